@@ -19,6 +19,13 @@ New entry points:
     O, L = decode_paged(q, k_pool, v_pool, page_table, ctx_lens, num_splits=16)
     part_o, part_lse = decode_partials(...);  O, L = lse_combine(part_o, part_lse)
 
+The same cache in 4 or 8 bits a value (MX pages, K and V each of its own width):
+
+    k_pool, v_pool = kv_pools_mx(num_pages, H_kv, D, k_bits=4, v_bits=4, device=...)
+    bad = kv_append_mx(k_new, v_new, k_pool, v_pool, page_table, start_pos)   # in place
+    k, v, bad = kv_read_mx(k_pool, v_pool, page_table, start_pos, num_tokens)
+    O, L = decode_paged_mx(q, k_pool, v_pool, page_table, ctx_lens)
+
 Every call runs the hand-written HIP kernels of ``libfa_mi355x.so`` through
 the C ABI in include/fa_mi355x.h. There is no fallback: importing this package
 without the built extension raises ImportError.
@@ -125,6 +132,59 @@ def decode_partials(q, k_pool, v_pool, page_table, ctx_lens, num_splits: int = 1
 def lse_combine(part_o, part_lse):
     """[O fp16 [B,H,D], L fp32 [B,H]] merged from split partials."""
     return _C.lse_combine(part_o, part_lse)
+
+
+def mx_page_bytes(D: int, bits: int) -> int:
+    """Bytes of an MX page (16 tokens of one head): 16 * D values of 4 or 8 bits
+    and a scale byte for every 32 of them."""
+    n = _C.mx_page_bytes(D, bits)
+    if n == 0:
+        raise RuntimeError("MX pages need a head dimension of 64 or 128 and 4 or 8 bits")
+    return n
+
+
+def kv_pools_mx(num_pages: int, H_kv: int, D: int, k_bits: int = 4, v_bits: int = 4, device="cuda"):
+    """(k_pool, v_pool): zeroed uint8 [num_pages, H_kv, mx_page_bytes(D, bits)].
+
+    Blocks of 32 values along D share a power-of-two scale; values are E2M1 (4
+    bits) or E4M3 (8 bits). The layout of a page is in include/fa_mi355x.h.
+    """
+    return tuple(torch.zeros(num_pages, H_kv, mx_page_bytes(D, b), dtype=torch.uint8, device=device)
+                 for b in (k_bits, v_bits))
+
+
+def kv_append_mx(k_new, v_new, k_pool, v_pool, page_table, start_pos, new_lens=None):
+    """kv_append into MX pages: k_new/v_new [B,H,T,D] (both fp16 or both bf16) are
+    quantised as they are written, in place; returns bad int32 [B] as kv_append.
+
+    Every value is rounded to the nearest its block's scale allows (blocks that
+    hold a NaN or an infinity read back as NaN).
+    """
+    return _C.kv_append_mx(k_new, v_new, k_pool, v_pool, page_table, start_pos, new_lens)
+
+
+def kv_read_mx(k_pool, v_pool, page_table, start_pos, num_tokens: int, lens=None,
+               dtype=torch.float16):
+    """[k, v, bad]: tokens start_pos[b] .. + num_tokens out of MX pages, k/v
+    [B,H_kv,num_tokens,D] in dtype (fp16 or bf16), without rounding for pages
+    written from rows of that dtype.
+
+    Rows from lens[b] on are zeros; a token with no valid page reads as NaN and
+    sets bad[b] (int32 [B]).
+    """
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise RuntimeError("dtype must be torch.float16 or torch.bfloat16")
+    return _C.kv_read_mx(k_pool, v_pool, page_table, start_pos, num_tokens, lens,
+                         dtype == torch.bfloat16)
+
+
+def decode_paged_mx(q, k_pool, v_pool, page_table, ctx_lens):
+    """[O, L] of one query token per sequence over its MX pages (decode_paged's
+    results for what the pages hold); q fp16 or bf16, O in q's dtype, L fp32.
+
+    The split over the pages follows the batch's lengths, on the device.
+    """
+    return _C.decode_paged_mx(q, k_pool, v_pool, page_table, ctx_lens)
 
 
 def loaded_libraries():

@@ -61,6 +61,13 @@ SIGNATURES = {
     "fa_fwd_splitkv_f16": (C.c_int, [_vp] * 6 + [_i64] * 5 + [C.c_int, _i64, _vp]),
     "fa_bwd_varlen_f16": (C.c_int, [_vp] * 11 + [_i64] * 6 + [C.c_int, _vp]),
     "fa_validate_bwd_varlen": (C.c_int, [_vp] * 11 + [_i64] * 6),
+    "fa_mx_page_bytes": (_i64, [_i64, _i64]),
+    "fa_validate_kv_append_mx": (C.c_int, [_vp] * 8 + [_i64] * 9),
+    "fa_kv_append_mx": (C.c_int, [_vp] * 8 + [_i64] * 9 + [C.c_int, _vp]),
+    "fa_kv_read_mx": (C.c_int, [_vp] * 8 + [_i64] * 9 + [C.c_int, _vp]),
+    "fa_validate_decode_mx": (C.c_int, [_vp] * 5 + [_i64] * 9 + [_vp] * 3),
+    "fa_decode_mx_workspace_floats": (_i64, [_i64] * 4),
+    "fa_decode_paged_mx": (C.c_int, [_vp] * 5 + [_i64] * 9 + [_vp] * 3 + [C.c_int, _vp]),
     "fa_probe_fwd_variant": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, C.c_int, C.c_int, _vp]),
     "fa_probe_fwd_variants": (C.c_int, [_vp, C.c_int, _i64, C.c_int]),
     "fa_probe_default_variant": (C.c_int, [_i64]),
@@ -80,6 +87,7 @@ STATUS = {
     "FA_ERR_BATCH_HEADS": 4, "FA_ERR_ALIGNMENT": 5, "FA_ERR_TOO_LARGE": 6,
     "FA_ERR_PAGE_SIZE": 7, "FA_ERR_NUM_SPLITS": 8, "FA_ERR_MAX_PAGES": 9,
     "FA_ERR_NUM_PAGES": 10, "FA_ERR_KV_HEADS": 11, "FA_ERR_SCRATCH_SIZE": 12,
+    "FA_ERR_MX_BITS": 13,
 }
 
 

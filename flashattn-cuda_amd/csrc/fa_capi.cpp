@@ -36,6 +36,7 @@ extern "C" const char* fa_status_str(int status) {
     case FA_ERR_KV_HEADS: return "H must be a positive multiple of H_kv";
     case FA_ERR_SCRATCH_SIZE:
       return "B*H*num_splits*(D+1) exceeds FA_DECODE_SCRATCH_FLOATS (no-alloc decode)";
+    case FA_ERR_MX_BITS: return "k_bits and v_bits must be 4 or 8";
     default: break;
   }
   if (status < 0) return "HIP error (negated hipError_t)";
@@ -187,4 +188,45 @@ extern "C" int64_t fa_decode_workspace_floats(int64_t B, int64_t H, int64_t D,
                                               int64_t num_splits) {
   if (B <= 0 || H <= 0 || D <= 0 || num_splits <= 0) return 0;
   return B * H * num_splits * (D + 1);
+}
+
+extern "C" int64_t fa_mx_page_bytes(int64_t D, int64_t bits) {
+  if ((D != 64 && D != 128) || (bits != 4 && bits != 8)) return 0;
+  return 16 * D * bits / 8 + 16 * D / 32;
+}
+
+// MX pages (no reference counterpart): the 16-bit writer's checks, the widths
+// and the flags, which the MX calls always write.
+extern "C" int fa_validate_kv_append_mx(const void* k, const void* v, const int32_t* page_table,
+                                        const int32_t* start_pos, const int32_t* lens,
+                                        const void* k_pool, const void* v_pool, const int32_t* bad,
+                                        int64_t B, int64_t H, int64_t T, int64_t D, int64_t k_bits,
+                                        int64_t v_bits, int64_t page_size, int64_t max_pages,
+                                        int64_t num_pages) {
+  if (!bad) return FA_ERR_NULL_POINTER;
+  const int st = fa_validate_kv_append(k, v, page_table, start_pos, lens, k_pool, v_pool, bad, B, H,
+                                       T, D, page_size, max_pages, num_pages);
+  if (st != FA_OK) return st;
+  if (fa_mx_page_bytes(D, k_bits) == 0 || fa_mx_page_bytes(D, v_bits) == 0) return FA_ERR_MX_BITS;
+  return FA_OK;
+}
+
+// The paged decode's checks, but for num_splits, which the MX decode has not.
+// Its grid is (chunks, head groups).
+extern "C" int fa_validate_decode_mx(const void* q, const void* k_pool, const void* v_pool,
+                                     const int32_t* page_table, const int32_t* ctx_lens, int64_t B,
+                                     int64_t H, int64_t H_kv, int64_t D, int64_t k_bits,
+                                     int64_t v_bits, int64_t page_size, int64_t max_pages,
+                                     int64_t num_pages, const float* workspace, const void* o,
+                                     const float* lse) {
+  const int st = fa_validate_decode(q, k_pool, v_pool, page_table, ctx_lens, B, H, D, page_size,
+                                    max_pages, num_pages, /*num_splits=*/1);
+  if (st != FA_OK) return st;
+  if (H_kv <= 0 || H % H_kv != 0) return FA_ERR_KV_HEADS;
+  if (fa_mx_page_bytes(D, k_bits) == 0 || fa_mx_page_bytes(D, v_bits) == 0) return FA_ERR_MX_BITS;
+  if (!workspace || !o) return FA_ERR_NULL_POINTER;
+  if (!aligned16(workspace) || !aligned16(o)) return FA_ERR_ALIGNMENT;
+  if (reinterpret_cast<uintptr_t>(lse) & 3u) return FA_ERR_ALIGNMENT;
+  if (num_pages > kMaxGrid) return FA_ERR_TOO_LARGE;
+  return FA_OK;
 }

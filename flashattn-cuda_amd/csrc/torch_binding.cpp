@@ -520,6 +520,153 @@ torch::Tensor kv_append(torch::Tensor k_new, torch::Tensor v_new, torch::Tensor 
   return bad;
 }
 
+// Pools of MX pages, uint8 [num_pages, H_kv, page_bytes]: page_bytes tells D and
+// the width.
+struct MxPools {
+  int64_t num_pages, Hkv, D, k_bits, v_bits;
+};
+
+MxPools check_mx_pools(const torch::Tensor& k_pool, const torch::Tensor& v_pool) {
+  TORCH_CHECK(k_pool.is_cuda() && v_pool.is_cuda(), "k_pool/v_pool must be CUDA tensors");
+  TORCH_CHECK(k_pool.dim() == 3 && v_pool.dim() == 3 && k_pool.scalar_type() == torch::kByte &&
+                  v_pool.scalar_type() == torch::kByte,
+              "k_pool and v_pool must be uint8 [num_pages, H_kv, page_bytes]");
+  TORCH_CHECK(v_pool.size(0) == k_pool.size(0) && v_pool.size(1) == k_pool.size(1),
+              "k_pool and v_pool must have the same num_pages and H_kv");
+  TORCH_CHECK(k_pool.is_contiguous() && v_pool.is_contiguous(), "MX pools must be contiguous");
+  TORCH_CHECK(k_pool.device() == v_pool.device(), "k_pool and v_pool must be on the same device");
+  MxPools m{k_pool.size(0), k_pool.size(1), 0, 0, 0};
+  for (const int64_t D : {64, 128}) {
+    int64_t kb = 0, vb = 0;
+    for (const int64_t bits : {4, 8}) {
+      if (k_pool.size(2) == fa_mx_page_bytes(D, bits)) kb = bits;
+      if (v_pool.size(2) == fa_mx_page_bytes(D, bits)) vb = bits;
+    }
+    if (kb && vb) m.D = D, m.k_bits = kb, m.v_bits = vb;
+  }
+  TORCH_CHECK(m.D != 0, "k_pool and v_pool must be pools of mx_page_bytes(D, bits) bytes a page "
+                        "with the same D (got ", k_pool.size(2), " and ", v_pool.size(2), ")");
+  return m;
+}
+
+// Page table and positions of an MX append or read.
+void check_mx_pages(const torch::Tensor& k_pool, const torch::Tensor& page_table,
+                    const torch::Tensor& start_pos, const c10::optional<torch::Tensor>& lens,
+                    int64_t B) {
+  const auto dev = k_pool.device();
+  TORCH_CHECK(page_table.is_cuda() && start_pos.is_cuda(),
+              "page_table/start_pos must be CUDA tensors");
+  TORCH_CHECK(page_table.dim() == 2 && page_table.scalar_type() == torch::kInt &&
+                  page_table.size(0) == B,
+              "page_table must be int32 [B, max_pages]");
+  TORCH_CHECK(start_pos.dim() == 1 && start_pos.scalar_type() == torch::kInt &&
+                  start_pos.size(0) == B,
+              "start_pos must be int32 [B]");
+  TORCH_CHECK(page_table.is_contiguous() && start_pos.is_contiguous(),
+              "page_table and start_pos must be contiguous");
+  TORCH_CHECK(page_table.device() == dev && start_pos.device() == dev,
+              "page_table and start_pos must be on the pools' device");
+  if (lens.has_value())
+    TORCH_CHECK(lens->is_cuda() && lens->dim() == 1 && lens->scalar_type() == torch::kInt &&
+                    lens->size(0) == B && lens->is_contiguous() && lens->device() == dev,
+                "lens must be a contiguous CUDA int32 [B] on the pools' device");
+}
+
+// kv_append_mx(k_new, v_new, k_pool, v_pool, page_table, start_pos,
+// new_lens=None) -> bad int32 [B]: kv_append into MX pages. No reference
+// counterpart.
+torch::Tensor kv_append_mx(torch::Tensor k_new, torch::Tensor v_new, torch::Tensor k_pool,
+                           torch::Tensor v_pool, torch::Tensor page_table, torch::Tensor start_pos,
+                           c10::optional<torch::Tensor> new_lens) {
+  TORCH_CHECK(k_new.is_cuda() && v_new.is_cuda(), "k_new/v_new must be CUDA tensors");
+  TORCH_CHECK(k_new.dim() == 4 && v_new.sizes() == k_new.sizes(),
+              "k_new and v_new must be [B, H, T, D] of the same shape");
+  TORCH_CHECK((k_new.scalar_type() == torch::kHalf || k_new.scalar_type() == torch::kBFloat16) &&
+                  v_new.scalar_type() == k_new.scalar_type(),
+              "k_new/v_new must be both float16 or both bfloat16");
+  TORCH_CHECK(k_new.is_contiguous() && v_new.is_contiguous(), "k_new and v_new must be contiguous");
+  const MxPools m = check_mx_pools(k_pool, v_pool);
+  const int64_t B = k_new.size(0), H = k_new.size(1), T = k_new.size(2), D = k_new.size(3);
+  TORCH_CHECK(m.Hkv == H && m.D == D, "the pools must have k_new's H and D");
+  check_mx_pages(k_pool, page_table, start_pos, new_lens, B);
+  const auto dev = k_pool.device();
+  TORCH_CHECK(k_new.device() == dev && v_new.device() == dev,
+              "kv_append_mx tensors must be on the same device");
+  const c10::DeviceGuard guard(dev);
+  auto bad = torch::empty({B}, page_table.options());
+  const int st = fa_kv_append_mx(
+      k_new.data_ptr(), v_new.data_ptr(), page_table.data_ptr<int32_t>(),
+      start_pos.data_ptr<int32_t>(), new_lens.has_value() ? new_lens->data_ptr<int32_t>() : nullptr,
+      k_pool.data_ptr(), v_pool.data_ptr(), bad.data_ptr<int32_t>(), B, H, T, D, m.k_bits, m.v_bits,
+      16, page_table.size(1), m.num_pages, k_new.scalar_type() == torch::kBFloat16,
+      current_stream(k_pool));
+  check_status(st, "fa_kv_append_mx");
+  return bad;
+}
+
+// kv_read_mx(k_pool, v_pool, page_table, start_pos, num_tokens, lens=None,
+// bf16=False) -> [k, v [B, H_kv, T, D], bad int32 [B]]. No reference counterpart.
+std::vector<torch::Tensor> kv_read_mx(torch::Tensor k_pool, torch::Tensor v_pool,
+                                      torch::Tensor page_table, torch::Tensor start_pos,
+                                      int64_t num_tokens, c10::optional<torch::Tensor> lens,
+                                      bool bf16) {
+  const MxPools m = check_mx_pools(k_pool, v_pool);
+  TORCH_CHECK(num_tokens >= 0, "num_tokens must be >= 0");
+  TORCH_CHECK(page_table.dim() == 2, "page_table must be int32 [B, max_pages]");
+  const int64_t B = page_table.size(0);
+  check_mx_pages(k_pool, page_table, start_pos, lens, B);
+  const c10::DeviceGuard guard(k_pool.device());
+  const auto opt = k_pool.options().dtype(bf16 ? torch::kBFloat16 : torch::kHalf);
+  auto k = torch::empty({B, m.Hkv, num_tokens, m.D}, opt), v = torch::empty_like(k);
+  auto bad = torch::empty({B}, page_table.options());
+  const int st = fa_kv_read_mx(
+      k_pool.data_ptr(), v_pool.data_ptr(), page_table.data_ptr<int32_t>(),
+      start_pos.data_ptr<int32_t>(), lens.has_value() ? lens->data_ptr<int32_t>() : nullptr,
+      k.data_ptr(), v.data_ptr(), bad.data_ptr<int32_t>(), B, m.Hkv, num_tokens, m.D, m.k_bits,
+      m.v_bits, 16, page_table.size(1), m.num_pages, bf16 ? 1 : 0, current_stream(k_pool));
+  check_status(st, "fa_kv_read_mx");
+  return {k, v, bad};
+}
+
+// decode_paged_mx(q, k_pool, v_pool, page_table, ctx_lens) -> [O, L]: the paged
+// decode over MX pages. No reference counterpart.
+std::vector<torch::Tensor> decode_paged_mx(torch::Tensor q, torch::Tensor k_pool,
+                                           torch::Tensor v_pool, torch::Tensor page_table,
+                                           torch::Tensor ctx_lens) {
+  TORCH_CHECK(q.is_cuda() && page_table.is_cuda() && ctx_lens.is_cuda(),
+              "q/page_table/ctx_lens must be CUDA tensors");
+  TORCH_CHECK(q.dim() == 3, "q must be 3D [B, H, D]");
+  TORCH_CHECK(q.scalar_type() == torch::kHalf || q.scalar_type() == torch::kBFloat16,
+              "q must be float16 or bfloat16");
+  const MxPools m = check_mx_pools(k_pool, v_pool);
+  const int64_t B = q.size(0), H = q.size(1), D = q.size(2);
+  TORCH_CHECK(m.D == D, "the pools must have q's D");
+  TORCH_CHECK(m.Hkv > 0 && H % m.Hkv == 0, "H must be a positive multiple of the pools' head count");
+  TORCH_CHECK(page_table.dim() == 2 && page_table.scalar_type() == torch::kInt,
+              "page_table must be int32 [B, max_pages]");
+  TORCH_CHECK(ctx_lens.dim() == 1 && ctx_lens.scalar_type() == torch::kInt,
+              "ctx_lens must be int32 [B]");
+  TORCH_CHECK(page_table.size(0) == B && ctx_lens.size(0) == B,
+              "page_table and ctx_lens must have q's batch size");
+  TORCH_CHECK(q.is_contiguous() && page_table.is_contiguous() && ctx_lens.is_contiguous(),
+              "decode tensors must be contiguous");
+  const auto dev = q.device();
+  TORCH_CHECK(k_pool.device() == dev && page_table.device() == dev && ctx_lens.device() == dev,
+              "decode tensors must be on the same device");
+  const c10::DeviceGuard guard(dev);
+  const auto f32 = q.options().dtype(torch::kFloat);
+  auto ws = torch::empty({fa_decode_mx_workspace_floats(B, H, m.Hkv, D)}, f32);
+  auto o = torch::empty({B, H, D}, q.options());
+  auto lse = torch::empty({B, H}, f32);
+  const int st = fa_decode_paged_mx(
+      q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), page_table.data_ptr<int32_t>(),
+      ctx_lens.data_ptr<int32_t>(), B, H, m.Hkv, D, m.k_bits, m.v_bits, 16, page_table.size(1),
+      m.num_pages, ws.data_ptr<float>(), o.data_ptr(), lse.data_ptr<float>(),
+      q.scalar_type() == torch::kBFloat16, current_stream(q));
+  check_status(st, "fa_decode_paged_mx");
+  return {o, lse};
+}
+
 // ---- layout probes (test support) ----
 torch::Tensor probe_mfma32(torch::Tensor a, torch::Tensor b, int64_t variant) {
   TORCH_CHECK(a.is_cuda() && a.sizes() == torch::IntArrayRef({32, 16}) && a.scalar_type() == torch::kHalf);
@@ -646,6 +793,16 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("kv_append", &kv_append, "write new K/V rows into the paged pools; returns bad [B]",
         py::arg("k_new"), py::arg("v_new"), py::arg("k_pool"), py::arg("v_pool"),
         py::arg("page_table"), py::arg("start_pos"), py::arg("new_lens") = py::none());
+  m.def("mx_page_bytes", &fa_mx_page_bytes, py::arg("D"), py::arg("bits"));
+  m.def("kv_append_mx", &kv_append_mx, "quantise new K/V rows into MX pages; returns bad [B]",
+        py::arg("k_new"), py::arg("v_new"), py::arg("k_pool"), py::arg("v_pool"),
+        py::arg("page_table"), py::arg("start_pos"), py::arg("new_lens") = py::none());
+  m.def("kv_read_mx", &kv_read_mx, "rows out of MX pages: returns [k, v, bad]", py::arg("k_pool"),
+        py::arg("v_pool"), py::arg("page_table"), py::arg("start_pos"), py::arg("num_tokens"),
+        py::arg("lens") = py::none(), py::arg("bf16") = false);
+  m.def("decode_paged_mx", &decode_paged_mx, "paged decode over MX pages: returns [O in q's dtype, L float]",
+        py::arg("q"), py::arg("k_pool"), py::arg("v_pool"), py::arg("page_table"),
+        py::arg("ctx_lens"));
   m.def("decode_paged", &decode_paged, "split-KV paged decode (fp16 or bf16): returns [O in q's dtype, L float]",
         py::arg("q"), py::arg("k_pool"), py::arg("v_pool"), py::arg("page_table"),
         py::arg("ctx_lens"), py::arg("num_splits") = 16);

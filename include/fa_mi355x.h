@@ -45,7 +45,8 @@ enum fa_status_code {
   FA_ERR_MAX_PAGES = 9,      /* max_pages <= 0 */
   FA_ERR_NUM_PAGES = 10,     /* num_pages <= 0 */
   FA_ERR_KV_HEADS = 11,      /* H_kv <= 0 or H not a multiple of H_kv */
-  FA_ERR_SCRATCH_SIZE = 12   /* split partials exceed FA_DECODE_SCRATCH_FLOATS */
+  FA_ERR_SCRATCH_SIZE = 12,  /* split partials exceed FA_DECODE_SCRATCH_FLOATS */
+  FA_ERR_MX_BITS = 13        /* k_bits or v_bits is not 4 or 8 */
 };
 
 /* Floats of the library's own split-partials array used by
@@ -415,6 +416,93 @@ int fa_bwd_cast_f32(const float* const f32[5], void* const h16[5], const float* 
 int fa_varlen_fill_outside(const int32_t* cu_seqlens, int64_t B, int64_t max_seqlen, int64_t total,
                            void* const buf[3], const int64_t heads[3], const int64_t words[3],
                            const uint32_t value[3], void* stream);
+
+/*
+ * KV cache in microscaling (MX) pages (no reference counterpart): the paged
+ * cache of fa_kv_append_f16 and fa_decode_paged_f16 in 4 or 8 bits a value, K
+ * and V each of its own width. A row's values lie in blocks of 32 along D,
+ * x = value * 2^(s - 127), with one byte s a block (255: NaN) and values in
+ * E2M1 (4 bits: 0, .5, 1, 1.5, 2, 3, 4, 6 and their negatives) or E4M3 (8 bits,
+ * up to 448).
+ *
+ * Pools are bytes, [num_pages, H_kv, fa_mx_page_bytes(D, bits)]: a page is 16
+ * tokens of one head, 16 * D * bits / 8 bytes of codes and then 16 * D / 32 of
+ * scales. In a byte of two values the one of even index is the low half. With
+ * w = D * bits / 8 the code bytes of a row:
+ *   K: byte j of row t at t w + j; for w = 128 at
+ *      1024 ((j % 32) / 16) + 16 (4 t + j / 32) + j % 16;
+ *      scale of block i of row t at 16 w + t D/32 + i.
+ *   V: with c = j / (w / 16), r = j % (w / 16), cell = 16 (t / 4) + c: byte j of
+ *      row t at cell w / 4 + (t % 4) w / 16 + r; for w = 128 at
+ *      1024 ((t % 4) / 2) + 16 cell + 8 (t % 2) + r;
+ *      scale of block i of row t at 16 w + 16 i + t.
+ */
+
+/* Bytes of a page of one head; 0 for a D or a width that has none. */
+int64_t fa_mx_page_bytes(int64_t D, int64_t bits);
+
+/* Host-only argument check of fa_kv_append_mx and fa_kv_read_mx (k, v: their 16-bit rows). */
+int fa_validate_kv_append_mx(const void* k, const void* v, const int32_t* page_table,
+                             const int32_t* start_pos, const int32_t* lens, const void* k_pool,
+                             const void* v_pool, const int32_t* bad, int64_t B, int64_t H, int64_t T,
+                             int64_t D, int64_t k_bits, int64_t v_bits, int64_t page_size,
+                             int64_t max_pages, int64_t num_pages);
+
+/*
+ * fa_kv_append_set_bad into MX pages: k_new, v_new (fp16, bf16 != 0: bfloat16,
+ * [B, H, T, D]) are quantised as they are written. The scale of a block whose
+ * largest magnitude is a is the smallest s >= 1 with a <= 7 * 2^(s - 127) (4
+ * bits) or 464 * 2^(s - 127) (8 bits), and at most the one for which the
+ * format's largest value is finite in the rows' type (4 bits: 140 in fp16, 252
+ * in bf16; 8 bits: 134, 246); values are rounded to nearest even and saturate.
+ * A block with a NaN or an infinity gets s = 255. Slots of the pages that the
+ * call does not cover keep what they hold. Every bad[b] is written.
+ */
+int fa_kv_append_mx(const void* k_new, const void* v_new, const int32_t* page_table,
+                    const int32_t* start_pos, const int32_t* new_lens, void* k_pool, void* v_pool,
+                    int32_t* bad, int64_t B, int64_t H, int64_t T, int64_t D, int64_t k_bits,
+                    int64_t v_bits, int64_t page_size, int64_t max_pages, int64_t num_pages,
+                    int bf16, void* stream);
+
+/*
+ * Tokens start_pos[b] .. + T of each sequence out of MX pages into k, v (fp16,
+ * bf16 != 0: bfloat16, [B, H, T, D]), exactly (a value beyond the type's range,
+ * which rows of that type do not leave in a page, is infinite). Rows from
+ * lens[b] (clamped to [0, T]; NULL: T) on are zeros. A token whose position is
+ * outside the table or whose page id is outside [0, num_pages) reads as NaN and
+ * sets bad[b] to 1; every other bad[b] is set to 0.
+ */
+int fa_kv_read_mx(const void* k_pool, const void* v_pool, const int32_t* page_table,
+                  const int32_t* start_pos, const int32_t* lens, void* k, void* v, int32_t* bad,
+                  int64_t B, int64_t H, int64_t T, int64_t D, int64_t k_bits, int64_t v_bits,
+                  int64_t page_size, int64_t max_pages, int64_t num_pages, int bf16, void* stream);
+
+/* Host-only argument check of fa_decode_paged_mx. */
+int fa_validate_decode_mx(const void* q, const void* k_pool, const void* v_pool,
+                          const int32_t* page_table, const int32_t* ctx_lens, int64_t B, int64_t H,
+                          int64_t H_kv, int64_t D, int64_t k_bits, int64_t v_bits,
+                          int64_t page_size, int64_t max_pages, int64_t num_pages,
+                          const float* workspace, const void* o, const float* lse);
+
+/* Floats of the workspace fa_decode_paged_mx needs (0 for invalid sizes). */
+int64_t fa_decode_mx_workspace_floats(int64_t B, int64_t H, int64_t H_kv, int64_t D);
+
+/*
+ * The paged decode over MX pages: q, o fp16 (bf16 != 0: bfloat16) [B, H, D],
+ * lse fp32 [B, H] or NULL, query head h reads pool head h / (H / H_kv). Results
+ * as fa_decode_paged_gqa_f16 over what the pages hold: o = 0 and lse = -inf of
+ * an empty context; a page id outside [0, num_pages), a negative length or one
+ * beyond max_pages * 16 make the sequence's o and lse NaN, and no memory outside the pools
+ * is read. How the pages are shared out follows from the lengths of the whole
+ * batch, so a sequence's last bits may depend on the others' lengths; the same
+ * call gives the same bits. workspace: 16-byte aligned, of the caller, need not
+ * be cleared; calls that may overlap need one each.
+ */
+int fa_decode_paged_mx(const void* q, const void* k_pool, const void* v_pool,
+                       const int32_t* page_table, const int32_t* ctx_lens, int64_t B, int64_t H,
+                       int64_t H_kv, int64_t D, int64_t k_bits, int64_t v_bits, int64_t page_size,
+                       int64_t max_pages, int64_t num_pages, float* workspace, void* o, float* lse,
+                       int bf16, void* stream);
 
 #ifdef __cplusplus
 }

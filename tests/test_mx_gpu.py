@@ -1,0 +1,466 @@
+"""GPU tier of the MX KV cache (kv_append_mx, kv_read_mx, decode_paged_mx)
+against its restatement in 64 bits (oracle/mx.py).
+
+Writer and reader have one rounding each, so the bar is equality: of every byte
+of both pools, slots that the call must not touch among them, and of every row
+read. The decode is held to a bound that follows from its roundings
+(oracle.mx.decode_mx).
+"""
+import numpy as np
+import pytest
+import torch
+
+from oracle import mx
+
+pytestmark = pytest.mark.gpu
+
+FORMS = [(64, 4, 4), (64, 8, 8), (64, 8, 4), (64, 4, 8), (128, 4, 4), (128, 8, 8), (128, 8, 4), (128, 4, 8)]
+TYPES = {False: torch.float16, True: torch.bfloat16}
+
+
+def _rows(rng, shape, bf16, spread=1.5):
+    """Rows whose blocks and channels differ in size, as bit patterns."""
+    x = rng.standard_normal(shape) * np.exp(spread * rng.standard_normal((*shape[:-1], 1)))
+    return mx.from_f64(x * np.exp(0.7 * rng.standard_normal(shape[-1])), bf16)
+
+
+def _pool(rng, pages, H, D, bits, is_v, bf16, spread=1.0):
+    codes, scales = mx.quantize(_rows(rng, (pages, H, 16, D), bf16, spread), bits, bf16)
+    return mx.pack_pages(codes, scales, bits, is_v)
+
+
+def _to(dev, *xs):
+    return [torch.from_numpy(np.ascontiguousarray(x)).to(dev) for x in xs]
+
+
+def _rows_to(dev, x16, bf16):
+    return torch.from_numpy(np.ascontiguousarray(x16).view(np.int16)).to(dev).view(TYPES[bf16])
+
+
+def _bits(t):
+    return t.cpu().view(torch.int16).numpy().view(np.uint16)
+
+
+def _append(fa, dev, kp, vp, table, start, k, v, bf16, lens=None):
+    tkp, tvp, tt, ts = _to(dev, kp, vp, table, start)
+    tl = None if lens is None else _to(dev, lens)[0]
+    bad = fa.kv_append_mx(_rows_to(dev, k, bf16), _rows_to(dev, v, bf16), tkp, tvp, tt, ts, tl)
+    return tkp.cpu().numpy(), tvp.cpu().numpy(), bad.cpu().numpy()
+
+
+def _same(got, want, tag):
+    for g, w, name in zip(got, want, ("k_pool", "v_pool", "bad")):
+        assert np.array_equal(g, w), f"{tag}: {name} differs in {(g != w).sum()} places"
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("D,kb,vb", FORMS)
+@pytest.mark.parametrize("B,H,T", [(1, 1, 1), (3, 2, 2), (2, 3, 37), (3, 1, 130)])
+def test_append_matches_oracle(fa, dev, B, H, T, D, kb, vb, bf16):
+    rng = np.random.default_rng(B * 100 + T + D + kb)
+    maxp = (T + 70) // 16 + 2
+    P = B * maxp + 3
+    table = rng.permutation(P).astype(np.int32)[:B * maxp].reshape(B, maxp)
+    kp = rng.integers(0, 256, (P, H, mx.page_bytes(D, kb))).astype(np.uint8)   # slots not covered keep theirs
+    vp = rng.integers(0, 256, (P, H, mx.page_bytes(D, vb))).astype(np.uint8)
+    k, v = _rows(rng, (B, H, T, D), bf16), _rows(rng, (B, H, T, D), bf16)
+    start = rng.integers(0, 60, B).astype(np.int32)
+    start[0] = 15   # the first token is a page's last slot
+    for lens in (None, rng.integers(-2, T + 3, B).astype(np.int32)):
+        want = mx.append_mx(kp, vp, table, start, k, v, kb, vb, bf16, lens)
+        _same(_append(fa, dev, kp, vp, table, start, k, v, bf16, lens), want, f"lens {lens}")
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("D,kb,vb", [(64, 4, 8), (128, 8, 4)])
+def test_append_of_every_value(fa, dev, D, kb, vb, bf16):
+    """All 65536 bit patterns, NaN, infinities, subnormals and both zeros among them, in blocks of
+    like size and shuffled, so that every scale and both of its limits come up."""
+    x = np.arange(65536, dtype=np.uint32).astype(np.uint16)
+    rng = np.random.default_rng(5)
+    x = np.concatenate([x, rng.permutation(x), rng.permutation(x[np.isfinite(mx.to_f64(x, bf16))])[:60000 // D * D]])
+    x = x.reshape(1, 1, -1, D)
+    T = x.shape[2]
+    P = -(-T // 16)
+    table = rng.permutation(P).astype(np.int32)[None]
+    kp, vp = (np.zeros((P, 1, mx.page_bytes(D, b)), np.uint8) for b in (kb, vb))
+    start = np.zeros(1, np.int32)
+    want = mx.append_mx(kp, vp, table, start, x, x, kb, vb, bf16)
+    got = _append(fa, dev, kp, vp, table, start, x, x, bf16)
+    _same(got, want, "every value")
+    k, v, bad = fa.kv_read_mx(*_to(dev, got[0], got[1], table, start), T, dtype=TYPES[bf16])
+    wk, wv, _ = mx.read_mx(want[0], want[1], table, start, T, D, kb, vb)
+    for g, w in ((k, wk), (v, wv)):
+        g = g.double().cpu().numpy()
+        assert ((g == w) | (np.isnan(g) & np.isnan(w))).all()
+
+
+@pytest.mark.parametrize("D,kb,vb", [(64, 4, 4), (128, 8, 4)])
+def test_append_bad_pages_and_positions(fa, dev, D, kb, vb):
+    B, H, T, maxp, P = 6, 2, 40, 5, 40
+    rng = np.random.default_rng(9)
+    table = rng.permutation(P).astype(np.int32)[:B * maxp].reshape(B, maxp).copy()
+    kp, vp = (rng.integers(0, 256, (P, H, mx.page_bytes(D, b))).astype(np.uint8) for b in (kb, vb))
+    k, v = _rows(rng, (B, H, T, D), False), _rows(rng, (B, H, T, D), False)
+    start = np.array([10, 0, maxp * 16 - 7, -2, -100, 2147483640], np.int32)
+    table[0, 1], table[1, 0] = -5, P
+    want = mx.append_mx(kp, vp, table, start, k, v, kb, vb, False)
+    assert want[2].tolist() == [1] * 6
+    _same(_append(fa, dev, kp, vp, table, start, k, v, False), want, "invalid")
+    tkp, tvp, tt, ts = _to(dev, want[0], want[1], table, start)
+    got = fa.kv_read_mx(tkp, tvp, tt, ts, T)
+    wk, wv, bad = mx.read_mx(want[0], want[1], table, start, T, D, kb, vb)
+    assert np.array_equal(got[2].cpu().numpy(), bad)
+    for g, w in zip(got[:2], (wk, wv)):
+        g, w = _bits(g), mx.from_f64(w, False)
+        ok = (g == w) | (((g & 0x7fff) > 0x7c00) & ((w & 0x7fff) > 0x7c00))   # NaN for NaN
+        assert ok.all()
+
+
+def test_flags_over_stale_memory_and_no_tokens(fa, dev):
+    B, H, D, P = 3, 2, 64, 30
+    kp, vp = fa.kv_pools_mx(P, H, D, 4, 8, device=dev)
+    table = torch.arange(P, dtype=torch.int32, device=dev).reshape(B, -1).contiguous()
+    start = torch.tensor([0, 16 * 10, -1], dtype=torch.int32, device=dev)
+    for T in (0, 3):
+        x = torch.randn(B, H, T, D, device=dev, dtype=torch.half)
+        stale = [torch.full((B,), 7, dtype=torch.int32, device=dev) for _ in range(4)]
+        del stale   # the caching allocator hands one of these blocks out next
+        assert fa.kv_append_mx(x, x, kp, vp, table, start).tolist() == [0, int(T > 0), int(T > 0)]
+        k, v, bad = fa.kv_read_mx(kp, vp, table, start, T)
+        assert bad.tolist() == [0, int(T > 0), int(T > 0)] and k.shape == v.shape == (B, H, T, D)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("D,kb,vb", FORMS)
+def test_read_matches_oracle(fa, dev, D, kb, vb, bf16):
+    """Any bytes: every code, and scales from below the type's range to above it (bf16: within it, as
+    its subnormal values are not told apart)."""
+    B, H, T, maxp, P = 3, 2, 75, 8, 26
+    rng = np.random.default_rng(D + kb + vb)
+    lo, hi = (30, 256) if bf16 else (80, 160)
+    pools = []
+    for bits, is_v in ((kb, False), (vb, True)):
+        codes = rng.integers(0, 16 if bits == 4 else 256, (P, H, 16, D)).astype(np.uint8)
+        scales = rng.integers(lo, hi, (P, H, 16, D // 32)).astype(np.uint8)
+        pools.append(mx.pack_pages(codes, scales, bits, is_v))
+    table = rng.permutation(P).astype(np.int32)[:B * maxp].reshape(B, maxp)
+    start = np.array([0, 13, 31], np.int32)
+    for lens in (None, np.array([1, T + 9, 16], np.int32), np.array([0, -4, T], np.int32)):
+        tl = None if lens is None else _to(dev, lens)[0]
+        k, v, bad = fa.kv_read_mx(*_to(dev, *pools, table, start), T, tl, dtype=TYPES[bf16])
+        wk, wv, wb = mx.read_mx(*pools, table, start, T, D, kb, vb, lens)
+        assert not bad.any() and not wb.any()
+        inf = 0x7f80 if bf16 else 0x7c00
+        for g, w, name in ((k, wk, "k"), (v, wv, "v")):
+            g, w = _bits(g), mx.from_f64(w, bf16)
+            same = (g == w) | (((g & 0x7fff) > inf) & ((w & 0x7fff) > inf))
+            assert same.all(), f"{name}: {(~same).sum()} differ"
+
+
+def _decode_case(seed, ctx, H, Hkv, D, kb, vb, bf16, poison=True, extra=0):
+    """Pools, table and queries; slots past the contexts and unused pages hold NaN."""
+    rng = np.random.default_rng(seed)
+    need = [-(-c // 16) for c in ctx]
+    P = sum(need) + 2
+    perm = rng.permutation(P).astype(np.int32)
+    table = np.full((len(ctx), max(max(need), 1) + extra), -1, np.int32)   # past a context: not looked at
+    kp, vp = _pool(rng, P, Hkv, D, kb, False, bf16), _pool(rng, P, Hkv, D, vb, True, bf16)
+    at = 0
+    for b, n in enumerate(need):
+        table[b, :n] = perm[at:at + n]
+        at += n
+        if poison and ctx[b] % 16:
+            for pool, bits, is_v in ((kp, kb, False), (vp, vb, True)):
+                co, so = mx.code_offsets(D, bits, is_v), mx.scale_offsets(D, bits, is_v)
+                for t in range(ctx[b] % 16, 16):
+                    pool[table[b, n - 1]][:, co[t]] = 0x7f
+                    pool[table[b, n - 1]][:, so[t]] = 255
+    if poison:
+        kp[perm[at:]] = 255
+        vp[perm[at:]] = 255
+    q = mx.from_f64(rng.standard_normal((len(ctx), H, D)), bf16)
+    return q, kp, vp, table, np.asarray(ctx, np.int32)
+
+
+def _check_decode(O, L, want, tag):
+    Ow, Lw, tO, tL = want
+    O, L = O.double().cpu().numpy(), L.double().cpu().numpy()
+    empty = np.isneginf(Lw)
+    assert np.array_equal(np.isneginf(L), empty) and (O[empty] == 0).all(), tag
+    eo = np.abs(O - Ow) / np.maximum(tO, 1e-300)
+    assert (np.abs(O - Ow) <= tO).all(), f"{tag}: O off by {np.nanmax(eo):.2f} of its bound"
+    el = np.abs(L[~empty] - Lw[~empty])
+    assert (el <= tL[~empty]).all(), f"{tag}: L off by {(el / tL[~empty]).max():.2f} of its bound"
+
+
+def _decode(fa, dev, case, kb, vb, bf16, tag):
+    q, kp, vp, table, ctx = case
+    print(f"[mx decode] {tag}: q {q.shape} ctx {ctx[:8]} K{kb} V{vb} bf16 {bf16}", flush=True)
+    tkp, tvp, tt, tc = _to(dev, kp, vp, table, ctx)
+    tq = _rows_to(dev, q, bf16)
+    O, L = fa.decode_paged_mx(tq, tkp, tvp, tt, tc)
+    _check_decode(O, L, mx.decode_mx(q, kp, vp, table, ctx, kb, vb, bf16), tag)
+    O2, L2 = fa.decode_paged_mx(tq, tkp, tvp, tt, tc)
+    assert torch.equal(O, O2) and torch.equal(L, L2), f"{tag}: two calls differ"
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("D,kb,vb", FORMS)
+@pytest.mark.parametrize("H,Hkv,ctx", [
+    (1, 1, [1]),
+    (4, 4, [0, 1, 15, 16, 17]),
+    (8, 2, [63, 64, 65, 250, 256, 257, 0]),
+    (6, 2, [1030]),
+])
+def test_decode_matches_oracle(fa, dev, H, Hkv, ctx, D, kb, vb, bf16):
+    _decode(fa, dev, _decode_case(H + D + kb, ctx, H, Hkv, D, kb, vb, bf16), kb, vb, bf16, f"H{H}/{Hkv}")
+
+
+@pytest.mark.parametrize("D,kb,vb,bf16,H,Hkv,ctx", [
+    (128, 4, 4, False, 32, 1, [9001]),            # two groups of 16 heads, one KV head, many chunks
+    (128, 4, 4, True, 40, 2, [3000, 5, 700]),     # groups of 20: 16 and 4
+    (64, 8, 8, False, 16, 4, [12000, 1, 0, 33]),  # one long sequence among short ones
+    (128, 8, 4, True, 8, 8, [4097, 4095, 16]),
+    (64, 4, 4, True, 4, 1, [20000]),
+])
+def test_decode_long_and_grouped(fa, dev, D, kb, vb, bf16, H, Hkv, ctx):
+    _decode(fa, dev, _decode_case(len(ctx) + H, ctx, H, Hkv, D, kb, vb, bf16), kb, vb, bf16, "long")
+
+
+@pytest.mark.parametrize("B", [64, 257, 1000])
+def test_decode_many_sequences(fa, dev, B):
+    """More sequences than a workgroup has threads, most of them short, empty ones among them."""
+    rng = np.random.default_rng(B)
+    ctx = rng.integers(0, 40, B)
+    ctx[rng.integers(0, B, 5)] = rng.integers(600, 2500, 5)
+    ctx[-1], ctx[0] = 1777, 0
+    _decode(fa, dev, _decode_case(B, ctx.tolist(), 2, 1, 64, 4, 8, False), 4, 8, False, f"B{B}")
+
+
+def test_decode_wide_table(fa, dev):
+    """A table far wider than the contexts: entries past them are not looked at."""
+    _decode(fa, dev, _decode_case(3, [5, 70, 16], 4, 2, 128, 4, 4, False, extra=3000), 4, 4, False, "wide")
+
+
+def test_decode_large_scores(fa, dev):
+    """One token far above the rest, and scores so large that all others vanish."""
+    D, n = 128, 500
+    q, kp, vp, table, ctx = _decode_case(2, [n, n], 2, 1, D, 8, 8, False)
+    for b, gain in ((0, 30.0), (1, 400.0)):
+        rows = np.zeros((1, 1, 1, D))
+        rows[..., :] = mx.to_f64(q[b, 0], False) * gain / np.sqrt(D)
+        k16 = mx.from_f64(rows, False)
+        kp, _, _ = mx.append_mx(kp, vp, table[b:b + 1], np.array([n // 3], np.int32), k16, k16, 8, 8, False)
+    _decode(fa, dev, (q, kp, vp, table, ctx), 8, 8, False, "large scores")
+
+
+def test_decode_bad_sequences_are_nan(fa, dev):
+    D, H = 64, 4
+    q, kp, vp, table, ctx = _decode_case(8, [40, 700, 100, 33, 16], H, 2, D, 4, 4, False)
+    want = mx.decode_mx(q, kp, vp, table, ctx, 4, 4, False)
+    table[0, 1] = kp.shape[0]
+    table[1, 17] = -1
+    ctx[2], ctx[3] = -1, table.shape[1] * 16 + 1
+    O, L = fa.decode_paged_mx(_rows_to(dev, q, False), *_to(dev, kp, vp, table, ctx))
+    assert torch.isnan(O[:4]).all() and torch.isnan(L[:4]).all()
+    _check_decode(O[4:], L[4:], [x[4:] for x in want], "the sequence that is valid")
+
+
+def test_decode_nan_block_reaches_its_heads_only(fa, dev):
+    D = 128
+    q, kp, vp, table, ctx = _decode_case(4, [50], 8, 4, D, 4, 4, True)
+    want = mx.decode_mx(q, kp, vp, table, ctx, 4, 4, True)
+    kp[table[0, 1], 2, mx.scale_offsets(D, 4, False)[3, 1]] = 255   # KV head 2: query heads 4 and 5
+    O, L = fa.decode_paged_mx(_rows_to(dev, q, True), *_to(dev, kp, vp, table, ctx))
+    assert torch.isnan(O[0, 4:6]).all() and torch.isnan(L[0, 4:6]).all()
+    keep = [0, 1, 2, 3, 6, 7]
+    _check_decode(O[:, keep], L[:, keep], [x[:, keep] for x in want], "other heads")
+
+
+def _serve(fa, dev, tk, tv, tq, kp, vp, table, prompt, steps):
+    """A prompt appended, then steps of append and decode: [O], [L]."""
+    ctx = prompt.clone()
+    bad = fa.kv_append_mx(tk[:, :, :int(prompt.max())].contiguous(), tv[:, :, :int(prompt.max())].contiguous(),
+                          kp, vp, table, torch.zeros_like(prompt), prompt)
+    assert not bad.any()
+    out = []
+    for i in range(steps):
+        sel = ctx.long()[:, None, None, None].expand(-1, tk.shape[1], 1, tk.shape[3])
+        fa.kv_append_mx(tk.gather(2, sel), tv.gather(2, sel), kp, vp, table, ctx)
+        ctx = ctx + 1
+        out.append(fa.decode_paged_mx(tq[i], kp, vp, table, ctx))
+    return out
+
+
+@pytest.mark.parametrize("D,kb,vb,bf16", [(128, 4, 4, True), (64, 8, 4, False)])
+def test_serving_run(fa, dev, D, kb, vb, bf16):
+    """Prompt, then 40 generated tokens, across page borders: every step against the oracle over the
+    cache as the oracle's writer fills it; at the end the cache read back equals it."""
+    B, H, Hkv, N = 3, 8, 2, 120
+    rng = np.random.default_rng(D)
+    k, v = _rows(rng, (B, Hkv, N, D), bf16, 0.5), _rows(rng, (B, Hkv, N, D), bf16, 0.5)
+    steps, prompt = 40, np.array([1, 47, 80], np.int32)
+    q = mx.from_f64(rng.standard_normal((steps, B, H, D)), bf16)
+    maxp, P = 8, 30
+    table = rng.permutation(P).astype(np.int32)[:B * maxp].reshape(B, maxp)
+    kp, vp = fa.kv_pools_mx(P, Hkv, D, kb, vb, device=dev)
+    tt, tp = _to(dev, table, prompt)
+    out = _serve(fa, dev, _rows_to(dev, k, bf16), _rows_to(dev, v, bf16), _rows_to(dev, q, bf16), kp, vp, tt, tp, steps)
+    wkp, wvp = np.zeros(tuple(kp.shape), np.uint8), np.zeros(tuple(vp.shape), np.uint8)
+    wkp, wvp, _ = mx.append_mx(wkp, wvp, table, np.zeros(B, np.int32), k, v, kb, vb, bf16, prompt + steps)
+    assert np.array_equal(kp.cpu().numpy(), wkp) and np.array_equal(vp.cpu().numpy(), wvp)
+    for i in range(0, steps, 3):
+        _check_decode(*out[i], mx.decode_mx(q[i], wkp, wvp, table, prompt + i + 1, kb, vb, bf16), f"step {i}")
+    rk, rv, bad = fa.kv_read_mx(kp, vp, tt, torch.zeros_like(tp), N, tp + steps, dtype=TYPES[bf16])
+    wk, wv, _ = mx.read_mx(wkp, wvp, table, np.zeros(B, np.int32), N, D, kb, vb, prompt + steps)
+    assert not bad.any()
+    assert np.array_equal(rk.double().cpu().numpy(), wk) and np.array_equal(rv.double().cpu().numpy(), wv)
+
+
+def test_captured_step_replays(fa, dev):
+    """Append and decode in one graph, replayed with new rows, lengths and eager calls of another
+    batch in between; two graphs of different shapes replayed in turn."""
+    rng = np.random.default_rng(11)
+    B, H, Hkv, D = 4, 8, 2, 128
+    graphs = []
+    for ctx in ([300, 17, 900, 64], [2000, 3, 16, 129]):
+        q, kp, vp, table, c = _decode_case(len(graphs), [n + 8 for n in ctx], H, Hkv, D, 4, 8, False, poison=False)
+        k, v = _rows(rng, (8, B, Hkv, 1, D), False, 0.5), _rows(rng, (8, B, Hkv, 1, D), False, 0.5)
+        st = dict(q=_rows_to(dev, q, False), table=table, host=(q, kp, vp), k=k, v=v, ctx=np.asarray(ctx, np.int32))
+        st["kp"], st["vp"], st["tt"], st["tc"] = _to(dev, kp, vp, table, st["ctx"])
+        st["tk"], st["tv"] = _rows_to(dev, k[0], False), _rows_to(dev, v[0], False)
+        graphs.append(st)
+
+    def step(s):
+        bad = fa.kv_append_mx(s["tk"], s["tv"], s["kp"], s["vp"], s["tt"], s["tc"])
+        s["tc"] += 1
+        return (*fa.decode_paged_mx(s["q"], s["kp"], s["vp"], s["tt"], s["tc"]), bad)
+
+    for s in graphs:   # first calls outside the capture; they take token 0
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(s)
+        torch.cuda.current_stream().wait_stream(side)
+        s["graph"] = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(s["graph"]):
+            s["out"] = step(s)
+    for i in range(1, 6):
+        for s in graphs:
+            s["tk"].copy_(_rows_to(dev, s["k"][i], False))
+            s["tv"].copy_(_rows_to(dev, s["v"][i], False))
+            s["graph"].replay()
+        e = graphs[i % 2]   # an eager call over the same memory between the replays
+        eo, el = fa.decode_paged_mx(e["q"], e["kp"], e["vp"], e["tt"], e["tc"])
+        torch.cuda.synchronize()
+        assert torch.equal(eo, e["out"][0]) and torch.equal(el, e["out"][1])
+        for s in graphs:
+            q, kp, vp = s["host"]
+            if i == 1:
+                kp, vp, _ = mx.append_mx(kp, vp, s["table"], s["ctx"], s["k"][0], s["v"][0], 4, 8, False)
+            kp, vp, _ = mx.append_mx(kp, vp, s["table"], s["ctx"] + i, s["k"][i], s["v"][i], 4, 8, False)
+            s["host"] = (q, kp, vp)
+            want = mx.decode_mx(q, kp, vp, s["table"], s["ctx"] + i + 1, 4, 8, False)
+            _check_decode(s["out"][0], s["out"][1], want, f"replay {i}")
+            assert not s["out"][2].any()
+
+
+def test_other_streams(fa, dev):
+    """Calls on two streams at once, each over its own batch, and the eager result of each."""
+    cases = [_decode_case(20 + i, [1500 + 700 * i, 40], 8, 2, 64, 4, 4, False) for i in range(2)]
+    args = [[_rows_to(dev, c[0], False), *_to(dev, *c[1:])] for c in cases]
+    want = [fa.decode_paged_mx(*a) for a in args]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(5):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(fa.decode_paged_mx(*args[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for O, L in got[i]:
+            assert torch.equal(O, want[i][0]) and torch.equal(L, want[i][1])
+
+
+def test_pool_beyond_4_gib(fa, dev):
+    """Pages whose byte offsets pass 2^32, written, read and attended."""
+    D, H, kb, vb, bf16 = 128, 8, 8, 4, False
+    P = (1 << 32) // (H * mx.page_bytes(D, kb)) + 3000
+    kp = torch.empty(P, H, mx.page_bytes(D, kb), dtype=torch.uint8, device=dev)
+    vp = torch.empty(P, H, mx.page_bytes(D, vb), dtype=torch.uint8, device=dev)
+    assert kp.numel() > 1 << 32
+    rng = np.random.default_rng(6)
+    n = 700
+    table = (P - 1 - rng.permutation(2000)[:-(-n // 16)]).astype(np.int32)[None]
+    k, v = _rows(rng, (1, H, n, D), bf16, 0.5), _rows(rng, (1, H, n, D), bf16, 0.5)
+    tt, ts, tc = _to(dev, table, np.zeros(1, np.int32), np.array([n], np.int32))
+    assert not fa.kv_append_mx(_rows_to(dev, k, bf16), _rows_to(dev, v, bf16), kp, vp, tt, ts).any()
+    used = table[0]
+    small = [mx.pack_pages(np.zeros((len(used), H, 16, D), np.uint8), np.zeros((len(used), H, 16, D // 32), np.uint8), b, z)
+             for b, z in ((kb, False), (vb, True))]
+    local = np.arange(len(used), dtype=np.int32)[None]
+    wk, wv, _ = mx.append_mx(*small, local, np.zeros(1, np.int32), k, v, kb, vb, bf16)
+    rk, rv, bad = fa.kv_read_mx(kp, vp, tt, ts, n)
+    ok, ov, _ = mx.read_mx(wk, wv, local, np.zeros(1, np.int32), n, D, kb, vb)
+    assert not bad.any() and np.array_equal(rk.double().cpu().numpy(), ok) and np.array_equal(rv.double().cpu().numpy(), ov)
+    q = mx.from_f64(rng.standard_normal((1, 16, D)), bf16)
+    O, L = fa.decode_paged_mx(_rows_to(dev, q, bf16), kp, vp, tt, tc)
+    _check_decode(O, L, mx.decode_mx(q, wk, wv, local, np.array([n]), kb, vb, bf16), "beyond 4 GiB")
+
+
+def test_agrees_with_16_bit_decode(fa, dev):
+    """The 16-bit decode over the rows that kv_read_mx returns is the same attention."""
+    B, H, Hkv, D, n = 2, 8, 2, 128, 1000
+    q, kp, vp, table, ctx = _decode_case(31, [n, 333], H, Hkv, D, 4, 4, False)
+    tq, (tkp, tvp, tt, tc) = _rows_to(dev, q, False), _to(dev, kp, vp, table, ctx)
+    k, v, _ = fa.kv_read_mx(tkp, tvp, tt, torch.zeros_like(tc), n, tc)
+    P = B * (-(-n // 16))
+    kp16 = torch.zeros(P, Hkv, 16, D, dtype=torch.half, device=dev)
+    vp16 = torch.zeros_like(kp16)
+    t16 = torch.arange(P, dtype=torch.int32, device=dev).reshape(B, -1)
+    fa.kv_append(k, v, kp16, vp16, t16, torch.zeros_like(tc))
+    O, L = fa.decode_paged_mx(tq, tkp, tvp, tt, tc)
+    O16, L16 = fa.decode_paged(tq, kp16, vp16, t16, tc)
+    _check_decode(O, L, mx.decode_mx(q, kp, vp, table, ctx, 4, 4, False), "MX")
+    # the 16-bit decode holds weights of at most 1 in fp16, in steps of 2^-24
+    _check_decode(O16, L16, mx.decode_mx(q, kp, vp, table, ctx, 4, 4, False, p_top=1.0), "16 bits")
+
+
+def test_rejects_bad_arguments(fa, dev):
+    kp, vp = fa.kv_pools_mx(4, 2, 64, 4, 8, device=dev)
+    x = torch.zeros(1, 2, 3, 64, dtype=torch.half, device=dev)
+    t = torch.zeros(1, 2, dtype=torch.int32, device=dev)
+    s = torch.zeros(1, dtype=torch.int32, device=dev)
+    q = torch.zeros(1, 4, 64, dtype=torch.half, device=dev)
+    k128, _ = fa.kv_pools_mx(4, 2, 128, 4, 4, device=dev)
+    for call, match in [
+        (lambda: fa.kv_append_mx(x.float(), x.float(), kp, vp, t, s), "float16"),
+        (lambda: fa.kv_append_mx(x, x.bfloat16(), kp, vp, t, s), "float16"),
+        (lambda: fa.kv_append_mx(x, x[:, :, :2], kp, vp, t, s), "same shape"),
+        (lambda: fa.kv_append_mx(x.transpose(1, 2), x.transpose(1, 2), kp, vp, t, s), "contiguous"),
+        (lambda: fa.kv_append_mx(x, x, kp.half(), vp, t, s), "uint8"),
+        (lambda: fa.kv_append_mx(x, x, k128, vp, t, s), "same D"),
+        (lambda: fa.kv_append_mx(x, x, kp[:, :, :500].contiguous(), vp, t, s), "page_bytes"),
+        (lambda: fa.kv_append_mx(x, x, kp[:2], vp, t, s), "num_pages"),
+        (lambda: fa.kv_append_mx(x, x, kp[:, :1], vp[:, :1], t, s), "contiguous"),
+        (lambda: fa.kv_append_mx(x[:, :1].contiguous(), x[:, :1].contiguous(), kp, vp, t, s), "H and D"),
+        (lambda: fa.kv_append_mx(x, x, kp, vp, t.long(), s), "int32"),
+        (lambda: fa.kv_append_mx(x, x, kp, vp, t, s.long()), "int32"),
+        (lambda: fa.kv_append_mx(x, x, kp, vp, t, s, s.long()), "int32"),
+        (lambda: fa.kv_append_mx(x, x, kp, vp, t.cpu(), s), "CUDA"),
+        (lambda: fa.kv_read_mx(kp, vp, t, s, -1), "num_tokens"),
+        (lambda: fa.kv_read_mx(kp, vp, t, s.cpu(), 1), "CUDA"),
+        (lambda: fa.kv_read_mx(kp, vp, t, torch.zeros(2, dtype=torch.int32, device=dev), 1), "start_pos"),
+        (lambda: fa.decode_paged_mx(q.float(), kp, vp, t, s), "float16 or bfloat16"),
+        (lambda: fa.decode_paged_mx(q[:, :3].contiguous(), kp, vp, t, s), "multiple"),
+        (lambda: fa.decode_paged_mx(q[:, :, :32].contiguous(), kp, vp, t, s), "q's D"),
+        (lambda: fa.decode_paged_mx(q.transpose(1, 2).contiguous().transpose(1, 2), kp, vp, t, s), "contiguous"),
+        (lambda: fa.decode_paged_mx(q, kp, vp, t[:0], s), "batch size"),
+        (lambda: fa.decode_paged_mx(q[:0], kp, vp, t[:0], s[:0]), "NULL"),
+        (lambda: fa.decode_paged_mx(q, kp, vp, t[:, :0], s), "max_pages"),
+        (lambda: fa.decode_paged_mx(q, kp[:0], vp[:0], t, s), "NULL|num_pages"),
+    ]:
+        with pytest.raises(RuntimeError, match=match):
+            call()
