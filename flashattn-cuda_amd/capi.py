@@ -66,7 +66,7 @@ SIGNATURES = {
     "fa_kv_append_mx": (C.c_int, [_vp] * 8 + [_i64] * 9 + [C.c_int, _vp]),
     "fa_kv_read_mx": (C.c_int, [_vp] * 8 + [_i64] * 9 + [C.c_int, _vp]),
     "fa_validate_decode_mx": (C.c_int, [_vp] * 5 + [_i64] * 9 + [_vp] * 3),
-    "fa_decode_mx_workspace_floats": (_i64, [_i64] * 4),
+    "fa_decode_mx_workspace_floats": (_i64, [_i64] * 5),
     "fa_decode_paged_mx": (C.c_int, [_vp] * 5 + [_i64] * 9 + [_vp] * 3 + [C.c_int, _vp]),
     "fa_probe_fwd_variant": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, C.c_int, C.c_int, _vp]),
     "fa_probe_fwd_variants": (C.c_int, [_vp, C.c_int, _i64, C.c_int]),
@@ -75,6 +75,7 @@ SIGNATURES = {
     "fa_probe_splitkv_plan_cus": (C.c_int, [_i64] * 4 + [C.c_int, C.c_int]),
     "fa_probe_unit_of": (C.c_int, [_i64, _i64, C.c_int, C.c_int, C.c_int, _i64, _vp, _vp]),
     "fa_probe_decode_ordered": (C.c_int, [_i64] * 5 + [C.c_int]),
+    "fa_probe_mx_chunks": (C.c_int, [_i64] * 5 + [C.POINTER(_i64)]),
     "fa_probe_bwd_block_rows": (C.c_int, [C.c_int, _i64, _i64, C.c_int]),
     "fa_probe_read_bw": (C.c_int, [_vp, _i64, C.c_int, _vp, _vp]),
     "fa_probe_gather_bw": (C.c_int, [_vp, _vp, _vp, _i64, C.c_int, C.c_int, _vp, _vp]),

@@ -22,123 +22,208 @@
 
 #include "fa_mi355x.h"
 #include "fa_mx.hpp"
+#include "fa_probe.h"
 
 namespace fa {
 namespace mx {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-constexpr int kBatch = 4;   // pages that a wave takes at a time
+constexpr int kXcds = 8;
+constexpr int kBatch = 2;   // pages that a wave takes at a time
 
-// Chunks. The pages of all sequences, T in all, are cut into runs of
-// C = max(kMinChunk, T / kTargetChunks per head group) pages, a sequence into
-// ceil(pages / C) nearly equal ones: workgroups of like size whatever the
-// lengths, about kTargetChunks of them, from lengths that only the device
-// knows. The grid has the most chunks that any lengths can give, and the rest
-// end at once.
-constexpr int kTargetChunks = 512;
-constexpr int kMinChunk = 16;
+// Chunks. The pages of all sequences, T in all, are cut into runs of C pages
+// (and a shorter one at a sequence's end): workgroups of like size
+// whatever the lengths, from lengths that only the device knows. The grid has
+// the most chunks that any lengths can give, and the rest end at once.
+//
+// C, for the batch's T pages (chunks are counted along the pages; a chunk is a
+// workgroup for every head group):
+//   kMinChunk pages while they make fewer than kFill workgroups,
+//   then what makes kFill of them, up to kMaxChunk pages,
+//   then kMaxChunk pages, until they make kMost workgroups.
+// kFill is four workgroups a CU (three of these are resident at a time); the
+// chunks past kMaxChunk pages buy balance at little cost. Besides, at most
+// kRowFill chunks a sequence (one of 131072 tokens over one KV head: 20.7 us in
+// 512 chunks, 16.0 in 256, 17.9 in 128), and where there are about as many
+// sequences as chunks wanted, only those of twice the mean length are cut (256
+// of 100 to 900 tokens over 4 KV heads: 20 -> 15.4 us).
+constexpr int kFill = 1024, kMost = 4096;
+constexpr int kMinChunk = 16, kMaxChunk = 128;
+constexpr int kRowFill = 256;
+
+// Rows up to which the join gives a row a workgroup for each 32 columns (one
+// sequence of 131072 tokens, 32 rows in 256 chunks: 6 us less).
+constexpr int kWideJoin = 1024;
+
+// Pools from this size on do not stay in the caches between two steps; their
+// codes are read with the non-temporal hint (2.5 GB: 440 -> 390 us, 300 MB: 64
+// -> 59; 35 MB, which do stay: 14.5 -> 16.0). Scales are read without it:
+// their lines are shared with the codes' ends and with the next page's.
+constexpr int64_t kPassThrough = 64 << 20;
 
 static int64_t head_groups(int64_t H, int64_t Hkv) { return Hkv * ((H / Hkv + 15) / 16); }
-// Chunks along the pages that each head group is cut into, at most this many
-// and one a sequence: sum ceil(p / C) <= T / C + B.
-static int64_t target_chunks(int64_t H, int64_t Hkv) {
+
+// Chunks along the pages that make kFill and kMost workgroups.
+struct Plan {
+  unsigned fill, most;
+};
+static Plan plan_of(int64_t B, int64_t H, int64_t Hkv) {
   const int64_t g = head_groups(H, Hkv);
-  return (kTargetChunks + g - 1) / g;
+  int64_t fill = (kFill + g - 1) / g;
+  if (fill > kRowFill * B) fill = kRowFill * B;
+  if (B >= fill && 3 * B < 4 * fill) fill = 3 * B / 4 > 0 ? 3 * B / 4 : 1;
+  return {(unsigned)fill, (unsigned)((kMost + g - 1) / g)};
 }
-// Chunks of the sequences that are cut at all: ceil(p / C) < 2 p / C of each.
-static int64_t partial_chunks(int64_t B, int64_t H, int64_t Hkv) {
-  const int64_t w = target_chunks(H, Hkv);
-  return w + (B < w ? B : w);
+
+// Pages of a chunk where the batch has `total`.
+__host__ __device__ inline int chunk_pages(int total, Plan plan) {
+  const unsigned c = ((unsigned)total + plan.fill - 1) / plan.fill;
+  if (c <= kMaxChunk) return c < kMinChunk ? kMinChunk : (int)c;
+  const unsigned d = ((unsigned)total + plan.most - 1) / plan.most;
+  return d < kMaxChunk ? kMaxChunk : (int)d;
 }
+
+// total / chunk_pages(total) for any total up to B * max_pages, at most: all
+// that the host knows. sum ceil(p / C) <= total / C + B, so the chunks are at
+// most this many and one a sequence.
+static int64_t most_chunks(int64_t B, int64_t H, int64_t Hkv, int64_t max_pages) {
+  const int64_t total = B * max_pages;
+  const int64_t fill = plan_of(B, H, Hkv).fill, most = plan_of(B, H, Hkv).most;
+  const int64_t by_max = total / kMaxChunk < most ? total / kMaxChunk : most;
+  const int64_t by_min = total / kMinChunk, n = fill > by_max ? fill : by_max;
+  return (n < by_min ? n : by_min) + 1;
+}
+// Chunks of the sequences that are cut at all, more than one a sequence: such a
+// sequence has more than C pages and less than 2 pages / C chunks.
+static int64_t partial_chunks(int64_t B, int64_t most) { return most + (B < most ? B : most); }
 
 // What a workgroup's chunk is.
 struct Chunk {
   int b;        // sequence, -1: none
-  int split, splits;
+  int ctx;      // its length
+  int split, splits;   // number of the chunk in the sequence, and how many there are
   int partial;  // of the sequence's first chunk, among those of cut sequences
-  int cut;      // the sequence's number among those
+  int index;    // the sequence's number among those
   int cuts;     // cut sequences in all
 };
 
 __device__ __forceinline__ int pages_of(int ctx, int max_pages) {
-  const int64_t p = ((int64_t)ctx + kTokens - 1) / kTokens;
-  return ctx <= 0 || p > max_pages ? 0 : (int)p;   // of an invalid length: none
+  const int p = (int)(((unsigned)max(ctx, 0) + kTokens - 1) / kTokens);
+  return p > max_pages ? 0 : p;   // of an invalid length: none
 }
 
-// Exclusive prefix over the workgroup's threads, and the sum.
-__device__ __forceinline__ int block_scan(int x, int* sh, int* total) {
+// Of a sequence of p pages: its chunks (p / C to the nearest, so that none is
+// under C / 2 longer or shorter than C by half), and what it adds to the count
+// of cut sequences (<< 16) and of their chunks. Those chunks are fewer than
+// 2 kMost.
+__device__ __forceinline__ int chunks_of(int p, int C, int* cut) {
+  const int s = max(1, (int)((2u * (unsigned)p + (unsigned)C) / (2u * (unsigned)C)));
+  *cut = s > 1 ? (s | 1 << 16) : 0;
+  return s;
+}
+
+// Exclusive prefixes of x and y over the workgroup's threads, and their sums.
+__device__ __forceinline__ void block_scan(int& x, int& y, int* sh, int* sum_x, int* sum_y) {
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int inc = scan_sum(x);
-  if (lane == 63) sh[wave] = inc;
-  __syncthreads();
-  int before = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    const int t = sh[w];
-    before += w < wave ? t : 0;
-    all += t;
+  const int ix = scan_sum(x), iy = scan_sum(y);
+  __syncthreads();   // sh may still be read
+  if (lane == 63) {
+    sh[wave] = ix;
+    sh[kWaves + wave] = iy;
   }
   __syncthreads();
-  *total = all;
-  return before + inc - x;
+  int bx = 0, by = 0;
+  *sum_x = *sum_y = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    bx += w < wave ? sh[w] : 0;
+    by += w < wave ? sh[kWaves + w] : 0;
+    *sum_x += sh[w];
+    *sum_y += sh[kWaves + w];
+  }
+  x = bx + ix - x;
+  y = by + iy - y;
 }
 
 // Chunk number x of the batch.
 __device__ __forceinline__ Chunk chunk_of(const int32_t* __restrict__ ctx_lens, int B,
-                                          int max_pages, int target, int x, int* sh) {
+                                          int max_pages, Plan plan, int x, int* sh) {
   Chunk r;
   if (B == 1) {
-    const int p = pages_of(ctx_lens[0], max_pages);
-    const int C = max(kMinChunk, (p + target - 1) / target);
-    r.splits = max(1, (p + C - 1) / C);
-    r.b = x < r.splits ? 0 : -1;
+    r.ctx = ctx_lens[0];
+    const int p = pages_of(r.ctx, max_pages);
+    r.splits = chunks_of(p, chunk_pages(p, plan), &r.cuts);
     r.split = x;
-    r.partial = 0;
-    r.cut = 0;
-    r.cuts = r.splits > 1;
+    r.b = x < r.splits ? 0 : -1;
+    r.partial = r.index = 0;
+    r.cuts >>= 16;
+    return r;
+  }
+  if (B <= 64) {   // a lane has a sequence; every wave finds the chunk by itself
+    const int lane = threadIdx.x & 63;
+    const int ctx = lane < B ? ctx_lens[lane] : 0;
+    const int p = pages_of(ctx, max_pages);
+    const int C = chunk_pages(__builtin_amdgcn_readlane(scan_sum(p), 63), plan);
+    int m, n = lane < B ? chunks_of(p, C, &m) : (m = 0);
+    const int in = scan_sum(n), im = scan_sum(m);
+    const int at = __popcll(__ballot(in <= x));   // lanes whose chunks end before x
+    if (at >= B) {
+      r.b = -1;
+      return r;
+    }
+    r.b = at;
+    r.ctx = __builtin_amdgcn_readlane(ctx, at);
+    r.split = x - __builtin_amdgcn_readlane(in - n, at);
+    r.splits = __builtin_amdgcn_readlane(n, at);
+    const int before = __builtin_amdgcn_readlane(im - m, at);
+    r.partial = before & 0xffff;
+    r.index = before >> 16;
+    r.cuts = __builtin_amdgcn_readlane(im, 63) >> 16;
     return r;
   }
   const int per = (B + kThreads - 1) / kThreads;
-  const int i0 = (int)threadIdx.x * per, i1 = min(i0 + per, B);
-  int mine = 0, total;
+  const int i0 = min((int)threadIdx.x * per, B), i1 = min(i0 + per, B);
+  int mine = 0, zero = 0, total, none;
   for (int i = i0; i < i1; ++i) mine += pages_of(ctx_lens[i], max_pages);
-  block_scan(mine, sh, &total);
-  const int C = max(kMinChunk, (total + target - 1) / target);
-  // Chunks, and of the cut sequences (chunks, sequences) in one number: their
-  // chunks are less than 2 target + 1.
-  int n = 0, m = 0, all;
+  block_scan(mine, zero, sh, &total, &none);
+  const int C = chunk_pages(total, plan);
+  int n = 0, m = 0, chunks, cuts;
   for (int i = i0; i < i1; ++i) {
-    const int s = (pages_of(ctx_lens[i], max_pages) + C - 1) / C;
-    n += max(1, s);
-    m += s > 1 ? (s | 1 << 16) : 0;
+    int cut;
+    n += chunks_of(pages_of(ctx_lens[i], max_pages), C, &cut);
+    m += cut;
   }
-  int e = block_scan(n, sh, &all);
-  int f = block_scan(m, sh, &total);
-  if (threadIdx.x == 0) sh[0] = -1;
+  const int end = n;
+  block_scan(n, m, sh, &chunks, &cuts);
+  if (x >= chunks) {   // the same in every thread
+    r.b = -1;
+    return r;
+  }
   __syncthreads();
-  if (x >= e && x < e + n) {   // one thread
+  if (x >= n && x < n + end) {   // one thread's
     for (int i = i0; i < i1; ++i) {
-      const int s = (pages_of(ctx_lens[i], max_pages) + C - 1) / C;
-      if (x < e + max(1, s)) {
+      int cut;
+      const int s = chunks_of(pages_of(ctx_lens[i], max_pages), C, &cut);
+      if (x < n + s) {
         sh[0] = i;
-        sh[1] = x - e;
-        sh[2] = max(1, s);
-        sh[3] = f;
+        sh[1] = x - n;
+        sh[2] = s;
+        sh[3] = m;
         break;
       }
-      e += max(1, s);
-      f += s > 1 ? (s | 1 << 16) : 0;
+      n += s;
+      m += cut;
     }
   }
   __syncthreads();
   r.b = sh[0];
+  r.ctx = ctx_lens[r.b];
   r.split = sh[1];
   r.splits = sh[2];
   r.partial = sh[3] & 0xffff;
-  r.cut = sh[3] >> 16;
-  r.cuts = total >> 16;
-  __syncthreads();
+  r.index = sh[3] >> 16;
+  r.cuts = cuts >> 16;
   return r;
 }
 
@@ -172,19 +257,36 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 }
 
 // A lane's piece of a page.
-template <int WORDS>
+template <bool NT, typename T>
+__device__ __forceinline__ T load_as(const char* p) {
+  if constexpr (NT) return __builtin_nontemporal_load(reinterpret_cast<const T*>(p));
+  return *reinterpret_cast<const T*>(p);
+}
+template <bool NT, int WORDS>
 __device__ __forceinline__ void load_piece(const char* p, uint32_t (&w)[WORDS]) {
   if constexpr (WORDS == 2) {
-    const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+    const u32x2 x = load_as<NT, u32x2>(p);
     w[0] = x[0];
     w[1] = x[1];
   } else {
 #pragma unroll
     for (int j = 0; j < WORDS / 4; ++j) {
-      const u32x4 x = *reinterpret_cast<const u32x4*>(p + 1024 * j);
+      const u32x4 x = load_as<NT, u32x4>(p + 1024 * j);
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[4 * j + i] = x[i];
     }
+  }
+}
+
+// Clears the codes of a V piece's tokens from n on.
+template <int WORDS>
+__device__ __forceinline__ void keep_tokens(uint32_t (&w)[WORDS], int n) {
+#pragma unroll
+  for (int j = 0; j < WORDS; ++j) {
+    if constexpr (WORDS == 2)
+      w[j] &= n >= 2 * j + 2 ? 0xffffffffu : n > 2 * j ? 0xffffu : 0u;
+    else
+      w[j] = j / (WORDS / 4) < n ? w[j] : 0u;
   }
 }
 
@@ -204,14 +306,15 @@ __device__ __forceinline__ uint32_t v_pair(const uint32_t (&w)[Page<D, VB>::WORD
   return values2<VB, BF16, N % PER / 2>(w[N / PER], scale);
 }
 
-template <int D, int KB, int VB, bool BF16>
+// NT: the pages are read with the non-temporal hint.
+template <int D, int KB, int VB, bool BF16, bool NT>
 __global__ void __launch_bounds__(kThreads)
 fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_pool,
                     const char* __restrict__ v_pool, const int32_t* __restrict__ page_table,
                     const int32_t* __restrict__ ctx_lens, float* __restrict__ part_o,
                     float* __restrict__ part_l, int32_t* __restrict__ plan,
                     uint16_t* __restrict__ o, float* __restrict__ lse, int B, int H, int Hkv,
-                    int max_pages, int num_pages, int target, float c) {
+                    int group, int ngrp, int max_pages, int num_pages, int slots, Plan chunk_plan, float c) {
   using PK = Page<D, KB>;
   using PV = Page<D, VB>;
   constexpr int KS = D / 32;   // steps of S = K Q^T
@@ -221,27 +324,31 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
   constexpr float kShift = BF16 ? 0.f : 15.f;
   __shared__ __attribute__((aligned(16))) float sh_o[kWaves][16][D + 4];   // heads in different banks
   __shared__ float sh_m[kWaves][16], sh_l[kWaves][16];
-  __shared__ int sh_i[4];
+  __shared__ int sh_i[2 * kWaves];
   __shared__ int sh_bad;
 
-  const int group = H / Hkv, ngrp = (group + 15) / 16;
-  const int hk = blockIdx.y / ngrp;
-  const int h0 = hk * group + 16 * (blockIdx.y % ngrp);   // first query head of this workgroup
-  const int G = min(16, hk * group + group - h0);
+  // Workgroups go to the XCDs in turn: an XCD has every eighth chunk, and the
+  // head groups of a chunk one after the other, so that what is read of a page
+  // at about the same time by one L2 is contiguous.
+  const int x = blockIdx.y * kXcds + blockIdx.x % kXcds, hg = blockIdx.x / kXcds;
+  const int hk = ngrp == 1 ? hg : hg / ngrp, sub = ngrp == 1 ? 0 : hg % ngrp;
+  const int h0 = hk * group + 16 * sub;   // first query head of this workgroup
+  const int G = min(16, group - 16 * sub);
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, grp = lane >> 4;
 
   if (tid == 0) sh_bad = 0;
-  Chunk ch = chunk_of(ctx_lens, B, max_pages, target, (int)blockIdx.x, sh_i);
+  Chunk ch = chunk_of(ctx_lens, B, max_pages, chunk_plan, x, sh_i);
   ch.b = __builtin_amdgcn_readfirstlane(ch.b);
   if (ch.b < 0) return;
+  const int ctx = __builtin_amdgcn_readfirstlane(ch.ctx);
+  const int pages = pages_of(ctx, max_pages);
   ch.split = __builtin_amdgcn_readfirstlane(ch.split);
   ch.splits = __builtin_amdgcn_readfirstlane(ch.splits);
-  const int ctx = ctx_lens[ch.b];
-  const int pages = __builtin_amdgcn_readfirstlane(pages_of(ctx, max_pages));
-  const int len = (pages + ch.splits - 1) / ch.splits;
-  const int p0 = min(ch.split * len, pages), p1 = min(p0 + len, pages);
+  // The first pages % splits chunks have a page more: none is empty.
+  const int each = (int)((unsigned)pages / (unsigned)ch.splits), more = pages - each * ch.splits;
+  const int p0 = ch.split * each + min(ch.split, more), p1 = p0 + each + (ch.split < more);
   // This wave's pages.
   const int w0 = p0 + (p1 - p0) * wave / kWaves, w1 = p0 + (p1 - p0) * (wave + 1) / kWaves;
   bool bad = ctx < 0 || (ctx > 0 && pages == 0);
@@ -256,10 +363,10 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
                                                grp * (D / 4) + 8 * kb);
   }
 
-  const int koff = (4 * col + grp) * (PK::PIECE < 16 ? PK::PIECE : 16);
-  const int voff = lane * (PV::PIECE < 16 ? PV::PIECE : 16);
-  const int ksoff = k_scale<D, KB>(col, grp * PK::BLOCKS / 4);
-  const int vsoff = v_scale<D, VB>(4 * grp, col * PV::BLOCKS / 16);
+  const uint32_t koff = (4 * col + grp) * (PK::PIECE < 16 ? PK::PIECE : 16);
+  const uint32_t voff = lane * (PV::PIECE < 16 ? PV::PIECE : 16);
+  const uint32_t ksoff = k_scale<D, KB>(col, grp * PK::BLOCKS / 4);
+  const uint32_t vsoff = v_scale<D, VB>(4 * grp, col * PV::BLOCKS / 16);
   const int32_t* pt = page_table + (size_t)ch.b * max_pages;
 
   float m = -INFINITY, l = 0.f;
@@ -267,26 +374,30 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
 #pragma unroll
   for (int db = 0; db < DB; ++db) acc[db] = f32x4{};
 
-  int ids = 0;   // lane i: page w0 + 64 j + i of the sequence
-  for (int w = w0; w < w1; w += kBatch) {
+  // Loads of the batch of pages w .. + kBatch - 1. Past the wave's last page they
+  // repeat it (masked below): without a branch the compiler keeps every load
+  // in flight over the batch before.
+  int ids = 0;   // lane i: id of the wave's page 64 j + i
+  const auto load = [&](Batch<D, KB, VB>& x, int w) {
     if (((w - w0) & 63) == 0) {
-      ids = w + lane < w1 ? pt[w + lane] : 0;
+      ids = pt[min(w + lane, w1 - 1)];
       const bool no = ids < 0 || ids >= num_pages;
       bad |= no;
       ids = no ? 0 : ids;   // read in place of a page that is not there; the result is NaN
     }
-    Batch<D, KB, VB> x;
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {   // past w1: page 0, masked below
+    for (int i = 0; i < kBatch; ++i) {
       const int pid = __builtin_amdgcn_readlane(ids, (w - w0 + i) & 63);
       const size_t rec = (size_t)pid * Hkv + hk;
       const char* kp = k_pool + rec * PK::BYTES;
       const char* vp = v_pool + rec * PV::BYTES;
-      load_piece(kp + koff, x.k[i]);
+      load_piece<NT>(kp + koff, x.k[i]);
       x.ks[i] = (uint8_t)kp[ksoff];
-      load_piece(vp + voff, x.v[i]);
+      load_piece<NT>(vp + voff, x.v[i]);
       x.vs[i] = *reinterpret_cast<const uint32_t*>(vp + vsoff);
     }
+  };
+  const auto attend = [&](Batch<D, KB, VB>& x, int w) {
     // Tokens of the batch that the wave has; from the lane's first.
     const int rem = min(ctx, w1 * kTokens) - w * kTokens, lim = rem - 4 * grp;
     const bool tail = rem < kBatch * kTokens;   // wave-uniform
@@ -306,10 +417,15 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
       });
     }
     if (tail) {
+      // Rows past the context may hold NaN, and 0 NaN is NaN: V's become zeros.
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i)
+      for (int i = 0; i < kBatch; ++i) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) s[i][r] = kTokens * i + r < lim ? s[i][r] : -INFINITY;
+        const int n = min(max(lim - kTokens * i, 0), 4);   // of the lane's four tokens
+        x.vs[i] &= (uint32_t)((1ull << (8 * n)) - 1);
+        keep_tokens<PV::WORDS>(x.v[i], n);
+      }
     }
     float top = s[0][0];
 #pragma unroll
@@ -359,8 +475,6 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
           static_for<0, 4>([&](auto r) {
             const uint32_t e = (x.vs[I] >> (8 * r.value)) & 0xffu;
             v[r.value] = v_pair<D, VB, BF16, r.value, qd.value>(x.v[I], scale_of(e));
-            // Rows past the context may hold NaN, and 0 NaN is NaN.
-            if (tail) v[r.value] = kTokens * I + r.value < lim ? v[r.value] : 0u;
           });
           even[2 * j.value] = __builtin_amdgcn_perm(v[1], v[0], 0x05040100u);
           even[2 * j.value + 1] = __builtin_amdgcn_perm(v[3], v[2], 0x05040100u);
@@ -376,6 +490,18 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
         }
       });
     });
+  };
+  if (w0 < w1) {
+    Batch<D, KB, VB> x, y;
+    load(x, w0);
+    for (int w = w0;;) {   // two batches a round: no copies between them
+      load(y, min(w + kBatch, w1 - 1));
+      attend(x, w);
+      if ((w += kBatch) >= w1) break;
+      load(x, min(w + kBatch, w1 - 1));
+      attend(y, w);
+      if ((w += kBatch) >= w1) break;
+    }
   }
   l = col_sum(l);
 
@@ -392,11 +518,11 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
     }
   }
   __syncthreads();
-  if (plan != nullptr && blockIdx.y == 0 && tid == 0) {   // for the pass that joins the chunks
-    if (blockIdx.x == 0) plan[0] = ch.cuts;
+  if (plan != nullptr && hg == 0 && tid == 0) {   // for the pass that joins
+    if (x == 0) plan[0] = ch.cuts;
     if (ch.splits > 1 && ch.split == 0) {
-      plan[1 + 2 * ch.cut] = ch.b;
-      plan[2 + 2 * ch.cut] = ch.partial | ch.splits << 16;
+      plan[1 + 2 * ch.index] = ch.b;
+      plan[2 + 2 * ch.index] = ch.partial | ch.splits << 16;
     }
   }
   for (int i = tid; i < G * D; i += kThreads) {
@@ -421,73 +547,103 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
       o[row * D + d] = (uint16_t)bits;
       if (lse != nullptr && d == 0) lse[row] = L * kLn2;
     } else {
-      const size_t row = (size_t)(ch.partial + ch.split) * H + h0 + g;
+      const size_t row = (size_t)(h0 + g) * slots + ch.partial + ch.split;
       part_o[row * D + d] = out;
       if (d == 0) part_l[row] = L;
     }
   }
 }
 
-// Joins the chunks of cut sequence blockIdx.x: a workgroup per row (sequence,
-// head), D / 4 threads for four values each, the chunks dealt out over
-// kThreads / (D / 4) groups of them.
-template <int D, bool BF16>
-__global__ void __launch_bounds__(kThreads)
+// Joins the chunks of cut sequence blockIdx.x, head blockIdx.y: a wave has 32
+// columns of the row (WAVES = 1) or kWaves waves share them, eight lanes for
+// four columns each in as many groups as there are, the chunks dealt out over
+// the groups. One pass, with a running maximum.
+template <int D, bool BF16, int WAVES>
+__global__ void __launch_bounds__(WAVES == 1 ? 2 * D : kThreads)
 fa_decode_mx_join_kernel(const float* __restrict__ part_o, const float* __restrict__ part_l,
                          const int32_t* __restrict__ plan, uint16_t* __restrict__ o,
-                         float* __restrict__ lse, int H) {
-  constexpr int PER = D / 4, GROUPS = kThreads / PER;
-  __shared__ float sh_m[kWaves], sh_z[GROUPS];
-  __shared__ __attribute__((aligned(16))) float sh_o[GROUPS][D];
-  if ((int)blockIdx.x >= plan[0]) return;
-  const int b = plan[1 + 2 * blockIdx.x], word = plan[2 + 2 * blockIdx.x];
+                         float* __restrict__ lse, int H, int slots) {
+  constexpr int GROUPS = 8 * WAVES, AHEAD = 4;
+  __shared__ __attribute__((aligned(16))) f32x4 sh_a[kWaves][8];
+  __shared__ float sh_m[kWaves], sh_z[kWaves];
+  const int cuts = plan[0], b = plan[1 + 2 * blockIdx.x], word = plan[2 + 2 * blockIdx.x];
+  if ((int)blockIdx.x >= cuts) return;
   const int first = word & 0xffff, n = word >> 16;
-  const int h = blockIdx.y, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  const float* pl = part_l + (size_t)first * H + h;
-  const float* po = part_o + ((size_t)first * H + h) * D;
+  const int h = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int d = 32 * (WAVES == 1 ? wave : (int)blockIdx.z) + 4 * (lane & 7);
+  const int g = WAVES == 1 ? lane >> 3 : 8 * wave + (lane >> 3);
+  const float* pl = part_l + (size_t)h * slots + first;
+  const float* po = part_o + ((size_t)h * slots + first) * D + d;
 
-  float M = -INFINITY;
-  bool nan = false;
-  for (int i = tid; i < n; i += kThreads) {
-    const float x = pl[(size_t)i * H];
-    nan |= x != x;
-    M = fmaxf(M, x);
-  }
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) M = fmaxf(M, __shfl_xor(M, d));
-  if (lane == 0) sh_m[wave] = M;
-  nan = __syncthreads_or(nan);
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) M = fmaxf(M, sh_m[w]);
-
-  const int g = tid / PER, d = 4 * (tid % PER);
+  float m = -INFINITY, z = 0.f;
   f32x4 a = f32x4{};
-  float z = 0.f;
-  for (int i = g; i < n; i += GROUPS) {   // a chunk of a cut sequence has tokens: its L is finite or NaN
-    const float e = exp2_hw(pl[(size_t)i * H] - M);
-    const f32x4 x = *reinterpret_cast<const f32x4*>(po + (size_t)i * H * D + d);
-    z += e;
+  for (int i = g; i < n; i += AHEAD * GROUPS) {
+    float x[AHEAD];
+    f32x4 v[AHEAD];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) a[j] = fmaf(e, x[j], a[j]);
+    for (int j = 0; j < AHEAD; ++j) {
+      const int k = min(i + j * GROUPS, n - 1);
+      x[j] = i + j * GROUPS < n ? pl[k] : -INFINITY;
+      v[j] = *reinterpret_cast<const f32x4*>(po + (size_t)k * D);
+    }
+    float top = m;   // finite or, with a NaN to come, -inf: a chunk of a cut sequence has tokens
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) top = fmaxf(top, x[j]);
+    const float e = exp2_hw(m - top);
+    z *= e;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) a[c] *= e;
+    m = top;
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const float w = exp2_hw(x[j] - m);
+      z += w;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) a[c] = fmaf(w, v[j][c], a[c]);
+    }
   }
-  *reinterpret_cast<f32x4*>(&sh_o[g][d]) = a;
-  if (d == 0) sh_z[g] = z;
-  __syncthreads();
-  if (g != 0) return;
-  a = f32x4{};
-  z = 0.f;
+  // The groups of the wave, then the waves.
+  float M = m;
 #pragma unroll
-  for (int i = 0; i < GROUPS; ++i) {
-    const f32x4 x = *reinterpret_cast<const f32x4*>(&sh_o[i][d]);
+  for (int k = 8; k < 64; k *= 2) M = fmaxf(M, __shfl_xor(M, k));
+  const float e = m == M ? 1.f : exp2_hw(m - M);   // a group without chunks: m = -inf, its sums 0
+  z *= e;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) a[j] += x[j];
-    z += sh_z[i];
+  for (int c = 0; c < 4; ++c) a[c] *= e;
+#pragma unroll
+  for (int k = 8; k < 64; k *= 2) {
+    z += __shfl_xor(z, k);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) a[c] += __shfl_xor(a[c], k);
   }
+  if constexpr (WAVES > 1) {
+    if (lane < 8) sh_a[wave][lane] = a;
+    if (lane == 0) {
+      sh_m[wave] = M;
+      sh_z[wave] = z;
+    }
+    __syncthreads();
+    if (wave != 0) return;
+    M = sh_m[0];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) M = fmaxf(M, sh_m[w]);
+    z = 0.f;
+    a = f32x4{};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float f = sh_m[w] == M ? 1.f : exp2_hw(sh_m[w] - M);
+      const f32x4 v = sh_a[w][lane & 7];
+      z = fmaf(f, sh_z[w], z);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) a[c] = fmaf(f, v[c], a[c]);
+    }
+  }
+  if (lane >= 8) return;
   const size_t row = (size_t)b * H + h;
-  const float inv = nan ? NAN : 1.f / z;
+  const float inv = 1.f / z;
   *reinterpret_cast<u32x2*>(o + row * D + d) =
       u32x2{pack2<BF16>(a[0] * inv, a[1] * inv), pack2<BF16>(a[2] * inv, a[3] * inv)};
-  if (lse != nullptr && d == 0) lse[row] = nan ? NAN : (M + log2_hw(z)) * kLn2;
+  if (lse != nullptr && d == 0) lse[row] = (M + log2_hw(z)) * kLn2;
 }
 
 template <int D, int KB, int VB, bool BF16>
@@ -495,24 +651,34 @@ static int decode(const void* q, const void* k_pool, const void* v_pool, const i
                   const int32_t* ctx_lens, int64_t B, int64_t H, int64_t Hkv, int64_t max_pages,
                   int64_t num_pages, float* workspace, void* o, float* lse, hipStream_t s) {
   const float c = (float)(1.0 / sqrt((double)D)) * kLog2e;
-  const int64_t target = target_chunks(H, Hkv);
+  const int64_t most = most_chunks(B, H, Hkv, max_pages);
   // No sequence of up to kMinChunk pages is cut.
   const bool one = max_pages <= kMinChunk;
-  const int64_t rows = partial_chunks(B, H, Hkv) * H;
+  const int64_t slots = partial_chunks(B, most), rows = slots * H;
   float* part_o = workspace;
   float* part_l = workspace + rows * D;
   int32_t* plan = one ? nullptr : reinterpret_cast<int32_t*>(part_l + rows);
-  const dim3 grid((unsigned)(one ? B : target + B), (unsigned)head_groups(H, Hkv));
-  hipLaunchKernelGGL((fa_decode_mx_kernel<D, KB, VB, BF16>), grid, dim3(kThreads), 0, s,
-                     (const uint16_t*)q, (const char*)k_pool, (const char*)v_pool, page_table,
-                     ctx_lens, part_o, part_l, plan, (uint16_t*)o, lse, (int)B, (int)H, (int)Hkv,
-                     (int)max_pages, (int)num_pages, (int)target, c);
+  const dim3 grid((unsigned)(kXcds * head_groups(H, Hkv)),
+                  (unsigned)(((one ? B : most + B) + kXcds - 1) / kXcds));
+  const bool nt = num_pages * Hkv * (Page<D, KB>::BYTES + Page<D, VB>::BYTES) >= kPassThrough;
+  const auto kernel = nt ? fa_decode_mx_kernel<D, KB, VB, BF16, true>
+                         : fa_decode_mx_kernel<D, KB, VB, BF16, false>;
+  hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, s, (const uint16_t*)q, (const char*)k_pool,
+                     (const char*)v_pool, page_table, ctx_lens, part_o, part_l, plan, (uint16_t*)o,
+                     lse, (int)B, (int)H, (int)Hkv, (int)(H / Hkv), (int)(head_groups(H, Hkv) / Hkv),
+                     (int)max_pages, (int)num_pages, (int)slots, plan_of(B, H, Hkv), c);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return -(int)e;
   if (one) return FA_OK;
-  const dim3 rest((unsigned)(B < target ? B : target), (unsigned)H);
-  hipLaunchKernelGGL((fa_decode_mx_join_kernel<D, BF16>), rest, dim3(kThreads), 0, s, part_o, part_l,
-                     plan, (uint16_t*)o, lse, (int)H);
+  // Few rows: a workgroup for each 32 columns; else one a row.
+  const unsigned cut = (unsigned)(B < most ? B : most);
+  if (B * H * (D / 32) <= kWideJoin)
+    hipLaunchKernelGGL((fa_decode_mx_join_kernel<D, BF16, kWaves>), dim3(cut, (unsigned)H, D / 32),
+                       dim3(kThreads), 0, s, part_o, part_l, plan, (uint16_t*)o, lse, (int)H,
+                       (int)slots);
+  else
+    hipLaunchKernelGGL((fa_decode_mx_join_kernel<D, BF16, 1>), dim3(cut, (unsigned)H), dim3(2 * D), 0,
+                       s, part_o, part_l, plan, (uint16_t*)o, lse, (int)H, (int)slots);
   e = hipGetLastError();
   return e == hipSuccess ? FA_OK : -(int)e;
 }
@@ -520,10 +686,14 @@ static int decode(const void* q, const void* k_pool, const void* v_pool, const i
 }  // namespace mx
 }  // namespace fa
 
-extern "C" int64_t fa_decode_mx_workspace_floats(int64_t B, int64_t H, int64_t H_kv, int64_t D) {
-  if (B <= 0 || H <= 0 || H_kv <= 0 || H % H_kv != 0 || D <= 0) return 0;
-  const int64_t cut = fa::mx::target_chunks(H, H_kv);   // sequences that are cut, at most
-  return fa::mx::partial_chunks(B, H, H_kv) * H * (D + 1) + 1 + 2 * (B < cut ? B : cut);
+extern "C" int64_t fa_decode_mx_workspace_floats(int64_t B, int64_t H, int64_t H_kv, int64_t D,
+                                                 int64_t max_pages) {
+  if (B <= 0 || H <= 0 || H_kv <= 0 || H % H_kv != 0 || D <= 0 || max_pages <= 0 ||
+      B > ((int64_t(1) << 31) - 1) / max_pages)
+    return 0;
+  if (max_pages <= fa::mx::kMinChunk) return 1;   // not used
+  const int64_t most = fa::mx::most_chunks(B, H, H_kv, max_pages);
+  return fa::mx::partial_chunks(B, most) * H * (D + 1) + 1 + 2 * (B < most ? B : most);
 }
 
 extern "C" int fa_decode_paged_mx(const void* q, const void* k_pool, const void* v_pool,
@@ -541,4 +711,13 @@ extern "C" int fa_decode_paged_mx(const void* q, const void* k_pool, const void*
                                         max_pages, num_pages, workspace, o, lse, s)
   FA_MX_DISPATCH(D, k_bits, v_bits, bf16, FA_MX_DECODE)
 #undef FA_MX_DECODE
+}
+
+extern "C" int fa_probe_mx_chunks(int64_t B, int64_t H, int64_t H_kv, int64_t max_pages, int64_t total,
+                                  int64_t* most) {
+  if (B <= 0 || H <= 0 || H_kv <= 0 || H % H_kv != 0 || max_pages <= 0 || total < 0 ||
+      B > ((int64_t(1) << 31) - 1) / max_pages || total > B * max_pages)
+    return 0;
+  if (most != nullptr) *most = fa::mx::most_chunks(B, H, H_kv, max_pages);
+  return fa::mx::chunk_pages((int)total, fa::mx::plan_of(B, H, H_kv));
 }

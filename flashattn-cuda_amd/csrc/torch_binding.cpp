@@ -655,7 +655,7 @@ std::vector<torch::Tensor> decode_paged_mx(torch::Tensor q, torch::Tensor k_pool
               "decode tensors must be on the same device");
   const c10::DeviceGuard guard(dev);
   const auto f32 = q.options().dtype(torch::kFloat);
-  auto ws = torch::empty({fa_decode_mx_workspace_floats(B, H, m.Hkv, D)}, f32);
+  auto ws = torch::empty({fa_decode_mx_workspace_floats(B, H, m.Hkv, D, page_table.size(1))}, f32);
   auto o = torch::empty({B, H, D}, q.options());
   auto lse = torch::empty({B, H}, f32);
   const int st = fa_decode_paged_mx(

@@ -485,7 +485,8 @@ int fa_validate_decode_mx(const void* q, const void* k_pool, const void* v_pool,
                           const float* workspace, const void* o, const float* lse);
 
 /* Floats of the workspace fa_decode_paged_mx needs (0 for invalid sizes). */
-int64_t fa_decode_mx_workspace_floats(int64_t B, int64_t H, int64_t H_kv, int64_t D);
+int64_t fa_decode_mx_workspace_floats(int64_t B, int64_t H, int64_t H_kv, int64_t D,
+                                      int64_t max_pages);
 
 /*
  * The paged decode over MX pages: q, o fp16 (bf16 != 0: bfloat16) [B, H, D],

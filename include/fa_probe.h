@@ -15,14 +15,14 @@
  * compute-unit count, without a device); 4 added fa_probe_gather_bw; 5 added
  * fa_probe_unit_of and variant 432; 6 added fa_probe_decode_ordered and
  * fa_probe_bwd_block_rows, lists variant 432, and fa_probe_frags dumps the
- * backward's fragments.
+ * backward's fragments; 7 added fa_probe_mx_chunks.
  */
 #ifndef FA_PROBE_H
 #define FA_PROBE_H
 
 #include <stdint.h>
 
-#define FA_PROBE_VERSION 6
+#define FA_PROBE_VERSION 7
 
 #ifdef __cplusplus
 extern "C" {
@@ -96,6 +96,12 @@ int fa_probe_unit_of(int64_t heads, int64_t per_head, int nxcd, int cus, int une
  * once run in index order), else 0. No device needed. */
 int fa_probe_decode_ordered(int64_t B, int64_t H, int64_t H_kv, int64_t D, int64_t num_splits,
                             int cus);
+
+/* Pages of a chunk of fa_decode_paged_mx where the batch's contexts have `total`
+ * pages, and in *most (may be NULL) the chunks its grid holds besides one a
+ * sequence; 0 for a bad argument. No device needed. */
+int fa_probe_mx_chunks(int64_t B, int64_t H, int64_t H_kv, int64_t max_pages, int64_t total,
+                       int64_t* most);
 
 /* Rows that a workgroup of the backward owns (128 or 64) for bh = B*H heads of
  * N rows on a device of `cus` compute units; 0 for a bad argument. No device

@@ -1,5 +1,7 @@
 """CPU tier of the MX KV cache: the oracle against the definition, the C ABI's
 argument checks, and the refusals of the Python entry points."""
+import ctypes as C
+
 import numpy as np
 import pytest
 import torch
@@ -131,11 +133,12 @@ def test_sizes_and_strings(capi):
     assert [lib.fa_mx_page_bytes(D, b) for D in (64, 128) for b in (4, 8)] == [544, 1056, 1088, 2112]
     assert lib.fa_mx_page_bytes(96, 4) == lib.fa_mx_page_bytes(128, 2) == 0
     assert lib.fa_status_str(capi.STATUS["FA_ERR_MX_BITS"]) == b"k_bits and v_bits must be 4 or 8"
-    assert lib.fa_decode_mx_workspace_floats(4, 32, 8, 128) > 0
-    assert lib.fa_decode_mx_workspace_floats(4, 32, 5, 128) == 0
+    assert lib.fa_decode_mx_workspace_floats(4, 32, 8, 128, 100) > 0
+    assert lib.fa_decode_mx_workspace_floats(4, 32, 5, 128, 100) == 0
+    assert lib.fa_decode_mx_workspace_floats(4, 32, 8, 128, 0) == 0
     # the workspace does not grow with a batch that fills the chip by itself
-    assert (lib.fa_decode_mx_workspace_floats(60000, 32, 8, 128) ==
-            lib.fa_decode_mx_workspace_floats(5000, 32, 8, 128) <= 1 << 24)
+    assert (lib.fa_decode_mx_workspace_floats(10000, 32, 8, 128, 2000) ==
+            lib.fa_decode_mx_workspace_floats(5000, 32, 8, 128, 2000) <= 1 << 24)
 
 
 def test_refusals_of_host_tensors(fa):
@@ -155,3 +158,29 @@ def test_refusals_of_host_tensors(fa):
         fa.kv_pools_mx(4, 2, 64, 4, 16, device="cpu")
     with pytest.raises(RuntimeError, match="dtype must be"):
         fa.kv_read_mx(kp, vp, i32[None], i32, 3, dtype=torch.float32)
+
+
+def test_chunk_plan_fits_its_grid(capi):
+    """The grid and the workspace are sized from B * max_pages; whatever the lengths (any total up to
+    that), the chunks that the device cuts fit them: at most `most` and one a sequence, of cut
+    sequences at most `most` and half a one a sequence."""
+    import random
+    lib = capi.load()
+    r = random.Random(3)
+    most = C.c_int64()
+    for _ in range(3000):
+        B = r.choice([1, 2, 3, 8, 60, 64, 65, 200, 256, 300, 1000])
+        Hkv = r.choice([1, 2, 4, 8, 32, 128])
+        H = Hkv * r.choice([1, 4, 20, 64])
+        maxp = int(2 ** r.uniform(0, 14))
+        lens = [min(maxp, int(2 ** r.uniform(0, 14)) - 1) for _ in range(B)]
+        Cp = lib.fa_probe_mx_chunks(B, H, Hkv, maxp, sum(lens), C.byref(most))
+        assert Cp >= 16
+        cut = [(2 * p + Cp) // (2 * Cp) for p in lens]
+        assert sum(max(1, n) for n in cut) <= most.value + B
+        cuts = [n for n in cut if n > 1]
+        assert sum(cuts) <= most.value + min(B, most.value) < 1 << 16 and len(cuts) <= min(B, most.value)
+        assert lib.fa_decode_mx_workspace_floats(B, H, Hkv, 64, maxp) >= 1
+        if maxp <= 16:
+            assert not cuts   # no second pass is launched
+    assert lib.fa_probe_mx_chunks(1, 4, 3, 10, 5, None) == lib.fa_probe_mx_chunks(1, 4, 4, 10, 11, None) == 0

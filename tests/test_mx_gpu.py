@@ -223,6 +223,8 @@ def test_decode_matches_oracle(fa, dev, H, Hkv, ctx, D, kb, vb, bf16):
     (64, 8, 8, False, 16, 4, [12000, 1, 0, 33]),  # one long sequence among short ones
     (128, 8, 4, True, 8, 8, [4097, 4095, 16]),
     (64, 4, 4, True, 4, 1, [20000]),
+    (64, 4, 4, False, 1, 1, [10350]),             # 647 pages in 40 chunks
+    (128, 4, 8, False, 2, 1, [10300, 10000, 9990, 400]),
 ])
 def test_decode_long_and_grouped(fa, dev, D, kb, vb, bf16, H, Hkv, ctx):
     _decode(fa, dev, _decode_case(len(ctx) + H, ctx, H, Hkv, D, kb, vb, bf16), kb, vb, bf16, "long")
