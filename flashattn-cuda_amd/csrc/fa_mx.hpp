@@ -83,6 +83,13 @@ __device__ __forceinline__ int v_scale(int t, int block) {
 // 2^(s - 127), or what the conversions take for NaN.
 __device__ __forceinline__ float scale_of(uint32_t s) { return __uint_as_float(s << 23); }
 
+// The scale in byte R of a word, the other bytes in its sign and fraction,
+// which the conversions from codes do not look at (checked over every scale).
+template <int R>
+__device__ __forceinline__ float scale_at(uint32_t w) {
+  return __uint_as_float(R == 3 ? w >> 1 : w << (23 - 8 * R));
+}
+
 // Values 2 I and 2 I + 1 of a word of codes (I < 4 at 4 bits, < 2 at 8), as
 // raw 16-bit pairs. Exact in both types, but for bf16 values below 2^-126.
 template <int BITS, bool BF16, int I>

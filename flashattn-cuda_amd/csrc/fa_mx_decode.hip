@@ -30,21 +30,27 @@ namespace mx {
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kXcds = 8;
-constexpr int kBatch = 2;   // pages that a wave takes at a time
 
-// Chunks. The pages of all sequences, T in all, are cut into runs of C pages
-// (and a shorter one at a sequence's end): workgroups of like size
-// whatever the lengths, from lengths that only the device knows. The grid has
-// the most chunks that any lengths can give, and the rest end at once.
+// Pages that a wave takes at a time: their loads are in flight together. Four
+// of up to 32 code bytes a lane (K and V), two of larger ones, whose registers
+// would leave three waves a SIMD and not four (K8V4 at D = 128 bf16, 24
+// sequences: 57.3 us with two, 57.9 with four; 4 bits, one sequence of 131072
+// tokens over one KV head: 14.7 and 13.9).
+template <int D, int KB, int VB>
+constexpr int kBatchOf = Page<D, KB>::PIECE + Page<D, VB>::PIECE <= 32 ? 4 : 2;
+
+// Chunks. The pages of all sequences, T in all, are cut into runs of about C
+// pages, a sequence into equal ones: workgroups of like size whatever the
+// lengths, from lengths that only the device knows. The grid has the most
+// chunks that any lengths can give, and the rest end at once.
 //
 // C, for the batch's T pages (chunks are counted along the pages; a chunk is a
 // workgroup for every head group):
 //   kMinChunk pages while they make fewer than kFill workgroups,
 //   then what makes kFill of them, up to kMaxChunk pages,
 //   then kMaxChunk pages, until they make kMost workgroups.
-// kFill is four workgroups a CU (three of these are resident at a time); the
-// chunks past kMaxChunk pages buy balance at little cost. Besides, at most
-// kRowFill chunks a sequence (one of 131072 tokens over one KV head: 20.7 us in
+// kFill is the four workgroups that a CU holds; chunks past kMaxChunk pages are
+// cut for balance, at little cost. Besides, at most kRowFill chunks a sequence (one of 131072 tokens over one KV head: 20.7 us in
 // 512 chunks, 16.0 in 256, 17.9 in 128), and where there are about as many
 // sequences as chunks wanted, only those of twice the mean length are cut (256
 // of 100 to 900 tokens over 4 KV heads: 20 -> 15.4 us).
@@ -257,21 +263,17 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 }
 
 // A lane's piece of a page.
-template <bool NT, typename T>
-__device__ __forceinline__ T load_as(const char* p) {
-  if constexpr (NT) return __builtin_nontemporal_load(reinterpret_cast<const T*>(p));
-  return *reinterpret_cast<const T*>(p);
-}
 template <bool NT, int WORDS>
-__device__ __forceinline__ void load_piece(const char* p, uint32_t (&w)[WORDS]) {
+__device__ __forceinline__ void load_piece(__amdgpu_buffer_rsrc_t r, uint32_t off, uint32_t (&w)[WORDS]) {
+  constexpr int kAux = NT ? 2 : 0;
   if constexpr (WORDS == 2) {
-    const u32x2 x = load_as<NT, u32x2>(p);
+    const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, kAux);
     w[0] = x[0];
     w[1] = x[1];
   } else {
 #pragma unroll
     for (int j = 0; j < WORDS / 4; ++j) {
-      const u32x4 x = load_as<NT, u32x4>(p + 1024 * j);
+      const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(r, off, 1024 * j, kAux);
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[4 * j + i] = x[i];
     }
@@ -293,6 +295,7 @@ __device__ __forceinline__ void keep_tokens(uint32_t (&w)[WORDS], int n) {
 // What a wave holds of a batch of pages before it is multiplied.
 template <int D, int KB, int VB>
 struct Batch {
+  static constexpr int kBatch = kBatchOf<D, KB, VB>;
   uint32_t k[kBatch][Page<D, KB>::WORDS];
   uint32_t v[kBatch][Page<D, VB>::WORDS];
   uint32_t ks[kBatch], vs[kBatch];
@@ -317,6 +320,7 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
                     int group, int ngrp, int max_pages, int num_pages, int slots, Plan chunk_plan, float c) {
   using PK = Page<D, KB>;
   using PV = Page<D, VB>;
+  constexpr int kBatch = kBatchOf<D, KB, VB>;
   constexpr int KS = D / 32;   // steps of S = K Q^T
   constexpr int DB = D / 16;   // blocks of O^T
   // P reaches 2^15 in fp16 rather than 1, so that it keeps all its bits down to
@@ -330,7 +334,7 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
   // Workgroups go to the XCDs in turn: an XCD has every eighth chunk, and the
   // head groups of a chunk one after the other, so that what is read of a page
   // at about the same time by one L2 is contiguous.
-  const int x = blockIdx.y * kXcds + blockIdx.x % kXcds, hg = blockIdx.x / kXcds;
+  const int number = blockIdx.y * kXcds + blockIdx.x % kXcds, hg = blockIdx.x / kXcds;
   const int hk = ngrp == 1 ? hg : hg / ngrp, sub = ngrp == 1 ? 0 : hg % ngrp;
   const int h0 = hk * group + 16 * sub;   // first query head of this workgroup
   const int G = min(16, group - 16 * sub);
@@ -339,7 +343,7 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
   const int col = lane & 15, grp = lane >> 4;
 
   if (tid == 0) sh_bad = 0;
-  Chunk ch = chunk_of(ctx_lens, B, max_pages, chunk_plan, x, sh_i);
+  Chunk ch = chunk_of(ctx_lens, B, max_pages, chunk_plan, number, sh_i);
   ch.b = __builtin_amdgcn_readfirstlane(ch.b);
   if (ch.b < 0) return;
   const int ctx = __builtin_amdgcn_readfirstlane(ch.ctx);
@@ -374,11 +378,15 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
 #pragma unroll
   for (int db = 0; db < DB; ++db) acc[db] = f32x4{};
 
-  // Loads of the batch of pages w .. + kBatch - 1. Past the wave's last page they
-  // repeat it (masked below): without a branch the compiler keeps every load
-  // in flight over the batch before.
+  // Pages w .. + kBatch - 1, all loads at once; past the wave's last page they
+  // repeat it (masked below). Four waves a SIMD hide each other's waits: a
+  // second set of registers, loaded one batch ahead, leaves three and measured
+  // slower (32 sequences of up to 32768 tokens 401 us, 384 without; one of
+  // 32000 14.4 and 13.2), and so did loading K and V each as soon as their
+  // registers are free (409 and 14.2).
   int ids = 0;   // lane i: id of the wave's page 64 j + i
-  const auto load = [&](Batch<D, KB, VB>& x, int w) {
+  Batch<D, KB, VB> x;
+  const auto load = [&](int w) {
     if (((w - w0) & 63) == 0) {
       ids = pt[min(w + lane, w1 - 1)];
       const bool no = ids < 0 || ids >= num_pages;
@@ -387,17 +395,17 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
     }
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-      const int pid = __builtin_amdgcn_readlane(ids, (w - w0 + i) & 63);
-      const size_t rec = (size_t)pid * Hkv + hk;
-      const char* kp = k_pool + rec * PK::BYTES;
-      const char* vp = v_pool + rec * PV::BYTES;
-      load_piece<NT>(kp + koff, x.k[i]);
-      x.ks[i] = (uint8_t)kp[ksoff];
-      load_piece<NT>(vp + voff, x.v[i]);
-      x.vs[i] = *reinterpret_cast<const uint32_t*>(vp + vsoff);
+      const size_t rec = (size_t)__builtin_amdgcn_readlane(ids, (w - w0 + i) & 63) * Hkv + hk;
+      const auto r = make_rsrc(k_pool + rec * PK::BYTES, PK::BYTES);
+      load_piece<NT>(r, koff, x.k[i]);
+      x.ks[i] = __builtin_amdgcn_raw_buffer_load_b8(r, ksoff, 0, 0);
+      const auto t = make_rsrc(v_pool + rec * PV::BYTES, PV::BYTES);
+      load_piece<NT>(t, voff, x.v[i]);
+      x.vs[i] = __builtin_amdgcn_raw_buffer_load_b32(t, vsoff, 0, 0);
     }
   };
-  const auto attend = [&](Batch<D, KB, VB>& x, int w) {
+  for (int w = w0; w < w1; w += kBatch) {
+    load(w);
     // Tokens of the batch that the wave has; from the lane's first.
     const int rem = min(ctx, w1 * kTokens) - w * kTokens, lim = rem - 4 * grp;
     const bool tail = rem < kBatch * kTokens;   // wave-uniform
@@ -417,6 +425,7 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
       });
     }
     if (tail) {
+      asm volatile("");   // a branch: not selects in every batch
       // Rows past the context may hold NaN, and 0 NaN is NaN: V's become zeros.
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
@@ -473,8 +482,7 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
           constexpr int I = I0 + j.value;
           uint32_t v[4];
           static_for<0, 4>([&](auto r) {
-            const uint32_t e = (x.vs[I] >> (8 * r.value)) & 0xffu;
-            v[r.value] = v_pair<D, VB, BF16, r.value, qd.value>(x.v[I], scale_of(e));
+            v[r.value] = v_pair<D, VB, BF16, r.value, qd.value>(x.v[I], scale_at<r.value>(x.vs[I]));
           });
           even[2 * j.value] = __builtin_amdgcn_perm(v[1], v[0], 0x05040100u);
           even[2 * j.value + 1] = __builtin_amdgcn_perm(v[3], v[2], 0x05040100u);
@@ -490,18 +498,6 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
         }
       });
     });
-  };
-  if (w0 < w1) {
-    Batch<D, KB, VB> x, y;
-    load(x, w0);
-    for (int w = w0;;) {   // two batches a round: no copies between them
-      load(y, min(w + kBatch, w1 - 1));
-      attend(x, w);
-      if ((w += kBatch) >= w1) break;
-      load(x, min(w + kBatch, w1 - 1));
-      attend(y, w);
-      if ((w += kBatch) >= w1) break;
-    }
   }
   l = col_sum(l);
 
@@ -519,36 +515,47 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
   }
   __syncthreads();
   if (plan != nullptr && hg == 0 && tid == 0) {   // for the pass that joins
-    if (x == 0) plan[0] = ch.cuts;
+    if (number == 0) plan[0] = ch.cuts;
     if (ch.splits > 1 && ch.split == 0) {
       plan[1 + 2 * ch.index] = ch.b;
       plan[2 + 2 * ch.index] = ch.partial | ch.splits << 16;
     }
   }
-  for (int i = tid; i < G * D; i += kThreads) {
-    const int g = i / D, d = i % D;
-    float M = sh_m[0][g];
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) M = fmaxf(M, sh_m[w][g]);
-    float a = 0.f, z = 0.f;
+  // A thread has four columns of a head.
+  for (int i = tid; i < G * (D / 4); i += kThreads) {
+    const int g = i / (D / 4), d = 4 * (i % (D / 4));
+    float wm[kWaves], wl[kWaves];
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-      // A wave without pages has m = -inf; its sum is 0.
-      const float e = sh_l[w][g] == 0.f ? 0.f : exp2_hw(sh_m[w][g] - M);
-      a = fmaf(e, sh_o[w][g][d], a);
-      z = fmaf(e, sh_l[w][g], z);
+      wm[w] = sh_m[w][g];
+      wl[w] = sh_l[w][g];
     }
-    float out = z == 0.f ? 0.f : a / z;
+    float M = wm[0];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) M = fmaxf(M, wm[w]);
+    f32x4 a = f32x4{};
+    float z = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      // A wave without pages has m = -inf; its sums are 0.
+      const float e = wl[w] == 0.f ? 0.f : exp2_hw(wm[w] - M);
+      const f32x4 v = *reinterpret_cast<const f32x4*>(&sh_o[w][g][d]);
+      z = fmaf(e, wl[w], z);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) a[j] = fmaf(e, v[j], a[j]);
+    }
+    float inv = z == 0.f ? 0.f : 1.f / z;
     float L = z == 0.f ? -INFINITY : M - kShift + log2_hw(z);   // in units of log 2
-    if (sh_bad) out = L = NAN;
+    if (sh_bad) inv = L = NAN;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) a[j] *= inv;
     if (ch.splits == 1) {
       const size_t row = (size_t)ch.b * H + h0 + g;
-      const uint32_t bits = pack2<BF16>(out, 0.f);
-      o[row * D + d] = (uint16_t)bits;
+      *reinterpret_cast<u32x2*>(o + row * D + d) = u32x2{pack2<BF16>(a[0], a[1]), pack2<BF16>(a[2], a[3])};
       if (lse != nullptr && d == 0) lse[row] = L * kLn2;
     } else {
       const size_t row = (size_t)(h0 + g) * slots + ch.partial + ch.split;
-      part_o[row * D + d] = out;
+      *reinterpret_cast<f32x4*>(part_o + row * D + d) = a;
       if (d == 0) part_l[row] = L;
     }
   }
