@@ -224,7 +224,8 @@ extern "C" int fa_validate_decode_mx(const void* q, const void* k_pool, const vo
   if (st != FA_OK) return st;
   if (H_kv <= 0 || H % H_kv != 0) return FA_ERR_KV_HEADS;
   if (fa_mx_page_bytes(D, k_bits) == 0 || fa_mx_page_bytes(D, v_bits) == 0) return FA_ERR_MX_BITS;
-  if (!workspace || !o) return FA_ERR_NULL_POINTER;
+  if (!o || (!workspace && fa_decode_mx_workspace_floats(B, H, H_kv, D, max_pages) > 0))
+    return FA_ERR_NULL_POINTER;
   if (!aligned16(workspace) || !aligned16(o)) return FA_ERR_ALIGNMENT;
   if (reinterpret_cast<uintptr_t>(lse) & 3u) return FA_ERR_ALIGNMENT;
   if (num_pages > kMaxGrid) return FA_ERR_TOO_LARGE;

@@ -46,7 +46,8 @@ constexpr int kBatchOf = Page<D, KB>::PIECE + Page<D, VB>::PIECE <= 32 ? 4 : 2;
 //
 // C, for the batch's T pages (chunks are counted along the pages; a chunk is a
 // workgroup for every head group):
-//   kMinChunk pages while they make fewer than kFill workgroups,
+//   kMinChunk pages while they make fewer than kFill workgroups (kMinFull where
+//   the sequences alone give every CU one),
 //   then what makes kFill of them, up to kMaxChunk pages,
 //   then kMaxChunk pages, until they make kMost workgroups.
 // kFill is the four workgroups that a CU holds; chunks past kMaxChunk pages are
@@ -55,7 +56,16 @@ constexpr int kBatchOf = Page<D, KB>::PIECE + Page<D, VB>::PIECE <= 32 ? 4 : 2;
 // sequences as chunks wanted, only those of twice the mean length are cut (256
 // of 100 to 900 tokens over 4 KV heads: 20 -> 15.4 us).
 constexpr int kFill = 1024, kMost = 4096;
-constexpr int kMinChunk = 16, kMaxChunk = 128;
+//
+// kMinChunk is a batch of four pages for each wave. Joining chunks costs a second
+// launch, 4 us: it is not made, and nothing is cut, for tables of up to
+// kOnePages pages (one sequence of 512 tokens 7.0 -> 5.3 us, 8 of them 8.2 ->
+// 6.3; at 768 tokens one sequence is faster cut, 7.0 and 7.4) or where no table
+// entry could make a second chunk (kMinFull: 32 sequences of 768 tokens over 8
+// KV heads 12.8 -> 9.6 us, of 2048 21.3 -> 20.8; under 256 workgroups it costs:
+// 8 sequences of 1024, 9.2 and 10.3).
+constexpr int kMinChunk = 16, kMaxChunk = 128, kMinFull = 96;
+constexpr int kOnePages = 32;
 constexpr int kRowFill = 256;
 
 // Rows up to which the join gives a row a workgroup for each 32 columns (one
@@ -70,22 +80,29 @@ constexpr int64_t kPassThrough = 64 << 20;
 
 static int64_t head_groups(int64_t H, int64_t Hkv) { return Hkv * ((H / Hkv + 15) / 16); }
 
-// Chunks along the pages that make kFill and kMost workgroups.
+// Chunks along the pages that make kFill and kMost workgroups; least pages of one.
 struct Plan {
-  unsigned fill, most;
+  unsigned fill, most, least;
 };
 static Plan plan_of(int64_t B, int64_t H, int64_t Hkv) {
   const int64_t g = head_groups(H, Hkv);
   int64_t fill = (kFill + g - 1) / g;
   if (fill > kRowFill * B) fill = kRowFill * B;
   if (B >= fill && 3 * B < 4 * fill) fill = 3 * B / 4 > 0 ? 3 * B / 4 : 1;
-  return {(unsigned)fill, (unsigned)((kMost + g - 1) / g)};
+  const unsigned least = B * g >= kFill / 4 ? kMinFull : kMinChunk;
+  return {(unsigned)fill, (unsigned)((kMost + g - 1) / g), least};
+}
+
+// Whether every sequence is one chunk, whatever the lengths: fewer than 3/2
+// chunks of the least length are one.
+static bool never_cut(int64_t B, int64_t H, int64_t Hkv, int64_t max_pages) {
+  return max_pages <= kOnePages || 2 * max_pages < 3 * (int64_t)plan_of(B, H, Hkv).least;
 }
 
 // Pages of a chunk where the batch has `total`.
 __host__ __device__ inline int chunk_pages(int total, Plan plan) {
   const unsigned c = ((unsigned)total + plan.fill - 1) / plan.fill;
-  if (c <= kMaxChunk) return c < kMinChunk ? kMinChunk : (int)c;
+  if (c <= kMaxChunk) return (int)(c < plan.least ? plan.least : c);
   const unsigned d = ((unsigned)total + plan.most - 1) / plan.most;
   return d < kMaxChunk ? kMaxChunk : (int)d;
 }
@@ -659,8 +676,7 @@ static int decode(const void* q, const void* k_pool, const void* v_pool, const i
                   int64_t num_pages, float* workspace, void* o, float* lse, hipStream_t s) {
   const float c = (float)(1.0 / sqrt((double)D)) * kLog2e;
   const int64_t most = most_chunks(B, H, Hkv, max_pages);
-  // No sequence of up to kMinChunk pages is cut.
-  const bool one = max_pages <= kMinChunk;
+  const bool one = never_cut(B, H, Hkv, max_pages);
   const int64_t slots = partial_chunks(B, most), rows = slots * H;
   float* part_o = workspace;
   float* part_l = workspace + rows * D;
@@ -673,7 +689,7 @@ static int decode(const void* q, const void* k_pool, const void* v_pool, const i
   hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, s, (const uint16_t*)q, (const char*)k_pool,
                      (const char*)v_pool, page_table, ctx_lens, part_o, part_l, plan, (uint16_t*)o,
                      lse, (int)B, (int)H, (int)Hkv, (int)(H / Hkv), (int)(head_groups(H, Hkv) / Hkv),
-                     (int)max_pages, (int)num_pages, (int)slots, plan_of(B, H, Hkv), c);
+                     (int)max_pages, (int)num_pages, (int)slots, one ? Plan{1, 1, 1} : plan_of(B, H, Hkv), c);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return -(int)e;
   if (one) return FA_OK;
@@ -698,7 +714,7 @@ extern "C" int64_t fa_decode_mx_workspace_floats(int64_t B, int64_t H, int64_t H
   if (B <= 0 || H <= 0 || H_kv <= 0 || H % H_kv != 0 || D <= 0 || max_pages <= 0 ||
       B > ((int64_t(1) << 31) - 1) / max_pages)
     return 0;
-  if (max_pages <= fa::mx::kMinChunk) return 1;   // not used
+  if (fa::mx::never_cut(B, H, H_kv, max_pages)) return 0;
   const int64_t most = fa::mx::most_chunks(B, H, H_kv, max_pages);
   return fa::mx::partial_chunks(B, most) * H * (D + 1) + 1 + 2 * (B < most ? B : most);
 }
@@ -725,6 +741,10 @@ extern "C" int fa_probe_mx_chunks(int64_t B, int64_t H, int64_t H_kv, int64_t ma
   if (B <= 0 || H <= 0 || H_kv <= 0 || H % H_kv != 0 || max_pages <= 0 || total < 0 ||
       B > ((int64_t(1) << 31) - 1) / max_pages || total > B * max_pages)
     return 0;
+  if (fa::mx::never_cut(B, H, H_kv, max_pages)) {
+    if (most != nullptr) *most = 0;
+    return (int)(total > 0 ? total : 1);
+  }
   if (most != nullptr) *most = fa::mx::most_chunks(B, H, H_kv, max_pages);
   return fa::mx::chunk_pages((int)total, fa::mx::plan_of(B, H, H_kv));
 }

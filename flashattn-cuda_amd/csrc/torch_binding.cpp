@@ -593,7 +593,7 @@ torch::Tensor kv_append_mx(torch::Tensor k_new, torch::Tensor v_new, torch::Tens
   TORCH_CHECK(k_new.device() == dev && v_new.device() == dev,
               "kv_append_mx tensors must be on the same device");
   const c10::DeviceGuard guard(dev);
-  auto bad = torch::empty({B}, page_table.options());
+  auto bad = at::empty({B}, page_table.options());
   const int st = fa_kv_append_mx(
       k_new.data_ptr(), v_new.data_ptr(), page_table.data_ptr<int32_t>(),
       start_pos.data_ptr<int32_t>(), new_lens.has_value() ? new_lens->data_ptr<int32_t>() : nullptr,
@@ -617,8 +617,8 @@ std::vector<torch::Tensor> kv_read_mx(torch::Tensor k_pool, torch::Tensor v_pool
   check_mx_pages(k_pool, page_table, start_pos, lens, B);
   const c10::DeviceGuard guard(k_pool.device());
   const auto opt = k_pool.options().dtype(bf16 ? torch::kBFloat16 : torch::kHalf);
-  auto k = torch::empty({B, m.Hkv, num_tokens, m.D}, opt), v = torch::empty_like(k);
-  auto bad = torch::empty({B}, page_table.options());
+  auto k = at::empty({B, m.Hkv, num_tokens, m.D}, opt), v = at::empty(k.sizes(), opt);
+  auto bad = at::empty({B}, page_table.options());
   const int st = fa_kv_read_mx(
       k_pool.data_ptr(), v_pool.data_ptr(), page_table.data_ptr<int32_t>(),
       start_pos.data_ptr<int32_t>(), lens.has_value() ? lens->data_ptr<int32_t>() : nullptr,
@@ -655,13 +655,14 @@ std::vector<torch::Tensor> decode_paged_mx(torch::Tensor q, torch::Tensor k_pool
               "decode tensors must be on the same device");
   const c10::DeviceGuard guard(dev);
   const auto f32 = q.options().dtype(torch::kFloat);
-  auto ws = torch::empty({fa_decode_mx_workspace_floats(B, H, m.Hkv, D, page_table.size(1))}, f32);
-  auto o = torch::empty({B, H, D}, q.options());
-  auto lse = torch::empty({B, H}, f32);
+  const int64_t floats = fa_decode_mx_workspace_floats(B, H, m.Hkv, D, page_table.size(1));
+  const auto ws = floats > 0 ? at::empty({floats}, f32) : torch::Tensor();
+  auto o = at::empty({B, H, D}, q.options());
+  auto lse = at::empty({B, H}, f32);
   const int st = fa_decode_paged_mx(
       q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), page_table.data_ptr<int32_t>(),
       ctx_lens.data_ptr<int32_t>(), B, H, m.Hkv, D, m.k_bits, m.v_bits, 16, page_table.size(1),
-      m.num_pages, ws.data_ptr<float>(), o.data_ptr(), lse.data_ptr<float>(),
+      m.num_pages, floats > 0 ? ws.data_ptr<float>() : nullptr, o.data_ptr(), lse.data_ptr<float>(),
       q.scalar_type() == torch::kBFloat16, current_stream(q));
   check_status(st, "fa_decode_paged_mx");
   return {o, lse};

@@ -484,7 +484,8 @@ int fa_validate_decode_mx(const void* q, const void* k_pool, const void* v_pool,
                           int64_t page_size, int64_t max_pages, int64_t num_pages,
                           const float* workspace, const void* o, const float* lse);
 
-/* Floats of the workspace fa_decode_paged_mx needs (0 for invalid sizes). */
+/* Floats of the workspace fa_decode_paged_mx needs: 0 for invalid sizes, and
+ * where no sequence is cut in chunks (few pages a sequence). */
 int64_t fa_decode_mx_workspace_floats(int64_t B, int64_t H, int64_t H_kv, int64_t D,
                                       int64_t max_pages);
 
@@ -497,7 +498,7 @@ int64_t fa_decode_mx_workspace_floats(int64_t B, int64_t H, int64_t H_kv, int64_
  * is read. How the pages are shared out follows from the lengths of the whole
  * batch, so a sequence's last bits may depend on the others' lengths; the same
  * call gives the same bits. workspace: 16-byte aligned, of the caller, need not
- * be cleared; calls that may overlap need one each.
+ * be cleared (NULL where none is needed); calls that may overlap need one each.
  */
 int fa_decode_paged_mx(const void* q, const void* k_pool, const void* v_pool,
                        const int32_t* page_table, const int32_t* ctx_lens, int64_t B, int64_t H,
