@@ -208,6 +208,8 @@ extern "C" int fa_validate_kv_append_mx(const void* k, const void* v, const int3
                                        T, D, page_size, max_pages, num_pages);
   if (st != FA_OK) return st;
   if (fa_mx_page_bytes(D, k_bits) == 0 || fa_mx_page_bytes(D, v_bits) == 0) return FA_ERR_MX_BITS;
+  // A workgroup of 256 threads has 16 tokens, and a grid fewer than 2^32 threads.
+  if (T > (int64_t(1) << 28) - 32) return FA_ERR_TOO_LARGE;
   return FA_OK;
 }
 

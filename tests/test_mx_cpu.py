@@ -92,6 +92,7 @@ def _app(**kw):
     (dict(ps=32), "FA_ERR_PAGE_SIZE"), (dict(maxp=0), "FA_ERR_MAX_PAGES"), (dict(np_=0), "FA_ERR_NUM_PAGES"),
     (dict(k=A + 8), "FA_ERR_ALIGNMENT"), (dict(kp=A + 8), "FA_ERR_ALIGNMENT"), (dict(bad=A + 2), "FA_ERR_ALIGNMENT"),
     (dict(H=70000), "FA_ERR_TOO_LARGE"), (dict(T=1 << 31), "FA_ERR_TOO_LARGE"),
+    (dict(T=1 << 28), "FA_ERR_TOO_LARGE"), (dict(T=(1 << 28) - 32), "FA_OK"),
 ])
 def test_validate_append_and_read(capi, kw, code):
     lib = capi.load()
