@@ -27,8 +27,6 @@
 namespace fa {
 namespace mx {
 
-constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / 64;
 constexpr int kXcds = 8;
 
 // Pages that a wave takes at a time: their loads are in flight together. Four
@@ -147,29 +145,31 @@ __device__ __forceinline__ int chunks_of(int p, int C, int* cut) {
 }
 
 // Exclusive prefixes of x and y over the workgroup's threads, and their sums.
+template <int WAVES>
 __device__ __forceinline__ void block_scan(int& x, int& y, int* sh, int* sum_x, int* sum_y) {
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int ix = scan_sum(x), iy = scan_sum(y);
   __syncthreads();   // sh may still be read
   if (lane == 63) {
     sh[wave] = ix;
-    sh[kWaves + wave] = iy;
+    sh[WAVES + wave] = iy;
   }
   __syncthreads();
   int bx = 0, by = 0;
   *sum_x = *sum_y = 0;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
+  for (int w = 0; w < WAVES; ++w) {
     bx += w < wave ? sh[w] : 0;
-    by += w < wave ? sh[kWaves + w] : 0;
+    by += w < wave ? sh[WAVES + w] : 0;
     *sum_x += sh[w];
-    *sum_y += sh[kWaves + w];
+    *sum_y += sh[WAVES + w];
   }
   x = bx + ix - x;
   y = by + iy - y;
 }
 
 // Chunk number x of the batch.
+template <int WAVES>
 __device__ __forceinline__ Chunk chunk_of(const int32_t* __restrict__ ctx_lens, int B,
                                           int max_pages, Plan plan, int x, int* sh) {
   Chunk r;
@@ -205,11 +205,11 @@ __device__ __forceinline__ Chunk chunk_of(const int32_t* __restrict__ ctx_lens, 
     r.cuts = __builtin_amdgcn_readlane(im, 63) >> 16;
     return r;
   }
-  const int per = (B + kThreads - 1) / kThreads;
+  const int per = (B + 64 * WAVES - 1) / (64 * WAVES);
   const int i0 = min((int)threadIdx.x * per, B), i1 = min(i0 + per, B);
   int mine = 0, zero = 0, total, none;
   for (int i = i0; i < i1; ++i) mine += pages_of(ctx_lens[i], max_pages);
-  block_scan(mine, zero, sh, &total, &none);
+  block_scan<WAVES>(mine, zero, sh, &total, &none);
   const int C = chunk_pages(total, plan);
   int n = 0, m = 0, chunks, cuts;
   for (int i = i0; i < i1; ++i) {
@@ -218,7 +218,7 @@ __device__ __forceinline__ Chunk chunk_of(const int32_t* __restrict__ ctx_lens, 
     m += cut;
   }
   const int end = n;
-  block_scan(n, m, sh, &chunks, &cuts);
+  block_scan<WAVES>(n, m, sh, &chunks, &cuts);
   if (x >= chunks) {   // the same in every thread
     r.b = -1;
     return r;
@@ -327,8 +327,8 @@ __device__ __forceinline__ uint32_t v_pair(const uint32_t (&w)[Page<D, VB>::WORD
 }
 
 // NT: the pages are read with the non-temporal hint.
-template <int D, int KB, int VB, bool BF16, bool NT>
-__global__ void __launch_bounds__(kThreads)
+template <int D, int KB, int VB, bool BF16, bool NT, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES)
 fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_pool,
                     const char* __restrict__ v_pool, const int32_t* __restrict__ page_table,
                     const int32_t* __restrict__ ctx_lens, float* __restrict__ part_o,
@@ -343,10 +343,10 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
   // P reaches 2^15 in fp16 rather than 1, so that it keeps all its bits down to
   // 2^-29 of the row's largest (and some to 2^-39); bf16 has fp32's range.
   constexpr float kShift = BF16 ? 0.f : 15.f;
-  __shared__ __attribute__((aligned(16))) float sh_o[kWaves][16][D + 4];   // heads in different banks
-  __shared__ float sh_m[kWaves][16], sh_l[kWaves][16];
-  __shared__ int sh_i[2 * kWaves];
-  __shared__ int sh_bad;
+  __shared__ __attribute__((aligned(16))) float sh_o[WAVES][16][D + 4];   // heads in different banks
+  __shared__ float sh_m[WAVES][16], sh_l[WAVES][16];
+  __shared__ int sh_i[2 * WAVES];
+  __shared__ int sh_bad[WAVES];
 
   // Workgroups go to the XCDs in turn: an XCD has every eighth chunk, and the
   // head groups of a chunk one after the other, so that what is read of a page
@@ -359,8 +359,7 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, grp = lane >> 4;
 
-  if (tid == 0) sh_bad = 0;
-  Chunk ch = chunk_of(ctx_lens, B, max_pages, chunk_plan, number, sh_i);
+  Chunk ch = chunk_of<WAVES>(ctx_lens, B, max_pages, chunk_plan, number, sh_i);
   ch.b = __builtin_amdgcn_readfirstlane(ch.b);
   if (ch.b < 0) return;
   const int ctx = __builtin_amdgcn_readfirstlane(ch.ctx);
@@ -371,7 +370,7 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
   const int each = (int)((unsigned)pages / (unsigned)ch.splits), more = pages - each * ch.splits;
   const int p0 = ch.split * each + min(ch.split, more), p1 = p0 + each + (ch.split < more);
   // This wave's pages.
-  const int w0 = p0 + (p1 - p0) * wave / kWaves, w1 = p0 + (p1 - p0) * (wave + 1) / kWaves;
+  const int w0 = p0 + (p1 - p0) * wave / WAVES, w1 = p0 + (p1 - p0) * (wave + 1) / WAVES;
   bool bad = ctx < 0 || (ctx > 0 && pages == 0);
 
   // Q^T operand: column col = head h0 + col, step kb of the lane's quarter of D.
@@ -519,7 +518,8 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
   l = col_sum(l);
 
   // The waves' parts join in LDS. acc[db][r] is value (4 grp + r) D/16 + db.
-  if (__any(bad) && lane == 0) sh_bad = 1;
+  const bool wave_bad = __any(bad);
+  if (lane == 0) sh_bad[wave] = wave_bad;
   if (col < G) {
 #pragma unroll
     for (int r = 0; r < 4; ++r)
@@ -531,6 +531,9 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
     }
   }
   __syncthreads();
+  bool any_bad = false;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) any_bad |= sh_bad[w] != 0;
   if (plan != nullptr && hg == 0 && tid == 0) {   // for the pass that joins
     if (number == 0) plan[0] = ch.cuts;
     if (ch.splits > 1 && ch.split == 0) {
@@ -539,21 +542,21 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
     }
   }
   // A thread has four columns of a head.
-  for (int i = tid; i < G * (D / 4); i += kThreads) {
+  for (int i = tid; i < G * (D / 4); i += 64 * WAVES) {
     const int g = i / (D / 4), d = 4 * (i % (D / 4));
-    float wm[kWaves], wl[kWaves];
+    float wm[WAVES], wl[WAVES];
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
       wm[w] = sh_m[w][g];
       wl[w] = sh_l[w][g];
     }
     float M = wm[0];
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) M = fmaxf(M, wm[w]);
+    for (int w = 1; w < WAVES; ++w) M = fmaxf(M, wm[w]);
     f32x4 a = f32x4{};
     float z = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
       // A wave without pages has m = -inf; its sums are 0.
       const float e = wl[w] == 0.f ? 0.f : exp2_hw(wm[w] - M);
       const f32x4 v = *reinterpret_cast<const f32x4*>(&sh_o[w][g][d]);
@@ -563,7 +566,7 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
     }
     float inv = z == 0.f ? 0.f : 1.f / z;
     float L = z == 0.f ? -INFINITY : M - kShift + log2_hw(z);   // in units of log 2
-    if (sh_bad) inv = L = NAN;
+    if (any_bad) inv = L = NAN;
 #pragma unroll
     for (int j = 0; j < 4; ++j) a[j] *= inv;
     if (ch.splits == 1) {
@@ -578,18 +581,20 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
   }
 }
 
+constexpr int kJoinWaves = 4;
+
 // Joins the chunks of cut sequence blockIdx.x, head blockIdx.y: a wave has 32
-// columns of the row (WAVES = 1) or kWaves waves share them, eight lanes for
+// columns of the row (WAVES = 1) or kJoinWaves waves share them, eight lanes for
 // four columns each in as many groups as there are, the chunks dealt out over
 // the groups. One pass, with a running maximum.
 template <int D, bool BF16, int WAVES>
-__global__ void __launch_bounds__(WAVES == 1 ? 2 * D : kThreads)
+__global__ void __launch_bounds__(WAVES == 1 ? 2 * D : 64 * kJoinWaves)
 fa_decode_mx_join_kernel(const float* __restrict__ part_o, const float* __restrict__ part_l,
                          const int32_t* __restrict__ plan, uint16_t* __restrict__ o,
                          float* __restrict__ lse, int H, int slots) {
   constexpr int GROUPS = 8 * WAVES, AHEAD = 4;
-  __shared__ __attribute__((aligned(16))) f32x4 sh_a[kWaves][8];
-  __shared__ float sh_m[kWaves], sh_z[kWaves];
+  __shared__ __attribute__((aligned(16))) f32x4 sh_a[kJoinWaves][8];
+  __shared__ float sh_m[kJoinWaves], sh_z[kJoinWaves];
   const int cuts = plan[0], b = plan[1 + 2 * blockIdx.x], word = plan[2 + 2 * blockIdx.x];
   if ((int)blockIdx.x >= cuts) return;
   const int first = word & 0xffff, n = word >> 16;
@@ -650,11 +655,11 @@ fa_decode_mx_join_kernel(const float* __restrict__ part_o, const float* __restri
     if (wave != 0) return;
     M = sh_m[0];
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) M = fmaxf(M, sh_m[w]);
+    for (int w = 1; w < kJoinWaves; ++w) M = fmaxf(M, sh_m[w]);
     z = 0.f;
     a = f32x4{};
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < kJoinWaves; ++w) {
       const float f = sh_m[w] == M ? 1.f : exp2_hw(sh_m[w] - M);
       const f32x4 v = sh_a[w][lane & 7];
       z = fmaf(f, sh_z[w], z);
@@ -684,20 +689,29 @@ static int decode(const void* q, const void* k_pool, const void* v_pool, const i
   const dim3 grid((unsigned)(kXcds * head_groups(H, Hkv)),
                   (unsigned)(((one ? B : most + B) + kXcds - 1) / kXcds));
   const bool nt = num_pages * Hkv * (Page<D, KB>::BYTES + Page<D, VB>::BYTES) >= kPassThrough;
-  const auto kernel = nt ? fa_decode_mx_kernel<D, KB, VB, BF16, true>
-                         : fa_decode_mx_kernel<D, KB, VB, BF16, false>;
-  hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, s, (const uint16_t*)q, (const char*)k_pool,
+  // Eight waves where nothing is cut and a CU has one workgroup at most (32
+  // sequences of 2048 tokens over 8 KV heads 20.5 -> 16.7 us, 8 of 512 6.3 ->
+  // 6.0; four where there are more: 32 of 768 over 32 heads 15.3 and 20.8) or
+  // where four take a batch each (one of 130 tokens, D = 64: 3.5 and 4.4).
+  const int64_t groups = head_groups(H, Hkv);
+  const int waves = one && max_pages > kMinChunk && B * groups <= kFill / 4 ? 8 : 4;
+  const auto kernel = waves == 8 ? (nt ? fa_decode_mx_kernel<D, KB, VB, BF16, true, 8>
+                                       : fa_decode_mx_kernel<D, KB, VB, BF16, false, 8>)
+                                 : (nt ? fa_decode_mx_kernel<D, KB, VB, BF16, true, 4>
+                                       : fa_decode_mx_kernel<D, KB, VB, BF16, false, 4>);
+  hipLaunchKernelGGL(kernel, grid, dim3(64 * waves), 0, s, (const uint16_t*)q, (const char*)k_pool,
                      (const char*)v_pool, page_table, ctx_lens, part_o, part_l, plan, (uint16_t*)o,
-                     lse, (int)B, (int)H, (int)Hkv, (int)(H / Hkv), (int)(head_groups(H, Hkv) / Hkv),
-                     (int)max_pages, (int)num_pages, (int)slots, one ? Plan{1, 1, 1} : plan_of(B, H, Hkv), c);
+                     lse, (int)B, (int)H, (int)Hkv, (int)(H / Hkv), (int)(groups / Hkv),
+                     (int)max_pages, (int)num_pages, (int)slots,
+                     one ? Plan{1, 1, 1} : plan_of(B, H, Hkv), c);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return -(int)e;
   if (one) return FA_OK;
   // Few rows: a workgroup for each 32 columns; else one a row.
   const unsigned cut = (unsigned)(B < most ? B : most);
   if (B * H * (D / 32) <= kWideJoin)
-    hipLaunchKernelGGL((fa_decode_mx_join_kernel<D, BF16, kWaves>), dim3(cut, (unsigned)H, D / 32),
-                       dim3(kThreads), 0, s, part_o, part_l, plan, (uint16_t*)o, lse, (int)H,
+    hipLaunchKernelGGL((fa_decode_mx_join_kernel<D, BF16, kJoinWaves>), dim3(cut, (unsigned)H, D / 32),
+                       dim3(64 * kJoinWaves), 0, s, part_o, part_l, plan, (uint16_t*)o, lse, (int)H,
                        (int)slots);
   else
     hipLaunchKernelGGL((fa_decode_mx_join_kernel<D, BF16, 1>), dim3(cut, (unsigned)H), dim3(2 * D), 0,
