@@ -373,16 +373,6 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
   const int w0 = p0 + (p1 - p0) * wave / WAVES, w1 = p0 + (p1 - p0) * (wave + 1) / WAVES;
   bool bad = ctx < 0 || (ctx > 0 && pages == 0);
 
-  // Q^T operand: column col = head h0 + col, step kb of the lane's quarter of D.
-  u32x4 qf[KS];
-#pragma unroll
-  for (int kb = 0; kb < KS; ++kb) {
-    qf[kb] = u32x4{};
-    if (col < G)
-      qf[kb] = *reinterpret_cast<const u32x4*>(q + ((size_t)ch.b * H + h0 + col) * D +
-                                               grp * (D / 4) + 8 * kb);
-  }
-
   const uint32_t koff = (4 * col + grp) * (PK::PIECE < 16 ? PK::PIECE : 16);
   const uint32_t voff = lane * (PV::PIECE < 16 ? PV::PIECE : 16);
   const uint32_t ksoff = k_scale<D, KB>(col, grp * PK::BLOCKS / 4);
@@ -402,9 +392,21 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
   // registers are free (409 and 14.2).
   int ids = 0;   // lane i: id of the wave's page 64 j + i
   Batch<D, KB, VB> x;
+  const auto load_ids = [&](int w) { ids = pt[min(w + lane, w1 - 1)]; };
+  if (w0 < w1) load_ids(w0);   // before Q, which is not waited for until the first scores
+  // Q^T operand: column col = head h0 + col, step kb of the lane's quarter of D.
+  u32x4 qf[KS];
+#pragma unroll
+  for (int kb = 0; kb < KS; ++kb) {
+    qf[kb] = u32x4{};
+    if (col < G)
+      qf[kb] = *reinterpret_cast<const u32x4*>(q + ((size_t)ch.b * H + h0 + col) * D +
+                                               grp * (D / 4) + 8 * kb);
+  }
+
   const auto load = [&](int w) {
     if (((w - w0) & 63) == 0) {
-      ids = pt[min(w + lane, w1 - 1)];
+      if (w != w0) load_ids(w);
       const bool no = ids < 0 || ids >= num_pages;
       bad |= no;
       ids = no ? 0 : ids;   // read in place of a page that is not there; the result is NaN

@@ -28,10 +28,12 @@ using pages::kThreads;
 template <int D>
 constexpr int kRows = kThreads / (D / 8);
 
-// Rows read back of this size and more pass the caches, which would not hold
-// them for their reader: 131 MB of 32000 tokens 35.4 -> 25.5 us, 65 MB 18.2 ->
-// 14.0 (15 MB 5.7 -> 4.7 too, but those the L2 keeps).
-constexpr int64_t kPassThrough = 32 << 20;
+// Rows read back of this size and more are written past the caches: alone 134
+// MB take 33.6 -> 23.2 us and 131 MB of one sequence 35.9 -> 25.5; with a kernel
+// after it that reads them all 61.8 -> 61.6 and 63.7 -> 65.0, as those then
+// come from memory. Smaller ones are left where their reader finds them (65 MB
+// alone 19.7 -> 12.7, with that kernel 33.3 -> 35.9).
+constexpr int64_t kPassThrough = 100 << 20;
 
 // Workgroups along a sequence that cover T tokens from any position: whole
 // pages, the first and the last of which may be covered in part.
@@ -206,7 +208,8 @@ fa_kv_append_mx_kernel(const u32x4* __restrict__ k_new, const u32x4* __restrict_
 }
 
 // NT: the rows are written with the non-temporal hint, and the heads of a page
-// are read one after the other (16 heads of 4 x 4096 tokens: 31.4 -> 24.3 us).
+// are read one after the other (16 heads of 4 x 4096 tokens with the hint alone
+// 31.4 us, 24.3 so).
 template <int D, int KB, int VB, bool BF16, bool NT>
 __global__ void __launch_bounds__(kThreads)
 fa_kv_read_mx_kernel(const char* __restrict__ k_pool, const char* __restrict__ v_pool,
