@@ -66,9 +66,10 @@ constexpr int kMinChunk = 16, kMaxChunk = 128, kMinFull = 96;
 constexpr int kOnePages = 32;
 constexpr int kRowFill = 256;
 
-// Rows up to which the join gives a row a workgroup for each 32 columns (one
-// sequence of 131072 tokens, 32 rows in 256 chunks: 6 us less).
-constexpr int kWideJoin = 1024;
+// Chunks a sequence from which the join gives a row a workgroup for each 32
+// columns (one sequence over one KV head, 256 chunks: 16.5 -> 13.5 us; 8
+// sequences of 8 chunks 12.85 and 13.2).
+constexpr int kWideJoin = 48;
 
 // Pools from this size on do not stay in the caches between two steps; their
 // codes are read with the non-temporal hint (2.5 GB: 440 -> 390 us, 300 MB: 64
@@ -709,9 +710,8 @@ static int decode(const void* q, const void* k_pool, const void* v_pool, const i
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return -(int)e;
   if (one) return FA_OK;
-  // Few rows: a workgroup for each 32 columns; else one a row.
   const unsigned cut = (unsigned)(B < most ? B : most);
-  if (B * H * (D / 32) <= kWideJoin)
+  if (most > kWideJoin * B)
     hipLaunchKernelGGL((fa_decode_mx_join_kernel<D, BF16, kJoinWaves>), dim3(cut, (unsigned)H, D / 32),
                        dim3(64 * kJoinWaves), 0, s, part_o, part_l, plan, (uint16_t*)o, lse, (int)H,
                        (int)slots);

@@ -262,6 +262,38 @@ def test_decode_many_sequences(fa, dev, B):
     _decode(fa, dev, _decode_case(B, ctx.tolist(), 2, 1, 64, 4, 8, False), 4, 8, False, f"B{B}")
 
 
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("D,kb,vb", FORMS)
+def test_decode_large_pools(fa, dev, D, kb, vb, bf16):
+    """Pools of 64 MB and more are read with the non-temporal hint: the same pages spread over such
+    pools give the same bits, in cut and uncut batches of four and of eight waves."""
+    for H, Hkv, ctx in ((4, 2, [1500, 40, 0]), (2, 2, [300, 511]), (2, 1, [9])):
+        q, kp, vp, table, c = _decode_case(D + H, ctx, H, Hkv, D, kb, vb, bf16)
+        P = (64 << 20) // (Hkv * (kp.shape[2] + vp.shape[2])) + 100
+        tkp, tvp, tt, tc = _to(dev, kp, vp, table, c)
+        at = torch.from_numpy(np.random.default_rng(1).choice(P, kp.shape[0], replace=False)).to(dev)
+        big = []
+        for t in (tkp, tvp):
+            x = torch.full((P, Hkv, t.shape[2]), 255, dtype=torch.uint8, device=dev)
+            x[at] = t
+            big.append(x)
+        moved = torch.where(tt >= 0, at[tt.clamp(min=0).long()].int(), tt)
+        tq = _rows_to(dev, q, bf16)
+        O, L = fa.decode_paged_mx(tq, *big, moved, tc)
+        Ow, Lw = fa.decode_paged_mx(tq, tkp, tvp, tt, tc)
+        assert torch.equal(O, Ow) and torch.equal(L, Lw)
+        _check_decode(O, L, mx.decode_mx(q, kp, vp, table, c, kb, vb, bf16), f"{ctx}")
+
+
+@pytest.mark.parametrize("H,Hkv,B,pages", [
+    (2, 2, 3, [32, 31, 1]), (2, 2, 3, [33, 24, 23]),          # the widest table of one launch, and the next
+    (64, 64, 4, [143, 1, 90, 0]), (64, 64, 4, [144, 143, 1, 8]),   # and where the sequences fill the chip
+])
+def test_decode_at_the_limits_of_one_launch(fa, dev, H, Hkv, B, pages):
+    ctx = [16 * p - (p > 1) * 3 for p in pages]
+    _decode(fa, dev, _decode_case(H, ctx, H, Hkv, 64, 4, 4, False), 4, 4, False, f"{pages}")
+
+
 def test_decode_wide_table(fa, dev):
     """A table far wider than the contexts: entries past them are not looked at."""
     _decode(fa, dev, _decode_case(3, [5, 70, 16], 4, 2, 128, 4, 4, False, extra=3000), 4, 4, False, "wide")
