@@ -135,12 +135,14 @@ __device__ __forceinline__ int pages_of(int ctx, int max_pages) {
   return p > max_pages ? 0 : p;   // of an invalid length: none
 }
 
-// Of a sequence of p pages: its chunks (p / C to the nearest, so that none is
-// under C / 2 longer or shorter than C by half), and what it adds to the count
-// of cut sequences (<< 16) and of their chunks. Those chunks are fewer than
-// 2 kMost.
+// Of a sequence of p pages: its chunks, and what it adds to the count of cut
+// sequences (<< 16) and of their chunks, which are fewer than 2 kMost. p / C to
+// the nearest, so that none is longer or shorter than C by half; of kMinChunk
+// pages not to the nearest but up, as a longer one takes its waves a second
+// batch (8 sequences of 200 to 4000 tokens 12.8 -> 11.8 us).
 __device__ __forceinline__ int chunks_of(int p, int C, int* cut) {
-  const int s = max(1, (int)((2u * (unsigned)p + (unsigned)C) / (2u * (unsigned)C)));
+  const unsigned c = (unsigned)C, up = C == kMinChunk ? 2 * c - 1 : c;
+  const int s = max(1, (int)((2u * (unsigned)p + up) / (2u * c)));
   *cut = s > 1 ? (s | 1 << 16) : 0;
   return s;
 }

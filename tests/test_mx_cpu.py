@@ -164,7 +164,7 @@ def test_refusals_of_host_tensors(fa):
 def test_chunk_plan_fits_its_grid(capi):
     """The grid and the workspace are sized from B * max_pages; whatever the lengths (any total up to
     that), the chunks that the device cuts fit them: at most `most` and one a sequence, of cut
-    sequences at most `most` and half a one a sequence."""
+    sequences at most `most` and one a cut sequence."""
     import random
     lib = capi.load()
     r = random.Random(3)
@@ -177,11 +177,12 @@ def test_chunk_plan_fits_its_grid(capi):
         lens = [min(maxp, int(2 ** r.uniform(0, 14)) - 1) for _ in range(B)]
         Cp = lib.fa_probe_mx_chunks(B, H, Hkv, maxp, sum(lens), C.byref(most))
         assert Cp >= min(16, max(1, sum(lens)))
-        cut = [(2 * p + Cp) // (2 * Cp) for p in lens]
+        cut = [-(-p // Cp) if Cp == 16 else (2 * p + Cp) // (2 * Cp) for p in lens]
+        if most.value == 0:   # one launch: a sequence is one chunk
+            assert Cp >= max(lens)
+            cut = [1] * B
         assert sum(max(1, n) for n in cut) <= most.value + B
         cuts = [n for n in cut if n > 1]
         assert sum(cuts) <= most.value + min(B, most.value) < 1 << 15 and len(cuts) <= min(B, most.value)
         assert (lib.fa_decode_mx_workspace_floats(B, H, Hkv, 64, maxp) > 0) == (most.value > 0)
-        if most.value == 0:
-            assert not cuts   # no second pass is launched
     assert lib.fa_probe_mx_chunks(1, 4, 3, 10, 5, None) == lib.fa_probe_mx_chunks(1, 4, 4, 10, 11, None) == 0
