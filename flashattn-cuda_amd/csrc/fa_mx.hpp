@@ -91,7 +91,7 @@ __device__ __forceinline__ float scale_at(uint32_t w) {
 }
 
 // Values 2 I and 2 I + 1 of a word of codes (I < 4 at 4 bits, < 2 at 8), as
-// raw 16-bit pairs. Exact in both types, but for bf16 values below 2^-126.
+// raw 16-bit pairs. Exact wherever the type has the value.
 template <int BITS, bool BF16, int I>
 __device__ __forceinline__ uint32_t values2(uint32_t w, float scale) {
   if constexpr (BITS == 4) {

@@ -49,11 +49,11 @@ constexpr int kBatchOf = Page<D, KB>::PIECE + Page<D, VB>::PIECE <= 32 ? 4 : 2;
 //   then what makes kFill of them, up to kMaxChunk pages,
 //   then kMaxChunk pages, until they make kMost workgroups.
 // kFill is the four workgroups that a CU holds; chunks past kMaxChunk pages are
-// cut for balance, at little cost. Besides, at most kRowFill chunks a sequence (one of 131072 tokens over one KV head: 20.7 us in
-// 512 chunks, 16.0 in 256, 17.9 in 128), and where there are about as many
-// sequences as chunks wanted, only those of twice the mean length are cut (256
-// of 100 to 900 tokens over 4 KV heads: 20 -> 15.4 us).
-constexpr int kFill = 1024, kMost = 4096;
+// cut for balance, at little cost. Besides, at most kRowFill chunks a sequence
+// (one of 131072 tokens over one KV head: 20.7 us in 512 chunks, 16.0 in 256,
+// 17.9 in 128), and where there are about as many sequences as chunks wanted,
+// only those of twice the mean length are cut (256 of 100 to 900 tokens over 4
+// KV heads: 20 -> 15.4 us).
 //
 // kMinChunk is a batch of four pages for each wave. Joining chunks costs a second
 // launch, 4 us: it is not made, and nothing is cut, for tables of up to
@@ -62,9 +62,16 @@ constexpr int kFill = 1024, kMost = 4096;
 // entry could make a second chunk (kMinFull: 32 sequences of 768 tokens over 8
 // KV heads 12.8 -> 9.6 us, of 2048 21.3 -> 20.8; under 256 workgroups it costs:
 // 8 sequences of 1024, 9.2 and 10.3).
+constexpr int kFill = 1024, kMost = 4096;
 constexpr int kMinChunk = 16, kMaxChunk = 128, kMinFull = 96;
 constexpr int kOnePages = 32;
 constexpr int kRowFill = 256;
+
+// Sequences up to which every wave finds its chunk by itself, a lane for up to
+// four of them; more are planned by a launch of their own, whose 8 us do not
+// show beside the work of so many (4096 sequences of about 300 tokens over 8 KV
+// heads, planned by every workgroup 752 us, 306 by none).
+constexpr int kWavePlan = 256;
 
 // Chunks a sequence from which the join gives a row a workgroup for each 32
 // columns (one sequence over one KV head, 256 chunks: 16.5 -> 13.5 us; 8
@@ -92,8 +99,8 @@ static Plan plan_of(int64_t B, int64_t H, int64_t Hkv) {
   return {(unsigned)fill, (unsigned)((kMost + g - 1) / g), least};
 }
 
-// Whether every sequence is one chunk, whatever the lengths: fewer than 3/2
-// chunks of the least length are one.
+// Whether every sequence is one chunk, whatever the lengths: none (kMinFull) has
+// 3/2 chunks of the least length.
 static bool never_cut(int64_t B, int64_t H, int64_t Hkv, int64_t max_pages) {
   return max_pages <= kOnePages || 2 * max_pages < 3 * (int64_t)plan_of(B, H, Hkv).least;
 }
@@ -116,18 +123,34 @@ static int64_t most_chunks(int64_t B, int64_t H, int64_t Hkv, int64_t max_pages)
   const int64_t by_min = total / kMinChunk, n = fill > by_max ? fill : by_max;
   return (n < by_min ? n : by_min) + 1;
 }
+// Rows of the grid: most chunks and one a sequence, a chunk to each XCD.
+static int64_t chunk_rows(int64_t B, int64_t most) { return (most + B + kXcds - 1) / kXcds; }
+
 // Chunks of the sequences that are cut at all, more than one a sequence: such a
 // sequence has more than C pages and less than 2 pages / C chunks.
 static int64_t partial_chunks(int64_t B, int64_t most) { return most + (B < most ? B : most); }
 
+// The workspace, in words of 4 bytes: the table of chunks where one is planned,
+// partial O and L, and the cut sequences for the join.
+struct Workspace {
+  int64_t slots, part_o, part_l, plan, words;
+};
+static Workspace workspace_of(int64_t B, int64_t H, int64_t D, int64_t most) {
+  Workspace w;
+  w.slots = partial_chunks(B, most);
+  w.part_o = B > kWavePlan ? 4 * (1 + chunk_rows(B, most) * kXcds) : 0;
+  w.part_l = w.part_o + w.slots * H * D;
+  w.plan = w.part_l + w.slots * H;
+  w.words = w.plan + 1 + 2 * (B < most ? B : most);
+  return w;
+}
+
 // What a workgroup's chunk is.
 struct Chunk {
-  int b;        // sequence, -1: none
-  int ctx;      // its length
-  int split, splits;   // number of the chunk in the sequence, and how many there are
-  int partial;  // of the sequence's first chunk, among those of cut sequences
-  int index;    // the sequence's number among those
-  int cuts;     // cut sequences in all
+  int b, ctx;           // sequence, -1: none; its length
+  int split, splits;    // number of the chunk in the sequence, and how many there are
+  int partial;          // of the chunk, among those of cut sequences
+  int index, cuts;      // the sequence's number among those, and how many there are
 };
 
 __device__ __forceinline__ int pages_of(int ctx, int max_pages) {
@@ -147,110 +170,142 @@ __device__ __forceinline__ int chunks_of(int p, int C, int* cut) {
   return s;
 }
 
+// Chunk number x of a batch of up to kWavePlan sequences.
+__device__ __forceinline__ Chunk chunk_of(const int32_t* __restrict__ ctx_lens, int B,
+                                          int max_pages, Plan plan, int x) {
+  Chunk r;
+  if (B == 1) {
+    r.ctx = ctx_lens[0];
+    const int p = pages_of(r.ctx, max_pages);
+    r.splits = chunks_of(p, chunk_pages(p, plan), &r.cuts);
+    r.b = x < r.splits ? 0 : -1;
+    r.split = r.partial = x;
+    r.index = 0;
+    r.cuts >>= 16;
+    return r;
+  }
+  constexpr int MOST = kWavePlan / 64;
+  const int per = (B + 63) / 64, i0 = (int)(threadIdx.x & 63) * per;
+  int ctx[MOST], n[MOST], m[MOST], pages = 0, ns = 0, ms = 0;
+#pragma unroll
+  for (int k = 0; k < MOST; ++k) {
+    ctx[k] = k < per && i0 + k < B ? ctx_lens[i0 + k] : 0;
+    pages += pages_of(ctx[k], max_pages);
+  }
+  const int C = chunk_pages(__builtin_amdgcn_readlane(scan_sum(pages), 63), plan);
+#pragma unroll
+  for (int k = 0; k < MOST; ++k) {
+    n[k] = m[k] = 0;
+    if (k < per && i0 + k < B) n[k] = chunks_of(pages_of(ctx[k], max_pages), C, &m[k]);
+    ns += n[k];
+    ms += m[k];
+  }
+  const int im = scan_sum(ms);
+  int e = scan_sum(ns) - ns, f = im - ms;   // of the lane's first sequence
+  int b = -1, len = 0, split = 0, splits = 0, before = 0;
+#pragma unroll
+  for (int k = 0; k < MOST; ++k) {
+    if (x >= e && x < e + n[k]) {
+      b = i0 + k;
+      len = ctx[k];
+      split = x - e;
+      splits = n[k];
+      before = f;
+    }
+    e += n[k];
+    f += m[k];
+  }
+  const uint64_t one = __ballot(b >= 0);
+  if (one == 0) {
+    r.b = -1;
+    return r;
+  }
+  const int at = __builtin_ctzll(one);
+  r.b = __builtin_amdgcn_readlane(b, at);
+  r.ctx = __builtin_amdgcn_readlane(len, at);
+  r.split = __builtin_amdgcn_readlane(split, at);
+  r.splits = __builtin_amdgcn_readlane(splits, at);
+  before = __builtin_amdgcn_readlane(before, at);
+  r.partial = (before & 0xffff) + r.split;
+  r.index = before >> 16;
+  r.cuts = __builtin_amdgcn_readlane(im, 63) >> 16;
+  return r;
+}
+
 // Exclusive prefixes of x and y over the workgroup's threads, and their sums.
 template <int WAVES>
-__device__ __forceinline__ void block_scan(int& x, int& y, int* sh, int* sum_x, int* sum_y) {
+__device__ __forceinline__ void block_scan(int& x, int& y, int (&sh)[2][WAVES], int* sum_x,
+                                           int* sum_y) {
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int ix = scan_sum(x), iy = scan_sum(y);
   __syncthreads();   // sh may still be read
   if (lane == 63) {
-    sh[wave] = ix;
-    sh[WAVES + wave] = iy;
+    sh[0][wave] = ix;
+    sh[1][wave] = iy;
   }
   __syncthreads();
   int bx = 0, by = 0;
   *sum_x = *sum_y = 0;
 #pragma unroll
   for (int w = 0; w < WAVES; ++w) {
-    bx += w < wave ? sh[w] : 0;
-    by += w < wave ? sh[WAVES + w] : 0;
-    *sum_x += sh[w];
-    *sum_y += sh[WAVES + w];
+    bx += w < wave ? sh[0][w] : 0;
+    by += w < wave ? sh[1][w] : 0;
+    *sum_x += sh[0][w];
+    *sum_y += sh[1][w];
   }
   x = bx + ix - x;
   y = by + iy - y;
 }
 
-// Chunk number x of the batch.
-template <int WAVES>
-__device__ __forceinline__ Chunk chunk_of(const int32_t* __restrict__ ctx_lens, int B,
-                                          int max_pages, Plan plan, int x, int* sh) {
-  Chunk r;
-  if (B == 1) {
-    r.ctx = ctx_lens[0];
-    const int p = pages_of(r.ctx, max_pages);
-    r.splits = chunks_of(p, chunk_pages(p, plan), &r.cuts);
-    r.split = x;
-    r.b = x < r.splits ? 0 : -1;
-    r.partial = r.index = 0;
-    r.cuts >>= 16;
-    return r;
-  }
-  if (B <= 64) {   // a lane has a sequence; every wave finds the chunk by itself
-    const int lane = threadIdx.x & 63;
-    const int ctx = lane < B ? ctx_lens[lane] : 0;
-    const int p = pages_of(ctx, max_pages);
-    const int C = chunk_pages(__builtin_amdgcn_readlane(scan_sum(p), 63), plan);
-    int m, n = lane < B ? chunks_of(p, C, &m) : (m = 0);
-    const int in = scan_sum(n), im = scan_sum(m);
-    const int at = __popcll(__ballot(in <= x));   // lanes whose chunks end before x
-    if (at >= B) {
-      r.b = -1;
-      return r;
-    }
-    r.b = at;
-    r.ctx = __builtin_amdgcn_readlane(ctx, at);
-    r.split = x - __builtin_amdgcn_readlane(in - n, at);
-    r.splits = __builtin_amdgcn_readlane(n, at);
-    const int before = __builtin_amdgcn_readlane(im - m, at);
-    r.partial = before & 0xffff;
-    r.index = before >> 16;
-    r.cuts = __builtin_amdgcn_readlane(im, 63) >> 16;
-    return r;
-  }
-  const int per = (B + 64 * WAVES - 1) / (64 * WAVES);
-  const int i0 = min((int)threadIdx.x * per, B), i1 = min(i0 + per, B);
+// The chunks of a batch of any size: table[0] has their number, table[1 + x]
+// chunk x as (sequence, its length, split | splits << 16, partial); plan as the join reads it. One
+// workgroup, a run of sequences a thread; a sequence's entries are written by
+// the whole wave.
+constexpr int kPlanWaves = 16;
+__global__ void __launch_bounds__(64 * kPlanWaves)
+fa_decode_mx_plan_kernel(const int32_t* __restrict__ ctx_lens, int B, int max_pages,
+                         Plan chunk_plan, int4* __restrict__ table, int32_t* __restrict__ plan) {
+  __shared__ int sh[2][kPlanWaves];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int per = (B + 64 * kPlanWaves - 1) / (64 * kPlanWaves);
+  const int i0 = min(tid * per, B), i1 = min(i0 + per, B);
   int mine = 0, zero = 0, total, none;
   for (int i = i0; i < i1; ++i) mine += pages_of(ctx_lens[i], max_pages);
-  block_scan<WAVES>(mine, zero, sh, &total, &none);
-  const int C = chunk_pages(total, plan);
+  block_scan<kPlanWaves>(mine, zero, sh, &total, &none);
+  const int C = chunk_pages(total, chunk_plan);
   int n = 0, m = 0, chunks, cuts;
   for (int i = i0; i < i1; ++i) {
     int cut;
     n += chunks_of(pages_of(ctx_lens[i], max_pages), C, &cut);
     m += cut;
   }
-  const int end = n;
-  block_scan<WAVES>(n, m, sh, &chunks, &cuts);
-  if (x >= chunks) {   // the same in every thread
-    r.b = -1;
-    return r;
+  block_scan<kPlanWaves>(n, m, sh, &chunks, &cuts);
+  if (tid == 0) {
+    table[0] = int4{chunks, 0, 0, 0};
+    plan[0] = cuts >> 16;
   }
-  __syncthreads();
-  if (x >= n && x < n + end) {   // one thread's
-    for (int i = i0; i < i1; ++i) {
-      int cut;
-      const int s = chunks_of(pages_of(ctx_lens[i], max_pages), C, &cut);
-      if (x < n + s) {
-        sh[0] = i;
-        sh[1] = x - n;
-        sh[2] = s;
-        sh[3] = m;
-        break;
+  for (int k = 0; k < per; ++k) {
+    const int i = i0 + k;
+    int cut = 0, s = 0, ctx = 0;
+    if (i < i1) {
+      ctx = ctx_lens[i];
+      s = chunks_of(pages_of(ctx, max_pages), C, &cut);
+      if (s > 1) {
+        plan[1 + 2 * (m >> 16)] = i;
+        plan[2 + 2 * (m >> 16)] = (m & 0xffff) | s << 16;
       }
-      n += s;
-      m += cut;
     }
+    if (s == 1) table[1 + n] = int4{i, ctx, 1 << 16, 0};
+    for (uint64_t rest = __ballot(s > 1); rest != 0; rest &= rest - 1) {
+      const int l = __builtin_ctzll(rest);
+      const int b = __builtin_amdgcn_readlane(i, l), cl = __builtin_amdgcn_readlane(ctx, l);
+      const int sl = __builtin_amdgcn_readlane(s, l);
+      const int nl = __builtin_amdgcn_readlane(n, l), ml = __builtin_amdgcn_readlane(m, l) & 0xffff;
+      for (int j = lane; j < sl; j += 64) table[1 + nl + j] = int4{b, cl, j | sl << 16, ml + j};
+    }
+    n += s;
+    m += cut;
   }
-  __syncthreads();
-  r.b = sh[0];
-  r.ctx = ctx_lens[r.b];
-  r.split = sh[1];
-  r.splits = sh[2];
-  r.partial = sh[3] & 0xffff;
-  r.index = sh[3] >> 16;
-  r.cuts = cuts >> 16;
-  return r;
 }
 
 // Max and sum over the four lane groups of a column.
@@ -335,9 +390,10 @@ __global__ void __launch_bounds__(64 * WAVES)
 fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_pool,
                     const char* __restrict__ v_pool, const int32_t* __restrict__ page_table,
                     const int32_t* __restrict__ ctx_lens, float* __restrict__ part_o,
-                    float* __restrict__ part_l, int32_t* __restrict__ plan,
-                    uint16_t* __restrict__ o, float* __restrict__ lse, int B, int H, int Hkv,
-                    int group, int ngrp, int max_pages, int num_pages, int slots, Plan chunk_plan, float c) {
+                    float* __restrict__ part_l, const int4* __restrict__ table,
+                    int32_t* __restrict__ plan, uint16_t* __restrict__ o, float* __restrict__ lse,
+                    int B, int H, int Hkv, int group, int ngrp, int max_pages, int num_pages,
+                    int slots, Plan chunk_plan, float c) {
   using PK = Page<D, KB>;
   using PV = Page<D, VB>;
   constexpr int kBatch = kBatchOf<D, KB, VB>;
@@ -348,7 +404,6 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
   constexpr float kShift = BF16 ? 0.f : 15.f;
   __shared__ __attribute__((aligned(16))) float sh_o[WAVES][16][D + 4];   // heads in different banks
   __shared__ float sh_m[WAVES][16], sh_l[WAVES][16];
-  __shared__ int sh_i[2 * WAVES];
   __shared__ int sh_bad[WAVES];
 
   // Workgroups go to the XCDs in turn: an XCD has every eighth chunk, and the
@@ -362,7 +417,23 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, grp = lane >> 4;
 
-  Chunk ch = chunk_of<WAVES>(ctx_lens, B, max_pages, chunk_plan, number, sh_i);
+  Chunk ch;
+  if (plan == nullptr) {   // nothing is cut: a chunk a sequence
+    ch.b = number < B ? number : -1;
+    ch.ctx = ctx_lens[min(number, B - 1)];
+    ch.split = ch.partial = 0;
+    ch.splits = 1;
+  } else if (table != nullptr) {
+    const int chunks = table[0].x;
+    const int4 e = table[1 + number];
+    ch.b = number < chunks ? e.x : -1;
+    ch.ctx = e.y;
+    ch.split = e.z & 0xffff;
+    ch.splits = e.z >> 16;
+    ch.partial = e.w;
+  } else {
+    ch = chunk_of(ctx_lens, B, max_pages, chunk_plan, number);
+  }
   ch.b = __builtin_amdgcn_readfirstlane(ch.b);
   if (ch.b < 0) return;
   const int ctx = __builtin_amdgcn_readfirstlane(ch.ctx);
@@ -539,7 +610,7 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
   bool any_bad = false;
 #pragma unroll
   for (int w = 0; w < WAVES; ++w) any_bad |= sh_bad[w] != 0;
-  if (plan != nullptr && hg == 0 && tid == 0) {   // for the pass that joins
+  if (plan != nullptr && table == nullptr && hg == 0 && tid == 0) {   // for the pass that joins
     if (number == 0) plan[0] = ch.cuts;
     if (ch.splits > 1 && ch.split == 0) {
       plan[1 + 2 * ch.index] = ch.b;
@@ -579,7 +650,7 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
       *reinterpret_cast<u32x2*>(o + row * D + d) = u32x2{pack2<BF16>(a[0], a[1]), pack2<BF16>(a[2], a[3])};
       if (lse != nullptr && d == 0) lse[row] = L * kLn2;
     } else {
-      const size_t row = (size_t)(h0 + g) * slots + ch.partial + ch.split;
+      const size_t row = (size_t)(h0 + g) * slots + ch.partial;
       *reinterpret_cast<f32x4*>(part_o + row * D + d) = a;
       if (d == 0) part_l[row] = L;
     }
@@ -687,12 +758,19 @@ static int decode(const void* q, const void* k_pool, const void* v_pool, const i
   const float c = (float)(1.0 / sqrt((double)D)) * kLog2e;
   const int64_t most = most_chunks(B, H, Hkv, max_pages);
   const bool one = never_cut(B, H, Hkv, max_pages);
-  const int64_t slots = partial_chunks(B, most), rows = slots * H;
-  float* part_o = workspace;
-  float* part_l = workspace + rows * D;
-  int32_t* plan = one ? nullptr : reinterpret_cast<int32_t*>(part_l + rows);
+  const Workspace w = workspace_of(B, H, D, most);
+  float* part_o = one ? nullptr : workspace + w.part_o;
+  float* part_l = one ? nullptr : workspace + w.part_l;
+  int32_t* plan = one ? nullptr : reinterpret_cast<int32_t*>(workspace + w.plan);
+  int4* table = one || B <= kWavePlan ? nullptr : reinterpret_cast<int4*>(workspace);
+  if (table != nullptr) {
+    hipLaunchKernelGGL(fa_decode_mx_plan_kernel, dim3(1), dim3(64 * kPlanWaves), 0, s, ctx_lens, (int)B,
+                       (int)max_pages, plan_of(B, H, Hkv), table, plan);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return -(int)e;
+  }
   const dim3 grid((unsigned)(kXcds * head_groups(H, Hkv)),
-                  (unsigned)(((one ? B : most + B) + kXcds - 1) / kXcds));
+                  (unsigned)chunk_rows(B, one ? 0 : most));
   const bool nt = num_pages * Hkv * (Page<D, KB>::BYTES + Page<D, VB>::BYTES) >= kPassThrough;
   // Eight waves where nothing is cut and a CU has one workgroup at most (32
   // sequences of 2048 tokens over 8 KV heads 20.5 -> 16.7 us, 8 of 512 6.3 ->
@@ -705,10 +783,10 @@ static int decode(const void* q, const void* k_pool, const void* v_pool, const i
                                  : (nt ? fa_decode_mx_kernel<D, KB, VB, BF16, true, 4>
                                        : fa_decode_mx_kernel<D, KB, VB, BF16, false, 4>);
   hipLaunchKernelGGL(kernel, grid, dim3(64 * waves), 0, s, (const uint16_t*)q, (const char*)k_pool,
-                     (const char*)v_pool, page_table, ctx_lens, part_o, part_l, plan, (uint16_t*)o,
-                     lse, (int)B, (int)H, (int)Hkv, (int)(H / Hkv), (int)(groups / Hkv),
-                     (int)max_pages, (int)num_pages, (int)slots,
-                     one ? Plan{1, 1, 1} : plan_of(B, H, Hkv), c);
+                     (const char*)v_pool, page_table, ctx_lens, part_o, part_l, table, plan,
+                     (uint16_t*)o, lse, (int)B, (int)H, (int)Hkv, (int)(H / Hkv),
+                     (int)(groups / Hkv), (int)max_pages, (int)num_pages, (int)w.slots,
+                     plan_of(B, H, Hkv), c);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return -(int)e;
   if (one) return FA_OK;
@@ -716,10 +794,10 @@ static int decode(const void* q, const void* k_pool, const void* v_pool, const i
   if (most > kWideJoin * B)
     hipLaunchKernelGGL((fa_decode_mx_join_kernel<D, BF16, kJoinWaves>), dim3(cut, (unsigned)H, D / 32),
                        dim3(64 * kJoinWaves), 0, s, part_o, part_l, plan, (uint16_t*)o, lse, (int)H,
-                       (int)slots);
+                       (int)w.slots);
   else
     hipLaunchKernelGGL((fa_decode_mx_join_kernel<D, BF16, 1>), dim3(cut, (unsigned)H), dim3(2 * D), 0,
-                       s, part_o, part_l, plan, (uint16_t*)o, lse, (int)H, (int)slots);
+                       s, part_o, part_l, plan, (uint16_t*)o, lse, (int)H, (int)w.slots);
   e = hipGetLastError();
   return e == hipSuccess ? FA_OK : -(int)e;
 }
@@ -733,8 +811,7 @@ extern "C" int64_t fa_decode_mx_workspace_floats(int64_t B, int64_t H, int64_t H
       B > ((int64_t(1) << 31) - 1) / max_pages)
     return 0;
   if (fa::mx::never_cut(B, H, H_kv, max_pages)) return 0;
-  const int64_t most = fa::mx::most_chunks(B, H, H_kv, max_pages);
-  return fa::mx::partial_chunks(B, most) * H * (D + 1) + 1 + 2 * (B < most ? B : most);
+  return fa::mx::workspace_of(B, H, D, fa::mx::most_chunks(B, H, H_kv, max_pages)).words;
 }
 
 extern "C" int fa_decode_paged_mx(const void* q, const void* k_pool, const void* v_pool,

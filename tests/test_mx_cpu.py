@@ -137,8 +137,9 @@ def test_sizes_and_strings(capi):
     assert lib.fa_decode_mx_workspace_floats(4, 32, 8, 128, 100) > 0
     assert lib.fa_decode_mx_workspace_floats(4, 32, 5, 128, 100) == 0
     assert lib.fa_decode_mx_workspace_floats(4, 32, 8, 128, 0) == 0
-    # the workspace does not grow with a batch that fills the chip by itself
-    assert (lib.fa_decode_mx_workspace_floats(10000, 32, 8, 128, 2000) ==
+    # the workspace grows with a batch that fills the chip by itself only by the table's four words a
+    # sequence
+    assert (lib.fa_decode_mx_workspace_floats(10000, 32, 8, 128, 2000) - 4 * 5000 ==
             lib.fa_decode_mx_workspace_floats(5000, 32, 8, 128, 2000) <= 1 << 24)
 
 

@@ -134,8 +134,7 @@ def test_flags_over_stale_memory_and_no_tokens(fa, dev):
 @pytest.mark.parametrize("bf16", [False, True])
 @pytest.mark.parametrize("D,kb,vb", FORMS)
 def test_read_matches_oracle(fa, dev, D, kb, vb, bf16):
-    """Any bytes: every code, and scales from below the type's range to above it (bf16: within it, as
-    its subnormal values are not told apart)."""
+    """Any bytes: every code, and scales from below the type's range to above it (bf16: from 2^-97 up)."""
     B, H, T, maxp, P = 3, 2, 75, 8, 26
     rng = np.random.default_rng(D + kb + vb)
     lo, hi = (30, 256) if bf16 else (80, 160)
@@ -260,6 +259,27 @@ def test_decode_many_sequences(fa, dev, B):
     ctx[rng.integers(0, B, 5)] = rng.integers(600, 2500, 5)
     ctx[-1], ctx[0] = 1777, 0
     _decode(fa, dev, _decode_case(B, ctx.tolist(), 2, 1, 64, 4, 8, False), 4, 8, False, f"B{B}")
+
+
+@pytest.mark.parametrize("B,long", [(70, [3000, 700]), (256, [9000, 2400, 2304]), (300, [131072, 2500, 4000]),
+                                    (2100, [4000, 2400])])
+def test_decode_of_planned_batches(fa, dev, B, long):
+    """A few long sequences among many short, empty and invalid ones: chunks found by the waves
+    (a lane for up to four sequences) and, past 256 sequences, planned by a launch."""
+    rng = np.random.default_rng(B)
+    ctx = rng.integers(0, 30, B)
+    ctx[rng.choice(B, len(long), replace=False)] = long
+    case = _decode_case(B, ctx.tolist(), 2, 1, 64, 4, 8, False)
+    _decode(fa, dev, case, 4, 8, False, f"B{B}")
+    q, kp, vp, table, c = case
+    bad = int(np.argmin(c))   # one sequence's length is invalid: the others stay as they are
+    O, L = fa.decode_paged_mx(_rows_to(dev, q, False), *_to(dev, kp, vp, table, c))
+    c2 = c.copy()
+    c2[bad] = -5
+    O2, L2 = fa.decode_paged_mx(_rows_to(dev, q, False), *_to(dev, kp, vp, table, c2))
+    keep = np.arange(B) != bad
+    assert torch.isnan(O2[bad]).all() and torch.isnan(L2[bad]).all()
+    assert torch.equal(O2[keep], O[keep]) and torch.equal(L2[keep], L[keep])
 
 
 @pytest.mark.parametrize("bf16", [False, True])
