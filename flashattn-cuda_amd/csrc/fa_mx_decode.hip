@@ -258,9 +258,9 @@ __device__ __forceinline__ void block_scan(int& x, int& y, int (&sh)[2][WAVES], 
 }
 
 // The chunks of a batch of any size: table[0] has their number, table[1 + x]
-// chunk x as (sequence, its length, split | splits << 16, partial); plan as the join reads it. One
-// workgroup, a run of sequences a thread; a sequence's entries are written by
-// the whole wave.
+// chunk x as (sequence, its length, split | splits << 16, partial); plan as the
+// join reads it. One workgroup, a run of sequences a thread; a sequence's
+// entries are written by the whole wave.
 constexpr int kPlanWaves = 16;
 __global__ void __launch_bounds__(64 * kPlanWaves)
 fa_decode_mx_plan_kernel(const int32_t* __restrict__ ctx_lens, int B, int max_pages,
@@ -461,9 +461,9 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
   // Pages w .. + kBatch - 1, all loads at once; past the wave's last page they
   // repeat it (masked below). Four waves a SIMD hide each other's waits: a
   // second set of registers, loaded one batch ahead, leaves three and measured
-  // slower (32 sequences of up to 32768 tokens 401 us, 384 without; one of
-  // 32000 14.4 and 13.2), and so did loading K and V each as soon as their
-  // registers are free (409 and 14.2).
+  // slower (32 sequences of up to 32768 tokens 402 us, 398 without; one of
+  // 32000 14.0 and 13.0), and so did loading K and V each as soon as their
+  // registers are free (409 and 14.2, when it was 384 and 13.2 without).
   int ids = 0;   // lane i: id of the wave's page 64 j + i
   Batch<D, KB, VB> x;
   const auto load_ids = [&](int w) { ids = pt[min(w + lane, w1 - 1)]; };

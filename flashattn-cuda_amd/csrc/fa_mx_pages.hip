@@ -282,8 +282,9 @@ static int read(const void* k_pool, const void* v_pool, const int32_t* page_tabl
   const dim3 grid((unsigned)(nt ? blocks * H : blocks), nt ? 1u : (unsigned)H, (unsigned)B);
   const auto kernel = nt ? fa_kv_read_mx_kernel<D, KB, VB, BF16, true>
                          : fa_kv_read_mx_kernel<D, KB, VB, BF16, false>;
-  hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, s, (const char*)k_pool, (const char*)v_pool, page_table, start_pos, lens,
-                     (u32x4*)k, (u32x4*)v, bad, (int)H, (int)T, (int)max_pages, (int)num_pages);
+  hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, s, (const char*)k_pool, (const char*)v_pool,
+                     page_table, start_pos, lens, (u32x4*)k, (u32x4*)v, bad, (int)H, (int)T,
+                     (int)max_pages, (int)num_pages);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? FA_OK : -(int)e;
 }
