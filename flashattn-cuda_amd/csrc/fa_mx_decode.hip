@@ -15,6 +15,12 @@
 //                    c D/16 + db, P^T straight from the S accumulators)
 // Lane l has head l % 16 in both products, so a head's maximum and sum stay in
 // its lane column.
+//
+// Maxima are kept as K Q^T gives them, and differences are scaled: s - m is 0 for
+// the largest score, so no weight passes 2^kShift however large the scores are.
+// (Of scaled scores s c and a rounded maximum m c the fma s c - m c is not 0 but
+// up to half a place of m c off: from 2^24 on, weights of 2 and more.) Chunks
+// are joined by (maximum, sum) for the same reason, not by their logsumexp.
 #include <hip/hip_runtime.h>
 
 #include <math.h>
@@ -131,19 +137,24 @@ static int64_t chunk_rows(int64_t B, int64_t most) { return (most + B + kXcds - 
 static int64_t partial_chunks(int64_t B, int64_t most) { return most + (B < most ? B : most); }
 
 // The workspace, in words of 4 bytes: the table of chunks where one is planned,
-// partial O and L, and the cut sequences for the join.
+// partial O, their maxima and sums, and the cut sequences for the join.
 struct Workspace {
-  int64_t slots, part_o, part_l, plan, words;
+  int64_t slots, part_o, part_ml, plan, words;
 };
 static Workspace workspace_of(int64_t B, int64_t H, int64_t D, int64_t most) {
   Workspace w;
   w.slots = partial_chunks(B, most);
   w.part_o = B > kWavePlan ? 4 * (1 + chunk_rows(B, most) * kXcds) : 0;
-  w.part_l = w.part_o + w.slots * H * D;
-  w.plan = w.part_l + w.slots * H;
+  w.part_ml = w.part_o + w.slots * H * D;
+  w.plan = w.part_ml + 2 * w.slots * H;
   w.words = w.plan + 1 + 2 * (B < most ? B : most);
   return w;
 }
+
+// P reaches 2^15 in fp16 rather than 1, so that it keeps all its bits down to
+// 2^-29 of the row's largest (and some to 2^-39); bf16 has fp32's range.
+template <bool BF16>
+constexpr float kShift = BF16 ? 0.f : 15.f;
 
 // What a workgroup's chunk is.
 struct Chunk {
@@ -390,7 +401,7 @@ __global__ void __launch_bounds__(64 * WAVES)
 fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_pool,
                     const char* __restrict__ v_pool, const int32_t* __restrict__ page_table,
                     const int32_t* __restrict__ ctx_lens, float* __restrict__ part_o,
-                    float* __restrict__ part_l, const int4* __restrict__ table,
+                    float2* __restrict__ part_ml, const int4* __restrict__ table,
                     int32_t* __restrict__ plan, uint16_t* __restrict__ o, float* __restrict__ lse,
                     int B, int H, int Hkv, int group, int ngrp, int max_pages, int num_pages,
                     int slots, Plan chunk_plan, float c) {
@@ -399,9 +410,6 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
   constexpr int kBatch = kBatchOf<D, KB, VB>;
   constexpr int KS = D / 32;   // steps of S = K Q^T
   constexpr int DB = D / 16;   // blocks of O^T
-  // P reaches 2^15 in fp16 rather than 1, so that it keeps all its bits down to
-  // 2^-29 of the row's largest (and some to 2^-39); bf16 has fp32's range.
-  constexpr float kShift = BF16 ? 0.f : 15.f;
   __shared__ __attribute__((aligned(16))) float sh_o[WAVES][16][D + 4];   // heads in different banks
   __shared__ float sh_m[WAVES][16], sh_l[WAVES][16];
   __shared__ int sh_bad[WAVES];
@@ -533,9 +541,9 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
     for (int i = 0; i < kBatch; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) top = fmaxf(top, s[i][r]);
-    const float m_new = fmaxf(m, col_max(top) * c);
+    const float m_new = fmaxf(m, col_max(top));
     if (__any(m_new != m)) {   // also where one of them is NaN
-      const float alpha = m_new == m ? 1.f : exp2_hw(m - m_new);
+      const float alpha = m_new == m ? 1.f : exp2_hw((m - m_new) * c);
       l *= alpha;
 #pragma unroll
       for (int db = 0; db < DB; ++db)
@@ -543,14 +551,13 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
         for (int r = 0; r < 4; ++r) acc[db][r] *= alpha;
       m = m_new;
     }
-    const float ref = m - kShift;
     u32x2 ph[kBatch], pl[kBatch];   // P as 16-bit operands, and in bf16 what the first leaves out
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
       float p[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        p[r] = exp2_hw(fmaf(s[i][r], c, -ref));
+        p[r] = exp2_hw(fmaf(s[i][r] - m, c, kShift<BF16>));
         l += p[r];
       }
       ph[i] = u32x2{pack2<BF16>(p[0], p[1]), pack2<BF16>(p[2], p[3])};
@@ -634,25 +641,25 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) {
       // A wave without pages has m = -inf; its sums are 0.
-      const float e = wl[w] == 0.f ? 0.f : exp2_hw(wm[w] - M);
+      const float e = wl[w] == 0.f ? 0.f : exp2_hw((wm[w] - M) * c);
       const f32x4 v = *reinterpret_cast<const f32x4*>(&sh_o[w][g][d]);
       z = fmaf(e, wl[w], z);
 #pragma unroll
       for (int j = 0; j < 4; ++j) a[j] = fmaf(e, v[j], a[j]);
     }
-    float inv = z == 0.f ? 0.f : 1.f / z;
-    float L = z == 0.f ? -INFINITY : M - kShift + log2_hw(z);   // in units of log 2
-    if (any_bad) inv = L = NAN;
+    if (any_bad) z = NAN;
+    const float inv = z == 0.f ? 0.f : 1.f / z;
 #pragma unroll
     for (int j = 0; j < 4; ++j) a[j] *= inv;
     if (ch.splits == 1) {
       const size_t row = (size_t)ch.b * H + h0 + g;
       *reinterpret_cast<u32x2*>(o + row * D + d) = u32x2{pack2<BF16>(a[0], a[1]), pack2<BF16>(a[2], a[3])};
-      if (lse != nullptr && d == 0) lse[row] = L * kLn2;
+      if (lse != nullptr && d == 0)
+        lse[row] = z == 0.f ? -INFINITY : fmaf(M, c, log2_hw(z) - kShift<BF16>) * kLn2;
     } else {
       const size_t row = (size_t)(h0 + g) * slots + ch.partial;
       *reinterpret_cast<f32x4*>(part_o + row * D + d) = a;
-      if (d == 0) part_l[row] = L;
+      if (d == 0) part_ml[row] = float2{M, z};
     }
   }
 }
@@ -665,9 +672,9 @@ constexpr int kJoinWaves = 4;
 // the groups. One pass, with a running maximum.
 template <int D, bool BF16, int WAVES>
 __global__ void __launch_bounds__(WAVES == 1 ? 2 * D : 64 * kJoinWaves)
-fa_decode_mx_join_kernel(const float* __restrict__ part_o, const float* __restrict__ part_l,
+fa_decode_mx_join_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml,
                          const int32_t* __restrict__ plan, uint16_t* __restrict__ o,
-                         float* __restrict__ lse, int H, int slots) {
+                         float* __restrict__ lse, int H, int slots, float c) {
   constexpr int GROUPS = 8 * WAVES, AHEAD = 4;
   __shared__ __attribute__((aligned(16))) f32x4 sh_a[kJoinWaves][8];
   __shared__ float sh_m[kJoinWaves], sh_z[kJoinWaves];
@@ -677,49 +684,49 @@ fa_decode_mx_join_kernel(const float* __restrict__ part_o, const float* __restri
   const int h = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int d = 32 * (WAVES == 1 ? wave : (int)blockIdx.z) + 4 * (lane & 7);
   const int g = WAVES == 1 ? lane >> 3 : 8 * wave + (lane >> 3);
-  const float* pl = part_l + (size_t)h * slots + first;
+  const float2* pl = part_ml + (size_t)h * slots + first;
   const float* po = part_o + ((size_t)h * slots + first) * D + d;
 
   float m = -INFINITY, z = 0.f;
   f32x4 a = f32x4{};
   for (int i = g; i < n; i += AHEAD * GROUPS) {
-    float x[AHEAD];
+    float2 x[AHEAD];
     f32x4 v[AHEAD];
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
       const int k = min(i + j * GROUPS, n - 1);
-      x[j] = i + j * GROUPS < n ? pl[k] : -INFINITY;
+      x[j] = i + j * GROUPS < n ? pl[k] : float2{-INFINITY, 0.f};
       v[j] = *reinterpret_cast<const f32x4*>(po + (size_t)k * D);
     }
     float top = m;   // finite or, with a NaN to come, -inf: a chunk of a cut sequence has tokens
 #pragma unroll
-    for (int j = 0; j < AHEAD; ++j) top = fmaxf(top, x[j]);
-    const float e = exp2_hw(m - top);
+    for (int j = 0; j < AHEAD; ++j) top = fmaxf(top, x[j].x);
+    const float e = exp2_hw((m - top) * c);
     z *= e;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) a[c] *= e;
+    for (int k = 0; k < 4; ++k) a[k] *= e;
     m = top;
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
-      const float w = exp2_hw(x[j] - m);
+      const float w = x[j].y * exp2_hw((x[j].x - m) * c);
       z += w;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) a[c] = fmaf(w, v[j][c], a[c]);
+      for (int k = 0; k < 4; ++k) a[k] = fmaf(w, v[j][k], a[k]);
     }
   }
   // The groups of the wave, then the waves.
   float M = m;
 #pragma unroll
   for (int k = 8; k < 64; k *= 2) M = fmaxf(M, __shfl_xor(M, k));
-  const float e = m == M ? 1.f : exp2_hw(m - M);   // a group without chunks: m = -inf, its sums 0
+  const float e = m == M ? 1.f : exp2_hw((m - M) * c);   // a group without chunks: m = -inf, its sums 0
   z *= e;
 #pragma unroll
-  for (int c = 0; c < 4; ++c) a[c] *= e;
+  for (int j = 0; j < 4; ++j) a[j] *= e;
 #pragma unroll
   for (int k = 8; k < 64; k *= 2) {
     z += __shfl_xor(z, k);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) a[c] += __shfl_xor(a[c], k);
+    for (int j = 0; j < 4; ++j) a[j] += __shfl_xor(a[j], k);
   }
   if constexpr (WAVES > 1) {
     if (lane < 8) sh_a[wave][lane] = a;
@@ -736,11 +743,11 @@ fa_decode_mx_join_kernel(const float* __restrict__ part_o, const float* __restri
     a = f32x4{};
 #pragma unroll
     for (int w = 0; w < kJoinWaves; ++w) {
-      const float f = sh_m[w] == M ? 1.f : exp2_hw(sh_m[w] - M);
+      const float f = sh_m[w] == M ? 1.f : exp2_hw((sh_m[w] - M) * c);
       const f32x4 v = sh_a[w][lane & 7];
       z = fmaf(f, sh_z[w], z);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) a[c] = fmaf(f, v[c], a[c]);
+      for (int j = 0; j < 4; ++j) a[j] = fmaf(f, v[j], a[j]);
     }
   }
   if (lane >= 8) return;
@@ -748,7 +755,7 @@ fa_decode_mx_join_kernel(const float* __restrict__ part_o, const float* __restri
   const float inv = 1.f / z;
   *reinterpret_cast<u32x2*>(o + row * D + d) =
       u32x2{pack2<BF16>(a[0] * inv, a[1] * inv), pack2<BF16>(a[2] * inv, a[3] * inv)};
-  if (lse != nullptr && d == 0) lse[row] = (M + log2_hw(z)) * kLn2;
+  if (lse != nullptr && d == 0) lse[row] = fmaf(M, c, log2_hw(z) - kShift<BF16>) * kLn2;
 }
 
 template <int D, int KB, int VB, bool BF16>
@@ -760,7 +767,7 @@ static int decode(const void* q, const void* k_pool, const void* v_pool, const i
   const bool one = never_cut(B, H, Hkv, max_pages);
   const Workspace w = workspace_of(B, H, D, most);
   float* part_o = one ? nullptr : workspace + w.part_o;
-  float* part_l = one ? nullptr : workspace + w.part_l;
+  float2* part_ml = one ? nullptr : reinterpret_cast<float2*>(workspace + w.part_ml);
   int32_t* plan = one ? nullptr : reinterpret_cast<int32_t*>(workspace + w.plan);
   int4* table = one || B <= kWavePlan ? nullptr : reinterpret_cast<int4*>(workspace);
   if (table != nullptr) {
@@ -783,7 +790,7 @@ static int decode(const void* q, const void* k_pool, const void* v_pool, const i
                                  : (nt ? fa_decode_mx_kernel<D, KB, VB, BF16, true, 4>
                                        : fa_decode_mx_kernel<D, KB, VB, BF16, false, 4>);
   hipLaunchKernelGGL(kernel, grid, dim3(64 * waves), 0, s, (const uint16_t*)q, (const char*)k_pool,
-                     (const char*)v_pool, page_table, ctx_lens, part_o, part_l, table, plan,
+                     (const char*)v_pool, page_table, ctx_lens, part_o, part_ml, table, plan,
                      (uint16_t*)o, lse, (int)B, (int)H, (int)Hkv, (int)(H / Hkv),
                      (int)(groups / Hkv), (int)max_pages, (int)num_pages, (int)w.slots,
                      plan_of(B, H, Hkv), c);
@@ -793,11 +800,11 @@ static int decode(const void* q, const void* k_pool, const void* v_pool, const i
   const unsigned cut = (unsigned)(B < most ? B : most);
   if (most > kWideJoin * B)
     hipLaunchKernelGGL((fa_decode_mx_join_kernel<D, BF16, kJoinWaves>), dim3(cut, (unsigned)H, D / 32),
-                       dim3(64 * kJoinWaves), 0, s, part_o, part_l, plan, (uint16_t*)o, lse, (int)H,
-                       (int)w.slots);
+                       dim3(64 * kJoinWaves), 0, s, part_o, part_ml, plan, (uint16_t*)o, lse, (int)H,
+                       (int)w.slots, c);
   else
     hipLaunchKernelGGL((fa_decode_mx_join_kernel<D, BF16, 1>), dim3(cut, (unsigned)H), dim3(2 * D), 0,
-                       s, part_o, part_l, plan, (uint16_t*)o, lse, (int)H, (int)w.slots);
+                       s, part_o, part_ml, plan, (uint16_t*)o, lse, (int)H, (int)w.slots, c);
   e = hipGetLastError();
   return e == hipSuccess ? FA_OK : -(int)e;
 }

@@ -540,3 +540,82 @@ def test_rejects_bad_arguments(fa, dev):
     ]:
         with pytest.raises(RuntimeError, match=match):
             call()
+
+
+def _huge_score_case(seed, ctx, D, kb, vb, bf16, b, qs):
+    """Scores far beyond 2^24, as rows of one KV head per b and query heads per (b, a): every value of
+    a K row is b but the first, b f with f of _STEPS; every value of a query is a but the first, which
+    makes the products a b (D - 1) +- 8 f g with g the last place of the product in 32 bits, so that
+    each is a number of 24 bits and any order of its sum is exact. Every seventh column of V is zero."""
+    q, kp, vp, table, ctx = _decode_case(seed, ctx, len(qs) * len(b), len(b), D, kb, vb, bf16)
+    rng = np.random.default_rng(seed)
+    B, n = len(ctx), int(ctx.max())
+    f = rng.choice(_STEPS, (B, 1, n))
+    k = np.broadcast_to(np.asarray(b)[None, :, None, None], (B, len(b), n, D)).copy()
+    k[..., 0] *= f
+    v = mx.to_f64(_rows(rng, (B, len(b), n, D), bf16, 0.5), bf16)
+    v[..., ::7] = 0
+    k16, v16 = mx.from_f64(k, bf16), mx.from_f64(v, bf16)
+    kp, vp, _ = mx.append_mx(kp, vp, table, np.zeros(B, np.int32), k16, v16, kb, vb, bf16, ctx)
+    q = np.zeros((B, len(b) * len(qs), D))
+    units = np.zeros(q.shape[1])   # of a head: its products are base + units f
+    base = np.zeros(q.shape[1])
+    for h in range(q.shape[1]):
+        bh, a = b[h // len(qs)], qs[h % len(qs)]
+        g = 2.0 ** (np.floor(np.log2(D * abs(a) * bh)) - 23)
+        q[:, h], q[:, h, 0] = a, 8 * g / bh * (1 if h % 2 else -1)
+        units[h], base[h] = q[0, h, 0] * bh, a * bh * (D - 1)
+    s = base[None, :, None] + units[None, :, None] * f
+    assert np.array_equal(s.astype(np.float32), s) and np.array_equal(mx.to_f64(mx.from_f64(q, bf16), bf16), q)
+    return (mx.from_f64(q, bf16), kp, vp, table, ctx), s
+
+
+_STEPS = np.array([0, 1, 2, 3, 4, 6, 8, 12]) / 8   # of b: values that both formats hold beside b
+
+
+def _exact_score_result(s, case, kb, vb, bf16):
+    """(O, L, tol_O, tol_L) where the products s are exact. With x_t = (s_t - max) / sqrt(D) log 2
+    exponents, u = 2^-24: a weight 2^x is off by the scale's and the product's rounding (4 u |x|, of
+    log 2), the argument's with the shift of 15 (u (15 + |x|)), and by 2 u of each exponential and u of
+    each product where it is taken in parts (in its wave, up to eight new maxima, waves, chunks):
+    u (4 |x| + 64) in all. Sums and roundings as in oracle.mx.decode_mx; L's scale, logarithm and
+    products are 8 u of it."""
+    q16, kp, vp, table, ctx = case
+    B, H, D = q16.shape
+    Hkv = kp.shape[1]
+    u, half, least = 2.0 ** -24, 2.0 ** -8 if bf16 else 2.0 ** -11, 2.0 ** -134 if bf16 else 2.0 ** -25
+    p_err, step = (2.0 ** -16, 2.0 ** -125) if bf16 else (2.0 ** -11, 2.0 ** -40)
+    O, L = np.zeros((B, H, D)), np.full((B, H), -np.inf)
+    tO, tL = np.zeros((B, H, D)), np.zeros((B, H))
+    for b in range(B):
+        n = int(ctx[b])
+        if n == 0:
+            continue
+        for h in range(H):
+            v = mx.page_values(vp[table[b, :-(-n // 16)], h // (H // Hkv)], D, vb, True).reshape(-1, D)[:n]
+            sh = s[b, h, :n] if s.shape[0] > 1 else s[0, h, :n]
+            m = sh.max()
+            x = (sh - m) / np.sqrt(D) / np.log(2)
+            e = np.exp2(x)
+            p = e / e.sum()
+            rel = p * u * (4 * np.abs(np.maximum(x, -200)) + 64)
+            w = rel.sum() + (n / 16 + 64) * u
+            O[b, h], L[b, h] = p @ v, m / np.sqrt(D) + np.log(e.sum())
+            av = p @ np.abs(v)
+            tO[b, h] = (rel @ np.abs(v) + w * np.abs(O[b, h]) + (n / 16 + 64) * u * av + p_err * av +
+                        step * np.abs(v).sum(0) / e.sum() + half * np.abs(O[b, h]) + least)
+            tL[b, h] = w + 8 * u * abs(L[b, h])
+    return O, L, tO, tL
+
+
+@pytest.mark.parametrize("ctx", [[1], [2, 17, 16, 500], [3000, 33, 1100], [20000]])
+@pytest.mark.parametrize("D,kb,vb,bf16", [(128, 4, 8, False), (64, 8, 4, False), (128, 8, 4, True), (64, 4, 8, True)])
+def test_decode_huge_scores(fa, dev, D, kb, vb, bf16, ctx):
+    """Scores (in units of log 2) of 2^22 to 2^32 in fp16 and 2^14 to 2^90 in bf16, of both signs: the
+    weights follow from the scores' differences, whatever the scores."""
+    b = [1024.0, 2.0 ** 45 if bf16 else 16384.0]
+    qs = [512.0, 1020.0, -2040.0, -2.0 ** 41, 1.5] if bf16 else [512.0, 1023.0, -2047.0, -1024.0, 16384.0]
+    case, s = _huge_score_case(len(ctx) + D, ctx, D, kb, vb, bf16, b, qs)
+    O, L = fa.decode_paged_mx(_rows_to(dev, case[0], bf16), *_to(dev, *case[1:]))
+    _check_decode(O, L, _exact_score_result(s, case, kb, vb, bf16), f"{ctx}")
+    assert (O.view(len(ctx), len(b) * len(qs), D)[..., ::7] == 0).all()
