@@ -151,8 +151,16 @@ static Workspace workspace_of(int64_t B, int64_t H, int64_t D, int64_t most) {
   return w;
 }
 
-// P reaches 2^15 in fp16 rather than 1, so that it keeps all its bits down to
-// 2^-29 of the row's largest (and some to 2^-39); bf16 has fp32's range.
+// P goes into its product as two 16-bit terms, itself rounded and then what that
+// leaves out: 22 bits in fp16, 16 in bf16, beside a sum of P that is not rounded
+// at all. (One fp16 term leaves half a place of 11 bits in each weight: O off by
+// up to six times the rest of its error. The second costs, in us, 1 % of large
+// batches (32 sequences of up to 32768 tokens 398 -> 402, one of 32000 13.0 ->
+// 13.15), 5 % where 16 heads have few pages a wave (one of 131072 over one KV
+// head 13.75 -> 14.45) and 8 % of many short uncut ones (256 of 100 to 900,
+// 16 heads over 4, 13.0 -> 14.0).) In fp16 P reaches 2^15 rather than 1, so that
+// what lies 2^-29 below a row's largest weight still has 11 bits and its rest
+// ends at 2^-39; bf16 has fp32's range.
 template <bool BF16>
 constexpr float kShift = BF16 ? 0.f : 15.f;
 
@@ -346,6 +354,22 @@ __device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f32x4 c) {
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return __builtin_bit_cast(uint32_t, cvt2x<BF16>(a, b));
+}
+
+// What pack2(a, b) = ab leaves out, rounded alike. fp16: a factor of -1 and words
+// that the compiler does not see through make each difference one mixed fma, and
+// keep it from rounding a and b a second time.
+template <bool BF16>
+__device__ __forceinline__ uint32_t rest2(float a, float b, uint32_t ab) {
+  if constexpr (BF16) {
+    return pack2<true>(a - __uint_as_float(ab << 16), b - __uint_as_float(ab & 0xffff0000u));
+  } else {
+    float neg = -1.f;
+    asm("" : "+s"(neg));
+    asm("" : "+v"(ab));
+    const f16x2 h = __builtin_bit_cast(f16x2, ab);
+    return pack2<false>(fmaf((float)h[0], neg, a), fmaf((float)h[1], neg, b));
+  }
 }
 
 // A lane's piece of a page.
@@ -551,7 +575,7 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
         for (int r = 0; r < 4; ++r) acc[db][r] *= alpha;
       m = m_new;
     }
-    u32x2 ph[kBatch], pl[kBatch];   // P as 16-bit operands, and in bf16 what the first leaves out
+    u32x2 ph[kBatch], pl[kBatch];   // P's two terms
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
       float p[4];
@@ -561,20 +585,14 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
         l += p[r];
       }
       ph[i] = u32x2{pack2<BF16>(p[0], p[1]), pack2<BF16>(p[2], p[3])};
-      if constexpr (BF16) {
-        // bf16 keeps 8 bits of P; a second product with the rounded remainder
-        // makes them 16.
-        const auto lo = [](uint32_t x) { return __uint_as_float(x << 16); };
-        const auto hi = [](uint32_t x) { return __uint_as_float(x & 0xffff0000u); };
-        pl[i] = u32x2{pack2<true>(p[0] - lo(ph[i][0]), p[1] - hi(ph[i][0])),
-                      pack2<true>(p[2] - lo(ph[i][1]), p[3] - hi(ph[i][1]))};
-      }
+      pl[i] = u32x2{rest2<BF16>(p[0], p[1], ph[i][0]), rest2<BF16>(p[2], p[3], ph[i][1])};
     }
     // Two pages a product: slots 0 .. 3 of the lane's reduction are tokens
     // 4 grp .. + 3 of the first, slots 4 .. 7 those of the second.
     static_for<0, kBatch / 2>([&](auto half) {
       constexpr int I0 = 2 * half.value;
       const u32x4 bh = u32x4{ph[I0][0], ph[I0][1], ph[I0 + 1][0], ph[I0 + 1][1]};
+      const u32x4 bl = u32x4{pl[I0][0], pl[I0][1], pl[I0 + 1][0], pl[I0 + 1][1]};
       static_for<0, DB / 2>([&](auto qd) {
         u32x4 even, odd;   // values 2 qd and 2 qd + 1 of the lane's sixteenth
         static_for<0, 2>([&](auto j) {
@@ -590,11 +608,8 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
         });
         acc[2 * qd.value] = mma16<BF16>(even, bh, acc[2 * qd.value]);
         acc[2 * qd.value + 1] = mma16<BF16>(odd, bh, acc[2 * qd.value + 1]);
-        if constexpr (BF16) {
-          const u32x4 bl = u32x4{pl[I0][0], pl[I0][1], pl[I0 + 1][0], pl[I0 + 1][1]};
-          acc[2 * qd.value] = mma16<true>(even, bl, acc[2 * qd.value]);
-          acc[2 * qd.value + 1] = mma16<true>(odd, bl, acc[2 * qd.value + 1]);
-        }
+        acc[2 * qd.value] = mma16<BF16>(even, bl, acc[2 * qd.value]);
+        acc[2 * qd.value + 1] = mma16<BF16>(odd, bl, acc[2 * qd.value + 1]);
       });
     });
   }

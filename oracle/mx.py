@@ -192,8 +192,9 @@ def decode_mx(q16, k_pool, v_pool, table, ctx, k_bits, v_bits, bf16, p_top=2.0 *
     """(O, L, tol_O, tol_L) in 64 bits, of valid sequences; q16 uint16 [B, H, D].
 
     tol_O and tol_L bound what a computation with exact 16-bit operands, 32-bit
-    sums and P rounded to fp16 (11 bits) or to two bf16 terms (16 bits) may be
-    off by, with u = 2^-24: the scores by D u sum |q k| / sqrt(D) (their sum)
+    sums and P rounded to two terms of fp16 (22 bits) or of bf16 (16) may be off
+    by (p_top = 1: to one fp16 term, 11 bits, as the 16-bit decode does), with
+    u = 2^-24: the scores by D u sum |q k| / sqrt(D) (their sum)
     and 4 u |s| (scaling, the exponential's argument), which P and so each
     weight take twice (numerator and sum), 16 u of the exponential, and the two
     sums over n tokens by (n / 16 + 64) u each (a lane adds a sixteenth of a
@@ -209,7 +210,7 @@ def decode_mx(q16, k_pool, v_pool, table, ctx, k_bits, v_bits, bf16, p_top=2.0 *
     O, L = np.zeros((B, H, D)), np.full((B, H), -np.inf)
     tO, tL = np.zeros((B, H, D)), np.zeros((B, H))
     u, half = 2.0 ** -24, 2.0 ** -8 if bf16 else 2.0 ** -11
-    p_err = 2.0 ** -16 if bf16 else 2.0 ** -11
+    p_err = 2.0 ** -16 if bf16 else 2.0 ** -11 if p_top == 1 else 2.0 ** -22
     step = 2.0 ** -125 if bf16 else 2.0 ** -25 / p_top
     least = 2.0 ** -134 if bf16 else 2.0 ** -25   # half the type's smallest step
     for b in range(B):

@@ -619,3 +619,31 @@ def test_decode_huge_scores(fa, dev, D, kb, vb, bf16, ctx):
     O, L = fa.decode_paged_mx(_rows_to(dev, case[0], bf16), *_to(dev, *case[1:]))
     _check_decode(O, L, _exact_score_result(s, case, kb, vb, bf16), f"{ctx}")
     assert (O.view(len(ctx), len(b) * len(qs), D)[..., ::7] == 0).all()
+
+
+@pytest.mark.parametrize("D,vb,ctx", [(64, 4, 1), (64, 8, 2), (128, 8, 3), (128, 4, 40), (64, 8, 1500)])
+def test_decode_weights_keep_32_bits_in_fp16(fa, dev, D, vb, ctx):
+    """V of 1 and -1 in nearly equal weights: O is the small rest of a difference, which half a place
+    of an 11-bit weight would show. With the scores' exponents below 2 (|q k| / sqrt(D) log 2), P's two
+    terms (2^-22), 16 u of an exponential, D u of a score and the sums' (n / 16 + 64) u, twice each,
+    O is off by that and by its own rounding (2^-11)."""
+    rng = np.random.default_rng(D + ctx)
+    H, n = 8, -(-ctx // 16) * 16
+    kc, ks = rng.integers(0, 16, (n // 16, 1, 16, D)).astype(np.uint8), np.full((n // 16, 1, 16, D // 32), 127, np.uint8)
+    vc = np.zeros((n // 16, 1, 16, D), np.uint8)
+    one = 2 if vb == 4 else 0x38
+    vc[:] = np.where(np.arange(n).reshape(-1, 1, 16, 1) % 2, one, one | (8 if vb == 4 else 128))
+    kp, vp = mx.pack_pages(kc, ks, 4, False), mx.pack_pages(vc, ks, vb, True)
+    q = mx.from_f64(rng.standard_normal((1, H, D)) * 0.1, False)
+    table, c = np.arange(n // 16, dtype=np.int32)[None], np.array([ctx], np.int32)
+    O, L = fa.decode_paged_mx(_rows_to(dev, q, False), *_to(dev, kp, vp, table, c))
+    k = mx.page_values(kp[:, 0], D, 4, False).reshape(-1, D)[:ctx]
+    s = k @ mx.to_f64(q[0], False).T / np.sqrt(D)
+    mag = (np.abs(k) @ np.abs(mx.to_f64(q[0], False)).T).max() / np.sqrt(D)
+    e = np.exp(s - s.max(0))
+    v = mx.page_values(vp[:, 0], D, vb, True).reshape(-1, D)[:ctx, :1]
+    want = (e * v).sum(0) / e.sum(0)
+    u = 2.0 ** -24
+    tol = 2.0 ** -22 + 2 * (16 + D * mag + 4 * np.abs(s).max() + n / 16 + 64) * u + 2.0 ** -11 * np.abs(want) + 2.0 ** -25
+    err = np.abs(O[0].double().cpu().numpy() - want[:, None])
+    assert (err <= tol[:, None]).all(), f"off by {(err / tol[:, None]).max():.2f} of the bound"
