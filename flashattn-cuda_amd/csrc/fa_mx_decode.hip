@@ -829,8 +829,11 @@ static int decode(const void* q, const void* k_pool, const void* v_pool, const i
 
 extern "C" int64_t fa_decode_mx_workspace_floats(int64_t B, int64_t H, int64_t H_kv, int64_t D,
                                                  int64_t max_pages) {
-  if (B <= 0 || H <= 0 || H_kv <= 0 || H % H_kv != 0 || D <= 0 || max_pages <= 0 ||
-      B > ((int64_t(1) << 31) - 1) / max_pages)
+  // the sizes that fa_validate_decode_mx refuses
+  constexpr int64_t kIndexes = (int64_t(1) << 31) - 1;
+  if (B <= 0 || B > 65535 || H <= 0 || H > 65535 || H_kv <= 0 || H % H_kv != 0 ||
+      (D != 64 && D != 128) || max_pages <= 0 || max_pages > kIndexes / fa::mx::kTokens ||
+      B > kIndexes / max_pages)
     return 0;
   if (fa::mx::never_cut(B, H, H_kv, max_pages)) return 0;
   return fa::mx::workspace_of(B, H, D, fa::mx::most_chunks(B, H, H_kv, max_pages)).words;

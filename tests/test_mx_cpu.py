@@ -187,3 +187,13 @@ def test_chunk_plan_fits_its_grid(capi):
         assert sum(cuts) <= most.value + min(B, most.value) < 1 << 15 and len(cuts) <= min(B, most.value)
         assert (lib.fa_decode_mx_workspace_floats(B, H, Hkv, 64, maxp) > 0) == (most.value > 0)
     assert lib.fa_probe_mx_chunks(1, 4, 3, 10, 5, None) == lib.fa_probe_mx_chunks(1, 4, 4, 10, 11, None) == 0
+
+
+@pytest.mark.parametrize("kw", [dict(B=0), dict(B=65536), dict(H=0), dict(H=65544), dict(Hkv=0), dict(Hkv=5), dict(D=96),
+                                dict(D=32), dict(D=0), dict(maxp=0), dict(maxp=1 << 27), dict(B=65535, maxp=1 << 20)])
+def test_no_workspace_for_sizes_that_are_refused(capi, kw):
+    lib = capi.load()
+    a = _dec(**kw)
+    B, H, Hkv, D, maxp = a[5], a[6], a[7], a[8], a[12]
+    assert lib.fa_validate_decode_mx(*a) != capi.STATUS["FA_OK"]
+    assert lib.fa_decode_mx_workspace_floats(B, H, Hkv, D, maxp) == 0
