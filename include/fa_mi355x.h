@@ -466,8 +466,9 @@ int fa_kv_append_mx(const void* k_new, const void* v_new, const int32_t* page_ta
 
 /*
  * Tokens start_pos[b] .. + T of each sequence out of MX pages into k, v (fp16,
- * bf16 != 0: bfloat16, [B, H, T, D]), exactly (a value beyond the type's range,
- * which rows of that type do not leave in a page, is infinite). Rows from
+ * bf16 != 0: bfloat16, [B, H, T, D]), exactly. (Of values that rows of that type
+ * do not leave in a page, one beyond the type's range is infinite and one between
+ * two of its subnormal numbers goes to the nearest, a tie to the even.) Rows from
  * lens[b] (clamped to [0, T]; NULL: T) on are zeros. A token whose position is
  * outside the table or whose page id is outside [0, num_pages) reads as NaN and
  * sets bad[b] to 1; every other bad[b] is set to 0.

@@ -647,3 +647,65 @@ def test_decode_weights_keep_32_bits_in_fp16(fa, dev, D, vb, ctx):
     tol = 2.0 ** -22 + 2 * (16 + D * mag + 4 * np.abs(s).max() + n / 16 + 64) * u + 2.0 ** -11 * np.abs(want) + 2.0 ** -25
     err = np.abs(O[0].double().cpu().numpy() - want[:, None])
     assert (err <= tol[:, None]).all(), f"off by {(err / tol[:, None]).max():.2f} of the bound"
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("bf16", [False, True])
+def test_read_of_every_code_and_scale(fa, dev, bf16, D):
+    """Every code under every scale, 0 and 255 among them: exact where the type has the value, to
+    nearest even where it lies between two of the type's subnormals, infinite past its range."""
+    rng = np.random.default_rng(D)
+    blocks = {4: np.tile(np.arange(32) % 16, (256 * 8, 1)), 8: np.tile(np.arange(256).reshape(8, 32), (256, 1))}
+    order = rng.permutation(256 * 8)   # neighbouring scales differ
+    scales = np.repeat(np.arange(256), 8)[order].reshape(-1, 1, 16, D // 32).astype(np.uint8)
+    P = len(scales)
+    table = np.arange(P, dtype=np.int32)[None]
+    for kb, vb in ((4, 8), (8, 4)):
+        codes = {n: blocks[n][order].reshape(P, 1, 16, D).astype(np.uint8) for n in (4, 8)}
+        kp, vp = mx.pack_pages(codes[kb], scales, kb, False), mx.pack_pages(codes[vb], scales, vb, True)
+        k, v, bad = fa.kv_read_mx(*_to(dev, kp, vp, table, np.zeros(1, np.int32)), 16 * P, dtype=TYPES[bf16])
+        assert not bad.any()
+        inf = 0x7f80 if bf16 else 0x7c00
+        for got, bits in ((k, kb), (v, vb)):
+            w = mx.from_f64(mx.dequantize(codes[bits], scales, bits).reshape(1, 1, -1, D), bf16)
+            g = _bits(got)
+            same = (g == w) | (((g & 0x7fff) > inf) & ((w & 0x7fff) > inf))
+            assert same.all(), f"{bits} bits: {(~same).sum()} differ"
+
+
+@pytest.mark.parametrize("vb", [4, 8])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("bf16", [False, True])
+def test_decode_of_every_value_code_and_scale(fa, dev, bf16, D, vb):
+    """One token of a page has all the weight, at each of a lane's four places; the other 15 hold zeros
+    under other scales. O is that token's V row: every code under every scale whose values the type
+    has, and scale 255. The weight is one up to 2^-22, the values have four bits: O is the value."""
+    rng = np.random.default_rng(D + vb)
+    per = 1 if vb == 4 else 8
+    codes = np.tile((np.arange(32) % 16)[None] if vb == 4 else np.arange(256).reshape(8, 32), (256, 1))
+    scales = np.repeat(np.arange(256), per)
+    val = mx.dequantize(codes.astype(np.uint8), scales[:, None].astype(np.uint8), vb)
+    back = mx.to_f64(mx.from_f64(val, bf16), bf16)
+    has = np.where(scales == 255, True, ((back == val) | np.isnan(val)).all(1))
+    codes, scales = codes[has], scales[has]
+    nb = D // 32
+    n = -(-len(scales) // nb) * nb
+    pick = np.concatenate([rng.permutation(len(scales)), np.arange(n - len(scales))])
+    rows, rs = codes[pick].reshape(-1, D), scales[pick].reshape(-1, nb)
+    rows, rs = np.tile(rows, (4, 1)), np.tile(rs, (4, 1))
+    B = len(rows)
+    slot = 4 * rng.integers(0, 4, B) + np.repeat(np.arange(4), B // 4)
+    vc, vs = np.zeros((B, 1, 16, D), np.uint8), rng.integers(0, 255, (B, 1, 16, nb)).astype(np.uint8)
+    vc[np.arange(B), 0, slot], vs[np.arange(B), 0, slot] = rows, rs
+    kc, ks = np.zeros((B, 1, 16, D), np.uint8), np.full((B, 1, 16, nb), 127, np.uint8)
+    kc[np.arange(B), 0, slot, 0] = 7   # 6: its score is 6000 / sqrt(D) above the others'
+    q = np.zeros((B, 1, D))
+    q[..., 0] = 1000
+    kp, vp = mx.pack_pages(kc, ks, 4, False), mx.pack_pages(vc, vs, vb, True)
+    O, _ = fa.decode_paged_mx(_rows_to(dev, mx.from_f64(q, bf16), bf16),
+                              *_to(dev, kp, vp, np.arange(B, dtype=np.int32)[:, None].copy(), np.full(B, 16, np.int32)))
+    w = mx.dequantize(rows.astype(np.uint8), rs.astype(np.uint8), vb)
+    g = mx.to_f64(_bits(O)[:, 0], bf16)
+    same = (g == w) | (np.isnan(g) & np.isnan(w))
+    i = np.argwhere(~same)
+    assert same.all(), f"{len(i)} differ, of scales {sorted(set(rs[i[:, 0], i[:, 1] // 32]))[:9]}, {g[~same][:4]} {w[~same][:4]}"
