@@ -197,3 +197,16 @@ def test_no_workspace_for_sizes_that_are_refused(capi, kw):
     B, H, Hkv, D, maxp = a[5], a[6], a[7], a[8], a[12]
     assert lib.fa_validate_decode_mx(*a) != capi.STATUS["FA_OK"]
     assert lib.fa_decode_mx_workspace_floats(B, H, Hkv, D, maxp) == 0
+
+
+@pytest.mark.parametrize("bits,bf16", [(b, t) for b in BITS for t in (False, True)])
+def test_quantised_rows_are_fixed_points(bits, bf16):
+    """What a page holds, quantised again, has the same codes under the same scales: a block's largest
+    value stays above half the scale's limit where a smaller scale could be taken."""
+    x = np.arange(65536, dtype=np.uint32).astype(np.uint16)
+    x = x[np.isfinite(mx.to_f64(x, bf16))]
+    rng = np.random.default_rng(2)
+    x = np.concatenate([x[:len(x) // 64 * 64], rng.permutation(x)[:len(x) // 64 * 64]]).reshape(-1, 64)
+    codes, scales = mx.quantize(x, bits, bf16)
+    again, scales2 = mx.quantize(mx.from_f64(mx.dequantize(codes, scales, bits), bf16), bits, bf16)
+    assert np.array_equal(again, codes) and np.array_equal(scales2, scales)
