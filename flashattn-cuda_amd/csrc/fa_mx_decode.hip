@@ -57,9 +57,7 @@ constexpr int kBatchOf = Page<D, KB>::PIECE + Page<D, VB>::PIECE <= 32 ? 4 : 2;
 // kFill is the four workgroups that a CU holds; chunks past kMaxChunk pages are
 // cut for balance, at little cost. Besides, at most kRowFill chunks a sequence
 // (one of 131072 tokens over one KV head: 20.7 us in 512 chunks, 16.0 in 256,
-// 17.9 in 128), and where there are about as many sequences as chunks wanted,
-// only those of twice the mean length are cut (256 of 100 to 900 tokens over 4
-// KV heads: 20 -> 15.4 us).
+// 17.9 in 128).
 //
 // kMinChunk is a batch of four pages for each wave. Joining chunks costs a second
 // launch, 4 us: it is not made, and nothing is cut, for tables of up to
@@ -74,9 +72,10 @@ constexpr int kOnePages = 32;
 constexpr int kRowFill = 256;
 
 // Sequences up to which every wave finds its chunk by itself, a lane for up to
-// four of them; more are planned by a launch of their own, whose 8 us do not
-// show beside the work of so many (4096 sequences of about 300 tokens over 8 KV
-// heads, planned by every workgroup 752 us, 306 by none).
+// four of them; more are planned by a launch of their own. In a table of 512
+// pages, sequences of 50 to 300 tokens: over 8 KV heads (D = 128) 257 take 24.5
+// us so and 34.8 planned by the waves with 16 a lane, 1024 take 69 and 137; over
+// one (D = 64) 257 take 9.5 and 9.2 (256 with four a lane 7.6), 1024 16 and 46.
 constexpr int kWavePlan = 256;
 
 // Chunks a sequence from which the join gives a row a workgroup for each 32
@@ -100,7 +99,6 @@ static Plan plan_of(int64_t B, int64_t H, int64_t Hkv) {
   const int64_t g = head_groups(H, Hkv);
   int64_t fill = (kFill + g - 1) / g;
   if (fill > kRowFill * B) fill = kRowFill * B;
-  if (B >= fill && 3 * B < 4 * fill) fill = 3 * B / 4 > 0 ? 3 * B / 4 : 1;
   const unsigned least = B * g >= kFill / 4 ? kMinFull : kMinChunk;
   return {(unsigned)fill, (unsigned)((kMost + g - 1) / g), least};
 }
