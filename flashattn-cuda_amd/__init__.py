@@ -182,6 +182,9 @@ def decode_paged_mx(q, k_pool, v_pool, page_table, ctx_lens):
     """[O, L] of one query token per sequence over its MX pages (decode_paged's
     results for what the pages hold); q fp16 or bf16, O in q's dtype, L fp32.
 
+    q has the dtype of the rows that were appended, which no call can check:
+    values of bf16 rows may lie beyond fp16's range.
+
     The split over the pages follows the batch's lengths, on the device.
     """
     return _C.decode_paged_mx(q, k_pool, v_pool, page_table, ctx_lens)

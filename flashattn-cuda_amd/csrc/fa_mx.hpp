@@ -109,10 +109,12 @@ __device__ __forceinline__ uint32_t values2(uint32_t w, float scale) {
 
 // The scale code of a block whose largest magnitude is a (finite): the
 // smallest s >= 1 with a <= lim 2^(s - 127), lim = 7 = 1.75 2^2 or
-// 464 = 1.8125 2^8, the largest value that rounds to the format's largest (6,
-// 448) and not past it. The fraction of a above that of lim carries into the
-// exponent. At most the code for which the format's largest value is finite in
-// the rows' type: values past it saturate.
+// 464 = 1.8125 2^8, half a step past the format's largest (6, 448), to which
+// values up to there go (464 by its tie, 7 by saturation: its tie is 8). The
+// fraction of a above that of lim carries into the exponent. At most the code
+// for which the format's largest value is finite in the rows' type: values past
+// it saturate, which leaves them more than half a step off (of fp16 rows 65504
+// becomes 49152 in 4 bits, 57344 in 8).
 template <int BITS, bool BF16>
 __device__ __forceinline__ int scale_code(float a) {
   constexpr uint32_t carry = BITS == 4 ? 0x7fffffu - 0x600000u : 0x7fffffu - 0x680000u;

@@ -13,6 +13,7 @@
 //   S   = K Q^T     (16x16x32: 16 tokens x 16 heads; heads past the group are zero columns)
 //   O^T += V^T P^T  (16x16x32 over two pages: rows c of block db are values
 //                    c D/16 + db, P^T straight from the S accumulators)
+// P^T goes in as two terms, so V's product is made twice.
 // Lane l has head l % 16 in both products, so a head's maximum and sum stay in
 // its lane column.
 //
@@ -38,8 +39,9 @@ constexpr int kXcds = 8;
 // Pages that a wave takes at a time: their loads are in flight together. Four
 // of up to 32 code bytes a lane (K and V), two of larger ones, whose registers
 // would leave three waves a SIMD and not four (K8V4 at D = 128 bf16, 24
-// sequences: 57.3 us with two, 57.9 with four; 4 bits, one sequence of 131072
-// tokens over one KV head: 14.7 and 13.9).
+// sequences: 57.4 us with two, 58.2 with four; 4 bits, one sequence of 131072
+// tokens over one KV head: 15.1 and 14.5). Times here are of the launches of one
+// call in a captured graph; a call from the outside adds the host's.
 template <int D, int KB, int VB>
 constexpr int kBatchOf = Page<D, KB>::PIECE + Page<D, VB>::PIECE <= 32 ? 4 : 2;
 
@@ -56,16 +58,19 @@ constexpr int kBatchOf = Page<D, KB>::PIECE + Page<D, VB>::PIECE <= 32 ? 4 : 2;
 //   then kMaxChunk pages, until they make kMost workgroups.
 // kFill is the four workgroups that a CU holds; chunks past kMaxChunk pages are
 // cut for balance, at little cost. Besides, at most kRowFill chunks a sequence
-// (one of 131072 tokens over one KV head: 20.7 us in 512 chunks, 16.0 in 256,
-// 17.9 in 128).
+// (one of 131072 tokens over one KV head, in 512, 256 and 128 chunks: 12.9, 11.8
+// and 12.9 us for 8 query heads, 17.6, 14.4 and 13.8 for 32).
 //
 // kMinChunk is a batch of four pages for each wave. Joining chunks costs a second
 // launch, 4 us: it is not made, and nothing is cut, for tables of up to
-// kOnePages pages (one sequence of 512 tokens 7.0 -> 5.3 us, 8 of them 8.2 ->
-// 6.3; at 768 tokens one sequence is faster cut, 7.0 and 7.4) or where no table
-// entry could make a second chunk (kMinFull: 32 sequences of 768 tokens over 8
-// KV heads 12.8 -> 9.6 us, of 2048 21.3 -> 20.8; under 256 workgroups it costs:
-// 8 sequences of 1024, 9.2 and 10.3).
+// kOnePages pages (one sequence of 512 tokens 7.0 -> 5.0 us, 8 of them 7.9 ->
+// 5.2; at 768 tokens one sequence is faster cut, 6.9 and 7.3, 8 are not, 8.0 and
+// 7.9) or where no table entry could make a second chunk (kMinFull: 32 sequences
+// of 768 tokens over 8 KV heads 12.8 -> 9.6 us, of 2048 20.8 -> 16.3; with fewer
+// than 256 workgroups 8 sequences of 1024 would gain, 8.7 -> 8.0, 8 of 2048 lose,
+// 10.9 -> 12.3). Both go by the table, which alone the host knows: a short context
+// in a wide table pays the second launch (one of 130 tokens 3.4 us in a table of 9
+// pages, 5.2 in one of 2048).
 constexpr int kFill = 1024, kMost = 4096;
 constexpr int kMinChunk = 16, kMaxChunk = 128, kMinFull = 96;
 constexpr int kOnePages = 32;
@@ -79,14 +84,19 @@ constexpr int kRowFill = 256;
 constexpr int kWavePlan = 256;
 
 // Chunks a sequence from which the join gives a row a workgroup for each 32
-// columns (one sequence over one KV head, 256 chunks: 16.5 -> 13.5 us; 8
-// sequences of 8 chunks 12.85 and 13.2).
+// columns (one sequence over one KV head, 256 chunks: 17.9 -> 14.5 us; two
+// sequences of 63 chunks 14.1 -> 13.7; four of 32 13.6 and 13.9, eight of 8 10.85
+// and 11.2).
 constexpr int kWideJoin = 48;
 
 // Pools from this size on do not stay in the caches between two steps; their
-// codes are read with the non-temporal hint (2.5 GB: 440 -> 390 us, 300 MB: 64
-// -> 59; 35 MB, which do stay: 14.5 -> 16.0). Scales are read without it:
-// their lines are shared with the codes' ends and with the next page's.
+// codes are read with the non-temporal hint. Of four batches in turn, each the
+// whole of its pools: 2.5 GB 452 -> 404 us, 299 MB 64.7 -> 57.4, 165 MB 39.8 ->
+// 36.2, 131 MB 33.5 -> 31.6, 65 MB 18.4 -> 19.8, 35 MB 13.3 -> 14.0. The rule goes
+// by the pools, as a step reads other layers' between two of this one; a small
+// batch in large pools that is read again at once loses by it (35 MB in 4 GB 12.0
+// -> 12.3 us, 165 MB 33.3 -> 36.4). Scales are read without the hint: their lines
+// are shared with the codes' ends and with the next page's.
 constexpr int64_t kPassThrough = 64 << 20;
 
 static int64_t head_groups(int64_t H, int64_t Hkv) { return Hkv * ((H / Hkv + 15) / 16); }
@@ -179,7 +189,7 @@ __device__ __forceinline__ int pages_of(int ctx, int max_pages) {
 // sequences (<< 16) and of their chunks, which are fewer than 2 kMost. p / C to
 // the nearest, so that none is longer or shorter than C by half; of kMinChunk
 // pages not to the nearest but up, as a longer one takes its waves a second
-// batch (8 sequences of 200 to 4000 tokens 12.8 -> 11.8 us).
+// batch (8 sequences of 200 to 4000 tokens 13.1 -> 12.2 us).
 __device__ __forceinline__ int chunks_of(int p, int C, int* cut) {
   const unsigned c = (unsigned)C, up = C == kMinChunk ? 2 * c - 1 : c;
   const int s = max(1, (int)((2u * (unsigned)p + up) / (2u * c)));
@@ -491,9 +501,8 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
   // Pages w .. + kBatch - 1, all loads at once; past the wave's last page they
   // repeat it (masked below). Four waves a SIMD hide each other's waits: a
   // second set of registers, loaded one batch ahead, leaves three and measured
-  // slower (32 sequences of up to 32768 tokens 402 us, 398 without; one of
-  // 32000 14.0 and 13.0), and so did loading K and V each as soon as their
-  // registers are free (409 and 14.2, when it was 384 and 13.2 without).
+  // slower (32 sequences of up to 32768 tokens by 1 %, one of 32000 by 8), and so
+  // did loading K and V each as soon as their registers are free (6 and 8 %).
   int ids = 0;   // lane i: id of the wave's page 64 j + i
   Batch<D, KB, VB> x;
   const auto load_ids = [&](int w) { ids = pt[min(w + lane, w1 - 1)]; };
@@ -793,9 +802,9 @@ static int decode(const void* q, const void* k_pool, const void* v_pool, const i
                   (unsigned)chunk_rows(B, one ? 0 : most));
   const bool nt = num_pages * Hkv * (Page<D, KB>::BYTES + Page<D, VB>::BYTES) >= kPassThrough;
   // Eight waves where nothing is cut and a CU has one workgroup at most (32
-  // sequences of 2048 tokens over 8 KV heads 20.5 -> 16.7 us, 8 of 512 6.3 ->
-  // 6.0; four where there are more: 32 of 768 over 32 heads 15.3 and 20.8) or
-  // where four take a batch each (one of 130 tokens, D = 64: 3.5 and 4.4).
+  // sequences of 2048 tokens over 8 KV heads 20.5 -> 16.3 us, 8 of 512 5.3 ->
+  // 5.2); four where there are more (32 of 768 over 32 heads, D = 64: 12.7 and
+  // 17.0) or where four take a batch each (one of 130 tokens, D = 64: 3.4 and 4.3).
   const int64_t groups = head_groups(H, Hkv);
   const int waves = one && max_pages > kMinChunk && B * groups <= kFill / 4 ? 8 : 4;
   const auto kernel = waves == 8 ? (nt ? fa_decode_mx_kernel<D, KB, VB, BF16, true, 8>

@@ -28,11 +28,15 @@ using pages::kThreads;
 template <int D>
 constexpr int kRows = kThreads / (D / 8);
 
-// Rows read back of this size and more are written past the caches: alone 134
-// MB take 33.6 -> 23.2 us and 131 MB of one sequence 35.9 -> 25.5; with a kernel
-// after it that reads them all 61.8 -> 61.6 and 63.7 -> 65.0, as those then
-// come from memory. Smaller ones are left where their reader finds them (65 MB
-// alone 19.7 -> 12.7, with that kernel 33.3 -> 35.9).
+// Rows read back of this size and more are written past the caches. The read
+// alone is faster by it at any size; a kernel after it that reads all rows at once
+// then finds them in memory and is slower by as much or more, until they outgrow
+// the caches (us, alone and with that kernel, one sequence over 8 heads, D = 128:
+//   65 MB 19.4 -> 14.0, 33.1 -> 35.2;  102 MB 28.6 -> 20.4, 49.1 -> 51.7;
+//   131 MB 35.5 -> 25.5, 63.6 -> 64.5; 205 MB 53.6 -> 38.4, 101.3 -> 104.3;
+//   262 MB, two sequences, 63.4 -> 45.7, 138.7 -> 126.0).
+// So a caller gains where more than a pass over memory comes between, or from
+// 256 MB on; smaller rows are left where their reader finds them.
 constexpr int64_t kPassThrough = 100 << 20;
 
 // Workgroups along a sequence that cover T tokens from any position: whole
@@ -209,7 +213,7 @@ fa_kv_append_mx_kernel(const u32x4* __restrict__ k_new, const u32x4* __restrict_
 
 // NT: the rows are written with the non-temporal hint, and the heads of a page
 // are read one after the other (16 heads of 4 x 4096 tokens with the hint alone
-// 31.4 us, 24.3 so).
+// 31.4 us, with the order alone 31.9, with both 23.0).
 template <int D, int KB, int VB, bool BF16, bool NT>
 __global__ void __launch_bounds__(kThreads)
 fa_kv_read_mx_kernel(const char* __restrict__ k_pool, const char* __restrict__ v_pool,

@@ -493,13 +493,15 @@ int64_t fa_decode_mx_workspace_floats(int64_t B, int64_t H, int64_t H_kv, int64_
 /*
  * The paged decode over MX pages: q, o fp16 (bf16 != 0: bfloat16) [B, H, D],
  * lse fp32 [B, H] or NULL, query head h reads pool head h / (H / H_kv). Results
- * as fa_decode_paged_gqa_f16 over what the pages hold: o = 0 and lse = -inf of
- * an empty context; a page id outside [0, num_pages), a negative length or one
- * beyond max_pages * 16 make the sequence's o and lse NaN, and no memory outside the pools
- * is read. How the pages are shared out follows from the lengths of the whole
- * batch, so a sequence's last bits may depend on the others' lengths; the same
- * call gives the same bits. workspace: 16-byte aligned, of the caller, need not
- * be cleared (NULL where none is needed); calls that may overlap need one each.
+ * as fa_decode_paged_gqa_f16 over what the pages hold: o = 0 and lse = -inf of an
+ * empty context; a page id outside [0, num_pages), a negative length or one beyond
+ * max_pages * 16 make the sequence's o and lse NaN, and no memory outside the pools
+ * is read. q is of the type of the rows that were written, which nothing in a page
+ * tells: over values that fp16 does not have o is infinite or NaN. How the pages
+ * are shared out follows from the lengths of the whole batch, so a sequence's last
+ * bits may depend on the others' lengths; the same call gives the same bits.
+ * workspace: 16-byte aligned, of the caller, need not be cleared (NULL where none
+ * is needed); calls that may overlap need one each.
  */
 int fa_decode_paged_mx(const void* q, const void* k_pool, const void* v_pool,
                        const int32_t* page_table, const int32_t* ctx_lens, int64_t B, int64_t H,

@@ -14,7 +14,7 @@ from __future__ import annotations
 import numpy as np
 
 PAGE = 16
-LIM = {4: 7.0, 8: 464.0}     # the largest value that rounds to the format's largest
+LIM = {4: 7.0, 8: 464.0}     # half a step past the format's largest, to which values up to there go
 TOP = {(4, False): 140, (4, True): 252, (8, False): 134, (8, True): 246}   # largest scale code, by (bits, bf16)
 
 
