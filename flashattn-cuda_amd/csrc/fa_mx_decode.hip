@@ -172,6 +172,14 @@ static Workspace workspace_of(int64_t B, int64_t H, int64_t D, int64_t most) {
 template <bool BF16>
 constexpr float kShift = BF16 ? 0.f : 15.f;
 
+// A chunk's sum as the join takes it for its weight: of n tokens the weights add
+// up to n 2^-12, less than a chunk's tokens in any context, so no value whose
+// chunk's own sums are in range leaves it there, and none near the range's lower
+// end either. Exact: powers of two, and a sum is 2^kShift at least.
+template <bool BF16>
+constexpr float kPartScale = BF16 ? 0x1p-12f : 0x1p-27f;
+constexpr float kJoinScale = 0x1p12f;   // of the joined weights: back to sums of exponentials
+
 // What a workgroup's chunk is.
 struct Chunk {
   int b, ctx;           // sequence, -1: none; its length
@@ -681,7 +689,7 @@ fa_decode_mx_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_p
     } else {
       const size_t row = (size_t)(h0 + g) * slots + ch.partial;
       *reinterpret_cast<f32x4*>(part_o + row * D + d) = a;
-      if (d == 0) part_ml[row] = float2{M, z};
+      if (d == 0) part_ml[row] = float2{M, z * kPartScale<BF16>};
     }
   }
 }
@@ -777,7 +785,7 @@ fa_decode_mx_join_kernel(const float* __restrict__ part_o, const float2* __restr
   const float inv = 1.f / z;
   *reinterpret_cast<u32x2*>(o + row * D + d) =
       u32x2{pack2<BF16>(a[0] * inv, a[1] * inv), pack2<BF16>(a[2] * inv, a[3] * inv)};
-  if (lse != nullptr && d == 0) lse[row] = fmaf(M, c, log2_hw(z) - kShift<BF16>) * kLn2;
+  if (lse != nullptr && d == 0) lse[row] = fmaf(M, c, log2_hw(z * kJoinScale)) * kLn2;
 }
 
 template <int D, int KB, int VB, bool BF16>

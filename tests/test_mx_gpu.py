@@ -709,3 +709,21 @@ def test_decode_of_every_value_code_and_scale(fa, dev, bf16, D, vb):
     same = (g == w) | (np.isnan(g) & np.isnan(w))
     i = np.argwhere(~same)
     assert same.all(), f"{len(i)} differ, of scales {sorted(set(rs[i[:, 0], i[:, 1] // 32]))[:9]}, {g[~same][:4]} {w[~same][:4]}"
+
+
+@pytest.mark.parametrize("top", [118, -118])
+@pytest.mark.parametrize("H,Hkv,ctx", [(4, 1, [20000]), (8, 8, [3000, 700, 40])])
+def test_decode_joins_the_range_of_bf16(fa, dev, H, Hkv, ctx, top):
+    """V of 2^118 and of 2^-118 in equal weights over many chunks: a chunk's sums stay in range, and so
+    must the joined ones, which are as many times larger as there are tokens. O is V, of one bit, with
+    equal weights that the sums leave (n / 16 + 64) u off, twice, below half a place of O."""
+    D, kb, vb = 64, 4, 8
+    q, kp, vp, table, c = _decode_case(3, ctx, H, Hkv, D, kb, vb, True)
+    B, n = len(ctx), max(ctx)
+    k = np.zeros((B, Hkv, n, D))
+    v = np.broadcast_to(2.0 ** top * np.where(np.arange(D) % 3 == 0, -1, 1), k.shape)
+    kp, vp, _ = mx.append_mx(kp, vp, table, np.zeros(B, np.int32), mx.from_f64(k, True), mx.from_f64(v, True), kb, vb, True, c)
+    O, L = fa.decode_paged_mx(_rows_to(dev, q, True), *_to(dev, kp, vp, table, c))
+    assert np.array_equal(mx.to_f64(_bits(O), True), np.broadcast_to(v[:1, :1, 0], O.shape))
+    want = np.log(c.astype(np.float64))[:, None]
+    assert (np.abs(L.double().cpu().numpy() - want) <= (n / 16 + 64) * 2.0 ** -24 + 2.0 ** -21 * want).all()
