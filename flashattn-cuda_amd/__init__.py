@@ -26,6 +26,17 @@ The same cache in 4 or 8 bits a value (MX pages, K and V each of its own width):
     k, v, bad = kv_read_mx(k_pool, v_pool, page_table, start_pos, num_tokens)
     O, L = decode_paged_mx(q, k_pool, v_pool, page_table, ctx_lens)
 
+Rotary positions, a prefix shared by a batch, and a cache kept within a budget:
+
+    freqs, scale = rope_frequencies(rot_dim, base=10000.0)
+    Qr, Kr = rope(Q, K, freqs, positions)
+    dQ, dK = rope_backward(dQr, dKr, freqs, positions)
+    q, bad = kv_append_rope(q, k_new, v_new, k_pool, v_pool, page_table, start_pos, freqs)
+    O, L = decode_shared(q, k_pool, v_pool, prefix_table, prefix_len, page_table, ctx_lens)
+    O, L, weights = decode_paged_weights(q, k_pool, v_pool, page_table, ctx_lens, weights)
+    kept, weights, lens, bad = kv_evict(k_pool, v_pool, page_table, ctx_lens, weights,
+                                        new_page_table, keep, recent)
+
 Every call runs the hand-written HIP kernels of ``libfa_mi355x.so`` through
 the C ABI in include/fa_mi355x.h. There is no fallback: importing this package
 without the built extension raises ImportError.
@@ -34,6 +45,7 @@ from __future__ import annotations
 
 import importlib.machinery
 import importlib.util
+import math
 import os
 import pathlib
 import sysconfig
@@ -188,6 +200,134 @@ def decode_paged_mx(q, k_pool, v_pool, page_table, ctx_lens):
     The split over the pages follows the batch's lengths, on the device.
     """
     return _C.decode_paged_mx(q, k_pool, v_pool, page_table, ctx_lens)
+
+
+def rope_frequencies(rot_dim: int, base: float = 10000.0, scaling=None, factor: float = 1.0,
+                     original_len: int = 0, slow_turns: float = 1.0, fast_turns: float = 32.0,
+                     device="cuda"):
+    """(freqs, scale) for rope(): freqs float64 [rot_dim / 2], radians a position.
+
+    freqs[i] = base ** (-2 i / rot_dim), and for contexts `factor` times as long as
+    the original_len positions that a model was trained on, by `scaling`:
+
+      None        as they are
+      "linear"    all divided by factor (positions interpolated)
+      "ntk"       base * factor ** (rot_dim / (rot_dim - 2)): the slowest is divided
+                  by factor, the fastest kept
+      "by_parts"  those that make fewer than slow_turns turns within original_len
+                  divided by factor, those that make more than fast_turns kept, a
+                  linear ramp over their index between the two; scale is 0.1 ln factor + 1
+
+    scale is 1 otherwise. It multiplies the rotated dims of Q and of K.
+    """
+    if rot_dim <= 0 or rot_dim % 2 != 0:
+        raise RuntimeError("rot_dim must be positive and even")
+    if not (base > 1.0 and factor >= 1.0):
+        raise RuntimeError("base must be > 1 and factor >= 1")
+    half = rot_dim // 2
+    i = torch.arange(half, dtype=torch.float64)
+    scale = 1.0
+    if scaling == "ntk":
+        if rot_dim < 4:
+            raise RuntimeError("scaling 'ntk' needs rot_dim >= 4")
+        base = base * factor ** (rot_dim / (rot_dim - 2))
+    freqs = base ** (-2.0 * i / rot_dim)
+    if scaling == "linear":
+        freqs = freqs / factor
+    elif scaling == "by_parts":
+        if original_len <= 0 or not 0.0 < slow_turns < fast_turns:
+            raise RuntimeError("scaling 'by_parts' needs original_len > 0 and 0 < slow_turns < fast_turns")
+
+        def index(turns):   # of the frequency that makes so many turns within original_len
+            return rot_dim * math.log(original_len / (2.0 * math.pi * turns)) / (2.0 * math.log(base))
+
+        lo = max(math.floor(index(fast_turns)), 0)
+        hi = min(math.ceil(index(slow_turns)), half - 1)
+        ramp = torch.clamp((i - lo) / max(hi - lo, 1e-3), 0.0, 1.0)   # 0: kept, 1: divided
+        freqs = freqs * (1.0 - ramp) + freqs / factor * ramp
+        scale = 0.1 * math.log(factor) + 1.0
+    elif scaling not in (None, "ntk"):
+        raise RuntimeError("scaling must be None, 'linear', 'ntk' or 'by_parts'")
+    return freqs.to(device), scale
+
+
+_ROPE_TYPES = {None: -1, torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+
+
+def rope(Q, K, freqs, positions=None, interleaved: bool = False, scale: float = 1.0):
+    """[Q', K']: the first R = 2 * len(freqs) dims of every row turned by its position,
+    contiguous, in the dtype of Q and K (fp16, bf16 or fp32). [Q'] if K is None.
+
+    Q [B,H,N,D] and K [B,H_kv,N,D] may be views (a projection's [B,N,H,D] transposed)
+    and are read as they lie where rows are contiguous and 16-byte aligned; packed
+    rows are [H,total,D]. positions: int32 [N] or [B,N] (packed [total]); None: 0 to
+    N - 1. Pairs are dims (i, i + R/2), or neighbours if interleaved. Angles are exact
+    for any position (reduced in 64 bits).
+    """
+    return _C.rope(Q, K, freqs, positions, interleaved, scale, False, -1)
+
+
+def rope_backward(dQ, dK, freqs, positions=None, interleaved: bool = False, scale: float = 1.0,
+                  dtype=None):
+    """[dQ, dK] of rope's inputs from those of its outputs (backward()'s fp32 ones, or
+    16-bit ones), in dtype: theirs, or for fp32 gradients also fp16 or bf16.
+
+    freqs, positions, interleaved and scale as in the call of rope.
+    """
+    if dtype not in _ROPE_TYPES:
+        raise RuntimeError("dtype must be torch.float16, torch.bfloat16 or torch.float32")
+    return _C.rope(dQ, dK, freqs, positions, interleaved, scale, True, _ROPE_TYPES[dtype])
+
+
+def kv_append_rope(q, k_new, v_new, k_pool, v_pool, page_table, start_pos, freqs, positions=None,
+                   new_lens=None, interleaved: bool = False, scale: float = 1.0, want_k: bool = False):
+    """[q', bad]: rope of q [B,H,T,D] and k_new [B,H_kv,T,D], and kv_append of the rotated
+    k_new and of v_new, in one launch. With want_k [q', k', bad] (a prompt's own attention
+    needs k').
+
+    positions: int32 [B], the position of each sequence's first new token where it is
+    not its slot start_pos[b] (after kv_evict). q, k_new, v_new may be views as in
+    rope (slices of a joined q, k, v). Rows of q' and k' from new_lens[b] on are zeros.
+    """
+    return _C.kv_append_rope(q, k_new, v_new, k_pool, v_pool, page_table, start_pos, freqs, positions,
+                             new_lens, interleaved, scale, want_k)
+
+
+def decode_shared(q, k_pool, v_pool, prefix_table, prefix_len, page_table, ctx_lens):
+    """[O, L] of one query token per sequence over a prefix that all sequences share and
+    then its own paged K/V, as one softmax; decode_paged's dtypes.
+
+    The prefix is the first prefix_len (int32, one value, on the device) tokens of the
+    pages prefix_table (int32 [prefix_pages]), read once for the whole batch;
+    page_table and ctx_lens are those of the sequences' own tokens (lengths may be 0).
+    An invalid prefix makes every O and L NaN, an invalid own page those of its sequence.
+    """
+    return _C.decode_shared(q, k_pool, v_pool, prefix_table, prefix_len, page_table, ctx_lens)
+
+
+def decode_paged_weights(q, k_pool, v_pool, page_table, ctx_lens, weights, num_splits: int = 16,
+                         inplace: bool = False):
+    """[O, L, W]: decode_paged, and W = weights with the attention weight of every cached
+    token added, summed over the query heads of its KV head (fp32 [B,H_kv,max_pages*16]).
+
+    inplace: W is weights itself. Slots past a context keep their value; where O and L
+    are NaN (an invalid page or length), W is NaN over the context.
+    """
+    return _C.decode_paged_weights(q, k_pool, v_pool, page_table, ctx_lens, weights, num_splits, inplace)
+
+
+def kv_evict(k_pool, v_pool, page_table, ctx_lens, weights, new_page_table, keep: int, recent: int):
+    """[kept, new_weights, new_lens, bad]: at most `keep` tokens of each head stay, the
+    `recent` last ones and of the others the heaviest by weights (of equal ones the
+    earliest; NaN counts as lightest), copied in order into the pages of new_page_table.
+
+    kept int32 [B,H_kv,keep]: old slot of each new one, then -1; new_weights fp32
+    [B,H_kv,new_max_pages*16]: their weights, then zeros; new_lens int32 [B]. bad int32
+    [B]: 1 where a row had no valid page, old or new (it is not copied), or the length
+    is invalid (then new_lens is 0). The new pages must not be among the old ones,
+    which are the caller's to free afterwards.
+    """
+    return _C.kv_evict(k_pool, v_pool, page_table, ctx_lens, weights, new_page_table, keep, recent)
 
 
 def loaded_libraries():

@@ -68,6 +68,19 @@ SIGNATURES = {
     "fa_validate_decode_mx": (C.c_int, [_vp] * 5 + [_i64] * 9 + [_vp] * 3),
     "fa_decode_mx_workspace_floats": (_i64, [_i64] * 5),
     "fa_decode_paged_mx": (C.c_int, [_vp] * 5 + [_i64] * 9 + [_vp] * 3 + [C.c_int, _vp]),
+    "fa_rope": (C.c_int, [_vp] * 6 + [_i64] + [_vp] * 2 + [_i64] * 6 + [C.c_float] + [C.c_int] * 4 + [_vp]),
+    "fa_validate_rope": (C.c_int, [_vp] * 6 + [_i64] + [_vp] * 2 + [_i64] * 6 + [C.c_int] * 2),
+    "fa_kv_append_rope": (C.c_int, [_vp] * 16 + [_i64] * 6 + [C.c_float, C.c_int] + [_i64] * 3 +
+                          [C.c_int, _vp]),
+    "fa_validate_kv_append_rope": (C.c_int, [_vp] * 16 + [_i64] * 9),
+    "fa_decode_shared": (C.c_int, [_vp] * 7 + [_i64] * 8 + [_vp] * 3 + [C.c_int, _vp]),
+    "fa_decode_shared_workspace_floats": (_i64, [_i64] * 6),
+    "fa_validate_decode_shared": (C.c_int, [_vp] * 7 + [_i64] * 8 + [_vp] * 3),
+    "fa_decode_paged_weights": (C.c_int, [_vp] * 6 + [_i64] * 8 + [_vp] * 4 + [C.c_int, _vp]),
+    "fa_decode_weights_workspace_floats": (_i64, [_i64] * 5),
+    "fa_validate_decode_weights": (C.c_int, [_vp] * 6 + [_i64] * 8 + [_vp] * 4),
+    "fa_kv_evict": (C.c_int, [_vp] * 10 + [_i64] * 9 + [_vp]),
+    "fa_validate_kv_evict": (C.c_int, [_vp] * 10 + [_i64] * 9),
     "fa_probe_fwd_variant": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, C.c_int, C.c_int, _vp]),
     "fa_probe_fwd_variants": (C.c_int, [_vp, C.c_int, _i64, C.c_int]),
     "fa_probe_default_variant": (C.c_int, [_i64]),
@@ -88,8 +101,11 @@ STATUS = {
     "FA_ERR_BATCH_HEADS": 4, "FA_ERR_ALIGNMENT": 5, "FA_ERR_TOO_LARGE": 6,
     "FA_ERR_PAGE_SIZE": 7, "FA_ERR_NUM_SPLITS": 8, "FA_ERR_MAX_PAGES": 9,
     "FA_ERR_NUM_PAGES": 10, "FA_ERR_KV_HEADS": 11, "FA_ERR_SCRATCH_SIZE": 12,
-    "FA_ERR_MX_BITS": 13,
+    "FA_ERR_MX_BITS": 13, "FA_ERR_ROT_DIM": 14, "FA_ERR_STRIDE": 15, "FA_ERR_TYPE": 16,
+    "FA_ERR_BUDGET": 17,
 }
+
+TYPES = {"FA_F16": 0, "FA_BF16": 1, "FA_F32": 2}
 
 
 def header_symbols() -> list[str]:

@@ -37,6 +37,10 @@ extern "C" const char* fa_status_str(int status) {
     case FA_ERR_SCRATCH_SIZE:
       return "B*H*num_splits*(D+1) exceeds FA_DECODE_SCRATCH_FLOATS (no-alloc decode)";
     case FA_ERR_MX_BITS: return "k_bits and v_bits must be 4 or 8";
+    case FA_ERR_ROT_DIM: return "rot_dim must be a positive multiple of 16, at most the head dimension";
+    case FA_ERR_STRIDE: return "row strides must be multiples of 16 bytes";
+    case FA_ERR_TYPE: return "element types must be alike, or float32 in";
+    case FA_ERR_BUDGET: return "keep must be in [1, new_max_pages * 16] and recent in [0, keep]";
     default: break;
   }
   if (status < 0) return "HIP error (negated hipError_t)";
@@ -231,5 +235,146 @@ extern "C" int fa_validate_decode_mx(const void* q, const void* k_pool, const vo
   if (!aligned16(workspace) || !aligned16(o)) return FA_ERR_ALIGNMENT;
   if (reinterpret_cast<uintptr_t>(lse) & 3u) return FA_ERR_ALIGNMENT;
   if (num_pages > kMaxGrid) return FA_ERR_TOO_LARGE;
+  return FA_OK;
+}
+
+// Rotary positions (no reference counterpart). Strides of dimensions of one index
+// are not looked at; rows are read as 16-byte pieces.
+static int check_rows(const void* p, const int64_t* st, int64_t B, int64_t H, int64_t N, int64_t size) {
+  if (!p) return FA_OK;
+  if (!st) return FA_ERR_NULL_POINTER;
+  const int64_t n[3] = {B, H, N};
+  for (int i = 0; i < 3; ++i)
+    if (n[i] > 1 && (st[i] < 0 || st[i] * size % 16 != 0)) return FA_ERR_STRIDE;
+  return aligned16(p) ? FA_OK : FA_ERR_ALIGNMENT;
+}
+
+static int check_rot(const double* freqs, int64_t B, int64_t H, int64_t H_kv, int64_t N, int64_t D,
+                     int64_t rot_dim) {
+  if (!freqs) return FA_ERR_NULL_POINTER;
+  if (D != 64 && D != 128) return FA_ERR_HEAD_DIM;
+  if (rot_dim <= 0 || rot_dim > D || rot_dim % 16 != 0) return FA_ERR_ROT_DIM;
+  if (B <= 0 || H <= 0) return FA_ERR_BATCH_HEADS;
+  if (reinterpret_cast<uintptr_t>(freqs) & 7u) return FA_ERR_ALIGNMENT;
+  // Grid (token blocks, head slots, B).
+  if (B > 65535 || H + 2 * H_kv > 65535 || N > (int64_t(1) << 28)) return FA_ERR_TOO_LARGE;
+  return FA_OK;
+}
+
+extern "C" int fa_validate_rope(const void* q, const int64_t q_strides[3], const void* k,
+                                const int64_t k_strides[3], const double* freqs,
+                                const int32_t* positions, int64_t pos_stride, const void* q_out,
+                                const void* k_out, int64_t B, int64_t H, int64_t H_kv, int64_t N,
+                                int64_t D, int64_t rot_dim, int in_type, int out_type) {
+  if (!q || !q_out || (H_kv != 0 && (!k || !k_out))) return FA_ERR_NULL_POINTER;
+  if (H_kv < 0) return FA_ERR_KV_HEADS;
+  if (N <= 0) return FA_ERR_SEQ_LEN;
+  int st = check_rot(freqs, B, H, H_kv, N, D, rot_dim);
+  if (st != FA_OK) return st;
+  if (in_type < FA_F16 || in_type > FA_F32 || out_type < FA_F16 || out_type > FA_F32 ||
+      (in_type != out_type && in_type != FA_F32))
+    return FA_ERR_TYPE;
+  const int64_t size = in_type == FA_F32 ? 4 : 2;
+  st = check_rows(q, q_strides, B, H, N, size);
+  if (st == FA_OK && H_kv > 0) st = check_rows(k, k_strides, B, H_kv, N, size);
+  if (st != FA_OK) return st;
+  if (!aligned16(q_out) || (H_kv > 0 && !aligned16(k_out))) return FA_ERR_ALIGNMENT;
+  if (reinterpret_cast<uintptr_t>(positions) & 3u) return FA_ERR_ALIGNMENT;
+  if (positions && pos_stride < 0) return FA_ERR_STRIDE;
+  return FA_OK;
+}
+
+extern "C" int fa_validate_kv_append_rope(const void* q, const int64_t q_strides[3], const void* k,
+                                          const int64_t k_strides[3], const void* v,
+                                          const int64_t v_strides[3], const double* freqs,
+                                          const int32_t* page_table, const int32_t* start_pos,
+                                          const int32_t* positions, const int32_t* new_lens,
+                                          const void* k_pool, const void* v_pool, const void* q_out,
+                                          const void* k_out, const int32_t* bad, int64_t B, int64_t H,
+                                          int64_t H_kv, int64_t T, int64_t D, int64_t rot_dim,
+                                          int64_t page_size, int64_t max_pages, int64_t num_pages) {
+  if (!bad || (T != 0 && (!q || !q_out))) return FA_ERR_NULL_POINTER;
+  int st = fa_validate_kv_append(k, v, page_table, start_pos, new_lens, k_pool, v_pool, bad, B, H_kv,
+                                 T, D, page_size, max_pages, num_pages);
+  if (st != FA_OK) return st;
+  if (H <= 0 || H % H_kv != 0) return FA_ERR_KV_HEADS;
+  st = check_rot(freqs, B, H, H_kv, T, D, rot_dim);
+  if (st == FA_OK) st = check_rows(q, q_strides, B, H, T, 2);
+  if (st == FA_OK) st = check_rows(k, k_strides, B, H_kv, T, 2);
+  if (st == FA_OK) st = check_rows(v, v_strides, B, H_kv, T, 2);
+  if (st != FA_OK) return st;
+  if (!aligned16(q_out) || !aligned16(k_out)) return FA_ERR_ALIGNMENT;
+  if (reinterpret_cast<uintptr_t>(positions) & 3u) return FA_ERR_ALIGNMENT;
+  return FA_OK;
+}
+
+// The paged decode's checks and those of the prefix: its grid is one-dimensional.
+extern "C" int fa_validate_decode_shared(const void* q, const void* k_pool, const void* v_pool,
+                                         const int32_t* prefix_table, const int32_t* prefix_len,
+                                         const int32_t* page_table, const int32_t* ctx_lens, int64_t B,
+                                         int64_t H, int64_t H_kv, int64_t D, int64_t page_size,
+                                         int64_t prefix_pages, int64_t max_pages, int64_t num_pages,
+                                         const float* workspace, const void* o, const float* lse) {
+  const int st = fa_validate_decode(q, k_pool, v_pool, page_table, ctx_lens, B, H, D, page_size,
+                                    max_pages, num_pages, /*num_splits=*/1);
+  if (st != FA_OK) return st;
+  if (H_kv <= 0 || H % H_kv != 0) return FA_ERR_KV_HEADS;
+  if (!prefix_table || !prefix_len || !workspace || !o || !lse) return FA_ERR_NULL_POINTER;
+  if (prefix_pages <= 0) return FA_ERR_MAX_PAGES;
+  if (!aligned16(workspace) || !aligned16(o)) return FA_ERR_ALIGNMENT;
+  const auto a4 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; };
+  if (!a4(prefix_table) || !a4(prefix_len) || !a4(lse)) return FA_ERR_ALIGNMENT;
+  // Positions within the prefix and rows (b, h) are 32-bit numbers.
+  if (prefix_pages > (int64_t(1) << 27) - 8 || num_pages > kMaxGrid) return FA_ERR_TOO_LARGE;
+  if (B * H > (int64_t(1) << 24)) return FA_ERR_TOO_LARGE;
+  return FA_OK;
+}
+
+extern "C" int fa_validate_decode_weights(const void* q, const void* k_pool, const void* v_pool,
+                                          const int32_t* page_table, const int32_t* ctx_lens,
+                                          const float* weights, int64_t B, int64_t H, int64_t H_kv,
+                                          int64_t D, int64_t page_size, int64_t max_pages,
+                                          int64_t num_pages, int64_t num_splits,
+                                          const float* workspace, const void* o, const float* lse,
+                                          const float* weights_out) {
+  const int st = fa_validate_decode(q, k_pool, v_pool, page_table, ctx_lens, B, H, D, page_size,
+                                    max_pages, num_pages, num_splits);
+  if (st != FA_OK) return st;
+  if (H_kv <= 0 || H % H_kv != 0) return FA_ERR_KV_HEADS;
+  if (!weights || !weights_out || !workspace || !o || !lse) return FA_ERR_NULL_POINTER;
+  if (!aligned16(workspace) || !aligned16(o) || !aligned16(weights) || !aligned16(weights_out))
+    return FA_ERR_ALIGNMENT;
+  if (reinterpret_cast<uintptr_t>(lse) & 3u) return FA_ERR_ALIGNMENT;
+  // The join has a workgroup for 1024 slots of a (b, KV head), and one for 8 rows.
+  const int64_t chunks = (max_pages * 16 + 1023) / 1024;
+  if (num_pages > kMaxGrid || B * H > (int64_t(1) << 24) || B * H_kv > ((int64_t(1) << 30) - 1) / chunks)
+    return FA_ERR_TOO_LARGE;
+  return FA_OK;
+}
+
+extern "C" int fa_validate_kv_evict(const void* k_pool, const void* v_pool, const int32_t* page_table,
+                                    const int32_t* ctx_lens, const float* weights,
+                                    const int32_t* new_page_table, const int32_t* kept,
+                                    const float* new_weights, const int32_t* new_lens,
+                                    const int32_t* bad, int64_t B, int64_t H_kv, int64_t D,
+                                    int64_t keep, int64_t recent, int64_t page_size,
+                                    int64_t max_pages, int64_t new_max_pages, int64_t num_pages) {
+  if (!k_pool || !v_pool || !page_table || !ctx_lens || !weights || !new_page_table || !kept ||
+      !new_weights || !new_lens || !bad)
+    return FA_ERR_NULL_POINTER;
+  if (D != 64 && D != 128) return FA_ERR_HEAD_DIM;
+  if (B <= 0 || H_kv <= 0) return FA_ERR_BATCH_HEADS;
+  if (page_size != 16) return FA_ERR_PAGE_SIZE;
+  if (max_pages <= 0 || new_max_pages <= 0) return FA_ERR_MAX_PAGES;
+  if (num_pages <= 0) return FA_ERR_NUM_PAGES;
+  if (!aligned16(k_pool) || !aligned16(v_pool)) return FA_ERR_ALIGNMENT;
+  const void* words[] = {page_table, ctx_lens, weights, new_page_table, kept, new_weights, new_lens, bad};
+  for (const void* p : words)
+    if (reinterpret_cast<uintptr_t>(p) & 3u) return FA_ERR_ALIGNMENT;
+  if (B > 65535 || H_kv > 65535 || num_pages > kMaxGrid) return FA_ERR_TOO_LARGE;
+  // Slots are 32-bit numbers, and a thread's steps of 1024 past the last one too.
+  constexpr int64_t kMaxSlotPages = (int64_t(1) << 27) - 128;
+  if (max_pages > kMaxSlotPages || new_max_pages > kMaxSlotPages) return FA_ERR_TOO_LARGE;
+  if (keep < 1 || keep > new_max_pages * 16 || recent < 0 || recent > keep) return FA_ERR_BUDGET;
   return FA_OK;
 }

@@ -668,6 +668,273 @@ std::vector<torch::Tensor> decode_paged_mx(torch::Tensor q, torch::Tensor k_pool
   return {o, lse};
 }
 
+// ---- rotary positions ----
+
+// Rows of x [B, H, N, D] as the rotary kernels read them: as they lie where rows
+// are contiguous and 16-byte aligned (a projection's [B, N, H, D] seen as
+// [B, H, N, D], a slice of a joined q, k, v), else a contiguous copy.
+struct RowView {
+  torch::Tensor t;
+  int64_t st[3] = {0, 0, 0};
+};
+
+RowView row_view(const torch::Tensor& x) {
+  RowView r;
+  r.t = x.is_neg() ? x.resolve_neg() : x;
+  const int64_t size = (int64_t)r.t.element_size();
+  bool plain = !r.t._is_zerotensor() && r.t.stride(3) == 1 &&
+               (reinterpret_cast<uintptr_t>(r.t.data_ptr()) & 15u) == 0;
+  for (int i = 0; i < 3; ++i)
+    plain = plain && (r.t.size(i) <= 1 || (r.t.stride(i) >= 0 && r.t.stride(i) * size % 16 == 0));
+  if (!plain) r.t = r.t.clone(at::MemoryFormat::Contiguous);
+  for (int i = 0; i < 3; ++i) r.st[i] = r.t.size(i) > 1 ? r.t.stride(i) : 0;
+  return r;
+}
+
+int fa_type_of(const torch::Tensor& t, const char* what) {
+  switch (t.scalar_type()) {
+    case torch::kHalf: return FA_F16;
+    case torch::kBFloat16: return FA_BF16;
+    case torch::kFloat: return FA_F32;
+    default: break;
+  }
+  TORCH_CHECK(false, what, " must be float16, bfloat16 or float32");
+  return -1;
+}
+
+void check_freqs(const torch::Tensor& freqs, const torch::Device& dev) {
+  TORCH_CHECK(freqs.is_cuda() && freqs.dim() == 1 && freqs.scalar_type() == torch::kDouble &&
+                  freqs.is_contiguous(),
+              "freqs must be a contiguous CUDA float64 [rot_dim / 2] (rope_frequencies)");
+  TORCH_CHECK(freqs.device() == dev, "freqs must be on the rows' device");
+}
+
+// rope(Q, K, freqs, positions, interleaved, scale, back, out_type) -> [Q, K]
+// rotated ([Q] without K). No reference counterpart.
+std::vector<torch::Tensor> rope(torch::Tensor Q, c10::optional<torch::Tensor> K, torch::Tensor freqs,
+                                c10::optional<torch::Tensor> positions, bool interleaved, double scale,
+                                bool back, int64_t out_type) {
+  TORCH_CHECK(Q.is_cuda() && (!K.has_value() || K->is_cuda()), "Q/K must be CUDA tensors");
+  TORCH_CHECK(Q.dim() == 4 || Q.dim() == 3, "Q must be [B, H, N, D], or packed [H, total, D]");
+  const bool packed = Q.dim() == 3;
+  const auto dev = Q.device();
+  TORCH_CHECK(!K.has_value() || (K->dim() == Q.dim() && K->size(-1) == Q.size(-1) &&
+                                 K->size(-2) == Q.size(-2) && (packed || K->size(0) == Q.size(0))),
+              "K must be [B, H_kv, N, D] (packed: [H_kv, total, D]) with Q's B, N and D");
+  TORCH_CHECK(!K.has_value() || (K->device() == dev && K->scalar_type() == Q.scalar_type()),
+              "Q and K must be on the same device and of the same dtype");
+  check_freqs(freqs, dev);
+  const int in_type = fa_type_of(Q, "Q and K");
+  TORCH_CHECK(out_type < 0 || out_type == in_type || in_type == FA_F32,
+              "dtype must be that of the rows, or any of float16, bfloat16, float32 for float32 rows");
+  if (out_type < 0) out_type = in_type;
+  const auto q4 = packed ? Q.unsqueeze(0) : Q;
+  const int64_t B = q4.size(0), H = q4.size(1), N = q4.size(2), D = q4.size(3);
+  TORCH_CHECK(N > 0, "N must be > 0");
+  const c10::DeviceGuard guard(dev);
+  const RowView q = row_view(q4);
+  RowView k;
+  if (K.has_value()) k = row_view(packed ? K->unsqueeze(0) : *K);
+  const int64_t Hkv = K.has_value() ? k.t.size(1) : 0;
+  const int32_t* pos = nullptr;
+  int64_t pos_stride = 0;
+  torch::Tensor p;
+  if (positions.has_value()) {
+    p = *positions;
+    TORCH_CHECK(p.is_cuda() && p.scalar_type() == torch::kInt && p.device() == dev,
+                "positions must be int32 on the rows' device");
+    TORCH_CHECK((p.dim() == 1 && p.size(0) == N) || (!packed && p.dim() == 2 && p.size(0) == B && p.size(1) == N),
+                "positions must be [N] or [B, N] (packed: [total])");
+    if ((N > 1 && p.stride(-1) != 1)) p = p.contiguous();
+    pos = p.data_ptr<int32_t>();
+    pos_stride = p.dim() == 2 && B > 1 ? p.stride(0) : 0;
+  }
+  const auto opt = q.t.options().dtype(out_type == FA_F16    ? torch::kHalf
+                                       : out_type == FA_BF16 ? torch::kBFloat16
+                                                             : torch::kFloat);
+  auto qo = at::empty({B, H, N, D}, opt);
+  auto ko = K.has_value() ? at::empty({B, Hkv, N, D}, opt) : torch::Tensor();
+  const int st = fa_rope(q.t.data_ptr(), q.st, Hkv > 0 ? k.t.data_ptr() : nullptr, k.st,
+                         freqs.data_ptr<double>(), pos, pos_stride, qo.data_ptr(),
+                         Hkv > 0 ? ko.data_ptr() : nullptr, B, H, Hkv, N, D, 2 * freqs.size(0),
+                         (float)scale, interleaved ? 1 : 0, back ? 1 : 0, in_type, (int)out_type,
+                         current_stream(q.t));
+  check_status(st, "fa_rope");
+  if (packed) {
+    qo = qo.squeeze(0);
+    if (ko.defined()) ko = ko.squeeze(0);
+  }
+  if (ko.defined()) return {qo, ko};
+  return {qo};
+}
+
+// kv_append_rope(...) -> [q rotated, (k rotated,) bad int32 [B]]: rotary positions
+// and kv_append in one launch. No reference counterpart.
+std::vector<torch::Tensor> kv_append_rope(torch::Tensor q, torch::Tensor k_new, torch::Tensor v_new,
+                                          torch::Tensor k_pool, torch::Tensor v_pool,
+                                          torch::Tensor page_table, torch::Tensor start_pos,
+                                          torch::Tensor freqs, c10::optional<torch::Tensor> positions,
+                                          c10::optional<torch::Tensor> new_lens, bool interleaved,
+                                          double scale, bool want_k) {
+  TORCH_CHECK(q.is_cuda() && k_new.is_cuda() && v_new.is_cuda() && k_pool.is_cuda() &&
+                  v_pool.is_cuda() && page_table.is_cuda() && start_pos.is_cuda(),
+              "q/k_new/v_new/k_pool/v_pool/page_table/start_pos must be CUDA tensors");
+  TORCH_CHECK(q.dim() == 4 && k_new.dim() == 4 && v_new.sizes() == k_new.sizes(),
+              "q must be [B, H, T, D], k_new and v_new [B, H_kv, T, D] of the same shape");
+  const int64_t B = q.size(0), H = q.size(1), T = q.size(2), D = q.size(3), Hkv = k_new.size(1);
+  TORCH_CHECK(k_new.size(0) == B && k_new.size(2) == T && k_new.size(3) == D && Hkv > 0 && H % Hkv == 0,
+              "k_new and v_new must be [B, H_kv, T, D] with q's B, T and D and H a multiple of H_kv");
+  TORCH_CHECK(k_pool.dim() == 4 && v_pool.sizes() == k_pool.sizes() && k_pool.size(1) == Hkv &&
+                  k_pool.size(3) == D,
+              "k_pool and v_pool must be [num_pages, H_kv, page_size, D] with k_new's H_kv and D");
+  const auto type = q.scalar_type();
+  TORCH_CHECK((type == torch::kHalf || type == torch::kBFloat16) && k_new.scalar_type() == type &&
+                  v_new.scalar_type() == type && k_pool.scalar_type() == type &&
+                  v_pool.scalar_type() == type,
+              "q/k_new/v_new/k_pool/v_pool must be all float16 or all bfloat16");
+  const auto dev = q.device();
+  TORCH_CHECK(page_table.dim() == 2 && page_table.scalar_type() == torch::kInt && page_table.size(0) == B,
+              "page_table must be int32 [B, max_pages]");
+  const auto ints = [&](const torch::Tensor& t, const char* name) {
+    TORCH_CHECK(t.is_cuda() && t.dim() == 1 && t.scalar_type() == torch::kInt && t.size(0) == B &&
+                    t.is_contiguous() && t.device() == dev,
+                name, " must be a contiguous int32 [B] on q's device");
+    return t.data_ptr<int32_t>();
+  };
+  const int32_t* start = ints(start_pos, "start_pos");
+  const int32_t* pos = positions.has_value() ? ints(*positions, "positions") : nullptr;
+  const int32_t* lens = new_lens.has_value() ? ints(*new_lens, "new_lens") : nullptr;
+  check_freqs(freqs, dev);
+  TORCH_CHECK(k_pool.is_contiguous() && v_pool.is_contiguous() && page_table.is_contiguous(),
+              "k_pool, v_pool and page_table must be contiguous");
+  TORCH_CHECK(k_new.device() == dev && v_new.device() == dev && k_pool.device() == dev &&
+                  v_pool.device() == dev && page_table.device() == dev,
+              "kv_append_rope tensors must be on the same device");
+  const c10::DeviceGuard guard(dev);
+  const RowView qv = row_view(q), kv = row_view(k_new), vv = row_view(v_new);
+  auto qo = at::empty({B, H, T, D}, q.options());
+  auto ko = want_k ? at::empty({B, Hkv, T, D}, q.options()) : torch::Tensor();
+  auto bad = at::empty({B}, page_table.options());
+  const int st = fa_kv_append_rope(
+      qv.t.data_ptr(), qv.st, kv.t.data_ptr(), kv.st, vv.t.data_ptr(), vv.st, freqs.data_ptr<double>(),
+      page_table.data_ptr<int32_t>(), start, pos, lens, k_pool.data_ptr(), v_pool.data_ptr(),
+      qo.data_ptr(), want_k ? ko.data_ptr() : nullptr, bad.data_ptr<int32_t>(), B, H, Hkv, T, D,
+      2 * freqs.size(0), (float)scale, interleaved ? 1 : 0, k_pool.size(2), page_table.size(1),
+      k_pool.size(0), type == torch::kBFloat16 ? 1 : 0, current_stream(k_pool));
+  check_status(st, "fa_kv_append_rope");
+  if (want_k) return {qo, ko, bad};
+  return {qo, bad};
+}
+
+// decode_shared(q, k_pool, v_pool, prefix_table, prefix_len, page_table, ctx_lens)
+// -> [O, L]: the paged decode of a batch that shares a prefix. No reference
+// counterpart.
+std::vector<torch::Tensor> decode_shared(torch::Tensor q, torch::Tensor k_pool, torch::Tensor v_pool,
+                                         torch::Tensor prefix_table, torch::Tensor prefix_len,
+                                         torch::Tensor page_table, torch::Tensor ctx_lens) {
+  const DecodeArgs a = check_decode(q, k_pool, v_pool, page_table, ctx_lens);
+  TORCH_CHECK(prefix_table.is_cuda() && prefix_table.dim() == 1 &&
+                  prefix_table.scalar_type() == torch::kInt && prefix_table.is_contiguous(),
+              "prefix_table must be a contiguous CUDA int32 [prefix_pages]");
+  TORCH_CHECK(prefix_len.is_cuda() && prefix_len.numel() == 1 && prefix_len.scalar_type() == torch::kInt,
+              "prefix_len must be a CUDA int32 tensor of one value");
+  TORCH_CHECK(prefix_table.device() == q.device() && prefix_len.device() == q.device(),
+              "decode tensors must be on the same device");
+  const c10::DeviceGuard guard(q.device());
+  const auto f32 = q.options().dtype(torch::kFloat);
+  auto ws = at::empty({fa_decode_shared_workspace_floats(a.B, a.H, a.Hkv, a.D, prefix_table.size(0),
+                                                         a.max_pages)}, f32);
+  auto o = at::empty({a.B, a.H, a.D}, q.options());
+  auto lse = at::empty({a.B, a.H}, f32);
+  const int st = fa_decode_shared(
+      q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), prefix_table.data_ptr<int32_t>(),
+      prefix_len.data_ptr<int32_t>(), page_table.data_ptr<int32_t>(), ctx_lens.data_ptr<int32_t>(), a.B,
+      a.H, a.Hkv, a.D, a.page_size, prefix_table.size(0), a.max_pages, a.num_pages,
+      ws.data_ptr<float>(), o.data_ptr(), lse.data_ptr<float>(), q.scalar_type() == torch::kBFloat16,
+      current_stream(q));
+  check_status(st, "fa_decode_shared");
+  return {o, lse};
+}
+
+// Weights of cached tokens: contiguous fp32 [B, H_kv, max_pages * 16].
+void check_weights(const torch::Tensor& w, int64_t B, int64_t Hkv, int64_t max_pages,
+                   const torch::Device& dev) {
+  TORCH_CHECK(w.is_cuda() && w.dim() == 3 && w.scalar_type() == torch::kFloat && w.is_contiguous() &&
+                  w.size(0) == B && w.size(1) == Hkv && w.size(2) == 16 * max_pages && w.device() == dev,
+              "weights must be contiguous float32 [B, H_kv, max_pages * 16] on the pools' device");
+}
+
+// decode_paged_weights(q, k_pool, v_pool, page_table, ctx_lens, weights,
+// num_splits=16, inplace=False) -> [O, L, weights + this step's]. No reference
+// counterpart.
+std::vector<torch::Tensor> decode_paged_weights(torch::Tensor q, torch::Tensor k_pool,
+                                                torch::Tensor v_pool, torch::Tensor page_table,
+                                                torch::Tensor ctx_lens, torch::Tensor weights,
+                                                int64_t num_splits, bool inplace) {
+  const DecodeArgs a = check_decode(q, k_pool, v_pool, page_table, ctx_lens);
+  check_weights(weights, a.B, a.Hkv, a.max_pages, q.device());
+  const c10::DeviceGuard guard(q.device());
+  const auto f32 = q.options().dtype(torch::kFloat);
+  auto ws = at::empty({fa_decode_weights_workspace_floats(a.B, a.H, a.D, a.max_pages, num_splits)}, f32);
+  auto o = at::empty({a.B, a.H, a.D}, q.options());
+  auto lse = at::empty({a.B, a.H}, f32);
+  auto w = inplace ? weights : at::empty(weights.sizes(), f32);
+  const int st = fa_decode_paged_weights(
+      q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), page_table.data_ptr<int32_t>(),
+      ctx_lens.data_ptr<int32_t>(), weights.data_ptr<float>(), a.B, a.H, a.Hkv, a.D, a.page_size,
+      a.max_pages, a.num_pages, num_splits, ws.data_ptr<float>(), o.data_ptr(), lse.data_ptr<float>(),
+      w.data_ptr<float>(), q.scalar_type() == torch::kBFloat16, current_stream(q));
+  check_status(st, "fa_decode_paged_weights");
+  return {o, lse, w};
+}
+
+// kv_evict(k_pool, v_pool, page_table, ctx_lens, weights, new_page_table, keep,
+// recent) -> [kept, new_weights, new_lens, bad]. No reference counterpart.
+std::vector<torch::Tensor> kv_evict(torch::Tensor k_pool, torch::Tensor v_pool, torch::Tensor page_table,
+                                    torch::Tensor ctx_lens, torch::Tensor weights,
+                                    torch::Tensor new_page_table, int64_t keep, int64_t recent) {
+  TORCH_CHECK(k_pool.is_cuda() && v_pool.is_cuda() && page_table.is_cuda() && ctx_lens.is_cuda() &&
+                  new_page_table.is_cuda(),
+              "k_pool/v_pool/page_table/ctx_lens/new_page_table must be CUDA tensors");
+  TORCH_CHECK(k_pool.dim() == 4 && v_pool.sizes() == k_pool.sizes(),
+              "k_pool and v_pool must be [num_pages, H_kv, page_size, D] of the same shape");
+  TORCH_CHECK((k_pool.scalar_type() == torch::kHalf || k_pool.scalar_type() == torch::kBFloat16) &&
+                  v_pool.scalar_type() == k_pool.scalar_type(),
+              "k_pool and v_pool must be both float16 or both bfloat16");
+  TORCH_CHECK(page_table.dim() == 2 && page_table.scalar_type() == torch::kInt,
+              "page_table must be int32 [B, max_pages]");
+  const int64_t B = page_table.size(0), Hkv = k_pool.size(1), max_pages = page_table.size(1);
+  TORCH_CHECK(new_page_table.dim() == 2 && new_page_table.scalar_type() == torch::kInt &&
+                  new_page_table.size(0) == B,
+              "new_page_table must be int32 [B, new_max_pages]");
+  TORCH_CHECK(ctx_lens.dim() == 1 && ctx_lens.scalar_type() == torch::kInt && ctx_lens.size(0) == B,
+              "ctx_lens must be int32 [B]");
+  TORCH_CHECK(k_pool.is_contiguous() && v_pool.is_contiguous() && page_table.is_contiguous() &&
+                  ctx_lens.is_contiguous() && new_page_table.is_contiguous(),
+              "kv_evict tensors must be contiguous");
+  const auto dev = k_pool.device();
+  TORCH_CHECK(v_pool.device() == dev && page_table.device() == dev && ctx_lens.device() == dev &&
+                  new_page_table.device() == dev,
+              "kv_evict tensors must be on the same device");
+  check_weights(weights, B, Hkv, max_pages, dev);
+  TORCH_CHECK(keep >= 1 && keep <= 16 * new_page_table.size(1) && recent >= 0 && recent <= keep,
+              "keep must be in [1, new_max_pages * 16] and recent in [0, keep]");
+  const c10::DeviceGuard guard(dev);
+  auto kept = at::empty({B, Hkv, keep}, page_table.options());
+  auto new_weights = at::empty({B, Hkv, 16 * new_page_table.size(1)}, weights.options());
+  auto new_lens = at::empty({B}, page_table.options());
+  auto bad = at::empty({B}, page_table.options());
+  const int st = fa_kv_evict(k_pool.data_ptr(), v_pool.data_ptr(), page_table.data_ptr<int32_t>(),
+                             ctx_lens.data_ptr<int32_t>(), weights.data_ptr<float>(),
+                             new_page_table.data_ptr<int32_t>(), kept.data_ptr<int32_t>(),
+                             new_weights.data_ptr<float>(), new_lens.data_ptr<int32_t>(),
+                             bad.data_ptr<int32_t>(), B, Hkv, k_pool.size(3), keep, recent,
+                             k_pool.size(2), max_pages, new_page_table.size(1), k_pool.size(0),
+                             current_stream(k_pool));
+  check_status(st, "fa_kv_evict");
+  return {kept, new_weights, new_lens, bad};
+}
+
 // ---- layout probes (test support) ----
 torch::Tensor probe_mfma32(torch::Tensor a, torch::Tensor b, int64_t variant) {
   TORCH_CHECK(a.is_cuda() && a.sizes() == torch::IntArrayRef({32, 16}) && a.scalar_type() == torch::kHalf);
@@ -804,6 +1071,27 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("decode_paged_mx", &decode_paged_mx, "paged decode over MX pages: returns [O in q's dtype, L float]",
         py::arg("q"), py::arg("k_pool"), py::arg("v_pool"), py::arg("page_table"),
         py::arg("ctx_lens"));
+  m.def("rope", &rope, "rotary positions: returns [Q, K] rotated ([Q] without K)", py::arg("Q"),
+        py::arg("K"), py::arg("freqs"), py::arg("positions"), py::arg("interleaved"), py::arg("scale"),
+        py::arg("back"), py::arg("out_type"));
+  m.def("kv_append_rope", &kv_append_rope,
+        "rotate q and k, write k and v into the paged pools: returns [q, (k,) bad]", py::arg("q"),
+        py::arg("k_new"), py::arg("v_new"), py::arg("k_pool"), py::arg("v_pool"), py::arg("page_table"),
+        py::arg("start_pos"), py::arg("freqs"), py::arg("positions") = py::none(),
+        py::arg("new_lens") = py::none(), py::arg("interleaved") = false, py::arg("scale") = 1.0,
+        py::arg("want_k") = false);
+  m.def("decode_shared", &decode_shared,
+        "paged decode of a batch that shares a prefix: returns [O in q's dtype, L float]", py::arg("q"),
+        py::arg("k_pool"), py::arg("v_pool"), py::arg("prefix_table"), py::arg("prefix_len"),
+        py::arg("page_table"), py::arg("ctx_lens"));
+  m.def("decode_paged_weights", &decode_paged_weights,
+        "paged decode that adds up attention weights: returns [O in q's dtype, L float, weights float]",
+        py::arg("q"), py::arg("k_pool"), py::arg("v_pool"), py::arg("page_table"), py::arg("ctx_lens"),
+        py::arg("weights"), py::arg("num_splits") = 16, py::arg("inplace") = false);
+  m.def("kv_evict", &kv_evict,
+        "pack each head's newest and heaviest tokens: returns [kept, new_weights, new_lens, bad]",
+        py::arg("k_pool"), py::arg("v_pool"), py::arg("page_table"), py::arg("ctx_lens"),
+        py::arg("weights"), py::arg("new_page_table"), py::arg("keep"), py::arg("recent"));
   m.def("decode_paged", &decode_paged, "split-KV paged decode (fp16 or bf16): returns [O in q's dtype, L float]",
         py::arg("q"), py::arg("k_pool"), py::arg("v_pool"), py::arg("page_table"),
         py::arg("ctx_lens"), py::arg("num_splits") = 16);

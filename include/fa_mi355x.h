@@ -46,8 +46,15 @@ enum fa_status_code {
   FA_ERR_NUM_PAGES = 10,     /* num_pages <= 0 */
   FA_ERR_KV_HEADS = 11,      /* H_kv <= 0 or H not a multiple of H_kv */
   FA_ERR_SCRATCH_SIZE = 12,  /* split partials exceed FA_DECODE_SCRATCH_FLOATS */
-  FA_ERR_MX_BITS = 13        /* k_bits or v_bits is not 4 or 8 */
+  FA_ERR_MX_BITS = 13,       /* k_bits or v_bits is not 4 or 8 */
+  FA_ERR_ROT_DIM = 14,       /* rot_dim is not a multiple of 16 in [16, D] */
+  FA_ERR_STRIDE = 15,        /* a row stride is negative or no multiple of 16 bytes */
+  FA_ERR_TYPE = 16,          /* element types that do not go together */
+  FA_ERR_BUDGET = 17         /* keep or recent outside its range */
 };
+
+/* Element types, where an entry point takes more than two. */
+enum fa_type { FA_F16 = 0, FA_BF16 = 1, FA_F32 = 2 };
 
 /* Floats of the library's own split-partials array used by
  * fa_decode_paged_noalloc_f16 (16 MiB per GPU). */
@@ -508,6 +515,158 @@ int fa_decode_paged_mx(const void* q, const void* k_pool, const void* v_pool,
                        int64_t H_kv, int64_t D, int64_t k_bits, int64_t v_bits, int64_t page_size,
                        int64_t max_pages, int64_t num_pages, float* workspace, void* o, float* lse,
                        int bf16, void* stream);
+
+/*
+ * Rotary positions (no reference counterpart). Of the first rot_dim = R dims of
+ * a row at position p, pair i becomes, with a = p * freqs[i],
+ *   y1 = scale (x1 cos a - x2 sin a),  y2 = scale (x2 cos a + x1 sin a);
+ * pairs are dims (i, i + R/2), or with interleaved != 0 dims (2i, 2i + 1); dims
+ * from R on are copied. freqs: fp64 [R / 2], radians a position; angles are
+ * reduced in fp64, so far positions are as exact as near ones. R is a multiple of
+ * 16 in [16, D].
+ *
+ * fa_rope: q [B, H, N, D] and k [B, H_kv, N, D] (k NULL with H_kv 0: q alone),
+ * each by element strides of (sequence, head, token), rows of D contiguous and
+ * 16-byte aligned, into contiguous q_out, k_out. Token n of sequence b is at
+ * positions[b * pos_stride + n] (pos_stride 0: one row for all; NULL: n). back !=
+ * 0 rotates by -a: the transpose, which takes gradients of the outputs to
+ * gradients of the inputs. in_type, out_type: FA_F16, FA_BF16 or FA_F32, alike or
+ * in_type FA_F32. Arithmetic in fp32, one rounding to out_type.
+ */
+int fa_rope(const void* q, const int64_t q_strides[3], const void* k, const int64_t k_strides[3],
+            const double* freqs, const int32_t* positions, int64_t pos_stride, void* q_out,
+            void* k_out, int64_t B, int64_t H, int64_t H_kv, int64_t N, int64_t D, int64_t rot_dim,
+            float scale, int interleaved, int back, int in_type, int out_type, void* stream);
+
+/* Host-only argument check of fa_rope. */
+int fa_validate_rope(const void* q, const int64_t q_strides[3], const void* k,
+                     const int64_t k_strides[3], const double* freqs, const int32_t* positions,
+                     int64_t pos_stride, const void* q_out, const void* k_out, int64_t B, int64_t H,
+                     int64_t H_kv, int64_t N, int64_t D, int64_t rot_dim, int in_type, int out_type);
+
+/*
+ * fa_rope and fa_kv_append_set_bad in one launch (fp16, bf16 != 0: bfloat16): of
+ * each sequence's new tokens t < n_b (n_b = new_lens[b] clamped to [0, T], or T),
+ * q [B, H, T, D] rotated goes to q_out, k [B, H_kv, T, D] rotated and v as it is go
+ * into the pools at slot start_pos[b] + t, and k to k_out too where that is not
+ * NULL. Token t is rotated to position positions[b] + t (NULL: start_pos[b] + t):
+ * after an eviction slots and positions differ. q, k, v by strides as in fa_rope;
+ * q_out [B, H, T, D] and k_out [B, H_kv, T, D] contiguous, zeros from n_b on. A
+ * token with no valid page is rotated, but not written, and sets bad[b] to 1;
+ * every other bad[b] is set to 0. With T = 0 only bad is written, and q, k, v and
+ * their outputs may be NULL.
+ */
+int fa_kv_append_rope(const void* q, const int64_t q_strides[3], const void* k,
+                      const int64_t k_strides[3], const void* v, const int64_t v_strides[3],
+                      const double* freqs, const int32_t* page_table, const int32_t* start_pos,
+                      const int32_t* positions, const int32_t* new_lens, void* k_pool, void* v_pool,
+                      void* q_out, void* k_out, int32_t* bad, int64_t B, int64_t H, int64_t H_kv,
+                      int64_t T, int64_t D, int64_t rot_dim, float scale, int interleaved,
+                      int64_t page_size, int64_t max_pages, int64_t num_pages, int bf16, void* stream);
+
+/* Host-only argument check of fa_kv_append_rope. */
+int fa_validate_kv_append_rope(const void* q, const int64_t q_strides[3], const void* k,
+                               const int64_t k_strides[3], const void* v,
+                               const int64_t v_strides[3], const double* freqs,
+                               const int32_t* page_table, const int32_t* start_pos,
+                               const int32_t* positions, const int32_t* new_lens,
+                               const void* k_pool, const void* v_pool, const void* q_out,
+                               const void* k_out, const int32_t* bad, int64_t B, int64_t H,
+                               int64_t H_kv, int64_t T, int64_t D, int64_t rot_dim,
+                               int64_t page_size, int64_t max_pages, int64_t num_pages);
+
+/*
+ * Paged decode of a batch that shares a prefix (no reference counterpart): query
+ * token b attends to the first prefix_len[0] tokens of the pages prefix_table[0 ..
+ * prefix_pages), the same for every b, and to the ctx_lens[b] tokens of its own
+ * pages (page_table, as in fa_decode_paged_gqa_f16; prefix_len: int32 [1] on the
+ * device). o, lse are those of one softmax over both; o = 0 and lse = -inf where
+ * both are empty. The prefix is read once per KV head for up to 128 query rows
+ * (b, h). A page id outside [0, num_pages), a negative length or one beyond its
+ * table makes o and lse of the sequence NaN, of every sequence where it is the
+ * prefix's. q, pools, o fp16 (bf16 != 0: bfloat16); weights of the prefix are
+ * rounded to that type for their product with V, as in the forward. workspace:
+ * fa_decode_shared_workspace_floats(...) floats, 16-byte aligned, need not be
+ * cleared; calls that may overlap need one each.
+ */
+int fa_decode_shared(const void* q, const void* k_pool, const void* v_pool,
+                     const int32_t* prefix_table, const int32_t* prefix_len,
+                     const int32_t* page_table, const int32_t* ctx_lens, int64_t B, int64_t H,
+                     int64_t H_kv, int64_t D, int64_t page_size, int64_t prefix_pages,
+                     int64_t max_pages, int64_t num_pages, float* workspace, void* o, float* lse,
+                     int bf16, void* stream);
+
+/* Floats of fa_decode_shared's workspace; 0 for invalid sizes. */
+int64_t fa_decode_shared_workspace_floats(int64_t B, int64_t H, int64_t H_kv, int64_t D,
+                                          int64_t prefix_pages, int64_t max_pages);
+
+/* Host-only argument check of fa_decode_shared. */
+int fa_validate_decode_shared(const void* q, const void* k_pool, const void* v_pool,
+                              const int32_t* prefix_table, const int32_t* prefix_len,
+                              const int32_t* page_table, const int32_t* ctx_lens, int64_t B,
+                              int64_t H, int64_t H_kv, int64_t D, int64_t page_size,
+                              int64_t prefix_pages, int64_t max_pages, int64_t num_pages,
+                              const float* workspace, const void* o, const float* lse);
+
+/*
+ * fa_decode_paged_gqa_f16 (bf16 != 0: fa_decode_paged_bf16) that also adds up the
+ * attention that each cached token gets (no reference counterpart):
+ *   weights_out[b, hk, j] = weights[b, hk, j] + sum over the query heads h of KV
+ *   head hk of exp(s_hj - lse_h),   j < ctx_lens[b],
+ * fp32 [B, H_kv, max_pages * 16], 16-byte aligned; slots past the context keep
+ * their value. weights_out may be weights (in place), but not overlap it
+ * otherwise. Where o and lse are NaN (an invalid page or length), so are the
+ * sequence's weights up to its context, cut to the table. workspace:
+ * fa_decode_weights_workspace_floats(...) floats, 16-byte aligned, need not be
+ * cleared; calls that may overlap need one each.
+ */
+int fa_decode_paged_weights(const void* q, const void* k_pool, const void* v_pool,
+                            const int32_t* page_table, const int32_t* ctx_lens,
+                            const float* weights, int64_t B, int64_t H, int64_t H_kv, int64_t D,
+                            int64_t page_size, int64_t max_pages, int64_t num_pages,
+                            int64_t num_splits, float* workspace, void* o, float* lse,
+                            float* weights_out, int bf16, void* stream);
+
+/* Floats of fa_decode_paged_weights' workspace; 0 for invalid sizes. */
+int64_t fa_decode_weights_workspace_floats(int64_t B, int64_t H, int64_t D, int64_t max_pages,
+                                           int64_t num_splits);
+
+/* Host-only argument check of fa_decode_paged_weights. */
+int fa_validate_decode_weights(const void* q, const void* k_pool, const void* v_pool,
+                               const int32_t* page_table, const int32_t* ctx_lens,
+                               const float* weights, int64_t B, int64_t H, int64_t H_kv, int64_t D,
+                               int64_t page_size, int64_t max_pages, int64_t num_pages,
+                               int64_t num_splits, const float* workspace, const void* o,
+                               const float* lse, const float* weights_out);
+
+/*
+ * Cuts each head's cache to at most `keep` tokens (no reference counterpart). With
+ * n = ctx_lens[b]: of n > keep tokens the `recent` last and the keep - recent
+ * heaviest of the others by weights (fp32 [B, H_kv, max_pages * 16]; of equal ones
+ * those of lower slots; a NaN is below every number) stay, else all of them. Their
+ * K and V rows are copied, in the order of their slots, to slots 0 .. of
+ * new_page_table (int32 [B, new_max_pages]). kept [B, H_kv, keep]: the old slot of
+ * each new one, -1 past the last; new_weights [B, H_kv, new_max_pages * 16]: their
+ * weights, then zeros; new_lens [B]: min(n, keep). Rows whose old or new page is
+ * invalid are not copied and set bad[b] to 1; a negative length, or one beyond the
+ * table, sets bad[b] and new_lens[b] = 0; every other bad[b] is set to 0. Pages of
+ * new_page_table that the call writes must not be among those it reads. 16-bit
+ * rows of any type. 0 <= recent <= keep <= new_max_pages * 16.
+ */
+int fa_kv_evict(void* k_pool, void* v_pool, const int32_t* page_table, const int32_t* ctx_lens,
+                const float* weights, const int32_t* new_page_table, int32_t* kept,
+                float* new_weights, int32_t* new_lens, int32_t* bad, int64_t B, int64_t H_kv,
+                int64_t D, int64_t keep, int64_t recent, int64_t page_size, int64_t max_pages,
+                int64_t new_max_pages, int64_t num_pages, void* stream);
+
+/* Host-only argument check of fa_kv_evict. */
+int fa_validate_kv_evict(const void* k_pool, const void* v_pool, const int32_t* page_table,
+                         const int32_t* ctx_lens, const float* weights,
+                         const int32_t* new_page_table, const int32_t* kept,
+                         const float* new_weights, const int32_t* new_lens, const int32_t* bad,
+                         int64_t B, int64_t H_kv, int64_t D, int64_t keep, int64_t recent,
+                         int64_t page_size, int64_t max_pages, int64_t new_max_pages,
+                         int64_t num_pages);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,261 @@
+"""CPU tier of the rotary positions, the shared prefix and the cache budget: arguments are refused before any HIP call, by
+the C ABI and by the torch binding; rope_frequencies; the oracles against each other."""
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import cache, rotary
+
+A = 0x10000   # a fake, 16-byte aligned address: never dereferenced by validation
+
+
+def _st(*x):
+    return C.cast((C.c_int64 * 3)(*x), C.c_void_p)
+
+
+def _rope(**kw):
+    a = dict(q=A, qs=_st(8 * 64 * 128, 64 * 128, 128), k=A, ks=_st(8 * 64 * 128, 64 * 128, 128), f=A, p=A, ps=64, qo=A, ko=A, B=2, H=8,
+             Hkv=8, N=64, D=128, R=128, it=0, ot=0)
+    a.update(kw)
+    return [a[x] for x in ("q", "qs", "k", "ks", "f", "p", "ps", "qo", "ko", "B", "H", "Hkv", "N", "D", "R", "it", "ot")]
+
+
+ROPE = [
+    (dict(), "FA_OK"), (dict(q=0), "FA_ERR_NULL_POINTER"), (dict(qs=None), "FA_ERR_NULL_POINTER"), (dict(f=0), "FA_ERR_NULL_POINTER"),
+    (dict(k=0), "FA_ERR_NULL_POINTER"), (dict(ko=0), "FA_ERR_NULL_POINTER"), (dict(k=0, ko=0, ks=None, Hkv=0), "FA_OK"),
+    (dict(p=0), "FA_OK"), (dict(D=96, R=96), "FA_ERR_HEAD_DIM"), (dict(N=0), "FA_ERR_SEQ_LEN"), (dict(B=0), "FA_ERR_BATCH_HEADS"),
+    (dict(Hkv=-1), "FA_ERR_KV_HEADS"), (dict(R=0), "FA_ERR_ROT_DIM"), (dict(R=24), "FA_ERR_ROT_DIM"), (dict(R=144), "FA_ERR_ROT_DIM"),
+    (dict(R=16), "FA_OK"), (dict(it=2, ot=0), "FA_OK"), (dict(it=2, ot=1), "FA_OK"), (dict(it=2, ot=2), "FA_OK"),
+    (dict(it=0, ot=1), "FA_ERR_TYPE"), (dict(it=1, ot=2), "FA_ERR_TYPE"), (dict(it=3, ot=3), "FA_ERR_TYPE"), (dict(it=-1, ot=-1), "FA_ERR_TYPE"),
+    (dict(q=A + 2), "FA_ERR_ALIGNMENT"), (dict(ko=A + 8), "FA_ERR_ALIGNMENT"), (dict(f=A + 4), "FA_ERR_ALIGNMENT"),
+    (dict(p=A + 2), "FA_ERR_ALIGNMENT"), (dict(qs=_st(4, 64 * 128, 128)), "FA_ERR_STRIDE"), (dict(ks=_st(8, 16, 129)), "FA_ERR_STRIDE"),
+    (dict(ks=_st(8, 16, -128)), "FA_ERR_STRIDE"), (dict(qs=_st(3, 0, 128), B=1), "FA_OK"), (dict(qs=_st(4, 4, 4), it=2, ot=2), "FA_OK"),
+    (dict(ps=-1), "FA_ERR_STRIDE"), (dict(B=70000), "FA_ERR_TOO_LARGE"), (dict(H=65530), "FA_ERR_TOO_LARGE"), (dict(N=1 << 29), "FA_ERR_TOO_LARGE"),
+]
+
+
+@pytest.mark.parametrize("i", range(len(ROPE)))
+def test_validate_rope(capi, i):
+    kw, code = ROPE[i]
+    lib, a = capi.load(), _rope(**kw)
+    assert lib.fa_validate_rope(*a) == capi.STATUS[code]
+    if code != "FA_OK":
+        assert lib.fa_rope(*a[:15], 1.0, 0, 0, *a[15:], None) == capi.STATUS[code]
+
+
+def _append(**kw):
+    st = _st(8 * 5 * 128, 5 * 128, 128)
+    a = dict(q=A, qs=st, k=A, ks=st, v=A, vs=st, f=A, t=A, s=A, p=0, n=0, kp=A, vp=A, qo=A, ko=0, bad=A, B=2, H=8, Hkv=8, T=5, D=128, R=64,
+             size=16, mp=10, pages=100)
+    a.update(kw)
+    return list(a.values())
+
+
+APPEND = [
+    (dict(), "FA_OK"), (dict(bad=0), "FA_ERR_NULL_POINTER"), (dict(q=0), "FA_ERR_NULL_POINTER"), (dict(v=0), "FA_ERR_NULL_POINTER"),
+    (dict(vs=None), "FA_ERR_NULL_POINTER"), (dict(qo=0), "FA_ERR_NULL_POINTER"), (dict(t=0), "FA_ERR_NULL_POINTER"),
+    (dict(f=0), "FA_ERR_NULL_POINTER"), (dict(T=0, q=0, k=0, v=0, qo=0, qs=None, ks=None, vs=None), "FA_OK"), (dict(T=-1), "FA_ERR_SEQ_LEN"),
+    (dict(H=9), "FA_ERR_KV_HEADS"), (dict(H=0), "FA_ERR_KV_HEADS"), (dict(Hkv=0), "FA_ERR_BATCH_HEADS"), (dict(D=32, R=32), "FA_ERR_HEAD_DIM"),
+    (dict(R=8), "FA_ERR_ROT_DIM"), (dict(size=32), "FA_ERR_PAGE_SIZE"), (dict(mp=0), "FA_ERR_MAX_PAGES"), (dict(pages=0), "FA_ERR_NUM_PAGES"),
+    (dict(qs=_st(8, 8, 4)), "FA_ERR_STRIDE"), (dict(vs=_st(8, 8, -8)), "FA_ERR_STRIDE"), (dict(ko=A + 4), "FA_ERR_ALIGNMENT"),
+    (dict(p=A + 1), "FA_ERR_ALIGNMENT"), (dict(k=A + 2), "FA_ERR_ALIGNMENT"), (dict(H=64000, Hkv=1000), "FA_ERR_TOO_LARGE"),
+    (dict(T=(1 << 28) + 1), "FA_ERR_TOO_LARGE"),
+]
+
+
+@pytest.mark.parametrize("i", range(len(APPEND)))
+def test_validate_append(capi, i):
+    kw, code = APPEND[i]
+    lib, a = capi.load(), _append(**kw)
+    assert lib.fa_validate_kv_append_rope(*a) == capi.STATUS[code]
+    if code != "FA_OK":
+        assert lib.fa_kv_append_rope(*a[:22], 1.0, 0, *a[22:], 0, None) == capi.STATUS[code]
+
+
+def _shared(**kw):
+    a = dict(q=A, kp=A, vp=A, pt=A, pl=A, t=A, c=A, B=4, H=32, Hkv=8, D=128, size=16, pp=100, mp=20, pages=500, ws=A, o=A, l=A)
+    a.update(kw)
+    return list(a.values())
+
+
+SHARED = [
+    (dict(), "FA_OK"), (dict(q=0), "FA_ERR_NULL_POINTER"), (dict(pt=0), "FA_ERR_NULL_POINTER"), (dict(pl=0), "FA_ERR_NULL_POINTER"),
+    (dict(ws=0), "FA_ERR_NULL_POINTER"), (dict(o=0), "FA_ERR_NULL_POINTER"), (dict(l=0), "FA_ERR_NULL_POINTER"), (dict(H=30), "FA_ERR_KV_HEADS"),
+    (dict(Hkv=0), "FA_ERR_KV_HEADS"), (dict(D=96), "FA_ERR_HEAD_DIM"), (dict(B=0), "FA_ERR_BATCH_HEADS"), (dict(size=8), "FA_ERR_PAGE_SIZE"),
+    (dict(pp=0), "FA_ERR_MAX_PAGES"), (dict(mp=0), "FA_ERR_MAX_PAGES"), (dict(pages=0), "FA_ERR_NUM_PAGES"), (dict(ws=A + 4), "FA_ERR_ALIGNMENT"),
+    (dict(pl=A + 2), "FA_ERR_ALIGNMENT"), (dict(o=A + 2), "FA_ERR_ALIGNMENT"), (dict(pp=1 << 27), "FA_ERR_TOO_LARGE"),
+    (dict(B=40000, H=1000, Hkv=1), "FA_ERR_TOO_LARGE"), (dict(B=70000), "FA_ERR_TOO_LARGE"),
+]
+
+
+@pytest.mark.parametrize("i", range(len(SHARED)))
+def test_validate_shared(capi, i):
+    kw, code = SHARED[i]
+    lib, a = capi.load(), _shared(**kw)
+    assert lib.fa_validate_decode_shared(*a) == capi.STATUS[code]
+    if code != "FA_OK":
+        assert lib.fa_decode_shared(*a, 0, None) == capi.STATUS[code]
+
+
+def _weights(**kw):
+    a = dict(q=A, kp=A, vp=A, t=A, c=A, w=A, B=4, H=32, Hkv=8, D=128, size=16, mp=20, pages=500, S=16, ws=A, o=A, l=A, wo=A)
+    a.update(kw)
+    return list(a.values())
+
+
+WEIGHTS = [
+    (dict(), "FA_OK"), (dict(w=0), "FA_ERR_NULL_POINTER"), (dict(wo=0), "FA_ERR_NULL_POINTER"), (dict(ws=0), "FA_ERR_NULL_POINTER"),
+    (dict(l=0), "FA_ERR_NULL_POINTER"), (dict(S=0), "FA_ERR_NUM_SPLITS"), (dict(S=17), "FA_ERR_NUM_SPLITS"), (dict(H=30), "FA_ERR_KV_HEADS"),
+    (dict(D=32), "FA_ERR_HEAD_DIM"), (dict(w=A + 4), "FA_ERR_ALIGNMENT"), (dict(wo=A + 8), "FA_ERR_ALIGNMENT"), (dict(l=A + 1), "FA_ERR_ALIGNMENT"),
+    (dict(mp=1 << 20, B=2000, Hkv=32), "FA_OK"), (dict(mp=1 << 20, B=2000, H=64, Hkv=64), "FA_ERR_TOO_LARGE"), (dict(B=40000, H=1000, Hkv=1), "FA_ERR_TOO_LARGE"),
+]
+
+
+@pytest.mark.parametrize("i", range(len(WEIGHTS)))
+def test_validate_weights(capi, i):
+    kw, code = WEIGHTS[i]
+    lib, a = capi.load(), _weights(**kw)
+    assert lib.fa_validate_decode_weights(*a) == capi.STATUS[code]
+    if code != "FA_OK":
+        assert lib.fa_decode_paged_weights(*a, 0, None) == capi.STATUS[code]
+
+
+def _evict(**kw):
+    a = dict(kp=A, vp=A, t=A, c=A, w=A, nt=A, kept=A, nw=A, nl=A, bad=A, B=4, Hkv=8, D=128, keep=100, recent=10, size=16, mp=20, nmp=7, pages=500)
+    a.update(kw)
+    return list(a.values())
+
+
+EVICT = [
+    (dict(), "FA_OK"), *((({x: 0}), "FA_ERR_NULL_POINTER") for x in ("kp", "vp", "t", "c", "w", "nt", "kept", "nw", "nl", "bad")),
+    (dict(D=96), "FA_ERR_HEAD_DIM"), (dict(B=0), "FA_ERR_BATCH_HEADS"), (dict(size=4), "FA_ERR_PAGE_SIZE"), (dict(mp=0), "FA_ERR_MAX_PAGES"),
+    (dict(nmp=0), "FA_ERR_MAX_PAGES"), (dict(pages=-1), "FA_ERR_NUM_PAGES"), (dict(kp=A + 8), "FA_ERR_ALIGNMENT"), (dict(kept=A + 2), "FA_ERR_ALIGNMENT"),
+    (dict(keep=0), "FA_ERR_BUDGET"), (dict(keep=113), "FA_ERR_BUDGET"), (dict(keep=112), "FA_OK"), (dict(recent=-1), "FA_ERR_BUDGET"),
+    (dict(recent=101), "FA_ERR_BUDGET"), (dict(recent=100), "FA_OK"), (dict(mp=1 << 27), "FA_ERR_TOO_LARGE"), (dict(Hkv=70000), "FA_ERR_TOO_LARGE"),
+]
+
+
+@pytest.mark.parametrize("i", range(len(EVICT)))
+def test_validate_evict(capi, i):
+    kw, code = EVICT[i]
+    lib, a = capi.load(), _evict(**kw)
+    assert lib.fa_validate_kv_evict(*a) == capi.STATUS[code]
+    if code != "FA_OK":
+        assert lib.fa_kv_evict(*a, None) == capi.STATUS[code]
+
+
+def test_status_strings(capi):
+    lib = capi.load()
+    for name, word in (("FA_ERR_ROT_DIM", b"rot_dim"), ("FA_ERR_STRIDE", b"stride"), ("FA_ERR_TYPE", b"type"), ("FA_ERR_BUDGET", b"recent")):
+        assert word in lib.fa_status_str(capi.STATUS[name])
+
+
+@pytest.mark.parametrize("B,H,Hkv,D,pp,mp", [(1, 1, 1, 64, 1, 1), (32, 32, 8, 128, 500, 94), (64, 32, 8, 128, 2048, 63), (1, 32, 1, 128, 8192, 1),
+                                             (300, 32, 32, 64, 625, 1), (1, 128, 1, 128, 50, 2), (2000, 8, 8, 64, 10, 4000)])
+def test_shared_workspace(capi, B, H, Hkv, D, pp, mp):
+    """Room for 1 to 256 parts of the prefix and 1 to 16 of the own pages, D + 2 floats each; none for invalid sizes."""
+    lib = capi.load()
+    n = lib.fa_decode_shared_workspace_floats(B, H, Hkv, D, pp, mp)
+    parts, rest = divmod(n, B * H * (D + 2))
+    assert rest == 0 and 2 <= parts <= min(256, -(-pp // 4)) + min(16, -(-mp // 8))
+    for bad in ((0, H, Hkv, D, pp, mp), (B, H, H + 1, D, pp, mp), (B, H, Hkv, D, 0, mp), (B, H, Hkv, D, pp, -1), (B, 70000, 1, D, pp, mp)):
+        assert lib.fa_decode_shared_workspace_floats(*bad) == 0
+    assert lib.fa_decode_weights_workspace_floats(B, H, D, mp, 5) == B * H * (16 * mp + 5 * (D + 2))
+    assert lib.fa_decode_weights_workspace_floats(B, H, D, 0, 5) == 0
+
+
+def test_binding_refuses_host_tensors(fa):
+    x = torch.zeros(1, 2, 3, 64)
+    i = torch.zeros(1, dtype=torch.int32)
+    t = i[:, None]
+    f, _ = fa.rope_frequencies(64, device="cpu")
+    pool = torch.zeros(2, 2, 16, 64, dtype=torch.half)
+    w = torch.zeros(1, 2, 16)
+    for call in (lambda: fa.rope(x, x, f), lambda: fa.rope_backward(x, None, f),
+                 lambda: fa.kv_append_rope(x, x, x, pool, pool, t, i, f),
+                 lambda: fa.decode_shared(x[:, :, 0].half(), pool, pool, i, i, t, i),
+                 lambda: fa.decode_paged_weights(x[:, :, 0].half(), pool, pool, t, i, w),
+                 lambda: fa.kv_evict(pool, pool, t, i, w, t, 4, 1)):
+        with pytest.raises(RuntimeError, match="must be CUDA tensors"):
+            call()
+    with pytest.raises(RuntimeError, match="dtype must be"):
+        fa.rope_backward(x, None, f, dtype=torch.float64)
+
+
+# ---------------------------------------------------------------------------
+# rope_frequencies
+# ---------------------------------------------------------------------------
+def test_frequencies(fa):
+    for R, base in ((64, 10000.0), (16, 500000.0), (128, 1e6)):
+        f, scale = fa.rope_frequencies(R, base, device="cpu")
+        assert f.dtype == torch.float64 and scale == 1.0
+        assert np.allclose(f.numpy(), [base ** (-2 * i / R) for i in range(R // 2)], rtol=1e-14)
+        lin, scale = fa.rope_frequencies(R, base, "linear", 4.0, device="cpu")
+        assert torch.equal(lin, f / 4) and scale == 1.0
+        ntk, scale = fa.rope_frequencies(R, base, "ntk", 8.0, device="cpu")
+        assert scale == 1.0 and ntk[0] == 1 and float(f[-1] / ntk[-1]) == pytest.approx(8.0, rel=1e-12)
+        assert (ntk[1:] < f[1:]).all()
+        n = 4096
+        parts, scale = fa.rope_frequencies(R, base, "by_parts", 16.0, n, device="cpu")
+        assert scale == pytest.approx(0.1 * math.log(16) + 1)
+        turns = n * f / (2 * math.pi)
+        assert torch.equal(parts[turns > 32 * base ** (2 / R)], f[turns > 32 * base ** (2 / R)])
+        slow = turns < base ** (-2 / R)
+        assert torch.allclose(parts[slow], f[slow] / 16, rtol=1e-12)
+        ratio = (parts / f).numpy()
+        assert (np.diff(ratio) <= 1e-15).all() and ratio.max() <= 1 and ratio.min() >= 1 / 16 - 1e-15
+        same, scale = fa.rope_frequencies(R, base, "by_parts", 1.0, n, device="cpu")
+        assert torch.allclose(same, f, rtol=1e-14) and scale == 1.0
+
+
+def test_frequencies_refuse(fa):
+    for kw, word in ((dict(rot_dim=0), "rot_dim"), (dict(rot_dim=15), "rot_dim"), (dict(rot_dim=16, base=1.0), "base"),
+                     (dict(rot_dim=16, factor=0.5), "factor"), (dict(rot_dim=16, scaling="ramp"), "scaling"),
+                     (dict(rot_dim=2, scaling="ntk"), "ntk"), (dict(rot_dim=16, scaling="by_parts"), "original_len"),
+                     (dict(rot_dim=16, scaling="by_parts", original_len=10, slow_turns=5.0, fast_turns=5.0), "slow_turns"),
+                     (dict(rot_dim=16, base=math.nan), "base")):
+        with pytest.raises(RuntimeError, match=word):
+            fa.rope_frequencies(**kw, device="cpu")
+
+
+# ---------------------------------------------------------------------------
+# The oracles
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("inter", [False, True])
+def test_rotation_oracle(inter):
+    """By hand for one pair; scores of rotated rows depend on the positions' difference alone; back is the transpose."""
+    f = np.array([0.5, 0.01])
+    x = np.array([[1.0, 2.0, 3.0, 4.0, 9.0]])
+    y = rotary.rotate(x, [3], f, inter, 2.0)
+    i, j = ((0, 1) if inter else (0, 2))
+    a = 1.5
+    assert np.allclose([y[0, i], y[0, j]], [2 * (x[0, i] * math.cos(a) - x[0, j] * math.sin(a)),
+                                            2 * (x[0, j] * math.cos(a) + x[0, i] * math.sin(a))])
+    assert y[0, 4] == 9.0
+    rng = np.random.default_rng(0)
+    q, k, g = rng.standard_normal((3, 6, 4))
+    at = lambda p: (rotary.rotate(q, p + 5, f, inter) * rotary.rotate(k, p, f, inter)).sum(-1)
+    assert np.allclose(at(np.arange(6)), at(np.arange(6) + 1000))
+    p = np.arange(6) * 11
+    assert np.allclose((g * rotary.rotate(q, p, f, inter, 1.5)).sum(), (rotary.rotate(g, p, f, inter, 1.5, True) * q).sum())
+
+
+def test_cache_oracles():
+    """A shared prefix is the same keys in every sequence; a head's weights sum to its query heads; eviction keeps what
+    a sort by hand keeps."""
+    rng = np.random.default_rng(0)
+    kp, vp = rng.standard_normal((2, 9, 2, 16, 8))
+    q = rng.standard_normal((2, 4, 8))
+    prefix, table = np.array([3, 0]), np.array([[5, 6], [7, 8]])
+    o, l, _, _ = cache.decode_shared(q, kp, vp, prefix, 32, table, [20, 3], 0.0)
+    joined = np.concatenate([np.tile(prefix, (2, 1)), table], 1)
+    o2, l2, w, _, _, _ = cache.decode_weights(q, kp, vp, joined, [52, 35], np.zeros((2, 2, 64)), 0.0)
+    assert np.allclose(o, o2) and np.allclose(l, l2) and np.allclose(w.sum(-1), 2.0) and not w[1, :, 35:].any()
+    w = np.array([[[5, 1, 5, 2, 5, 9, 0, 0, 1, 3] + [0] * 6]], np.float32)
+    k, v = rng.standard_normal((2, 4, 1, 16, 8))
+    k2, v2, kept, nw, n, bad = cache.evict(k, v, np.array([[2]]), [10], w, np.array([[1]]), 5, 2)
+    assert kept.tolist() == [[[0, 2, 5, 8, 9]]] and nw[0, 0, :6].tolist() == [5, 5, 9, 1, 3, 0] and n == [5] and bad == [0]
+    assert np.array_equal(k2[1, 0, :5], k[2, 0, [0, 2, 5, 8, 9]]) and np.array_equal(k2[1, 0, 5:], k[1, 0, 5:])

@@ -1,0 +1,268 @@
+"""GPU tier of the decode over a shared prefix (decode_shared) against its
+restatement in 64 bits (oracle/cache.py, which derives the bounds)."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import cache
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"fp16": torch.float16, "bf16": torch.bfloat16}
+HALF = {"fp16": 2.0 ** -11, "bf16": 2.0 ** -8}
+
+
+def _i32(dev, x):
+    return torch.tensor(x, dtype=torch.int32, device=dev)
+
+
+def _case(dev, seed, B, H, Hkv, D, P, ctx, dtype, poison=True, spare=3, extra=0, amp=1.0):
+    """Pools, tables and lengths; slots that no sequence has hold NaN, spare table entries an invalid page."""
+    rng = np.random.default_rng(seed)
+    need = [-(-n // 16) for n in [P, *ctx]]
+    pages = sum(need) + spare
+    perm = rng.permutation(pages).astype(np.int32)
+    prefix = np.full(max(1, need[0] + extra), -1 if extra else 0, np.int32)
+    table = np.full((B, max(1, max(need[1:], default=0) + extra)), -1 if extra else 0, np.int32)
+    prefix[:need[0]] = perm[:need[0]]
+    at = need[0]
+    for b, n in enumerate(need[1:]):
+        table[b, :n] = perm[at:at + n]
+        at += n
+    g = torch.Generator(device=dev)
+    g.manual_seed(seed)
+    pools = []
+    for _ in range(2):
+        x = torch.randn((pages, Hkv, 16, D), generator=g, device=dev, dtype=TYPES[dtype])
+        if poison:
+            keep = torch.zeros(pages, 16, dtype=torch.bool)
+            for n, ids in zip([P, *ctx], [prefix, *table]):
+                for j in range(-(-n // 16)):
+                    keep[int(ids[j]), :min(16, n - 16 * j)] = True
+            x = torch.where(keep.to(dev)[:, None, :, None], x, torch.full_like(x, math.nan))
+        pools.append(x)
+    q = (torch.randn((B, H, D), generator=g, device=dev) * amp).to(TYPES[dtype])
+    return q, *pools, torch.from_numpy(prefix).to(dev), _i32(dev, [P]), torch.from_numpy(table).to(dev), _i32(dev, ctx)
+
+
+def _want(case, dtype):
+    q, kp, vp, prefix, plen, table, ctx = case
+    f = lambda t: t.cpu().double().numpy()
+    return cache.decode_shared(f(q), f(kp), f(vp), prefix.cpu().numpy(), int(plen), table.cpu().numpy(),
+                               ctx.tolist(), HALF[dtype])
+
+
+def _check(got, want, dtype, tag=""):
+    O, L = got
+    o, l, to, tl = want
+    assert O.dtype == TYPES[dtype] and L.dtype == torch.float32 and O.shape == o.shape and L.shape == l.shape
+    eo = np.abs(O.cpu().double().numpy() - o)
+    assert (eo <= to).all(), f"{tag} O: worst {np.nanmax(eo / to):.2f} of the bound, {np.isnan(eo).sum()} NaN"
+    lg = L.cpu().double().numpy()
+    empty = np.isneginf(l)
+    assert np.array_equal(np.isneginf(lg), empty), tag
+    el = np.abs(lg[~empty] - l[~empty])
+    assert (el <= tl[~empty]).all(), f"{tag} L: worst {(el / tl[~empty]).max():.2f} of the bound"
+
+
+CASES = [
+    # B, H, Hkv, D, P, own lengths
+    (1, 1, 1, 64, 1, [0]), (1, 1, 1, 128, 16, [1]), (2, 8, 2, 64, 63, [0, 5]), (3, 4, 4, 128, 64, [1, 16, 17]),
+    (4, 8, 8, 64, 65, [300, 0, 2, 64]), (2, 32, 8, 128, 500, [33, 700]), (5, 6, 2, 128, 129, [1, 2, 3, 4, 5]),
+    (9, 16, 4, 64, 1000, [40] * 9), (16, 32, 8, 128, 700, list(range(0, 160, 10))), (33, 4, 1, 64, 257, [7] * 33),
+    (31, 36, 4, 128, 300, [9 * i % 50 for i in range(31)]), (70, 8, 2, 64, 333, [3 * i for i in range(70)]),
+    (1, 128, 1, 128, 800, [20]), (3, 40, 2, 64, 2100, [100, 0, 17]), (2, 2, 1, 128, 0, [70, 0]), (2, 4, 2, 64, 15, [0, 0]),
+    (40, 32, 8, 128, 70, [2] * 40),
+]
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("i", range(len(CASES)))
+def test_matches_oracle(fa, dev, i, dtype):
+    B, H, Hkv, D, P, ctx = CASES[i]
+    case = _case(dev, i, B, H, Hkv, D, P, ctx, dtype, extra=i % 3)
+    got = fa.decode_shared(*case)
+    _check(got, _want(case, dtype), dtype, f"case {CASES[i][:5]}")
+    again = fa.decode_shared(*case)
+    assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
+
+
+@pytest.mark.parametrize("P", [1, 15, 16, 17, 31, 32, 33, 48, 63, 64, 65, 127, 128, 129, 191, 193, 255, 256, 257])
+@pytest.mark.parametrize("D,dtype", [(64, "bf16"), (128, "fp16")])
+def test_prefix_lengths(fa, dev, P, D, dtype):
+    """The prefix ends at every place of a page, a tile and the ring of tiles."""
+    case = _case(dev, P, 3, 8, 2, D, P, [5, 0, 31], dtype)
+    _check(fa.decode_shared(*case), _want(case, dtype), dtype)
+
+
+@pytest.mark.parametrize("B,H,Hkv,D,dtype", [(8, 32, 8, 128, "fp16"), (40, 32, 8, 128, "bf16"), (33, 8, 8, 64, "fp16"), (20, 32, 2, 64, "bf16")])
+def test_long_prefix(fa, dev, B, H, Hkv, D, dtype):
+    """Long enough for more than 64 tiles a workgroup in a table far wider than the prefix, and for splits of a few."""
+    for P, extra in ((20000, 0), (9001, 700)):
+        case = _case(dev, P, B, H, Hkv, D, P, [11 * b for b in range(B)], dtype, poison=False, extra=extra)
+        q, kp, vp, prefix, plen, table, ctx = case
+        some = [0, B // 2, B - 1]   # the oracle's time: some sequences
+        got = fa.decode_shared(*case)
+        sub = (q[some], kp, vp, prefix, plen, table[some], ctx[some])
+        _check([x[some] for x in got], _want(sub, dtype), dtype, f"P {P}")
+
+
+def test_many_tiles_a_workgroup(fa, dev):
+    """32 KV heads and 300 query rows of each: one run of over 64 tiles, three row blocks."""
+    case = _case(dev, 3, 300, 32, 32, 64, 10000, [b % 3 for b in range(300)], "fp16", poison=False)
+    q, kp, vp, prefix, plen, table, ctx = case
+    some = [0, 127, 128, 299]
+    got = fa.decode_shared(*case)
+    _check([x[some] for x in got], _want((q[some], kp, vp, prefix, plen, table[some], ctx[some]), "fp16"), "fp16")
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_invalid_pages_and_lengths(fa, dev, D, dtype):
+    """An invalid own page or length makes its sequence NaN, an invalid prefix all of them."""
+    ctx = [40, 40, 40, 0, 16]
+    case = list(_case(dev, 4, 5, 8, 2, D, 200, ctx, dtype, spare=1))
+    good = fa.decode_shared(*case)
+    pages = case[1].shape[0]
+    t = case[5].clone()
+    t[0, 1], t[1, 2] = -1, pages
+    c = case[6].clone()
+    c[2] = 16 * t.shape[1] + 1
+    c[4] = -1
+    O, L = fa.decode_shared(*case[:5], t, c)
+    for b in (0, 1, 2, 4):
+        assert torch.isnan(O[b]).all() and torch.isnan(L[b]).all(), b
+    assert torch.equal(O[3], good[0][3]) and torch.equal(L[3], good[1][3])
+    for at, page in ((0, -5), (12, pages), (5, 2 ** 31 - 1)):
+        p = case[3].clone()
+        p[at] = page
+        O, L = fa.decode_shared(*case[:3], p, *case[4:])
+        assert torch.isnan(O).all() and torch.isnan(L).all(), (at, page)
+    for n in (-1, 16 * case[3].numel() + 1, 2 ** 31 - 1):
+        O, L = fa.decode_shared(*case[:4], _i32(dev, [n]), *case[5:])
+        assert torch.isnan(O).all() and torch.isnan(L).all(), n
+    p = case[3].clone()   # entries past the prefix are not looked at
+    p[4:] = -1
+    O, L = fa.decode_shared(*case[:3], p, _i32(dev, [64]), *case[5:])
+    assert torch.isfinite(O).all() and torch.isfinite(L).all()
+
+
+def test_no_prefix_is_the_paged_decode(fa, dev):
+    """Of an empty prefix O and L are decode_paged's, within both bounds."""
+    case = _case(dev, 5, 4, 8, 2, 128, 0, [100, 1, 0, 777], "fp16")
+    got = fa.decode_shared(*case)
+    _check(got, _want(case, "fp16"), "fp16")
+    assert (got[0][2] == 0).all() and torch.isneginf(got[1][2]).all()
+
+
+def test_prefix_in_the_own_pages(fa, dev):
+    """The same keys shared, and as the start of every sequence's own pages: one result within the bounds."""
+    case = _case(dev, 6, 6, 16, 4, 64, 160, [30, 1, 0, 64, 15, 16], "bf16")
+    q, kp, vp, prefix, plen, table, ctx = case
+    joined = torch.cat((prefix[:10].expand(6, 10), table), 1).contiguous()
+    _check(fa.decode_shared(q, kp, vp, prefix, plen * 0, joined, ctx + 160), _want(case, "bf16"), "bf16")
+    _check(fa.decode_shared(*case), _want(case, "bf16"), "bf16")
+
+
+def test_sharp_and_large_scores(fa, dev):
+    """Scores of hundreds: a few keys carry the weight, and the maximum moves along the keys."""
+    for amp in (8.0, 60.0):
+        case = _case(dev, 7, 4, 8, 2, 64, 700, [50, 0, 3, 100], "fp16", amp=amp)
+        _check(fa.decode_shared(*case), _want(case, "fp16"), "fp16", f"amp {amp}")
+
+
+def test_masked_by_minus_infinity(fa, dev):
+    """Keys whose scores are -inf (their K holds infinities) have no weight, a whole tile of them included."""
+    D, P = 64, 256
+    q, kp, vp, prefix, plen, table, ctx = _case(dev, 8, 2, 4, 2, D, P, [16, 3], "fp16")
+    q[..., 0] = q[..., 0].abs() + 0.5
+    kp[prefix[:8].long(), :, :, 0] = -math.inf   # the first 128 keys
+    kp[prefix[12].long(), :, 3:9, 0] = -math.inf
+    O, L = fa.decode_shared(q, kp, vp, prefix, plen, table, ctx)
+    f = lambda t: t.cpu().double().numpy()
+    live = np.ones(P, bool)
+    live[:128] = False
+    live[12 * 16 + 3:12 * 16 + 9] = False
+    for b in range(2):
+        for h in range(4):
+            k, v = (np.concatenate([cache.rows(f(x), prefix.cpu().numpy(), P, h // 2)[live],
+                                    cache.rows(f(x), table[b].cpu().numpy(), int(ctx[b]), h // 2)]) for x in (kp, vp))
+            o, l, _, to, tl, _ = cache.attend(f(q[b, h:h + 1]), k, v, HALF["fp16"])
+            assert (np.abs(f(O[b, h]) - o[0]) <= to[0]).all() and abs(float(L[b, h]) - l[0]) <= tl[0]
+
+
+def test_nan_stays_in_its_head(fa, dev):
+    """A NaN in a key of the prefix, or in an own value, reaches every query that sees it and no other."""
+    case = _case(dev, 9, 3, 8, 4, 64, 100, [20, 20, 20], "fp16")
+    q, kp, vp, prefix, plen, table, ctx = case
+    good = fa.decode_shared(*case)
+    kp[int(prefix[2]), 1, 5, 7] = math.nan
+    vp[int(table[2, 0]), 3, 4, 9] = math.nan
+    O, L = fa.decode_shared(*case)
+    hit = torch.zeros(3, 8, dtype=torch.bool, device=dev)
+    hit[:, 2:4] = True
+    assert torch.isnan(O[hit]).all() and torch.isnan(L[hit]).all()
+    hit[2, 6:8] = True
+    assert torch.isnan(O[2, 6:8, 9]).all()
+    assert torch.equal(O[~hit], good[0][~hit]) and torch.equal(L[~hit], good[1][~hit])
+
+
+def test_far_pages(fa, dev):
+    """Pages past 2^31 values of a pool."""
+    Hkv, D = 8, 128
+    pages = (1 << 31) // (Hkv * 16 * D) + 40
+    case = _case(dev, 10, 2, 16, Hkv, D, 150, [40, 9], "bf16", spare=0)
+    q, kp, vp, prefix, plen, table, ctx = case
+    n = kp.shape[0]
+    far = []
+    for x in (kp, vp):
+        y = torch.empty(pages, Hkv, 16, D, dtype=x.dtype, device=dev)
+        y[pages - n:] = x
+        far.append(y)
+    got = fa.decode_shared(q, *far, prefix + (pages - n), plen, table + (pages - n), ctx)
+    want = fa.decode_shared(*case)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_graphs_replayed_in_turn(fa, dev):
+    """Two captured calls that may share a workspace's memory, replayed with new lengths and queries, eager calls between."""
+    side = torch.cuda.Stream()
+    runs = []
+    for seed, shape in ((11, (3, 8, 2, 64, 300, [50, 3, 0])), (12, (17, 32, 8, 128, 900, [5 * i for i in range(17)]))):
+        case = _case(dev, seed, *shape, "fp16", poison=False)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            fa.decode_shared(*case)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = fa.decode_shared(*case)
+        runs.append((case, graph, out))
+    for i in range(4):
+        for case, graph, out in runs:
+            case[0].copy_(torch.randn_like(case[0]))
+            case[4].fill_(17 * i + 1)
+            case[6].clamp_(max=40 - 9 * i)
+            graph.replay()
+        for case, graph, out in runs:
+            want = fa.decode_shared(*case)
+            torch.cuda.synchronize()
+            assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1]), i
+            _check(out, _want(case, "fp16"), "fp16")
+
+
+def test_two_streams(fa, dev):
+    cases = [_case(dev, 13 + i, 6, 16, 4, 128, 600 + 100 * i, [40, 0, 9, 100, 1, 64], "bf16") for i in range(2)]
+    want = [fa.decode_shared(*c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(fa.decode_shared(*cases[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(a, want[i][0]) and torch.equal(b, want[i][1]) for a, b in got[i])
