@@ -305,15 +305,15 @@ def decode_shared(q, k_pool, v_pool, prefix_table, prefix_len, page_table, ctx_l
     return _C.decode_shared(q, k_pool, v_pool, prefix_table, prefix_len, page_table, ctx_lens)
 
 
-def decode_paged_weights(q, k_pool, v_pool, page_table, ctx_lens, weights, num_splits: int = 16,
-                         inplace: bool = False):
+def decode_paged_weights(q, k_pool, v_pool, page_table, ctx_lens, weights, inplace: bool = False):
     """[O, L, W]: decode_paged, and W = weights with the attention weight of every cached
     token added, summed over the query heads of its KV head (fp32 [B,H_kv,max_pages*16]).
 
     inplace: W is weights itself. Slots past a context keep their value; where O and L
-    are NaN (an invalid page or length), W is NaN over the context.
+    are NaN (an invalid page or length), W is NaN over the context. The split over the
+    pages follows the batch's lengths, on the device.
     """
-    return _C.decode_paged_weights(q, k_pool, v_pool, page_table, ctx_lens, weights, num_splits, inplace)
+    return _C.decode_paged_weights(q, k_pool, v_pool, page_table, ctx_lens, weights, inplace)
 
 
 def kv_evict(k_pool, v_pool, page_table, ctx_lens, weights, new_page_table, keep: int, recent: int):

@@ -14,127 +14,107 @@
 #include <math.h>
 #include <stdint.h>
 
-#include "fa_decode.hpp"
 #include "fa_mi355x.h"
 #include "fa_pages.hpp"
+#include "fa_stream.hpp"
 #include "fa_tile.hpp"
 
 namespace fa {
 namespace cache {
 
+using namespace stream;
 using pages::kPageSize;
-constexpr int kThreads = 256;
-constexpr int kMaxSplits = 16;
 
-template <int D, bool BF16>
-__global__ void __launch_bounds__(kDecThreads)
-fa_weights_split_kernel(const typename DecT<BF16>::e* __restrict__ q,
-                        const typename DecT<BF16>::e* __restrict__ kpool,
-                        const typename DecT<BF16>::e* __restrict__ vpool,
-                        const int32_t* __restrict__ page_table,
-                        const int32_t* __restrict__ ctx_lens, float* __restrict__ part_o,
-                        float* __restrict__ part_ml, float* __restrict__ scores, int H, int Hkv,
-                        int max_pages, int num_pages, int S, int ordered, float c) {
-  __shared__ DecShared<D> sh;
-  decode_split_body<D, BF16, true, true>(sh, blockIdx.x, blockIdx.y, blockIdx.z, gridDim.z, q, kpool,
-                                         vpool, page_table, ctx_lens, part_o, part_ml, nullptr, nullptr,
-                                         H, Hkv, max_pages, num_pages, S, ordered, c, scores);
+// Pools from this size on do not stay in the caches between two steps; their pages
+// are read with the non-temporal hint.
+constexpr int64_t kPassThrough = 64 << 20;
+
+// Floats from a head's scores to the next head's: an odd number of 256 bytes, not
+// the table's power of two, at which all heads' scores of a page would meet in the
+// same memory channels.
+__host__ __device__ inline int64_t score_row(int64_t max_pages) {
+  return ((max_pages * kPageSize + 63) / 64 | 1) * 64;
 }
 
-// Maximum and sum over a row's S splits, in units of log 2: (-inf, 0) where all
-// are empty, a NaN sum where one is.
-__device__ __forceinline__ float2 join_splits(const float2* __restrict__ ml, int S) {
-  float2 x[kMaxSplits];
-#pragma unroll
-  for (int s = 0; s < kMaxSplits; ++s) x[s] = s < S ? ml[s] : make_float2(-INFINITY, 0.f);
-  float M = -INFINITY, z = 0.f;
-#pragma unroll
-  for (int s = 0; s < kMaxSplits; ++s) M = fmaxf(M, x[s].x);
-#pragma unroll
-  for (int s = 0; s < kMaxSplits; ++s) z += x[s].x == -INFINITY ? x[s].y : x[s].y * exp2_hw(x[s].x - M);
-  return make_float2(M, z);
+template <int D, bool BF16, bool NT>
+__global__ void __launch_bounds__(stream::kThreads)
+fa_weights_chunk_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_pool,
+                        const char* __restrict__ v_pool, const int32_t* __restrict__ page_table,
+                        const int32_t* __restrict__ ctx_lens, const int4* __restrict__ table,
+                        float* __restrict__ part_o, float2* __restrict__ part_ml,
+                        int2* __restrict__ first, float* __restrict__ scores, int B, int H, int Hkv,
+                        int group, int ngrp, int max_pages, int num_pages, Plan plan, float c) {
+  __shared__ Shared<D> sh;
+  const Place at = place_of(blockIdx.x, Hkv * ngrp);
+  const Run r = run_of(ctx_lens, table, B, max_pages, plan, at.number);
+  if (r.b < 0) return;
+  if (at.hg == 0 && r.split == 0 && threadIdx.x == 0) first[r.b] = make_int2(at.number, r.splits);
+  const int hk = at.hg / ngrp, sub = at.hg - hk * ngrp, col = threadIdx.x & 15;
+  const int h = hk * group + 16 * sub + col;
+  const bool live = 16 * sub + col < group;
+  chunk_body<D, BF16, NT, true>(sh, q, k_pool, v_pool, page_table + (size_t)r.b * max_pages, r.p0, r.p1,
+                                r.ctx, r.bad, live, ((int64_t)r.b * H + h) * D, hk, Hkv, num_pages, c,
+                                scores + ((int64_t)r.b * H + h - col) * score_row(max_pages),
+                                score_row(max_pages), min(16, group - 16 * sub), part_o, part_ml,
+                                (int64_t)at.number * H + h);
 }
 
-constexpr int kChunk = 4 * kThreads;   // slots of a workgroup that writes weights
+constexpr int kChunk = 4 * kJoinThreads;   // slots of a workgroup that writes weights
 
-// Workgroups [0, rows): O and L of one row (b, h) out of its S partials. The
-// others: weights of kChunk slots of one (b, KV head), group heads in order, so
-// the same call gives the same bits.
+// Workgroups [0, rows): O and L of one row (b, h) out of its chunks. The others:
+// weights of kChunk slots of one (b, KV head), group heads in order, so the same
+// call gives the same bits.
 template <int D, bool BF16>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kJoinThreads)
 fa_weights_join_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml,
-                       const float* __restrict__ scores, const int32_t* __restrict__ ctx_lens,
-                       const float* w_in, float* w_out, typename DecT<BF16>::e* __restrict__ o,
-                       float* __restrict__ lse, int H, int Hkv, int max_pages, int S, int rows,
-                       int row_blocks, int chunks) {
-  typedef typename DecT<BF16>::e e4 __attribute__((ext_vector_type(4)));
-  const int tid = threadIdx.x;
-  constexpr int PER = D / 4;
-  if ((int)blockIdx.x < row_blocks) {
-    const int row = blockIdx.x * (kThreads / PER) + tid / PER;
-    if (row >= rows) return;
-    const int d = 4 * (tid % PER);
-    const float2* ml = part_ml + (size_t)row * S;
-    const float* po = part_o + (size_t)row * S * D + d;
-    f32x4 ps[kMaxSplits];
-#pragma unroll
-    for (int s = 0; s < kMaxSplits; ++s)
-      ps[s] = s < S ? *reinterpret_cast<const f32x4*>(po + (size_t)s * D) : f32x4{};
-    const float2 J = join_splits(ml, S);
-    f32x4 out = f32x4{};
-    if (J.y != 0.f) {   // a NaN sum: NaN
-      const float inv = 1.f / J.y;
-#pragma unroll
-      for (int s = 0; s < kMaxSplits; ++s) {
-        if (s < S) {
-          const float2 x = ml[s];
-          const float w = x.x == -INFINITY ? x.y : x.y * exp2_hw(x.x - J.x) * inv;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) out[i] = fmaf(w, ps[s][i], out[i]);
-        }
-      }
-    }
-    e4 v;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = (typename DecT<BF16>::e)out[i];
-    *reinterpret_cast<e4*>(o + (size_t)row * D + d) = v;
-    if (d == 0) lse[row] = J.y == 0.f ? -INFINITY : (J.x + log2_hw(J.y)) * kLn2;
+                       const int2* __restrict__ first_of, const float* __restrict__ scores,
+                       const int32_t* __restrict__ ctx_lens, const float* w_in, float* w_out,
+                       uint16_t* __restrict__ o, float* __restrict__ lse, int H, int Hkv,
+                       int max_pages, int rows, int chunks, float c) {
+  const int tid = threadIdx.x, wave = tid >> 6;
+  if ((int)blockIdx.x < rows) {
+    __shared__ JoinShared<D> sh;
+    const int row = blockIdx.x, b = row / H;
+    const int2 f = first_of[b];
+    const Parts a{part_o, part_ml, (int64_t)f.x * H + (row - b * H), H, f.y};
+    join_row<D, BF16>(sh, a, Parts{part_o, part_ml, 0, 0, 0}, c, o + (int64_t)row * D, lse + row);
     return;
   }
-  const int unit = (int)blockIdx.x - row_blocks;
+  const int unit = (int)blockIdx.x - rows;
   const int bh = unit / chunks;   // b * Hkv + hk
   const int b = bh / Hkv, hk = bh - b * Hkv;
   const int G = H / Hkv;
   const int64_t width = (int64_t)max_pages * kPageSize;
-  const int64_t first = (int64_t)(unit - bh * chunks) * kChunk;
+  const int64_t start = (int64_t)(unit - bh * chunks) * kChunk;
   int64_t ctx = ctx_lens[b];
   ctx = ctx < 0 ? 0 : (ctx > width ? width : ctx);
-  const bool in_place = w_in == w_out;
-  if (first >= ctx && in_place) return;
-  const int64_t j = first + 4 * tid;
+  if (start >= ctx && w_in == w_out) return;
+  const int64_t j = start + 4 * tid;
   const bool there = j < width;   // width is a multiple of 16
   const int64_t at = (int64_t)bh * width + j;
   f32x4 w = f32x4{};
   if (there) w = *reinterpret_cast<const f32x4*>(w_in + at);
-  if (first < ctx) {
-    __shared__ float M[kThreads], inv[kThreads];   // of a group's heads
+  if (start < ctx) {
+    __shared__ float2 J[kJoinThreads];   // of a group's heads: maximum, 1 / sum
+    const int2 f = first_of[b];
     f32x4 sum = f32x4{};
-    for (int g0 = 0; g0 < G; g0 += kThreads) {
-      const int gs = min(kThreads, G - g0);
+    for (int g0 = 0; g0 < G; g0 += kJoinThreads) {
+      const int gs = min(kJoinThreads, G - g0);
       if (g0 > 0) __syncthreads();
-      if (tid < gs) {
-        const float2 J = join_splits(part_ml + ((size_t)b * H + (size_t)hk * G + g0 + tid) * S, S);
-        M[tid] = J.x;
-        inv[tid] = 1.f / J.y;
+      for (int g = wave; g < gs; g += kJoinThreads / 64) {
+        const float2 x = join_wave(Parts{part_o, part_ml, (int64_t)f.x * H + hk * G + g0 + g, H, f.y}, c);
+        if ((tid & 63) == 0) J[g] = make_float2(x.x, 1.f / x.y);
       }
       __syncthreads();
       if (there && j < ctx) {
-        const float* sc = scores + ((size_t)b * H + (size_t)hk * G + g0) * width + j;
+        const int64_t next = score_row(max_pages);
+        const float* sc = scores + ((int64_t)b * H + hk * G + g0) * next + j;
 #pragma unroll 4
         for (int g = 0; g < gs; ++g) {
-          const f32x4 x = *reinterpret_cast<const f32x4*>(sc + (size_t)g * width);
+          const f32x4 x = *reinterpret_cast<const f32x4*>(sc + g * next);
+          const float2 Jg = J[g];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) sum[i] = fmaf(exp2_hw(x[i] - M[g]), inv[g], sum[i]);
+          for (int i = 0; i < 4; ++i) sum[i] = fmaf(exp2_hw((x[i] - Jg.x) * c), Jg.y, sum[i]);
         }
       }
     }
@@ -145,37 +125,50 @@ fa_weights_join_kernel(const float* __restrict__ part_o, const float2* __restric
   if (there) *reinterpret_cast<f32x4*>(w_out + at) = w;
 }
 
-template <bool BF16>
+// The workspace, in floats: the scores first, then the
+// chunks' partial O, their maxima and sums, the sequences' first chunks and, of
+// more sequences than a wave plans, the table of chunks.
+struct Workspace {
+  int64_t most, part_o, part_ml, first, table, floats;
+};
+static Workspace workspace_of(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t max_pages) {
+  Workspace w;
+  w.most = most_chunks(B, max_pages, plan_of(head_groups(H, Hkv)));
+  w.part_o = B * H * score_row(max_pages);
+  w.part_ml = w.part_o + w.most * H * D;
+  w.table = w.part_ml + (2 * w.most * H + 3) / 4 * 4;
+  w.first = w.table + (B > kWavePlan ? 4 * (1 + w.most) : 0);
+  w.floats = w.first + 2 * B;
+  return w;
+}
+
+template <int D, bool BF16>
 static int decode_weights(const void* q, const void* k_pool, const void* v_pool,
                           const int32_t* page_table, const int32_t* ctx_lens, const float* w_in,
-                          int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t max_pages,
-                          int64_t num_pages, int64_t S, float* ws, void* o, float* lse, float* w_out,
-                          void* stream) {
-  using E = typename DecT<BF16>::e;
+                          int64_t B, int64_t H, int64_t Hkv, int64_t max_pages, int64_t num_pages,
+                          float* ws, void* o, float* lse, float* w_out, void* stream) {
   const float c = (float)(1.0 / sqrt((double)D)) * kLog2e;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const int64_t width = max_pages * kPageSize, rows = B * H;
-  float* scores = ws;   // first: 16-byte aligned rows
-  float* part_o = scores + rows * width;
-  float* part_ml = part_o + rows * S * D;
-  const dim3 grid((unsigned)S, (unsigned)decode_head_groups(H, Hkv), (unsigned)B);
-  const int ordered = decode_ordered(B, H, Hkv, D, S, stream_topology(s).cus);
-  const int64_t row_blocks = (rows + kThreads / (D / 4) - 1) / (kThreads / (D / 4));
-  const int64_t chunks = (width + kChunk - 1) / kChunk;
-  const int64_t join = row_blocks + B * Hkv * chunks;
-#define FA_WEIGHTS(DD)                                                                             \
-  do {                                                                                             \
-    hipLaunchKernelGGL((fa_weights_split_kernel<DD, BF16>), grid, dim3(kDecThreads), 0, s,         \
-                       (const E*)q, (const E*)k_pool, (const E*)v_pool, page_table, ctx_lens,      \
-                       part_o, part_ml, scores, (int)H, (int)Hkv, (int)max_pages, (int)num_pages, \
-                       (int)S, ordered, c);                                                        \
-    hipLaunchKernelGGL((fa_weights_join_kernel<DD, BF16>), dim3((unsigned)join), dim3(kThreads), 0, \
-                       s, part_o, (const float2*)part_ml, scores, ctx_lens, w_in, w_out, (E*)o, lse, (int)H,     \
-                       (int)Hkv, (int)max_pages, (int)S, (int)rows, (int)row_blocks, (int)chunks); \
-  } while (0)
-  if (D == 128) FA_WEIGHTS(128);
-  else FA_WEIGHTS(64);
-#undef FA_WEIGHTS
+  const Workspace w = workspace_of(B, H, Hkv, D, max_pages);
+  const int64_t groups = head_groups(H, Hkv), rows = B * H;
+  const Plan plan = plan_of(groups);
+  float* part_o = ws + w.part_o;
+  float2* part_ml = (float2*)(ws + w.part_ml);
+  int2* first = (int2*)(ws + w.first);
+  int4* table = B > kWavePlan ? (int4*)(ws + w.table) : nullptr;
+  if (table != nullptr)
+    hipLaunchKernelGGL(fa_stream_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, ctx_lens, (int)B,
+                       (int)max_pages, plan, table);
+  const bool nt = num_pages * Hkv * kPageSize * D * 4 >= kPassThrough;
+  const auto kernel = nt ? fa_weights_chunk_kernel<D, BF16, true> : fa_weights_chunk_kernel<D, BF16, false>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)chunk_blocks(w.most, groups)), dim3(stream::kThreads), 0, s,
+                     (const uint16_t*)q, (const char*)k_pool, (const char*)v_pool, page_table, ctx_lens,
+                     table, part_o, part_ml, first, ws, (int)B, (int)H, (int)Hkv, (int)(H / Hkv),
+                     (int)(groups / Hkv), (int)max_pages, (int)num_pages, plan, c);
+  const int64_t chunks = (max_pages * kPageSize + kChunk - 1) / kChunk;
+  hipLaunchKernelGGL((fa_weights_join_kernel<D, BF16>), dim3((unsigned)(rows + B * Hkv * chunks)),
+                     dim3(kJoinThreads), 0, s, part_o, part_ml, first, ws, ctx_lens, w_in, w_out,
+                     (uint16_t*)o, lse, (int)H, (int)Hkv, (int)max_pages, (int)rows, (int)chunks, c);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? FA_OK : -(int)e;
 }
@@ -193,218 +186,404 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 
 constexpr int kSelThreads = 1024;
 constexpr int kSelWaves = kSelThreads / 64;
-constexpr int kCopies = 16;   // histograms side by side: lanes of a wave share a counter four at most
+constexpr int kBins = 2048, kCopies = 4;   // counters of a digit, side by side for lanes of a wave
+constexpr int kMostKeys = 32;              // of a thread's keys in registers
+constexpr int kListKeys = 4;               // up to which the selection also lists the stayers
+constexpr int kSubRuns = 4, kRuns = kSelWaves * kSubRuns;   // of a wave's slots, of the candidates
+
+// What is known of a (b, KV head) after its selection: tokens with keys above
+// `key` stay, and of those equal to it the first `left`. The candidates, all but
+// the newest tokens, are cut into runs: kSelWaves of `per` slots, of each kSubRuns
+// of `sub`. gt and eq count the keys above and equal before a run.
+struct Selection {
+  int n, cand, per, sub, left;   // n: the length, 0 of an invalid one; cand 0: every token stays
+  uint32_t key;
+  int gt[kRuns], eq[kRuns];
+};
+constexpr int kSelWords = sizeof(Selection) / 4;
 
 // One workgroup per (b, KV head): which tokens stay. The `recent` last ones do,
 // and of the others the keep - recent heaviest: the key of the last of these is
-// found digit by digit (8 bits, histograms in LDS), equal ones stay from the
-// lowest slot on. Then the stayers are written out in order, waves taking one
-// run of slots each.
+// found digit by digit (11, 11 and 10 bits, histograms in LDS). A wave has one run of
+// slots, 64 E of them in registers, read once and all at a time; E = 0: longer
+// tables, read again for every digit. Slots that there are not have the lowest key:
+// beside real ones they come last, so none of them ever stays. With up to kListKeys
+// keys a thread it also writes the stayers' old slots and weights, in order; beyond,
+// that is spread over the chip (fa_evict_list_kernel: 32000 slots of 64 heads 28 us in
+// one launch, 17 + 6.5 in two; 1100 slots of 32 heads 6.9 and 6.9 + 3.6).
+template <int E>
 __global__ void __launch_bounds__(kSelThreads)
 fa_evict_select_kernel(const float* __restrict__ weights, const int32_t* __restrict__ ctx_lens,
                        int32_t* __restrict__ kept, float* __restrict__ w_new,
-                       int32_t* __restrict__ new_lens, int32_t* __restrict__ bad, int Hkv,
-                       int max_pages, int keep, int recent, int new_width) {
-  __shared__ uint32_t hist[256 * kCopies];
+                       int32_t* __restrict__ new_lens, int32_t* __restrict__ bad,
+                       Selection* __restrict__ out, int Hkv, int max_pages, int keep, int recent,
+                       int new_width) {
+  constexpr int N = E > 0 ? E : 1;
+  __shared__ __attribute__((aligned(16))) uint32_t hist[kBins * kCopies];
   __shared__ uint32_t sh_digit, sh_above;
-  __shared__ int sh_gt[kSelWaves], sh_eq[kSelWaves];
+  __shared__ int sh_sum[kSelWaves], sh_gt[kSelWaves], sh_eq[kSelWaves];
+  __shared__ int sh_run[2][kRuns];
   const int hk = blockIdx.x, b = blockIdx.y;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t width = (int64_t)max_pages * kPageSize;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int width = max_pages * kPageSize;
   const size_t bh = (size_t)b * Hkv + hk;
+  const float* w = weights + bh * width;
   int n = ctx_lens[b];
   const bool invalid = n < 0 || n > width;
   if (invalid) n = 0;
   const int m = min(n, keep);
-  const float* w = weights + bh * width;
-  int32_t* kp = kept + bh * keep;
-  float* wn = w_new + bh * new_width;
-  if (hk == 0 && tid == 0) {
-    new_lens[b] = m;
-    bad[b] = invalid;
-  }
   for (int j = m + tid; j < new_width; j += kSelThreads) {
-    wn[j] = 0.f;
-    if (j < keep) kp[j] = -1;
+    w_new[bh * new_width + j] = 0.f;
+    if (j < keep) kept[bh * keep + j] = -1;
   }
-  if (n <= keep) {
-    for (int j = tid; j < m; j += kSelThreads) {
-      kp[j] = j;
-      wn[j] = w[j];
+  const int cand = n > keep ? n - recent : 0, need = keep - recent;   // 0 <= need < cand
+  if (tid == 0) {
+    out[bh].n = n;
+    out[bh].cand = cand;
+    if (hk == 0) {
+      new_lens[b] = m;
+      bad[b] = invalid;
     }
-    return;
   }
-  const int cand = n - recent, need = keep - recent;   // 0 <= need < cand
-  for (int j = tid; j < recent; j += kSelThreads) {
-    kp[need + j] = cand + j;
-    wn[need + j] = w[cand + j];
+  constexpr bool LIST = E > 0 && E <= kListKeys;
+  if constexpr (LIST) {   // those that stay unseen
+    const int stay = cand > 0 ? recent : n, to = cand > 0 ? need : 0;
+    for (int j = tid; j < stay; j += kSelThreads) {
+      kept[bh * keep + to + j] = cand + j;
+      w_new[bh * new_width + to + j] = w[cand + j];
+    }
   }
-  if (need == 0) return;
+  if (cand == 0) return;
+  // The wave's slots lo + 64 i + lane < hi: as many for every wave, so that their
+  // runs give the packing workgroups of like size.
+  const int per = (cand + kSelWaves * 64 - 1) / (kSelWaves * 64) * 64;   // at most 64 E
+  const int lo = min(wave * per, cand), hi = min(lo + per, cand);
+  uint32_t key[N];
+  if constexpr (E > 0) {
+    float x[N];
+#pragma unroll
+    for (int i = 0; i < E; ++i) x[i] = w[min(lo + 64 * i + lane, cand - 1)];
+#pragma unroll
+    for (int i = 0; i < E; ++i) key[i] = lo + 64 * i + lane < hi ? weight_key(x[i]) : 0;
+  }
+  const auto each = [&](auto&& f) {   // f(first slot of 64 - lo, key)
+    if constexpr (E > 0) {
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        if (lo + 64 * i < hi) f(64 * i, key[i]);
+    } else {
+      for (int j = lo; j < hi; j += 64) f(j - lo, j + lane < hi ? weight_key(w[j + lane]) : 0);
+    }
+  };
+  // Thread t has the counters of bins 2047 - 2 t and one below.
+  u32x4* const mine = reinterpret_cast<u32x4*>(hist + (kBins - 2 - 2 * tid) * kCopies);
+  mine[0] = mine[1] = u32x4{};
   uint32_t prefix = 0;   // digits of the threshold found so far
   int left = need;       // of the tokens that share them, how many stay
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256 * kCopies; i += kSelThreads) hist[i] = 0;
+  for (int pass = 0; pass < 3 && need > 0; ++pass) {
+    const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
+    const int above_bits = pass == 0 ? 31 : (pass == 1 ? 21 : 10);   // of pass 0 nothing is compared
+    const uint32_t same = pass == 0 ? 0 : prefix >> above_bits, mask = pass == 2 ? 1023 : 2047;
     __syncthreads();
-    for (int j = tid; j < cand; j += kSelThreads) {
-      const uint32_t k = weight_key(w[j]);
-      if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8)))
-        atomicAdd(&hist[((k >> shift) & 255) * kCopies + (lane & (kCopies - 1))], 1u);
-    }
+    each([&](int, uint32_t k) {
+      if (pass == 0 || (k >> above_bits) == same)
+        atomicAdd(&hist[((k >> shift) & mask) * kCopies + (lane & (kCopies - 1))], 1u);
+    });
     __syncthreads();
-    // Wave 0: lane l has digits 255 - 4 l down to 252 - 4 l.
-    if (wave == 0) {
-      uint32_t c[4], sum = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        c[i] = 0;
-        for (int x = 0; x < kCopies; ++x) c[i] += hist[(255 - 4 * lane - i) * kCopies + x];
-        sum += c[i];
-      }
-      uint32_t above = (uint32_t)scan_sum((int)sum) - sum;   // tokens of larger digits
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (above < (uint32_t)left && above + c[i] >= (uint32_t)left) {   // exactly one lane and i
-          sh_digit = 255 - 4 * lane - i;
-          sh_above = above;
-        }
-        above += c[i];
-      }
+    const u32x4 x1 = mine[0], x0 = mine[1];   // x0: the larger bin
+    mine[0] = mine[1] = u32x4{};
+    const int c0 = (int)(x0[0] + x0[1] + x0[2] + x0[3]), c1 = (int)(x1[0] + x1[1] + x1[2] + x1[3]);
+    int above = scan_sum(c0 + c1);
+    if (lane == 63) sh_sum[wave] = above;
+    above -= c0 + c1;
+    __syncthreads();
+    for (int i = 0; i < wave; ++i) above += sh_sum[i];   // tokens of larger digits
+    if (above < left && above + c0 + c1 >= left) {        // exactly one thread
+      const bool first = above + c0 >= left;
+      sh_digit = kBins - 1 - 2 * tid - (first ? 0 : 1);
+      sh_above = above + (first ? 0 : c0);
     }
     __syncthreads();
     prefix |= sh_digit << shift;
     left -= (int)sh_above;
   }
-  // Keys above `prefix` stay, and the first `left` equal to it.
-  const int run = (cand + kSelWaves * 64 - 1) / (kSelWaves * 64) * 64;   // slots of a wave
-  const int lo = min(wave * run, cand), hi = min(lo + run, cand);
-  int gt = 0, eq = 0;
-  for (int j0 = lo; j0 < hi; j0 += 64) {
-    const int j = j0 + lane;
-    const uint32_t k = j < hi ? weight_key(w[j]) : 0;
-    gt += __popcll(__ballot(j < hi && k > prefix));
-    eq += __popcll(__ballot(j < hi && k == prefix));
+  if (need == 0) prefix = 0xffffffffu;   // of no number: every NaN has 0
+  if constexpr (LIST) {
+    int gt = 0, eq = 0;
+    each([&](int, uint32_t k) {
+      gt += __popcll(__ballot(k > prefix));
+      eq += __popcll(__ballot(k == prefix));
+    });
+    if (lane == 0) {
+      sh_gt[wave] = gt;
+      sh_eq[wave] = eq;
+    }
+    __syncthreads();
+    gt = eq = 0;
+    for (int i = 0; i < wave; ++i) {
+      gt += sh_gt[i];
+      eq += sh_eq[i];
+    }
+    const uint64_t below = ((uint64_t)1 << lane) - 1;
+    each([&](int at, uint32_t k) {
+      const uint64_t mg = __ballot(k > prefix), me = __ballot(k == prefix);
+      const int q = eq + __popcll(me & below);
+      if (k > prefix || (k == prefix && q < left)) {
+        const int to = gt + __popcll(mg & below) + min(q, left), j = lo + at + lane;
+        kept[bh * keep + to] = j;
+        w_new[bh * new_width + to] = w[j];
+      }
+      gt += __popcll(mg);
+      eq += __popcll(me);
+    });
+    return;
   }
+  const int sub = (per / 64 + kSubRuns - 1) / kSubRuns * 64;
+  int gt = 0, eq = 0, next = 0, r = wave * kSubRuns;
+  each([&](int at, uint32_t k) {
+    if (at == next) {   // a run starts
+      if (lane == 0) {
+        sh_run[0][r] = gt;
+        sh_run[1][r] = eq;
+      }
+      next += sub;
+      ++r;
+    }
+    gt += __popcll(__ballot(k > prefix));
+    eq += __popcll(__ballot(k == prefix));
+  });
   if (lane == 0) {
     sh_gt[wave] = gt;
     sh_eq[wave] = eq;
   }
   __syncthreads();
-  gt = eq = 0;
-  for (int i = 0; i < wave; ++i) {
-    gt += sh_gt[i];
-    eq += sh_eq[i];
-  }
-  const uint64_t below = ((uint64_t)1 << lane) - 1;
-  for (int j0 = lo; j0 < hi; j0 += 64) {
-    const int j = j0 + lane;
-    const float x = j < hi ? w[j] : 0.f;
-    const uint32_t k = weight_key(x);
-    const uint64_t mg = __ballot(j < hi && k > prefix), me = __ballot(j < hi && k == prefix);
-    const int g = gt + __popcll(mg & below), e = eq + __popcll(me & below);
-    const bool is_eq = (me >> lane) & 1;
-    if (((mg >> lane) & 1) || (is_eq && e < left)) {
-      const int at = g + min(e, left);
-      kp[at] = j;
-      wn[at] = x;
+  if (tid < kRuns) {
+    gt = sh_run[0][tid];   // of a run that there is not: nothing, never read
+    eq = sh_run[1][tid];
+    for (int i = 0; i < tid / kSubRuns; ++i) {
+      gt += sh_gt[i];
+      eq += sh_eq[i];
     }
-    gt += __popcll(mg);
-    eq += __popcll(me);
+    out[bh].gt[tid] = gt;
+    out[bh].eq[tid] = eq;
+    if (tid == 0) {
+      out[bh].per = per;
+      out[bh].sub = sub;
+      out[bh].left = left;
+      out[bh].key = prefix;
+    }
+  }
+}
+
+constexpr int kMoveThreads = 256;
+constexpr int kListSlots = 512;   // slots that a workgroup looks through at a time
+
+// Old slots and weights of the stayers, in order. Workgroups x < kRuns have a run of
+// candidates, the others kListSlots of the tokens that stay unseen (the newest, or
+// all of a short cache).
+__global__ void __launch_bounds__(kMoveThreads)
+fa_evict_list_kernel(const float* __restrict__ weights, const Selection* __restrict__ sel,
+                     int32_t* __restrict__ kept, float* __restrict__ w_new, int Hkv, int max_pages,
+                     int new_max_pages, int keep, int recent) {
+  constexpr int WAVES = kMoveThreads / 64;
+  constexpr int ROUNDS = kListSlots / kMoveThreads;
+  __shared__ int sh_gt[WAVES], sh_eq[WAVES];
+  const int hk = blockIdx.y, b = blockIdx.z;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const size_t bh = (size_t)b * Hkv + hk;
+  const Selection& se = sel[bh];
+  const float* w = weights + bh * ((size_t)max_pages * kPageSize);
+  int32_t* kp = kept + bh * keep;
+  float* wn = w_new + bh * ((size_t)new_max_pages * kPageSize);
+  const int cand = se.cand;
+  if (blockIdx.x >= kRuns) {
+    const int stay = cand > 0 ? recent : se.n;    // tokens cand .. + stay - 1
+    const int to = cand > 0 ? keep - recent : 0;
+    const int first = ((int)blockIdx.x - kRuns) * kListSlots;
+    for (int i = first + tid; i < min(first + kListSlots, stay); i += kMoveThreads) {
+      kp[to + i] = cand + i;
+      wn[to + i] = w[cand + i];
+    }
+    return;
+  }
+  if (cand == 0) return;
+  const int per = se.per, sub = se.sub, left = se.left;
+  const int start = (int)blockIdx.x / kSubRuns * per, lo = start + (int)blockIdx.x % kSubRuns * sub;
+  const int hi = min(min(lo + sub, start + per), cand);
+  if (lo >= hi) return;
+  const uint32_t key = se.key;
+  int gt = se.gt[blockIdx.x], eq = se.eq[blockIdx.x];
+  for (int j0 = lo; j0 < hi; j0 += kListSlots) {
+    // A wave has kListSlots / WAVES slots in a row, so that the waves' counts
+    // follow one another.
+    float x[ROUNDS];
+    const int mine = j0 + wave * (kListSlots / WAVES) + lane;
+#pragma unroll
+    for (int i = 0; i < ROUNDS; ++i) x[i] = w[min(mine + 64 * i, hi - 1)];
+    int g = 0, e = 0;
+#pragma unroll
+    for (int i = 0; i < ROUNDS; ++i) {
+      const uint32_t k = weight_key(x[i]);
+      const bool in = mine + 64 * i < hi;
+      g += __popcll(__ballot(in && k > key));
+      e += __popcll(__ballot(in && k == key));
+    }
+    if (j0 > lo) __syncthreads();
+    if (lane == 0) {
+      sh_gt[wave] = g;
+      sh_eq[wave] = e;
+    }
+    __syncthreads();
+    int G = gt, Q = eq;
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) {
+      if (i < wave) {
+        G += sh_gt[i];
+        Q += sh_eq[i];
+      }
+      gt += sh_gt[i];
+      eq += sh_eq[i];
+    }
+    const uint64_t below = ((uint64_t)1 << lane) - 1;
+#pragma unroll
+    for (int i = 0; i < ROUNDS; ++i) {
+      const uint32_t k = weight_key(x[i]);
+      const bool in = mine + 64 * i < hi;
+      const uint64_t mg = __ballot(in && k > key), me = __ballot(in && k == key);
+      const int q = Q + __popcll(me & below);
+      if (in && (k > key || (k == key && q < left))) {
+        const int at = G + __popcll(mg & below) + min(q, left);
+        kp[at] = mine + 64 * i;
+        wn[at] = x[i];
+      }
+      G += __popcll(mg);
+      Q += __popcll(me);
+    }
   }
 }
 
 constexpr int kMoveRows = 4;   // rows a thread has in flight
 
-// The stayers' rows into the new pages: 16-byte pieces, each row read and
-// written once. Bound: memory, by the gather of 2 D byte rows.
+// The stayers' rows into the new pages: 16-byte pieces, each row read and written
+// once, the reads past the caches. Bound: memory, by the gather of 2 D byte rows.
+// Slots, page ids and rows each are asked for together.
 template <int D>
-__global__ void __launch_bounds__(kThreads)
-fa_evict_move_kernel(uint4* k_pool, uint4* v_pool, const int32_t* __restrict__ page_table,
+__global__ void __launch_bounds__(kMoveThreads)
+fa_evict_move_kernel(u32x4* k_pool, u32x4* v_pool, const int32_t* __restrict__ page_table,
                      const int32_t* __restrict__ new_table, const int32_t* __restrict__ kept,
                      int32_t* __restrict__ bad, int Hkv, int max_pages, int new_max_pages,
                      int num_pages, int keep) {
-  constexpr int CH = D / 8;            // pieces of a row
-  constexpr int SIDE = kThreads / CH;  // rows side by side
+  constexpr int CH = D / 8;                // pieces of a row
+  constexpr int SIDE = kMoveThreads / CH;  // rows side by side
   const int hk = blockIdx.y, b = blockIdx.z;
   const int c = (int)threadIdx.x % CH;
   const int32_t* kp = kept + ((size_t)b * Hkv + hk) * keep;
-  uint4 x[kMoveRows], y[kMoveRows];
-  int64_t dst[kMoveRows];
+  int j[kMoveRows], old[kMoveRows], from[kMoveRows], to[kMoveRows];
+  u32x4 x[kMoveRows], y[kMoveRows];
+  bool miss = false;
 #pragma unroll
   for (int i = 0; i < kMoveRows; ++i) {
-    const int j = ((int)blockIdx.x * kMoveRows + i) * SIDE + (int)threadIdx.x / CH;
-    dst[i] = -1;
-    const int old = j < keep ? kp[j] : -1;
-    if (old >= 0) {
-      const int from = page_table[(size_t)b * max_pages + old / kPageSize];
-      const int to = new_table[(size_t)b * new_max_pages + j / kPageSize];
-      if (from >= 0 && from < num_pages && to >= 0 && to < num_pages) {
-        const int64_t src = (((int64_t)from * Hkv + hk) * kPageSize + old % kPageSize) * CH + c;
-        dst[i] = (((int64_t)to * Hkv + hk) * kPageSize + j % kPageSize) * CH + c;
-        x[i] = k_pool[src];
-        y[i] = v_pool[src];
-      } else if (c == 0) {
-        bad[b] = 1;   // the same value from every writer
-      }
-    }
+    j[i] = ((int)blockIdx.x * kMoveRows + i) * SIDE + (int)threadIdx.x / CH;
+    old[i] = kp[min(j[i], keep - 1)];
+    to[i] = new_table[(size_t)b * new_max_pages + min(j[i], keep - 1) / kPageSize];
   }
 #pragma unroll
   for (int i = 0; i < kMoveRows; ++i) {
-    if (dst[i] >= 0) {
-      k_pool[dst[i]] = x[i];
-      v_pool[dst[i]] = y[i];
-    }
+    if (j[i] >= keep) old[i] = -1;
+    from[i] = page_table[(size_t)b * max_pages + max(old[i], 0) / kPageSize];
   }
+#pragma unroll
+  for (int i = 0; i < kMoveRows; ++i) {
+    const bool ok = from[i] >= 0 && from[i] < num_pages && to[i] >= 0 && to[i] < num_pages;
+    miss |= old[i] >= 0 && !ok;
+    if (!ok) old[i] = -1;
+    // Rows that do not move read the pool's first one.
+    const int64_t src = old[i] < 0 ? c : (((int64_t)from[i] * Hkv + hk) * kPageSize + old[i] % kPageSize) * CH + c;
+    x[i] = __builtin_nontemporal_load(k_pool + src);
+    y[i] = __builtin_nontemporal_load(v_pool + src);
+  }
+#pragma unroll
+  for (int i = 0; i < kMoveRows; ++i) {
+    if (old[i] < 0) continue;
+    const int64_t dst = (((int64_t)to[i] * Hkv + hk) * kPageSize + j[i] % kPageSize) * CH + c;
+    k_pool[dst] = x[i];
+    v_pool[dst] = y[i];
+  }
+  if (miss) bad[b] = 1;   // the same value from every writer
 }
 
 }  // namespace cache
 }  // namespace fa
 
-extern "C" int64_t fa_decode_weights_workspace_floats(int64_t B, int64_t H, int64_t D,
-                                                      int64_t max_pages, int64_t num_splits) {
-  if (B <= 0 || H <= 0 || D <= 0 || max_pages <= 0 || num_splits <= 0) return 0;
-  return B * H * (max_pages * 16 + num_splits * (D + 2));
+extern "C" int64_t fa_decode_weights_workspace_floats(int64_t B, int64_t H, int64_t H_kv, int64_t D,
+                                                      int64_t max_pages) {
+  // the sizes that fa_validate_decode_weights refuses
+  constexpr int64_t kIndexes = (int64_t(1) << 31) - 1;
+  if (B <= 0 || B > 65535 || H <= 0 || H > 65535 || H_kv <= 0 || H % H_kv != 0 ||
+      (D != 64 && D != 128) || max_pages <= 0 || max_pages > kIndexes / 16 || B > kIndexes / max_pages)
+    return 0;
+  return fa::cache::workspace_of(B, H, H_kv, D, max_pages).floats;
 }
 
 extern "C" int fa_decode_paged_weights(const void* q, const void* k_pool, const void* v_pool,
                                        const int32_t* page_table, const int32_t* ctx_lens,
                                        const float* weights, int64_t B, int64_t H, int64_t H_kv,
                                        int64_t D, int64_t page_size, int64_t max_pages,
-                                       int64_t num_pages, int64_t num_splits, float* workspace,
-                                       void* o, float* lse, float* weights_out, int bf16,
-                                       void* stream) {
+                                       int64_t num_pages, float* workspace, void* o, float* lse,
+                                       float* weights_out, int bf16, void* stream) {
   const int st = fa_validate_decode_weights(q, k_pool, v_pool, page_table, ctx_lens, weights, B, H,
-                                            H_kv, D, page_size, max_pages, num_pages, num_splits,
-                                            workspace, o, lse, weights_out);
+                                            H_kv, D, page_size, max_pages, num_pages, workspace, o, lse,
+                                            weights_out);
   if (st != FA_OK) return st;
-  const auto fn = bf16 ? fa::cache::decode_weights<true> : fa::cache::decode_weights<false>;
-  return fn(q, k_pool, v_pool, page_table, ctx_lens, weights, B, H, H_kv, D, max_pages, num_pages,
-            num_splits, workspace, o, lse, weights_out, stream);
+  using fa::cache::decode_weights;
+  const auto fn = D == 128 ? (bf16 ? decode_weights<128, true> : decode_weights<128, false>)
+                           : (bf16 ? decode_weights<64, true> : decode_weights<64, false>);
+  return fn(q, k_pool, v_pool, page_table, ctx_lens, weights, B, H, H_kv, max_pages, num_pages, workspace,
+            o, lse, weights_out, stream);
+}
+
+extern "C" int64_t fa_kv_evict_workspace_words(int64_t B, int64_t H_kv) {
+  if (B <= 0 || H_kv <= 0 || B > 65535 || H_kv > 65535) return 0;
+  return B * H_kv * fa::cache::kSelWords;
 }
 
 extern "C" int fa_kv_evict(void* k_pool, void* v_pool, const int32_t* page_table,
                            const int32_t* ctx_lens, const float* weights,
                            const int32_t* new_page_table, int32_t* kept, float* new_weights,
-                           int32_t* new_lens, int32_t* bad, int64_t B, int64_t H_kv, int64_t D,
-                           int64_t keep, int64_t recent, int64_t page_size, int64_t max_pages,
-                           int64_t new_max_pages, int64_t num_pages, void* stream) {
+                           int32_t* new_lens, int32_t* bad, int32_t* workspace, int64_t B, int64_t H_kv,
+                           int64_t D, int64_t keep, int64_t recent, int64_t page_size,
+                           int64_t max_pages, int64_t new_max_pages, int64_t num_pages, void* stream) {
   using namespace fa::cache;
   const int st = fa_validate_kv_evict(k_pool, v_pool, page_table, ctx_lens, weights, new_page_table,
-                                      kept, new_weights, new_lens, bad, B, H_kv, D, keep, recent,
-                                      page_size, max_pages, new_max_pages, num_pages);
+                                      kept, new_weights, new_lens, bad, workspace, B, H_kv, D, keep,
+                                      recent, page_size, max_pages, new_max_pages, num_pages);
   if (st != FA_OK) return st;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(fa_evict_select_kernel, dim3((unsigned)H_kv, (unsigned)B), dim3(kSelThreads), 0,
-                     s, weights, ctx_lens, kept, new_weights, new_lens, bad, (int)H_kv,
-                     (int)max_pages, (int)keep, (int)recent, (int)(new_max_pages * kPageSize));
-  const int64_t rows = kMoveRows * (kThreads / (D / 8));
+  Selection* sel = reinterpret_cast<Selection*>(workspace);
+  const int64_t width = max_pages * kPageSize;
+  const int64_t keys = (width + kSelThreads - 1) / kSelThreads;   // of a thread
+  const auto select = keys <= 1    ? fa_evict_select_kernel<1>
+                      : keys <= 4  ? fa_evict_select_kernel<4>
+                      : keys <= 16 ? fa_evict_select_kernel<16>
+                      : keys <= kMostKeys ? fa_evict_select_kernel<kMostKeys>
+                                          : fa_evict_select_kernel<0>;
+  hipLaunchKernelGGL(select, dim3((unsigned)H_kv, (unsigned)B), dim3(kSelThreads), 0, s, weights, ctx_lens,
+                     kept, new_weights, new_lens, bad, sel, (int)H_kv, (int)max_pages, (int)keep,
+                     (int)recent, (int)(new_max_pages * kPageSize));
+  if (keys > kListKeys) {
+    const int64_t plain = ((keep < width ? keep : width) + kListSlots - 1) / kListSlots;
+    hipLaunchKernelGGL(fa_evict_list_kernel, dim3((unsigned)(kRuns + plain), (unsigned)H_kv, (unsigned)B),
+                       dim3(kMoveThreads), 0, s, weights, sel, kept, new_weights, (int)H_kv,
+                       (int)max_pages, (int)new_max_pages, (int)keep, (int)recent);
+  }
+  const int64_t rows = kMoveRows * (kMoveThreads / (D / 8));
   const dim3 grid((unsigned)((keep + rows - 1) / rows), (unsigned)H_kv, (unsigned)B);
-#define FA_MOVE(DD)                                                                                \
-  hipLaunchKernelGGL((fa_evict_move_kernel<DD>), grid, dim3(kThreads), 0, s, (uint4*)k_pool,       \
-                     (uint4*)v_pool, page_table, new_page_table, kept, bad, (int)H_kv,             \
-                     (int)max_pages, (int)new_max_pages, (int)num_pages, (int)keep)
-  if (D == 128) FA_MOVE(128);
-  else FA_MOVE(64);
-#undef FA_MOVE
+  const auto move = D == 128 ? fa_evict_move_kernel<128> : fa_evict_move_kernel<64>;
+  hipLaunchKernelGGL(move, grid, dim3(kMoveThreads), 0, s, (fa::u32x4*)k_pool, (fa::u32x4*)v_pool,
+                     page_table, new_page_table, kept, bad, (int)H_kv, (int)max_pages,
+                     (int)new_max_pages, (int)num_pages, (int)keep);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? FA_OK : -(int)e;
 }

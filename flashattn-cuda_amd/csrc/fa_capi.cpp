@@ -334,18 +334,17 @@ extern "C" int fa_validate_decode_weights(const void* q, const void* k_pool, con
                                           const int32_t* page_table, const int32_t* ctx_lens,
                                           const float* weights, int64_t B, int64_t H, int64_t H_kv,
                                           int64_t D, int64_t page_size, int64_t max_pages,
-                                          int64_t num_pages, int64_t num_splits,
-                                          const float* workspace, const void* o, const float* lse,
-                                          const float* weights_out) {
+                                          int64_t num_pages, const float* workspace, const void* o,
+                                          const float* lse, const float* weights_out) {
   const int st = fa_validate_decode(q, k_pool, v_pool, page_table, ctx_lens, B, H, D, page_size,
-                                    max_pages, num_pages, num_splits);
+                                    max_pages, num_pages, /*num_splits=*/1);
   if (st != FA_OK) return st;
   if (H_kv <= 0 || H % H_kv != 0) return FA_ERR_KV_HEADS;
   if (!weights || !weights_out || !workspace || !o || !lse) return FA_ERR_NULL_POINTER;
   if (!aligned16(workspace) || !aligned16(o) || !aligned16(weights) || !aligned16(weights_out))
     return FA_ERR_ALIGNMENT;
   if (reinterpret_cast<uintptr_t>(lse) & 3u) return FA_ERR_ALIGNMENT;
-  // The join has a workgroup for 1024 slots of a (b, KV head), and one for 8 rows.
+  // The join has a workgroup for 1024 slots of a (b, KV head), and one for a row.
   const int64_t chunks = (max_pages * 16 + 1023) / 1024;
   if (num_pages > kMaxGrid || B * H > (int64_t(1) << 24) || B * H_kv > ((int64_t(1) << 30) - 1) / chunks)
     return FA_ERR_TOO_LARGE;
@@ -356,11 +355,11 @@ extern "C" int fa_validate_kv_evict(const void* k_pool, const void* v_pool, cons
                                     const int32_t* ctx_lens, const float* weights,
                                     const int32_t* new_page_table, const int32_t* kept,
                                     const float* new_weights, const int32_t* new_lens,
-                                    const int32_t* bad, int64_t B, int64_t H_kv, int64_t D,
-                                    int64_t keep, int64_t recent, int64_t page_size,
+                                    const int32_t* bad, const int32_t* workspace, int64_t B,
+                                    int64_t H_kv, int64_t D, int64_t keep, int64_t recent, int64_t page_size,
                                     int64_t max_pages, int64_t new_max_pages, int64_t num_pages) {
   if (!k_pool || !v_pool || !page_table || !ctx_lens || !weights || !new_page_table || !kept ||
-      !new_weights || !new_lens || !bad)
+      !new_weights || !new_lens || !bad || !workspace)
     return FA_ERR_NULL_POINTER;
   if (D != 64 && D != 128) return FA_ERR_HEAD_DIM;
   if (B <= 0 || H_kv <= 0) return FA_ERR_BATCH_HEADS;
@@ -368,7 +367,8 @@ extern "C" int fa_validate_kv_evict(const void* k_pool, const void* v_pool, cons
   if (max_pages <= 0 || new_max_pages <= 0) return FA_ERR_MAX_PAGES;
   if (num_pages <= 0) return FA_ERR_NUM_PAGES;
   if (!aligned16(k_pool) || !aligned16(v_pool)) return FA_ERR_ALIGNMENT;
-  const void* words[] = {page_table, ctx_lens, weights, new_page_table, kept, new_weights, new_lens, bad};
+  const void* words[] = {page_table, ctx_lens, weights, new_page_table, kept, new_weights, new_lens, bad,
+                         workspace};
   for (const void* p : words)
     if (reinterpret_cast<uintptr_t>(p) & 3u) return FA_ERR_ALIGNMENT;
   if (B > 65535 || H_kv > 65535 || num_pages > kMaxGrid) return FA_ERR_TOO_LARGE;

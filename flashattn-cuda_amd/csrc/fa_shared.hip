@@ -6,19 +6,22 @@
 // The paged decode would read the prefix once per sequence. Here its keys are
 // read once per KV head: the query rows of all sequences and of all heads that
 // share a KV head, B * H / H_kv of them, form one product with them, as in a
-// forward pass without a mask. The own pages go through the split pass of the
-// paged decode, and one launch joins the partials of both by their (maximum, sum).
+// forward pass without a mask. Few rows (kFewRows) go through the chunks of
+// fa_stream.hpp instead, as the own pages do, and in their launch. One launch joins
+// the partials of both by their (maximum, sum).
 #include <hip/hip_runtime.h>
 
 #include <math.h>
 #include <stdint.h>
 
-#include "fa_decode.hpp"
 #include "fa_mi355x.h"
+#include "fa_stream.hpp"
 #include "fa_tile.hpp"
 
 namespace fa {
 namespace shared {
+
+using namespace stream;
 
 constexpr int kTile = 64;     // keys of a tile: 4 pages
 constexpr int kStages = 4;    // tiles in LDS, three of them in flight
@@ -39,10 +42,10 @@ fa_prefix_split_kernel(const f16* __restrict__ q, const f16* __restrict__ kpool,
                        float2* __restrict__ part_ml, int rows, int H, int Hkv, int max_pages,
                        int num_pages, int S, int row_blocks, int nxcd, float c) {
   constexpr int NW = WM * kKeyGroups;
-  constexpr int PAGE = kPage * D * 2;
+  constexpr int PAGE = kTokens * D * 2;
   constexpr int CPR = D / 8;
   constexpr int NC = PAGE / 1024;            // 1 KiB copies of a page
-  constexpr int PAGES = kTile / kPage;
+  constexpr int PAGES = kTile / kTokens;
   constexpr int NU = 2 * PAGES / NW;         // pages, of K or V, a wave copies of a tile
   constexpr int STAGE = 2 * PAGES * PAGE;    // K, then V
   constexpr int DB = D / 32;
@@ -62,9 +65,9 @@ fa_prefix_split_kernel(const f16* __restrict__ q, const f16* __restrict__ kpool,
   if (tid == 0) sh_bad = 0;
   __syncthreads();
   int P = prefix_len[0];
-  bool bad = P < 0 || P > max_pages * kPage;
+  bool bad = P < 0 || P > max_pages * kTokens;
   if (bad) P = 0;
-  const int pages = (P + kPage - 1) / kPage;
+  const int pages = (P + kTokens - 1) / kTokens;
   const int tiles = (pages + PAGES - 1) / PAGES;
   const int t0 = (int)((int64_t)tiles * s / S), t1 = (int)((int64_t)tiles * (s + 1) / S);
 
@@ -103,8 +106,8 @@ fa_prefix_split_kernel(const f16* __restrict__ q, const f16* __restrict__ kpool,
       const bool in = t0 + k < t1 && pi < pages;
       const bool ok = in && pid >= 0 && pid < num_pages;
       bad |= in && !ok;
-      const size_t off = ok ? ((size_t)pid * Hkv + hk) * (size_t)(kPage * D) : 0;
-      const auto r = make_rsrc_s(((unit & 1) ? vpool : kpool) + off, ok ? min(kPage, P - pi * kPage) * D * 2 : 0);
+      const size_t off = ok ? ((size_t)pid * Hkv + hk) * (size_t)(kTokens * D) : 0;
+      const auto r = make_rsrc_s(((unit & 1) ? vpool : kpool) + off, ok ? min(kTokens, P - pi * kTokens) * D * 2 : 0);
       const uint32_t dst = lds0 + (k % kStages) * STAGE + (unit & 1) * (PAGES * PAGE) + unit / 2 * PAGE;
 #pragma unroll
       for (int i = 0; i < NC; ++i) dma16(r, dst + 1024 * i, coff[i]);
@@ -131,8 +134,6 @@ fa_prefix_split_kernel(const f16* __restrict__ q, const f16* __restrict__ kpool,
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) sc = mma32<BF16>(load_row_frag<D>(kb, 0, kk), qf[kk], sc);
       float mx = -INFINITY;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) sc[r] *= c;
       if (key0 + 32 > P) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
@@ -143,7 +144,7 @@ fa_prefix_split_kernel(const f16* __restrict__ q, const f16* __restrict__ kpool,
       mx = max_xor32(mx);
       const float m_new = fmaxf(m, mx);
       if (__any(m_new != m)) {
-        const float alpha = m == m_new ? 1.f : exp2_hw(m - m_new);
+        const float alpha = m == m_new ? 1.f : exp2_hw((m - m_new) * c);
         l *= alpha;
 #pragma unroll
         for (int db = 0; db < DB; ++db)
@@ -155,7 +156,7 @@ fa_prefix_split_kernel(const f16* __restrict__ q, const f16* __restrict__ kpool,
       float ps = 0.f;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        sc[r] = exp2_hw(sc[r] - mu);
+        sc[r] = exp2_hw((sc[r] - mu) * c);
         ps += sc[r];
       }
       l += ps;
@@ -186,7 +187,8 @@ fa_prefix_split_kernel(const f16* __restrict__ q, const f16* __restrict__ kpool,
   __syncthreads();
   if (kg == 1 || !live) return;
   const float m1 = sh_m[rm][lane], M = fmaxf(m, m1);
-  const float e0 = m == -INFINITY ? 0.f : exp2_hw(m - M), e1 = m1 == -INFINITY ? 0.f : exp2_hw(m1 - M);
+  const float e0 = m == -INFINITY ? 0.f : exp2_hw((m - M) * c);
+  const float e1 = m1 == -INFINITY ? 0.f : exp2_hw((m1 - M) * c);
   const float z = e0 * l + e1 * sh_l[rm][lane];
   const bool nan = sh_bad || z != z;
   const float inv = nan ? NAN : (z > 0.f ? 1.f / z : 0.f);
@@ -204,143 +206,155 @@ fa_prefix_split_kernel(const f16* __restrict__ q, const f16* __restrict__ kpool,
   if (lane < 32) part_ml[at] = make_float2(M, nan ? NAN : z);
 }
 
-// The split pass of the paged decode over the own pages, partials as it leaves them.
-template <int D, bool BF16>
-__global__ void __launch_bounds__(kDecThreads)
-fa_own_split_kernel(const typename DecT<BF16>::e* __restrict__ q,
-                    const typename DecT<BF16>::e* __restrict__ kpool,
-                    const typename DecT<BF16>::e* __restrict__ vpool,
-                    const int32_t* __restrict__ page_table, const int32_t* __restrict__ ctx_lens,
-                    float* __restrict__ part_o, float* __restrict__ part_ml, int H, int Hkv,
-                    int max_pages, int num_pages, int S, int ordered, float c) {
-  __shared__ DecShared<D> sh;
-  decode_split_body<D, BF16, true>(sh, blockIdx.x, blockIdx.y, blockIdx.z, gridDim.z, q, kpool, vpool,
-                                   page_table, ctx_lens, part_o, part_ml, nullptr, nullptr, H, Hkv,
-                                   max_pages, num_pages, S, ordered, c);
+// Splits of a short list of prefix pages in the chunk pass: SP at most.
+__device__ __forceinline__ int prefix_splits(int P, int max_pages, int SP) {
+  const int n = pages_of(P, max_pages) / kMinChunk;
+  return n < 1 ? 1 : min(n, SP);
 }
 
-// O and L of a row out of the partials of both passes: one workgroup a row, D / 4
-// threads a partial, the sums in a fixed order.
-constexpr int kJoinThreads = 256;
-constexpr int kMaxPrefixSplits = 256;
-constexpr int kMaxOwnSplits = 16;
+// Workgroups [0, pre_blocks): chunks of the prefix for 16 of the `rows` query rows
+// of a KV head; partial number split * B * H + row. The others: chunks of the own
+// pages, partial number chunk * H + h.
+template <int D, bool BF16, bool NT>
+__global__ void __launch_bounds__(stream::kThreads)
+fa_shared_chunk_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_pool,
+                       const char* __restrict__ v_pool, const int32_t* __restrict__ prefix_table,
+                       const int32_t* __restrict__ prefix_len, const int32_t* __restrict__ page_table,
+                       const int32_t* __restrict__ ctx_lens, const int4* __restrict__ table,
+                       float* __restrict__ pre_o, float2* __restrict__ pre_ml, float* __restrict__ own_o,
+                       float2* __restrict__ own_ml, int2* __restrict__ first, int B, int H, int Hkv,
+                       int group, int ngrp, int rows, int pre_blocks, int pre_grp, int SP,
+                       int prefix_pages, int max_pages, int num_pages, Plan plan, float c) {
+  __shared__ Shared<D> sh;
+  const int col = threadIdx.x & 15;
+  if ((int)blockIdx.x < pre_blocks) {
+    const Place at = place_of(blockIdx.x, Hkv * pre_grp);
+    const int P = prefix_len[0], pages = pages_of(P, prefix_pages);
+    const int n = prefix_splits(P, prefix_pages, SP);
+    if (at.number >= n) return;
+    const int hk = at.hg / pre_grp, r = 16 * (at.hg - hk * pre_grp) + col;
+    const bool live = r < rows;
+    const int64_t row = live ? (int64_t)(r / group) * H + hk * group + r % group : 0;
+    const int p0 = (int)((int64_t)pages * at.number / n), p1 = (int)((int64_t)pages * (at.number + 1) / n);
+    chunk_body<D, BF16, NT, false>(sh, q, k_pool, v_pool, prefix_table, p0, p1, P,
+                                   P < 0 || (P > 0 && pages == 0), live, row * D, hk, Hkv, num_pages, c,
+                                   nullptr, 0, 0, pre_o, pre_ml, (int64_t)at.number * B * H + row);
+    return;
+  }
+  const Place at = place_of((int)blockIdx.x - pre_blocks, Hkv * ngrp);
+  const Run r = run_of(ctx_lens, table, B, max_pages, plan, at.number);
+  if (r.b < 0) return;
+  if (at.hg == 0 && r.split == 0 && threadIdx.x == 0) first[r.b] = make_int2(at.number, r.splits);
+  const int hk = at.hg / ngrp, sub = at.hg - hk * ngrp;
+  const int h = hk * group + 16 * sub + col;
+  const bool live = 16 * sub + col < group;
+  chunk_body<D, BF16, NT, false>(sh, q, k_pool, v_pool, page_table + (size_t)r.b * max_pages, r.p0, r.p1,
+                                 r.ctx, r.bad, live, ((int64_t)r.b * H + h) * D, hk, Hkv, num_pages, c,
+                                 nullptr, 0, 0, own_o, own_ml, (int64_t)at.number * H + h);
+}
 
+// O and L of row blockIdx.x out of the partials of the prefix (SP of them, or, of
+// few rows, as many as the prefix's length gives) and of the own pages.
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kJoinThreads)
-fa_shared_join_kernel(const float* __restrict__ pre_o, const float2* __restrict__ pre_ml, int SP,
-                      const float* __restrict__ own_o, const float2* __restrict__ own_ml, int SO,
-                      typename DecT<BF16>::e* __restrict__ o, float* __restrict__ lse) {
-  typedef typename DecT<BF16>::e e4 __attribute__((ext_vector_type(4)));
-  constexpr int PER = D / 4, SIDE = kJoinThreads / PER, WAVES = kJoinThreads / 64;
-  __shared__ float w[kMaxPrefixSplits + kMaxOwnSplits];
-  __shared__ float red[2 * WAVES];
-  __shared__ float acc[SIDE][D];
-  const int tid = threadIdx.x, wave = tid >> 6;
-  const int64_t row = blockIdx.x;
-  const int S = SP + SO;
-  const auto ml = [&](int i) { return i < SP ? pre_ml[row * SP + i] : own_ml[row * SO + i - SP]; };
-  float M = -INFINITY;
-  for (int i = tid; i < S; i += kJoinThreads) M = fmaxf(M, ml(i).x);
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) M = fmaxf(M, __shfl_xor(M, d));
-  if ((tid & 63) == 0) red[wave] = M;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < WAVES; ++i) M = fmaxf(M, red[i]);
-  float z = 0.f;
-  for (int i = tid; i < S; i += kJoinThreads) {
-    const float2 x = ml(i);   // an empty part: (-inf, 0), or NaN
-    const float e = x.x == -INFINITY ? x.y : x.y * exp2_hw(x.x - M);
-    w[i] = e;
-    z += e;
-  }
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) z += __shfl_xor(z, d);
-  if ((tid & 63) == 0) red[WAVES + wave] = z;
-  __syncthreads();
-  z = 0.f;
-#pragma unroll
-  for (int i = 0; i < WAVES; ++i) z += red[WAVES + i];
-  f32x4 v = f32x4{};
-  const int d = 4 * (tid % PER), side = tid / PER;
-#pragma unroll 4
-  for (int i = side; i < S; i += SIDE) {
-    const float* p = i < SP ? pre_o + (row * SP + i) * D : own_o + (row * SO + i - SP) * D;
-    const f32x4 x = *reinterpret_cast<const f32x4*>(p + d);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) v[r] = fmaf(w[i], x[r], v[r]);
-  }
-#pragma unroll
-  for (int r = 0; r < 4; ++r) acc[side][d + r] = v[r];
-  __syncthreads();
-  if (side > 0) return;
-  for (int i = 1; i < SIDE; ++i)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) v[r] += acc[i][d + r];
-  const float inv = z == 0.f ? 0.f : 1.f / z;   // a NaN sum: NaN
-  e4 out;
-#pragma unroll
-  for (int r = 0; r < 4; ++r) out[r] = (typename DecT<BF16>::e)(v[r] * inv);
-  *reinterpret_cast<e4*>(o + row * D + d) = out;
-  if (tid == 0) lse[row] = z == 0.f ? -INFINITY : (M + log2_hw(z)) * kLn2;
+fa_shared_join_kernel(const float* __restrict__ pre_o, const float2* __restrict__ pre_ml,
+                      const float* __restrict__ own_o, const float2* __restrict__ own_ml,
+                      const int2* __restrict__ first, const int32_t* __restrict__ prefix_len,
+                      uint16_t* __restrict__ o, float* __restrict__ lse, int H, int rows, int SP,
+                      int few, int prefix_pages, float c) {
+  __shared__ JoinShared<D> sh;
+  const int row = blockIdx.x, b = row / H;
+  const int2 f = first[b];
+  const int n = few ? prefix_splits(prefix_len[0], prefix_pages, SP) : SP;
+  const Parts pre = few ? Parts{pre_o, pre_ml, row, rows, n} : Parts{pre_o, pre_ml, (int64_t)row * SP, 1, n};
+  join_row<D, BF16>(sh, pre, Parts{own_o, own_ml, (int64_t)f.x * H + (row - b * H), H, f.y}, c,
+                    o + (int64_t)row * D, lse + row);
 }
 
-// How a call is cut: rows of a workgroup of the prefix pass, its runs of tiles,
-// the splits of the own pages.
-struct Plan {
-  int wm, row_blocks, sp, so;
+// Query rows of a KV head up to which the prefix goes through the chunk pass: one
+// or two workgroups of 16 rows for a chunk.
+constexpr int kFewRows = 32;
+constexpr int kMaxSplits = 256;   // of the prefix
+// The cut is made for the 256 CUs of a whole MI355X, whatever the device has: the
+// workspace follows from the sizes alone.
+constexpr int kCus = 256;
+constexpr int64_t kPassThrough = 64 << 20;   // bytes of pools read past the caches
+
+// How a call is cut: the prefix pass and its splits, the own pages' chunks, and the
+// workspace in floats.
+struct Cut {
+  bool few;
+  int wm, row_blocks, sp;
+  int64_t rows, own, pre_ml, own_o, own_ml, first, table, floats;
 };
 
-// Made for the 256 CUs of a whole MI355X, whatever the device has: the workspace
-// follows from the sizes alone.
-constexpr int kCus = 256;
-
-static Plan plan(int64_t B, int64_t H, int64_t Hkv, int64_t prefix_pages, int64_t max_pages) {
-  Plan p;
-  const int64_t rows = B * (H / Hkv);
-  p.wm = rows <= 32 ? 1 : (rows <= 64 ? 2 : 4);
-  p.row_blocks = (int)((rows + 32 * p.wm - 1) / (32 * p.wm));
-  const int64_t tiles = (prefix_pages * kPage + kTile - 1) / kTile;
-  int64_t sp = kCus / (Hkv * p.row_blocks);
-  sp = sp < 1 ? 1 : (sp > kMaxPrefixSplits ? kMaxPrefixSplits : sp);
-  p.sp = (int)(sp > tiles ? tiles : sp);
-  int64_t so = 2 * kCus / (B * decode_head_groups(H, Hkv));
-  const int64_t most = (max_pages + 7) / 8;
-  so = so > most ? most : so;
-  p.so = (int)(so < 1 ? 1 : (so > kMaxOwnSplits ? kMaxOwnSplits : so));
+static Cut cut_of(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t prefix_pages, int64_t max_pages) {
+  Cut p;
+  p.rows = B * (H / Hkv);
+  p.few = p.rows <= kFewRows;
+  p.wm = p.rows <= 64 ? 2 : 4;
+  int64_t sp, most;
+  if (p.few) {
+    p.row_blocks = (int)((p.rows + 15) / 16);
+    sp = kFill / (Hkv * p.row_blocks);
+    most = prefix_pages / kMinChunk;
+  } else {
+    p.row_blocks = (int)((p.rows + 32 * p.wm - 1) / (32 * p.wm));
+    sp = kCus / (Hkv * p.row_blocks);
+    most = (prefix_pages * kTokens + kTile - 1) / kTile;
+  }
+  sp = sp > most ? most : sp;
+  p.sp = (int)(sp < 1 ? 1 : (sp > kMaxSplits ? kMaxSplits : sp));
+  p.own = most_chunks(B, max_pages, plan_of(head_groups(H, Hkv)));
+  p.own_o = B * H * p.sp * D;
+  p.pre_ml = p.own_o + p.own * H * D;
+  p.own_ml = p.pre_ml + 2 * B * H * p.sp;
+  p.table = p.own_ml + (2 * p.own * H + 3) / 4 * 4;
+  p.first = p.table + (B > kWavePlan ? 4 * (1 + p.own) : 0);
+  p.floats = p.first + 2 * B;
   return p;
 }
 
 template <int D, bool BF16>
-static int launch(const Plan& p, const void* q, const void* k_pool, const void* v_pool,
+static int launch(const Cut& p, const void* q, const void* k_pool, const void* v_pool,
                   const int32_t* prefix_table, const int32_t* prefix_len, const int32_t* page_table,
                   const int32_t* ctx_lens, int64_t B, int64_t H, int64_t Hkv, int64_t prefix_pages,
                   int64_t max_pages, int64_t num_pages, const Topology& topo, float* ws, void* o,
                   float* lse, hipStream_t s) {
-  using E = typename DecT<BF16>::e;
   const float c = (float)(1.0 / sqrt((double)D)) * kLog2e;
-  const int64_t rows = B * H;
-  float* pre_o = ws;
-  float* own_o = pre_o + rows * p.sp * D;
-  float* pre_ml = own_o + rows * p.so * D;
-  float* own_ml = pre_ml + 2 * rows * p.sp;
-  const dim3 grid((unsigned)(Hkv * p.sp * p.row_blocks));
+  const int64_t groups = head_groups(H, Hkv);
+  const Plan plan = plan_of(groups);
+  float* own_o = ws + p.own_o;
+  float2* pre_ml = (float2*)(ws + p.pre_ml);
+  float2* own_ml = (float2*)(ws + p.own_ml);
+  int2* first = (int2*)(ws + p.first);
+  int4* table = B > kWavePlan ? (int4*)(ws + p.table) : nullptr;
+  if (table != nullptr)
+    hipLaunchKernelGGL(fa_stream_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, ctx_lens, (int)B,
+                       (int)max_pages, plan, table);
+  if (!p.few) {
+    const dim3 grid((unsigned)(Hkv * p.sp * p.row_blocks));
 #define FA_PREFIX(WM)                                                                              \
   hipLaunchKernelGGL((fa_prefix_split_kernel<D, BF16, WM>), grid, dim3(64 * WM * kKeyGroups), 0, s, \
                      (const f16*)q, (const f16*)k_pool, (const f16*)v_pool, prefix_table,          \
-                     prefix_len, pre_o, (float2*)pre_ml, (int)(B * (H / Hkv)), (int)H, (int)Hkv,           \
-                     (int)prefix_pages, (int)num_pages, p.sp, p.row_blocks, topo.xcds, c)
-  if (p.wm == 1) FA_PREFIX(1);
-  else if (p.wm == 2) FA_PREFIX(2);
-  else FA_PREFIX(4);
+                     prefix_len, ws, pre_ml, (int)p.rows, (int)H, (int)Hkv, (int)prefix_pages,     \
+                     (int)num_pages, p.sp, p.row_blocks, topo.xcds, c)
+    if (p.wm == 2) FA_PREFIX(2);
+    else FA_PREFIX(4);
 #undef FA_PREFIX
-  hipLaunchKernelGGL((fa_own_split_kernel<D, BF16>),
-                     dim3((unsigned)p.so, (unsigned)decode_head_groups(H, Hkv), (unsigned)B),
-                     dim3(kDecThreads), 0, s, (const E*)q, (const E*)k_pool, (const E*)v_pool,
-                     page_table, ctx_lens, own_o, own_ml, (int)H, (int)Hkv, (int)max_pages,
-                     (int)num_pages, p.so, (int)decode_ordered(B, H, Hkv, D, p.so, topo.cus), c);
-  hipLaunchKernelGGL((fa_shared_join_kernel<D, BF16>), dim3((unsigned)rows), dim3(kJoinThreads), 0, s,
-                     pre_o, (const float2*)pre_ml, p.sp, own_o, (const float2*)own_ml, p.so, (E*)o, lse);
+  }
+  const int64_t pre_blocks = p.few ? chunk_blocks(p.sp, Hkv * p.row_blocks) : 0;
+  const bool nt = num_pages * Hkv * kTokens * D * 4 >= kPassThrough;
+  const auto kernel = nt ? fa_shared_chunk_kernel<D, BF16, true> : fa_shared_chunk_kernel<D, BF16, false>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(pre_blocks + chunk_blocks(p.own, groups))),
+                     dim3(stream::kThreads), 0, s, (const uint16_t*)q, (const char*)k_pool,
+                     (const char*)v_pool, prefix_table, prefix_len, page_table, ctx_lens, table, ws, pre_ml,
+                     own_o, own_ml, first, (int)B, (int)H, (int)Hkv, (int)(H / Hkv), (int)(groups / Hkv),
+                     (int)p.rows, (int)pre_blocks, p.row_blocks, p.sp, (int)prefix_pages, (int)max_pages,
+                     (int)num_pages, plan, c);
+  hipLaunchKernelGGL((fa_shared_join_kernel<D, BF16>), dim3((unsigned)(B * H)), dim3(kJoinThreads), 0, s,
+                     ws, pre_ml, own_o, own_ml, first, prefix_len, (uint16_t*)o, lse, (int)H, (int)(B * H),
+                     p.sp, (int)p.few, (int)prefix_pages, c);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? FA_OK : -(int)e;
 }
@@ -350,12 +364,13 @@ static int launch(const Plan& p, const void* q, const void* k_pool, const void* 
 
 extern "C" int64_t fa_decode_shared_workspace_floats(int64_t B, int64_t H, int64_t H_kv, int64_t D,
                                                      int64_t prefix_pages, int64_t max_pages) {
-  if (B <= 0 || H <= 0 || H_kv <= 0 || H % H_kv != 0 || D <= 0 || prefix_pages <= 0 || max_pages <= 0)
+  // the sizes that fa_validate_decode_shared refuses
+  constexpr int64_t kIndexes = (int64_t(1) << 31) - 1;
+  if (B <= 0 || H <= 0 || H_kv <= 0 || H % H_kv != 0 || (D != 64 && D != 128) || prefix_pages <= 0 ||
+      max_pages <= 0 || B > 65535 || H > 65535 || prefix_pages > (1 << 27) - 8 ||
+      max_pages > kIndexes / 16 || B > kIndexes / max_pages)
     return 0;
-  if (B > 65535 || H > 65535 || D > 128 || prefix_pages > (1 << 27) || max_pages > (1 << 27))
-    return 0;   // sizes that the call refuses
-  const fa::shared::Plan p = fa::shared::plan(B, H, H_kv, prefix_pages, max_pages);
-  return B * H * (D + 2) * (p.sp + p.so);
+  return fa::shared::cut_of(B, H, H_kv, D, prefix_pages, max_pages).floats;
 }
 
 extern "C" int fa_decode_shared(const void* q, const void* k_pool, const void* v_pool,
@@ -370,7 +385,7 @@ extern "C" int fa_decode_shared(const void* q, const void* k_pool, const void* v
                                            ctx_lens, B, H, H_kv, D, page_size, prefix_pages,
                                            max_pages, num_pages, workspace, o, lse);
   if (st != FA_OK) return st;
-  const Plan p = shared::plan(B, H, H_kv, prefix_pages, max_pages);
+  const Cut p = cut_of(B, H, H_kv, D, prefix_pages, max_pages);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const auto fn = D == 128 ? (bf16 ? launch<128, true> : launch<128, false>)
                            : (bf16 ? launch<64, true> : launch<64, false>);

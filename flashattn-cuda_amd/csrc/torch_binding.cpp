@@ -865,24 +865,23 @@ void check_weights(const torch::Tensor& w, int64_t B, int64_t Hkv, int64_t max_p
 }
 
 // decode_paged_weights(q, k_pool, v_pool, page_table, ctx_lens, weights,
-// num_splits=16, inplace=False) -> [O, L, weights + this step's]. No reference
-// counterpart.
+// inplace=False) -> [O, L, weights + this step's]. No reference counterpart.
 std::vector<torch::Tensor> decode_paged_weights(torch::Tensor q, torch::Tensor k_pool,
                                                 torch::Tensor v_pool, torch::Tensor page_table,
                                                 torch::Tensor ctx_lens, torch::Tensor weights,
-                                                int64_t num_splits, bool inplace) {
+                                                bool inplace) {
   const DecodeArgs a = check_decode(q, k_pool, v_pool, page_table, ctx_lens);
   check_weights(weights, a.B, a.Hkv, a.max_pages, q.device());
   const c10::DeviceGuard guard(q.device());
   const auto f32 = q.options().dtype(torch::kFloat);
-  auto ws = at::empty({fa_decode_weights_workspace_floats(a.B, a.H, a.D, a.max_pages, num_splits)}, f32);
+  auto ws = at::empty({fa_decode_weights_workspace_floats(a.B, a.H, a.Hkv, a.D, a.max_pages)}, f32);
   auto o = at::empty({a.B, a.H, a.D}, q.options());
   auto lse = at::empty({a.B, a.H}, f32);
   auto w = inplace ? weights : at::empty(weights.sizes(), f32);
   const int st = fa_decode_paged_weights(
       q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), page_table.data_ptr<int32_t>(),
       ctx_lens.data_ptr<int32_t>(), weights.data_ptr<float>(), a.B, a.H, a.Hkv, a.D, a.page_size,
-      a.max_pages, a.num_pages, num_splits, ws.data_ptr<float>(), o.data_ptr(), lse.data_ptr<float>(),
+      a.max_pages, a.num_pages, ws.data_ptr<float>(), o.data_ptr(), lse.data_ptr<float>(),
       w.data_ptr<float>(), q.scalar_type() == torch::kBFloat16, current_stream(q));
   check_status(st, "fa_decode_paged_weights");
   return {o, lse, w};
@@ -924,12 +923,13 @@ std::vector<torch::Tensor> kv_evict(torch::Tensor k_pool, torch::Tensor v_pool, 
   auto new_weights = at::empty({B, Hkv, 16 * new_page_table.size(1)}, weights.options());
   auto new_lens = at::empty({B}, page_table.options());
   auto bad = at::empty({B}, page_table.options());
+  auto ws = at::empty({fa_kv_evict_workspace_words(B, Hkv)}, page_table.options());
   const int st = fa_kv_evict(k_pool.data_ptr(), v_pool.data_ptr(), page_table.data_ptr<int32_t>(),
                              ctx_lens.data_ptr<int32_t>(), weights.data_ptr<float>(),
                              new_page_table.data_ptr<int32_t>(), kept.data_ptr<int32_t>(),
                              new_weights.data_ptr<float>(), new_lens.data_ptr<int32_t>(),
-                             bad.data_ptr<int32_t>(), B, Hkv, k_pool.size(3), keep, recent,
-                             k_pool.size(2), max_pages, new_page_table.size(1), k_pool.size(0),
+                             bad.data_ptr<int32_t>(), ws.data_ptr<int32_t>(), B, Hkv, k_pool.size(3), keep,
+                             recent, k_pool.size(2), max_pages, new_page_table.size(1), k_pool.size(0),
                              current_stream(k_pool));
   check_status(st, "fa_kv_evict");
   return {kept, new_weights, new_lens, bad};
@@ -1087,7 +1087,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("decode_paged_weights", &decode_paged_weights,
         "paged decode that adds up attention weights: returns [O in q's dtype, L float, weights float]",
         py::arg("q"), py::arg("k_pool"), py::arg("v_pool"), py::arg("page_table"), py::arg("ctx_lens"),
-        py::arg("weights"), py::arg("num_splits") = 16, py::arg("inplace") = false);
+        py::arg("weights"), py::arg("inplace") = false);
   m.def("kv_evict", &kv_evict,
         "pack each head's newest and heaviest tokens: returns [kept, new_weights, new_lens, bad]",
         py::arg("k_pool"), py::arg("v_pool"), py::arg("page_table"), py::arg("ctx_lens"),

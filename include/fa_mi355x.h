@@ -609,35 +609,37 @@ int fa_validate_decode_shared(const void* q, const void* k_pool, const void* v_p
                               const float* workspace, const void* o, const float* lse);
 
 /*
- * fa_decode_paged_gqa_f16 (bf16 != 0: fa_decode_paged_bf16) that also adds up the
- * attention that each cached token gets (no reference counterpart):
+ * The paged decode (o, lse as fa_decode_paged_gqa_f16's; bf16 != 0:
+ * fa_decode_paged_bf16's) that also adds up the attention that each cached token
+ * gets (no reference counterpart):
  *   weights_out[b, hk, j] = weights[b, hk, j] + sum over the query heads h of KV
  *   head hk of exp(s_hj - lse_h),   j < ctx_lens[b],
  * fp32 [B, H_kv, max_pages * 16], 16-byte aligned; slots past the context keep
  * their value. weights_out may be weights (in place), but not overlap it
  * otherwise. Where o and lse are NaN (an invalid page or length), so are the
- * sequence's weights up to its context, cut to the table. workspace:
+ * sequence's weights up to its context, cut to the table. How the pages are shared
+ * out follows from the lengths of the whole batch, so a sequence's last bits may
+ * depend on the others' lengths; the same call gives the same bits. workspace:
  * fa_decode_weights_workspace_floats(...) floats, 16-byte aligned, need not be
  * cleared; calls that may overlap need one each.
  */
 int fa_decode_paged_weights(const void* q, const void* k_pool, const void* v_pool,
                             const int32_t* page_table, const int32_t* ctx_lens,
                             const float* weights, int64_t B, int64_t H, int64_t H_kv, int64_t D,
-                            int64_t page_size, int64_t max_pages, int64_t num_pages,
-                            int64_t num_splits, float* workspace, void* o, float* lse,
-                            float* weights_out, int bf16, void* stream);
+                            int64_t page_size, int64_t max_pages, int64_t num_pages, float* workspace,
+                            void* o, float* lse, float* weights_out, int bf16, void* stream);
 
 /* Floats of fa_decode_paged_weights' workspace; 0 for invalid sizes. */
-int64_t fa_decode_weights_workspace_floats(int64_t B, int64_t H, int64_t D, int64_t max_pages,
-                                           int64_t num_splits);
+int64_t fa_decode_weights_workspace_floats(int64_t B, int64_t H, int64_t H_kv, int64_t D,
+                                           int64_t max_pages);
 
 /* Host-only argument check of fa_decode_paged_weights. */
 int fa_validate_decode_weights(const void* q, const void* k_pool, const void* v_pool,
                                const int32_t* page_table, const int32_t* ctx_lens,
                                const float* weights, int64_t B, int64_t H, int64_t H_kv, int64_t D,
                                int64_t page_size, int64_t max_pages, int64_t num_pages,
-                               int64_t num_splits, const float* workspace, const void* o,
-                               const float* lse, const float* weights_out);
+                               const float* workspace, const void* o, const float* lse,
+                               const float* weights_out);
 
 /*
  * Cuts each head's cache to at most `keep` tokens (no reference counterpart). With
@@ -651,22 +653,27 @@ int fa_validate_decode_weights(const void* q, const void* k_pool, const void* v_
  * invalid are not copied and set bad[b] to 1; a negative length, or one beyond the
  * table, sets bad[b] and new_lens[b] = 0; every other bad[b] is set to 0. Pages of
  * new_page_table that the call writes must not be among those it reads. 16-bit
- * rows of any type. 0 <= recent <= keep <= new_max_pages * 16.
+ * rows of any type. 0 <= recent <= keep <= new_max_pages * 16. workspace:
+ * fa_kv_evict_workspace_words(...) words of 4 bytes that need not be cleared; calls
+ * that may overlap need one each.
  */
 int fa_kv_evict(void* k_pool, void* v_pool, const int32_t* page_table, const int32_t* ctx_lens,
                 const float* weights, const int32_t* new_page_table, int32_t* kept,
-                float* new_weights, int32_t* new_lens, int32_t* bad, int64_t B, int64_t H_kv,
-                int64_t D, int64_t keep, int64_t recent, int64_t page_size, int64_t max_pages,
-                int64_t new_max_pages, int64_t num_pages, void* stream);
+                float* new_weights, int32_t* new_lens, int32_t* bad, int32_t* workspace, int64_t B,
+                int64_t H_kv, int64_t D, int64_t keep, int64_t recent, int64_t page_size,
+                int64_t max_pages, int64_t new_max_pages, int64_t num_pages, void* stream);
+
+/* Words of fa_kv_evict's workspace; 0 for invalid sizes. */
+int64_t fa_kv_evict_workspace_words(int64_t B, int64_t H_kv);
 
 /* Host-only argument check of fa_kv_evict. */
 int fa_validate_kv_evict(const void* k_pool, const void* v_pool, const int32_t* page_table,
                          const int32_t* ctx_lens, const float* weights,
                          const int32_t* new_page_table, const int32_t* kept,
                          const float* new_weights, const int32_t* new_lens, const int32_t* bad,
-                         int64_t B, int64_t H_kv, int64_t D, int64_t keep, int64_t recent,
-                         int64_t page_size, int64_t max_pages, int64_t new_max_pages,
-                         int64_t num_pages);
+                         const int32_t* workspace, int64_t B, int64_t H_kv, int64_t D, int64_t keep,
+                         int64_t recent, int64_t page_size, int64_t max_pages,
+                         int64_t new_max_pages, int64_t num_pages);
 
 #ifdef __cplusplus
 }

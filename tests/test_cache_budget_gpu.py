@@ -39,7 +39,8 @@ def _check_weights(got, case, dtype, tag=""):
 
 CASES = [(1, 1, 1, 64, [1]), (2, 8, 2, 64, [0, 5]), (3, 4, 4, 128, [1, 16, 17]), (4, 8, 8, 64, [300, 0, 2, 64]),
          (2, 32, 8, 128, [33, 1700]), (3, 40, 2, 64, [100, 2500, 17]), (1, 128, 1, 128, [800]), (2, 36, 2, 128, [1023, 1025]),
-         (20, 4, 2, 64, [13 * i for i in range(20)]), (1, 300, 1, 64, [1100])]
+         (20, 4, 2, 64, [13 * i for i in range(20)]), (1, 300, 1, 64, [1100]), (300, 4, 2, 64, [7 * i % 90 for i in range(300)]),
+         (1500, 2, 1, 64, [i % 5 for i in range(1500)]), (1, 8, 1, 128, [9000]), (65, 2, 2, 128, [40] * 64 + [3000])]
 
 
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
@@ -47,16 +48,15 @@ CASES = [(1, 1, 1, 64, [1]), (2, 8, 2, 64, [0, 5]), (3, 4, 4, 128, [1, 16, 17]),
 def test_weights_match_oracle(fa, dev, i, dtype):
     B, H, Hkv, D, ctx = CASES[i]
     case = _paged(dev, i, B, H, Hkv, D, ctx, dtype, extra=i % 3)
-    for S in (16, 1, 5):
-        before = case[5].clone()
-        got = fa.decode_paged_weights(*case, num_splits=S)
-        _check_weights(got, case, dtype, f"{CASES[i]} S{S}")
-        assert torch.equal(case[5], before)
-        again = fa.decode_paged_weights(*case, num_splits=S)
-        assert all(torch.equal(x, y) for x, y in zip(got, again))
-        w = before.clone()
-        inplace = fa.decode_paged_weights(*case[:5], w, num_splits=S, inplace=True)
-        assert inplace[2].data_ptr() == w.data_ptr() and all(torch.equal(x, y) for x, y in zip(got, inplace))
+    before = case[5].clone()
+    got = fa.decode_paged_weights(*case)
+    _check_weights(got, case, dtype, f"{CASES[i]}")
+    assert torch.equal(case[5], before)
+    again = fa.decode_paged_weights(*case)
+    assert all(torch.equal(x, y) for x, y in zip(got, again))
+    w = before.clone()
+    inplace = fa.decode_paged_weights(*case[:5], w, inplace=True)
+    assert inplace[2].data_ptr() == w.data_ptr() and all(torch.equal(x, y) for x, y in zip(got, inplace))
 
 
 def test_weights_of_a_step_sum_to_the_heads(fa, dev):
@@ -71,8 +71,7 @@ def test_weights_of_a_step_sum_to_the_heads(fa, dev):
 def test_weights_large_scores(fa, dev):
     for amp in (8.0, 60.0):
         case = _paged(dev, 4, 3, 8, 2, 64, [700, 3, 1200], "fp16", amp=amp)
-        for S in (16, 3):
-            _check_weights(fa.decode_paged_weights(*case, num_splits=S), case, "fp16", f"amp {amp}")
+        _check_weights(fa.decode_paged_weights(*case), case, "fp16", f"amp {amp}")
 
 
 @pytest.mark.parametrize("D", [64, 128])

@@ -101,14 +101,14 @@ def test_validate_shared(capi, i):
 
 
 def _weights(**kw):
-    a = dict(q=A, kp=A, vp=A, t=A, c=A, w=A, B=4, H=32, Hkv=8, D=128, size=16, mp=20, pages=500, S=16, ws=A, o=A, l=A, wo=A)
+    a = dict(q=A, kp=A, vp=A, t=A, c=A, w=A, B=4, H=32, Hkv=8, D=128, size=16, mp=20, pages=500, ws=A, o=A, l=A, wo=A)
     a.update(kw)
     return list(a.values())
 
 
 WEIGHTS = [
     (dict(), "FA_OK"), (dict(w=0), "FA_ERR_NULL_POINTER"), (dict(wo=0), "FA_ERR_NULL_POINTER"), (dict(ws=0), "FA_ERR_NULL_POINTER"),
-    (dict(l=0), "FA_ERR_NULL_POINTER"), (dict(S=0), "FA_ERR_NUM_SPLITS"), (dict(S=17), "FA_ERR_NUM_SPLITS"), (dict(H=30), "FA_ERR_KV_HEADS"),
+    (dict(l=0), "FA_ERR_NULL_POINTER"), (dict(H=30), "FA_ERR_KV_HEADS"),
     (dict(D=32), "FA_ERR_HEAD_DIM"), (dict(w=A + 4), "FA_ERR_ALIGNMENT"), (dict(wo=A + 8), "FA_ERR_ALIGNMENT"), (dict(l=A + 1), "FA_ERR_ALIGNMENT"),
     (dict(mp=1 << 20, B=2000, Hkv=32), "FA_OK"), (dict(mp=1 << 20, B=2000, H=64, Hkv=64), "FA_ERR_TOO_LARGE"), (dict(B=40000, H=1000, Hkv=1), "FA_ERR_TOO_LARGE"),
 ]
@@ -124,13 +124,13 @@ def test_validate_weights(capi, i):
 
 
 def _evict(**kw):
-    a = dict(kp=A, vp=A, t=A, c=A, w=A, nt=A, kept=A, nw=A, nl=A, bad=A, B=4, Hkv=8, D=128, keep=100, recent=10, size=16, mp=20, nmp=7, pages=500)
+    a = dict(kp=A, vp=A, t=A, c=A, w=A, nt=A, kept=A, nw=A, nl=A, bad=A, ws=A, B=4, Hkv=8, D=128, keep=100, recent=10, size=16, mp=20, nmp=7, pages=500)
     a.update(kw)
     return list(a.values())
 
 
 EVICT = [
-    (dict(), "FA_OK"), *((({x: 0}), "FA_ERR_NULL_POINTER") for x in ("kp", "vp", "t", "c", "w", "nt", "kept", "nw", "nl", "bad")),
+    (dict(), "FA_OK"), *((({x: 0}), "FA_ERR_NULL_POINTER") for x in ("kp", "vp", "t", "c", "w", "nt", "kept", "nw", "nl", "bad", "ws")),
     (dict(D=96), "FA_ERR_HEAD_DIM"), (dict(B=0), "FA_ERR_BATCH_HEADS"), (dict(size=4), "FA_ERR_PAGE_SIZE"), (dict(mp=0), "FA_ERR_MAX_PAGES"),
     (dict(nmp=0), "FA_ERR_MAX_PAGES"), (dict(pages=-1), "FA_ERR_NUM_PAGES"), (dict(kp=A + 8), "FA_ERR_ALIGNMENT"), (dict(kept=A + 2), "FA_ERR_ALIGNMENT"),
     (dict(keep=0), "FA_ERR_BUDGET"), (dict(keep=113), "FA_ERR_BUDGET"), (dict(keep=112), "FA_OK"), (dict(recent=-1), "FA_ERR_BUDGET"),
@@ -154,17 +154,28 @@ def test_status_strings(capi):
 
 
 @pytest.mark.parametrize("B,H,Hkv,D,pp,mp", [(1, 1, 1, 64, 1, 1), (32, 32, 8, 128, 500, 94), (64, 32, 8, 128, 2048, 63), (1, 32, 1, 128, 8192, 1),
-                                             (300, 32, 32, 64, 625, 1), (1, 128, 1, 128, 50, 2), (2000, 8, 8, 64, 10, 4000)])
-def test_shared_workspace(capi, B, H, Hkv, D, pp, mp):
-    """Room for 1 to 256 parts of the prefix and 1 to 16 of the own pages, D + 2 floats each; none for invalid sizes."""
+                                             (300, 32, 32, 64, 625, 1), (1, 128, 1, 128, 50, 2), (2000, 8, 8, 64, 10, 4000), (65535, 1, 1, 64, 4, 8)])
+def test_workspaces(capi, B, H, Hkv, D, pp, mp):
+    """Room for a part of the prefix and a chunk a sequence at least, at most 256 parts and 4096 workgroups' chunks or a
+    chunk for 8 pages beside one a sequence; none for sizes that are refused."""
     lib = capi.load()
+    part = B * H * (D + 2)
+    chunk = H * (D + 2)
+    groups = Hkv * -(-H // Hkv // 16)
+    most = min(B * mp // 8, -(-4096 // groups)) + B
+    small = 3 + 2 * B + (4 * (1 + most) if B > 256 else 0)
     n = lib.fa_decode_shared_workspace_floats(B, H, Hkv, D, pp, mp)
-    parts, rest = divmod(n, B * H * (D + 2))
-    assert rest == 0 and 2 <= parts <= min(256, -(-pp // 4)) + min(16, -(-mp // 8))
-    for bad in ((0, H, Hkv, D, pp, mp), (B, H, H + 1, D, pp, mp), (B, H, Hkv, D, 0, mp), (B, H, Hkv, D, pp, -1), (B, 70000, 1, D, pp, mp)):
+    assert part + B * chunk <= n <= min(256, -(-pp // 4)) * part + most * chunk + small
+    w = lib.fa_decode_weights_workspace_floats(B, H, Hkv, D, mp)
+    scores = B * H * (((16 * mp + 63) // 64) | 1) * 64   # rows of an odd number of 256 bytes
+    assert scores + B * chunk <= w <= scores + most * chunk + small
+    for bad in ((0, H, Hkv, D, pp, mp), (B, H, H + 1, D, pp, mp), (B, H, Hkv, 96, pp, mp), (B, H, Hkv, D, 0, mp), (B, H, Hkv, D, pp, -1),
+                (B, 70000, 1, D, pp, mp), (B, H, Hkv, D, 1 << 27, mp), (65535, H, Hkv, D, pp, 1 << 16)):
         assert lib.fa_decode_shared_workspace_floats(*bad) == 0
-    assert lib.fa_decode_weights_workspace_floats(B, H, D, mp, 5) == B * H * (16 * mp + 5 * (D + 2))
-    assert lib.fa_decode_weights_workspace_floats(B, H, D, 0, 5) == 0
+        if bad[0] == 0 or bad[1] == 70000:
+            assert lib.fa_kv_evict_workspace_words(bad[0], bad[1]) == 0
+        if bad[4] not in (0, 1 << 27):
+            assert lib.fa_decode_weights_workspace_floats(*bad[:4], bad[5]) == 0
 
 
 def test_binding_refuses_host_tensors(fa):

@@ -74,7 +74,8 @@ CASES = [
     (9, 16, 4, 64, 1000, [40] * 9), (16, 32, 8, 128, 700, list(range(0, 160, 10))), (33, 4, 1, 64, 257, [7] * 33),
     (31, 36, 4, 128, 300, [9 * i % 50 for i in range(31)]), (70, 8, 2, 64, 333, [3 * i for i in range(70)]),
     (1, 128, 1, 128, 800, [20]), (3, 40, 2, 64, 2100, [100, 0, 17]), (2, 2, 1, 128, 0, [70, 0]), (2, 4, 2, 64, 15, [0, 0]),
-    (40, 32, 8, 128, 70, [2] * 40),
+    (40, 32, 8, 128, 70, [2] * 40), (300, 2, 1, 64, 90, [5 * i % 70 for i in range(300)]), (600, 4, 4, 128, 40, [i % 3 for i in range(600)]),
+    (16, 2, 1, 64, 1500, [3] * 16), (17, 2, 1, 64, 1500, [40] * 16 + [2000]),
 ]
 
 
