@@ -52,7 +52,8 @@ fa_weights_chunk_kernel(const uint16_t* __restrict__ q, const char* __restrict__
   const int hk = at.hg / ngrp, sub = at.hg - hk * ngrp, col = threadIdx.x & 15;
   const int h = hk * group + 16 * sub + col;
   const bool live = 16 * sub + col < group;
-  chunk_body<D, BF16, NT, true>(sh, q, k_pool, v_pool, page_table + (size_t)r.b * max_pages, r.p0, r.p1,
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  chunk_body<D, BF16, NT, true>(sh, wave, q, k_pool, v_pool, page_table + (size_t)r.b * max_pages, r.p0, r.p1,
                                 r.ctx, r.bad, live, ((int64_t)r.b * H + h) * D, hk, Hkv, num_pages, c,
                                 scores + ((int64_t)r.b * H + h - col) * score_row(max_pages),
                                 score_row(max_pages), min(16, group - 16 * sub), part_o, part_ml,
@@ -77,7 +78,7 @@ fa_weights_join_kernel(const float* __restrict__ part_o, const float2* __restric
     const int row = blockIdx.x, b = row / H;
     const int2 f = first_of[b];
     const Parts a{part_o, part_ml, (int64_t)f.x * H + (row - b * H), H, f.y};
-    join_row<D, BF16>(sh, a, Parts{part_o, part_ml, 0, 0, 0}, c, o + (int64_t)row * D, lse + row);
+    join_row<D, BF16>(sh, a, Parts{part_o, part_ml, 0, 0, 0}, o + (int64_t)row * D, lse + row);
     return;
   }
   const int unit = (int)blockIdx.x - rows;
@@ -95,14 +96,14 @@ fa_weights_join_kernel(const float* __restrict__ part_o, const float2* __restric
   f32x4 w = f32x4{};
   if (there) w = *reinterpret_cast<const f32x4*>(w_in + at);
   if (start < ctx) {
-    __shared__ float2 J[kJoinThreads];   // of a group's heads: maximum, 1 / sum
+    __shared__ float2 J[kJoinThreads];   // of a group's heads: reference, 1 / sum
     const int2 f = first_of[b];
     f32x4 sum = f32x4{};
     for (int g0 = 0; g0 < G; g0 += kJoinThreads) {
       const int gs = min(kJoinThreads, G - g0);
       if (g0 > 0) __syncthreads();
       for (int g = wave; g < gs; g += kJoinThreads / 64) {
-        const float2 x = join_wave(Parts{part_o, part_ml, (int64_t)f.x * H + hk * G + g0 + g, H, f.y}, c);
+        const float2 x = join_wave(Parts{part_o, part_ml, (int64_t)f.x * H + hk * G + g0 + g, H, f.y});
         if ((tid & 63) == 0) J[g] = make_float2(x.x, 1.f / x.y);
       }
       __syncthreads();
@@ -114,7 +115,7 @@ fa_weights_join_kernel(const float* __restrict__ part_o, const float2* __restric
           const f32x4 x = *reinterpret_cast<const f32x4*>(sc + g * next);
           const float2 Jg = J[g];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) sum[i] = fmaf(exp2_hw((x[i] - Jg.x) * c), Jg.y, sum[i]);
+          for (int i = 0; i < 4; ++i) sum[i] = fmaf(exp2_hw(fmaf(x[i], c, -Jg.x)), Jg.y, sum[i]);
         }
       }
     }

@@ -8,7 +8,7 @@
 // share a KV head, B * H / H_kv of them, form one product with them, as in a
 // forward pass without a mask. Few rows (kFewRows) go through the chunks of
 // fa_stream.hpp instead, as the own pages do, and in their launch. One launch joins
-// the partials of both by their (maximum, sum).
+// the partials of both by their references and sums.
 #include <hip/hip_runtime.h>
 
 #include <math.h>
@@ -25,44 +25,54 @@ using namespace stream;
 
 constexpr int kTile = 64;     // keys of a tile: 4 pages
 constexpr int kStages = 4;    // tiles in LDS, three of them in flight
+constexpr float kSlack = 8.f;   // of weights' exponents; see there
 constexpr int kKeyGroups = 2; // waves side by side over the keys of a tile
+constexpr int kRowGroups = 4, kTileRows = 32 * kRowGroups;   // and over the query rows of a unit
+constexpr int kTileWaves = kKeyGroups * kRowGroups;
 
-// Prefix pass. One workgroup per (KV head, run of tiles, 32 WM query rows): WM x
-// 2 waves, wave (rm, kg) with rows 32 rm .. + 31 and the tile's keys 32 kg .. +
-// 31. Tiles are copied global -> LDS (buffer_load ... lds), the rows past the
-// prefix as zeros (the copy's range ends there), and wait in a ring of kStages.
-// Scores and products are those of the forward: S^T = K Q^T with Q in registers,
-// O^T += V^T P^T with P^T straight from the accumulators (fa_tile.hpp), P rounded
-// to the operands' type beside an unrounded sum, as the forward rounds it.
-template <int D, bool BF16, int WM>
-__global__ void __launch_bounds__(64 * WM * kKeyGroups)
-fa_prefix_split_kernel(const f16* __restrict__ q, const f16* __restrict__ kpool,
-                       const f16* __restrict__ vpool, const int32_t* __restrict__ prefix_table,
-                       const int32_t* __restrict__ prefix_len, float* __restrict__ part_o,
-                       float2* __restrict__ part_ml, int rows, int H, int Hkv, int max_pages,
-                       int num_pages, int S, int row_blocks, int nxcd, float c) {
-  constexpr int NW = WM * kKeyGroups;
-  constexpr int PAGE = kTokens * D * 2;
+// LDS of a workgroup that runs either a run of tiles or two chunks.
+template <int D>
+struct TileShared {
+  static constexpr int kPage = kTokens * D * 2;
+  static constexpr int kStage = 2 * (kTile / kTokens) * kPage;   // K, then V
+  __attribute__((aligned(1024))) char ring[kStages * kStage];
+  float m[kTileWaves][64], l[kTileWaves][64];
+  int bad;
+};
+
+// Prefix pass, unit g of `units`: (KV head, run of tiles, kTileRows query rows) by
+// kRowGroups x 2 waves, wave (rm, kg) with rows 32 rm .. + 31 and the tile's keys 32
+// kg .. + 31; rm the slow one, so that of a few rows every SIMD has some. Tiles are
+// copied global -> LDS (buffer_load ... lds), the rows past the prefix as zeros (the
+// copy's range ends there), and wait in a ring of kStages. Scores and products are
+// those of the forward: S^T = K Q^T with Q in registers, O^T += V^T P^T with P^T
+// straight from the accumulators (fa_tile.hpp), P rounded to the operands' type beside
+// an unrounded sum, as the forward rounds it.
+template <int D, bool BF16>
+__device__ __forceinline__ void
+tile_unit(TileShared<D>& sh, const int unit, const int units, const f16* __restrict__ q,
+          const f16* __restrict__ kpool, const f16* __restrict__ vpool,
+          const int32_t* __restrict__ prefix_table, const int32_t* __restrict__ prefix_len,
+          float* __restrict__ part_o, float2* __restrict__ part_ml, int rows, int H, int Hkv,
+          int max_pages, int num_pages, int S, int row_blocks, int nxcd, float c) {
+  constexpr int WM = kRowGroups, NW = kTileWaves;
+  constexpr int PAGE = TileShared<D>::kPage, STAGE = TileShared<D>::kStage;
   constexpr int CPR = D / 8;
   constexpr int NC = PAGE / 1024;            // 1 KiB copies of a page
   constexpr int PAGES = kTile / kTokens;
   constexpr int NU = 2 * PAGES / NW;         // pages, of K or V, a wave copies of a tile
-  constexpr int STAGE = 2 * PAGES * PAGE;    // K, then V
   constexpr int DB = D / 32;
-  static_assert(WM * DB * 16 * 64 * 4 <= kStages * STAGE, "merge area within the ring");
-  __shared__ __attribute__((aligned(1024))) char smem[kStages * STAGE];
-  __shared__ float sh_m[WM][64], sh_l[WM][64];
-  __shared__ int sh_bad;
+  static_assert(NW * DB * 8 * 64 * 4 <= kStages * STAGE, "merge area within the ring");
 
   // Row blocks that read the same tiles are neighbours on one XCD.
-  const int g = xcd_remap(blockIdx.x, gridDim.x, nxcd);
+  const int g = xcd_remap(unit, units, nxcd);
   const int rb = g % row_blocks, s = (g / row_blocks) % S, hk = g / row_blocks / S;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int rm = wave % WM, kg = wave / WM;
+  const int rm = wave / kKeyGroups, kg = wave % kKeyGroups;
   const int G = H / Hkv;
 
-  if (tid == 0) sh_bad = 0;
+  if (tid == 0) sh.bad = 0;
   __syncthreads();
   int P = prefix_len[0];
   bool bad = P < 0 || P > max_pages * kTokens;
@@ -74,6 +84,7 @@ fa_prefix_split_kernel(const f16* __restrict__ q, const f16* __restrict__ kpool,
   // Query row of this lane: row r is head r % G of the group, sequence r / G.
   const int row = (rb * WM + rm) * 32 + (lane & 31);
   const bool live = row < rows;
+  const bool some = (rb * WM + rm) * 32 < rows;   // of the wave's rows; without, it only copies
   const int64_t qrow = live ? (int64_t)(row / G) * H + hk * G + row % G : 0;
   f16x8 qf[D / 16];
 #pragma unroll
@@ -90,7 +101,7 @@ fa_prefix_split_kernel(const f16* __restrict__ q, const f16* __restrict__ kpool,
     const int L = 64 * i + lane, t = L / CPR;
     coff[i] = (uint32_t)((t * CPR + ((L % CPR) ^ t_swz<D>(t))) * 16);
   }
-  const uint32_t lds0 = lds_addr(smem);
+  const uint32_t lds0 = lds_addr(sh.ring);
   // Page ids of the wave's pages, 64 tiles at a time, read with readlane.
   int pidv[NU];
   auto issue = [&](int k) {   // tile t0 + k
@@ -100,6 +111,9 @@ fa_prefix_split_kernel(const f16* __restrict__ q, const f16* __restrict__ kpool,
       if ((k & 63) == 0) {
         const int pi = (t0 + k + lane) * PAGES + unit / 2;
         pidv[x] = t0 + k + lane < t1 && pi < pages ? prefix_table[pi] : -1;
+        // Used up here: after the branch the compiler would wait for the load on
+        // either path, and with it, every tile, for all copies in flight.
+        asm volatile("" : "+v"(pidv[x]));
       }
       const int pi = (t0 + k) * PAGES + unit / 2;
       const int pid = __builtin_amdgcn_readlane(pidv[x], k & 63);
@@ -114,96 +128,153 @@ fa_prefix_split_kernel(const f16* __restrict__ q, const f16* __restrict__ kpool,
     }
   };
 
-  float m = -INFINITY, l = 0.f;
+  float mc = -INFINITY, l = 0.f;   // reference of the weights, in units of log 2; their sum
   f32x16 o[DB];
 #pragma unroll
   for (int db = 0; db < DB; ++db) o[db] = f32x16{};
-
+  f16x8 kf[D / 16];
+  // K's operands of the wave's 32 keys of tile t0 + k.
+  const auto load_k = [&](int k) {
+    const uint32_t kb = row_base<D>(lds0 + (k % kStages) * STAGE + kg * (32 * 2 * D), lane);
 #pragma unroll
-  for (int k = 0; k < kStages - 1; ++k) issue(k);
-  for (int t = t0; t < t1; ++t) {
-    const int k = t - t0;
-    wait_vmcnt<(kStages - 2) * NU * NC>();   // this wave's copies of tile t have landed
-    __syncthreads();                         // everyone's, and tile t - 1 is used up
-    issue(k + kStages - 1);
-    const int key0 = t * kTile + 32 * kg;
-    if (key0 < P) {
-      const uint32_t ks = lds0 + (k % kStages) * STAGE + kg * (32 * 2 * D);
-      const uint32_t kb = row_base<D>(ks, lane), vb = col_base<D>(ks + PAGES * PAGE, lane);
-      f32x16 sc = f32x16{};
+    for (int kk = 0; kk < D / 16; ++kk) kf[kk] = load_row_frag<D>(kb, 0, kk);
+  };
+  const auto scores = [&]() {
+    f32x16 x = f32x16{};
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) sc = mma32<BF16>(load_row_frag<D>(kb, 0, kk), qf[kk], sc);
-      float mx = -INFINITY;
-      if (key0 + 32 > P) {
+    for (int kk = 0; kk < D / 16; ++kk) x = mma32<BF16>(kf[kk], qf[kk], x);
+    return x;
+  };
+  // The wave's keys of tile t0 + k, whose scores are sc; NEXT: and the scores of its
+  // keys of the next tile, whose products run under this one's exponentials. LDS reads
+  // go out a phase before their products: one after the other each product waited
+  // for its own.
+  const auto step = [&](int k, f32x16& sc, auto next) {
+    if constexpr (decltype(next)::value) load_k(k + 1);
+    const int key0 = (t0 + k) * kTile + 32 * kg;
+    if (key0 + 32 > P) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (key0 + st_key(0, r, lane) >= P) sc[r] = -INFINITY;
-      }
-#pragma unroll
-      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[r]);
-      mx = max_xor32(mx);
-      const float m_new = fmaxf(m, mx);
-      if (__any(m_new != m)) {
-        const float alpha = m == m_new ? 1.f : exp2_hw((m - m_new) * c);
-        l *= alpha;
-#pragma unroll
-        for (int db = 0; db < DB; ++db)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
-        m = m_new;
-      }
-      const float mu = m == -INFINITY ? 0.f : m;   // no score above -inf so far: weights of 0
-      float ps = 0.f;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        sc[r] = exp2_hw((sc[r] - mu) * c);
-        ps += sc[r];
-      }
-      l += ps;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const f16x8 p = pack_px<BF16>(sc, j);
-#pragma unroll
-        for (int db = 0; db < DB; ++db) o[db] = mma32<BF16>(load_col_frag<D>(vb, 0, j, db), p, o[db]);
-      }
+      for (int r = 0; r < 16; ++r)
+        if (key0 + st_key(0, r, lane) >= P) sc[r] = -INFINITY;
     }
+    float mx = sc[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) mx = fmaxf(mx, sc[r]);
+    mx = max_xor32(mx) * c;
+    // The reference follows the maximum only where that is kSlack above it: of 32 rows
+    // one has a new maximum in most steps. Weights reach 2^kSlack.
+    if (__any(mx > mc + kSlack)) {
+      const float m_new = fmaxf(mc, mx);
+      const float alpha = m_new == mc ? 1.f : exp2_hw(mc - m_new);
+      l *= alpha;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
+      mc = m_new;
+    }
+    const float mu = mc == -INFINITY ? 0.f : mc;   // no score above -inf so far: weights of 0
+    __builtin_amdgcn_sched_barrier(0);
+    const uint32_t vb = col_base<D>(lds0 + (k % kStages) * STAGE + PAGES * PAGE + kg * (32 * 2 * D), lane);
+    f16x8 vf[2][DB];
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int db = 0; db < DB; ++db) vf[j][db] = load_col_frag<D>(vb, 0, j, db);
+    __builtin_amdgcn_sched_barrier(0);
+    f32x16 sn;
+    if constexpr (decltype(next)::value) sn = scores();
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sc[r] = exp2_hw(fmaf(sc[r], c, -mu));
+    f16x8 p[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) p[j] = pack_px<BF16>(sc, j);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int db = 0; db < DB; ++db) o[db] = mma32<BF16>(vf[j][db], p[j], o[db]);
+    float ps[4] = {sc[0], sc[1], sc[2], sc[3]};
+#pragma unroll
+    for (int r = 4; r < 16; ++r) ps[r & 3] += sc[r];
+    l += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+    if constexpr (decltype(next)::value) sc = sn;
+  };
+
+  const int n = t1 - t0;
+  if (n > 0) {
+#pragma unroll
+    for (int k = 0; k < kStages - 1; ++k) issue(k);
+    wait_vmcnt<(kStages - 2) * NU * NC>();   // this wave's copies of the first tile have landed
+    __syncthreads();                         // and everyone's
+    f32x16 sc;
+    if (some) {
+      load_k(0);
+      sc = scores();
+    }
+    for (int k = 0; k < n - 1; ++k) {
+      wait_vmcnt<(kStages - 3) * NU * NC>();   // tile k + 1
+      __syncthreads();                         // everyone's, and tile k - 1 is used up
+      issue(k + kStages - 1);
+      if (some) step(k, sc, std::true_type{});
+    }
+    if (some) step(n - 1, sc, std::false_type{});
   }
   l = sum_xor32(l);
 
-  // Merge the two key groups through LDS, register by register: lanes of the two
-  // waves hold the same elements.
+  // Merge the two key groups through LDS, each for half of the columns: a wave
+  // leaves the other's half register by register, lanes of the two hold the same
+  // elements.
   wait_vmem();
-  if (bad) sh_bad = 1;
+  if (bad) sh.bad = 1;
   __syncthreads();
-  float* sh_o = reinterpret_cast<float*>(smem) + rm * (DB * 16 * 64);
-  if (kg == 1) {
+  constexpr int HB = DB / 2, XCH = HB * 16 * 64;   // words a wave leaves
+  float* const area = reinterpret_cast<float*>(sh.ring);
+  {
+    float* to = area + (wave)*XCH;
 #pragma unroll
-    for (int db = 0; db < DB; ++db)
+    for (int h = 0; h < HB; ++h)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) sh_o[(db * 16 + r) * 64 + lane] = o[db][r];
-    sh_m[rm][lane] = m;
-    sh_l[rm][lane] = l;
+      for (int r = 0; r < 16; ++r) to[(h * 16 + r) * 64 + lane] = kg == 0 ? o[HB + h][r] : o[h][r];
+    sh.m[wave][lane] = mc;
+    sh.l[wave][lane] = l;
   }
   __syncthreads();
-  if (kg == 1 || !live) return;
-  const float m1 = sh_m[rm][lane], M = fmaxf(m, m1);
-  const float e0 = m == -INFINITY ? 0.f : exp2_hw((m - M) * c);
-  const float e1 = m1 == -INFINITY ? 0.f : exp2_hw((m1 - M) * c);
-  const float z = e0 * l + e1 * sh_l[rm][lane];
-  const bool nan = sh_bad || z != z;
+  const int other = wave ^ 1;   // the same rows, the other keys
+  const float m1 = sh.m[other][lane], M = fmaxf(mc, m1);
+  const float e0 = mc == -INFINITY ? 0.f : exp2_hw(mc - M), e1 = m1 == -INFINITY ? 0.f : exp2_hw(m1 - M);
+  const float z = e0 * l + e1 * sh.l[other][lane];
+  const bool nan = sh.bad || z != z;
   const float inv = nan ? NAN : (z > 0.f ? 1.f / z : 0.f);
-  const size_t at = (size_t)qrow * S + s;
+  const float f0 = e0 * inv, f1 = e1 * inv;
+  float v[HB][16];
+  const float* from = area + other * XCH;
 #pragma unroll
-  for (int db = 0; db < DB; ++db)
+  for (int h = 0; h < HB; ++h)
 #pragma unroll
-    for (int r4 = 0; r4 < 4; ++r4) {
-      f32x4 v;
+    for (int r = 0; r < 16; ++r)
+      v[h][r] = f0 * (kg == 0 ? o[h][r] : o[HB + h][r]) + f1 * from[(h * 16 + r) * 64 + lane];
+  __syncthreads();
+  // Through LDS once more, rows of the wave's half in a row: 32 rows of D / 2 (and 4
+  // words, for the banks), stored a row's 2 D bytes at a time.
+  constexpr int ROW = D / 2 + 4;
+  static_assert(NW * 32 * ROW * 4 <= kStages * STAGE, "rows within the ring");
+  float* const mine = area + wave * (32 * ROW);
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        v[r] = (e0 * o[db][4 * r4 + r] + e1 * sh_o[(db * 16 + 4 * r4 + r) * 64 + lane]) * inv;
-      *reinterpret_cast<f32x4*>(part_o + at * D + 32 * db + 8 * r4 + 4 * (lane >> 5)) = v;
-    }
-  if (lane < 32) part_ml[at] = make_float2(M, nan ? NAN : z);
+  for (int h = 0; h < HB; ++h)
+#pragma unroll
+    for (int r4 = 0; r4 < 4; ++r4)
+      *reinterpret_cast<f32x4*>(mine + (lane & 31) * ROW + 32 * h + 8 * r4 + 4 * (lane >> 5)) =
+          f32x4{v[h][4 * r4], v[h][4 * r4 + 1], v[h][4 * r4 + 2], v[h][4 * r4 + 3]};
+  if (kg == 0 && lane < 32 && live) part_ml[(size_t)qrow * S + s] = make_float2(M, nan ? NAN : z);
+  constexpr int PER = D / 8;   // lanes of a row's half
+#pragma unroll 4
+  for (int i = 0; i < 32; i += 64 / PER) {
+    const int x = i + lane / PER, r = (rb * WM + rm) * 32 + x, d = 4 * (lane % PER);
+    if (r >= rows) continue;
+    const size_t at = ((size_t)(r / G) * H + hk * G + r % G) * S + s;
+    *reinterpret_cast<f32x4*>(part_o + at * D + kg * (D / 2) + d) = *reinterpret_cast<const f32x4*>(mine + x * ROW + d);
+  }
 }
 
 // Splits of a short list of prefix pages in the chunk pass: SP at most.
@@ -227,6 +298,7 @@ fa_shared_chunk_kernel(const uint16_t* __restrict__ q, const char* __restrict__ 
                        int prefix_pages, int max_pages, int num_pages, Plan plan, float c) {
   __shared__ Shared<D> sh;
   const int col = threadIdx.x & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if ((int)blockIdx.x < pre_blocks) {
     const Place at = place_of(blockIdx.x, Hkv * pre_grp);
     const int P = prefix_len[0], pages = pages_of(P, prefix_pages);
@@ -236,7 +308,7 @@ fa_shared_chunk_kernel(const uint16_t* __restrict__ q, const char* __restrict__ 
     const bool live = r < rows;
     const int64_t row = live ? (int64_t)(r / group) * H + hk * group + r % group : 0;
     const int p0 = (int)((int64_t)pages * at.number / n), p1 = (int)((int64_t)pages * (at.number + 1) / n);
-    chunk_body<D, BF16, NT, false>(sh, q, k_pool, v_pool, prefix_table, p0, p1, P,
+    chunk_body<D, BF16, NT, false>(sh, wave, q, k_pool, v_pool, prefix_table, p0, p1, P,
                                    P < 0 || (P > 0 && pages == 0), live, row * D, hk, Hkv, num_pages, c,
                                    nullptr, 0, 0, pre_o, pre_ml, (int64_t)at.number * B * H + row);
     return;
@@ -248,9 +320,51 @@ fa_shared_chunk_kernel(const uint16_t* __restrict__ q, const char* __restrict__ 
   const int hk = at.hg / ngrp, sub = at.hg - hk * ngrp;
   const int h = hk * group + 16 * sub + col;
   const bool live = 16 * sub + col < group;
-  chunk_body<D, BF16, NT, false>(sh, q, k_pool, v_pool, page_table + (size_t)r.b * max_pages, r.p0, r.p1,
+  chunk_body<D, BF16, NT, false>(sh, wave, q, k_pool, v_pool, page_table + (size_t)r.b * max_pages, r.p0, r.p1,
                                  r.ctx, r.bad, live, ((int64_t)r.b * H + h) * D, hk, Hkv, num_pages, c,
                                  nullptr, 0, 0, own_o, own_ml, (int64_t)at.number * H + h);
+}
+
+// Workgroups [0, units): runs of tiles of the prefix. The others: two chunks of the
+// own pages each, of neighbouring head groups (see place_of: here an XCD's chunks and
+// head groups follow one another over its workgroups' halves). The own pages are bound
+// by memory and the tiles by their products, so one launch has both under way.
+template <int D, bool BF16, bool NT>
+__global__ void __launch_bounds__(64 * kTileWaves)
+fa_shared_tile_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_pool,
+                      const char* __restrict__ v_pool, const int32_t* __restrict__ prefix_table,
+                      const int32_t* __restrict__ prefix_len, const int32_t* __restrict__ page_table,
+                      const int32_t* __restrict__ ctx_lens, const int4* __restrict__ table,
+                      float* __restrict__ pre_o, float2* __restrict__ pre_ml, float* __restrict__ own_o,
+                      float2* __restrict__ own_ml, int2* __restrict__ first, int B, int H, int Hkv,
+                      int group, int ngrp, int rows, int units, int row_blocks, int SP,
+                      int prefix_pages, int max_pages, int num_pages, Plan plan, int nxcd, float c) {
+  constexpr int kHalves = kTileWaves / kWaves;
+  __shared__ union Lds {
+    TileShared<D> tile;
+    Shared<D> chunk[kHalves];
+    __device__ Lds() {}
+  } sh;
+  if ((int)blockIdx.x < units) {
+    tile_unit<D, BF16>(sh.tile, blockIdx.x, units, (const f16*)q, (const f16*)k_pool, (const f16*)v_pool,
+                       prefix_table, prefix_len, pre_o, pre_ml, rows, H, Hkv, prefix_pages, num_pages, SP,
+                       row_blocks, nxcd, c);
+    return;
+  }
+  const int w = (int)blockIdx.x - units, col = threadIdx.x & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = wave / kWaves;
+  const int seq = kHalves * (w / kXcds) + half, groups = Hkv * ngrp;
+  const int number = seq / groups * kXcds + w % kXcds, hg = seq % groups;
+  const Run r = run_of(ctx_lens, table, B, max_pages, plan, number);
+  if (r.b >= 0 && hg == 0 && r.split == 0 && threadIdx.x % (64 * kWaves) == 0)
+    first[r.b] = make_int2(number, r.splits);
+  const int hk = hg / ngrp, sub = hg - hk * ngrp;
+  const int h = hk * group + 16 * sub + col;
+  const bool live = r.b >= 0 && 16 * sub + col < group;
+  chunk_body<D, BF16, NT, false>(sh.chunk[half], wave % kWaves, q, k_pool, v_pool,
+                                 page_table + (size_t)max(r.b, 0) * max_pages, r.p0, r.p1, r.ctx, r.bad, live,
+                                 ((int64_t)r.b * H + h) * D, hk, Hkv, num_pages, c, nullptr, 0, 0, own_o,
+                                 own_ml, (int64_t)number * H + h);
 }
 
 // O and L of row blockIdx.x out of the partials of the prefix (SP of them, or, of
@@ -261,13 +375,13 @@ fa_shared_join_kernel(const float* __restrict__ pre_o, const float2* __restrict_
                       const float* __restrict__ own_o, const float2* __restrict__ own_ml,
                       const int2* __restrict__ first, const int32_t* __restrict__ prefix_len,
                       uint16_t* __restrict__ o, float* __restrict__ lse, int H, int rows, int SP,
-                      int few, int prefix_pages, float c) {
+                      int few, int prefix_pages) {
   __shared__ JoinShared<D> sh;
   const int row = blockIdx.x, b = row / H;
   const int2 f = first[b];
   const int n = few ? prefix_splits(prefix_len[0], prefix_pages, SP) : SP;
   const Parts pre = few ? Parts{pre_o, pre_ml, row, rows, n} : Parts{pre_o, pre_ml, (int64_t)row * SP, 1, n};
-  join_row<D, BF16>(sh, pre, Parts{own_o, own_ml, (int64_t)f.x * H + (row - b * H), H, f.y}, c,
+  join_row<D, BF16>(sh, pre, Parts{own_o, own_ml, (int64_t)f.x * H + (row - b * H), H, f.y},
                     o + (int64_t)row * D, lse + row);
 }
 
@@ -278,13 +392,22 @@ constexpr int kMaxSplits = 256;   // of the prefix
 // The cut is made for the 256 CUs of a whole MI355X, whatever the device has: the
 // workspace follows from the sizes alone.
 constexpr int kCus = 256;
+// Units of the prefix pass in the launch of tiles: five eighths of the CUs, so that the
+// own pages are read beside the tiles' products and not after them, and chunks of the
+// own pages that make kTileFill workgroups' halves (32 sequences of 50 to 1500 tokens
+// under 7999, H32 over 8 D128: 33.3 us, with 256 units 38, with chunks for 1024 halves
+// 36.9, in launches of their own 17 + 20.4; 64 of 20 to 1000 under 32768: 69, 83, 74,
+// 48.5 + 24.7). Where the own pages are few, by their table, all CUs (64 of one token
+// under 30000: 61.2 -> 52.6).
+constexpr int kTileUnits = 160, kTileFill = 512;
 constexpr int64_t kPassThrough = 64 << 20;   // bytes of pools read past the caches
 
 // How a call is cut: the prefix pass and its splits, the own pages' chunks, and the
 // workspace in floats.
 struct Cut {
   bool few;
-  int wm, row_blocks, sp;
+  int row_blocks, sp;
+  Plan plan;   // of the own pages' chunks
   int64_t rows, own, pre_ml, own_o, own_ml, first, table, floats;
 };
 
@@ -292,20 +415,20 @@ static Cut cut_of(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t prefix_p
   Cut p;
   p.rows = B * (H / Hkv);
   p.few = p.rows <= kFewRows;
-  p.wm = p.rows <= 64 ? 2 : 4;
   int64_t sp, most;
   if (p.few) {
     p.row_blocks = (int)((p.rows + 15) / 16);
     sp = kFill / (Hkv * p.row_blocks);
     most = prefix_pages / kMinChunk;
   } else {
-    p.row_blocks = (int)((p.rows + 32 * p.wm - 1) / (32 * p.wm));
-    sp = kCus / (Hkv * p.row_blocks);
+    p.row_blocks = (int)((p.rows + kTileRows - 1) / kTileRows);
+    sp = (4 * B * max_pages < prefix_pages ? kCus : kTileUnits) / (Hkv * p.row_blocks);
     most = (prefix_pages * kTokens + kTile - 1) / kTile;
   }
   sp = sp > most ? most : sp;
   p.sp = (int)(sp < 1 ? 1 : (sp > kMaxSplits ? kMaxSplits : sp));
-  p.own = most_chunks(B, max_pages, plan_of(head_groups(H, Hkv)));
+  p.plan = plan_of(head_groups(H, Hkv), p.few ? kFill : kTileFill);
+  p.own = most_chunks(B, max_pages, p.plan);
   p.own_o = B * H * p.sp * D;
   p.pre_ml = p.own_o + p.own * H * D;
   p.own_ml = p.pre_ml + 2 * B * H * p.sp;
@@ -323,7 +446,7 @@ static int launch(const Cut& p, const void* q, const void* k_pool, const void* v
                   float* lse, hipStream_t s) {
   const float c = (float)(1.0 / sqrt((double)D)) * kLog2e;
   const int64_t groups = head_groups(H, Hkv);
-  const Plan plan = plan_of(groups);
+  const Plan plan = p.plan;
   float* own_o = ws + p.own_o;
   float2* pre_ml = (float2*)(ws + p.pre_ml);
   float2* own_ml = (float2*)(ws + p.own_ml);
@@ -332,29 +455,31 @@ static int launch(const Cut& p, const void* q, const void* k_pool, const void* v
   if (table != nullptr)
     hipLaunchKernelGGL(fa_stream_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, ctx_lens, (int)B,
                        (int)max_pages, plan, table);
-  if (!p.few) {
-    const dim3 grid((unsigned)(Hkv * p.sp * p.row_blocks));
-#define FA_PREFIX(WM)                                                                              \
-  hipLaunchKernelGGL((fa_prefix_split_kernel<D, BF16, WM>), grid, dim3(64 * WM * kKeyGroups), 0, s, \
-                     (const f16*)q, (const f16*)k_pool, (const f16*)v_pool, prefix_table,          \
-                     prefix_len, ws, pre_ml, (int)p.rows, (int)H, (int)Hkv, (int)prefix_pages,     \
-                     (int)num_pages, p.sp, p.row_blocks, topo.xcds, c)
-    if (p.wm == 2) FA_PREFIX(2);
-    else FA_PREFIX(4);
-#undef FA_PREFIX
-  }
-  const int64_t pre_blocks = p.few ? chunk_blocks(p.sp, Hkv * p.row_blocks) : 0;
   const bool nt = num_pages * Hkv * kTokens * D * 4 >= kPassThrough;
-  const auto kernel = nt ? fa_shared_chunk_kernel<D, BF16, true> : fa_shared_chunk_kernel<D, BF16, false>;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)(pre_blocks + chunk_blocks(p.own, groups))),
-                     dim3(stream::kThreads), 0, s, (const uint16_t*)q, (const char*)k_pool,
-                     (const char*)v_pool, prefix_table, prefix_len, page_table, ctx_lens, table, ws, pre_ml,
-                     own_o, own_ml, first, (int)B, (int)H, (int)Hkv, (int)(H / Hkv), (int)(groups / Hkv),
-                     (int)p.rows, (int)pre_blocks, p.row_blocks, p.sp, (int)prefix_pages, (int)max_pages,
-                     (int)num_pages, plan, c);
+  if (p.few) {
+    const int64_t pre_blocks = chunk_blocks(p.sp, Hkv * p.row_blocks);
+    const auto kernel = nt ? fa_shared_chunk_kernel<D, BF16, true> : fa_shared_chunk_kernel<D, BF16, false>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(pre_blocks + chunk_blocks(p.own, groups))),
+                       dim3(stream::kThreads), 0, s, (const uint16_t*)q, (const char*)k_pool,
+                       (const char*)v_pool, prefix_table, prefix_len, page_table, ctx_lens, table, ws,
+                       pre_ml, own_o, own_ml, first, (int)B, (int)H, (int)Hkv, (int)(H / Hkv),
+                       (int)(groups / Hkv), (int)p.rows, (int)pre_blocks, p.row_blocks, p.sp,
+                       (int)prefix_pages, (int)max_pages, (int)num_pages, plan, c);
+  } else {
+    const int64_t units = Hkv * p.sp * p.row_blocks;
+    const int64_t halves = kTileWaves / kWaves;
+    const int64_t own = ((p.own + kXcds - 1) / kXcds * groups + halves - 1) / halves * kXcds;
+    const auto kernel = nt ? fa_shared_tile_kernel<D, BF16, true> : fa_shared_tile_kernel<D, BF16, false>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(units + own)), dim3(64 * kTileWaves), 0, s,
+                       (const uint16_t*)q, (const char*)k_pool, (const char*)v_pool, prefix_table,
+                       prefix_len, page_table, ctx_lens, table, ws, pre_ml, own_o, own_ml, first, (int)B,
+                       (int)H, (int)Hkv, (int)(H / Hkv), (int)(groups / Hkv), (int)p.rows, (int)units,
+                       p.row_blocks, p.sp, (int)prefix_pages, (int)max_pages, (int)num_pages, plan,
+                       topo.xcds, c);
+  }
   hipLaunchKernelGGL((fa_shared_join_kernel<D, BF16>), dim3((unsigned)(B * H)), dim3(kJoinThreads), 0, s,
                      ws, pre_ml, own_o, own_ml, first, prefix_len, (uint16_t*)o, lse, (int)H, (int)(B * H),
-                     p.sp, (int)p.few, (int)prefix_pages, c);
+                     p.sp, (int)p.few, (int)prefix_pages);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? FA_OK : -(int)e;
 }

@@ -1,6 +1,6 @@
 // fa_stream.hpp — decode attention over runs of 16-bit pages, for the kernels
 // that run it: one query token per sequence, cut into chunks of pages that a
-// later launch joins by their maxima and sums.
+// later launch joins by their references and sums (see part_ml below).
 //
 // Bound by memory: a page of 16 tokens of one KV head is 32 D bytes each of K and
 // V, read once for up to 16 query rows. A wave loads whole pages straight into
@@ -47,8 +47,8 @@ constexpr int kMinChunk = kWaves * kBatch, kMaxChunk = 32;
 struct Plan {
   unsigned fill, most;   // chunks along the pages that make kFill and kMost workgroups
 };
-inline Plan plan_of(int64_t groups) {
-  return {(unsigned)((kFill + groups - 1) / groups), (unsigned)((kMost + groups - 1) / groups)};
+inline Plan plan_of(int64_t groups, int64_t fill = kFill) {
+  return {(unsigned)((fill + groups - 1) / groups), (unsigned)((kMost + groups - 1) / groups)};
 }
 
 // Pages of a chunk where the batch has `total`.
@@ -282,17 +282,18 @@ struct Shared {
   int bad[kWaves];
 };
 
-// One chunk by the whole workgroup: pages p0 .. p1 - 1 of a list `pt` of a
+// One chunk by kWaves waves, `wave` their number: pages p0 .. p1 - 1 of a list `pt` of a
 // sequence of ctx tokens, for up to 16 query rows. Column col of the products is
 // the query row at element qoff of q (live: there is one), and takes partial
-// number `part`: part_o[part * D ..] normalised, part_ml[part] = (maximum of
-// K Q^T, sum); (-inf, 0) of no pages, a NaN sum where a page or the length is
-// invalid. scores (SCORES): where the scores of column 0 go, K Q^T unscaled, a float
+// number `part`: part_o[part * D ..] normalised, part_ml[part] = (reference, sum of
+// weights to it, in units of log 2): (-inf, 0) of no pages, a NaN sum where a page or
+// the length is invalid. scores (SCORES): where the scores of column 0 go, K Q^T unscaled, a float
 // a slot of the sequence, and score_stride on those of the next of `heads` columns.
-// NT: V is read with the non-temporal hint (K's lines are read in two halves).
+// NT: pages are read with the non-temporal hint. Has one barrier of the workgroup, so
+// waves without a chunk call it too, with no pages and no live row.
 template <int D, bool BF16, bool NT, bool SCORES>
 __device__ __forceinline__ void
-chunk_body(Shared<D>& sh, const uint16_t* __restrict__ q, const char* __restrict__ k_pool,
+chunk_body(Shared<D>& sh, const int wave, const uint16_t* __restrict__ q, const char* __restrict__ k_pool,
            const char* __restrict__ v_pool, const int32_t* __restrict__ pt, int p0, int p1, int ctx,
            bool bad, bool live, int64_t qoff, int hk, int Hkv, int num_pages, float c,
            float* __restrict__ scores, int64_t score_stride, int heads, float* __restrict__ part_o,
@@ -302,8 +303,7 @@ chunk_body(Shared<D>& sh, const uint16_t* __restrict__ q, const char* __restrict
   constexpr int DB = D / 16;               // blocks of O^T
   constexpr int VW = D / 32;               // words of a lane's V piece of a token
   constexpr int kAux = NT ? 2 : 0;
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = threadIdx.x & 63;
   const int col = lane & 15, grp = lane >> 4;
   // This wave's pages, in whole batches but for the last wave's.
   const int per = ((p1 - p0 + kBatch - 1) / kBatch + kWaves - 1) / kWaves * kBatch;
@@ -495,7 +495,10 @@ chunk_body(Shared<D>& sh, const uint16_t* __restrict__ q, const char* __restrict
     for (int j = 0; j < 4; ++j) a[j] *= inv;
     *reinterpret_cast<f32x4*>(part_o + part * D + d) = a;
   }
-  if (wave == 0 && grp == 0) part_ml[part] = make_float2(M, z);
+  // The reference is the scaled maximum, rounded; the sum takes up what that left.
+  const float mc = M * c;
+  if (wave == 0 && grp == 0)
+    part_ml[part] = make_float2(mc, mc == -INFINITY ? z : z * exp2_hw(fmaf(M, c, -mc)));
 }
 
 // Partials of one row: number at + i * stride, i < n.
@@ -516,23 +519,23 @@ struct JoinShared {
   float acc[4 * kJoinThreads / D][D];
 };
 
-// Maximum and sum over a row's parts, for the whole wave: (-inf, 0) of empty
+// Reference and sum over a row's parts, for the whole wave: (-inf, 0) of empty
 // ones, a NaN sum where one is.
-__device__ __forceinline__ float2 join_wave(const Parts& p, float c) {
+__device__ __forceinline__ float2 join_wave(const Parts& p) {
   const int lane = threadIdx.x & 63;
   float M = -INFINITY, z = 0.f;
   for (int i = lane; i < p.n; i += 64) {
     const float2 x = p.ml[p.at + i * p.stride];
     if (x.x > M) {
-      z *= exp2_hw((M - x.x) * c);   // M = -inf: z is 0 or NaN
+      z *= exp2_hw(M - x.x);   // M = -inf: z is 0 or NaN
       M = x.x;
     }
-    z += x.x == -INFINITY ? x.y : x.y * exp2_hw((x.x - M) * c);
+    z += x.x == -INFINITY ? x.y : x.y * exp2_hw(x.x - M);
   }
   float top = M;
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
-  z = M == -INFINITY ? z : z * exp2_hw((M - top) * c);
+  z = M == -INFINITY ? z : z * exp2_hw(M - top);
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) z += __shfl_xor(z, d);
   return make_float2(top, z);
@@ -541,7 +544,7 @@ __device__ __forceinline__ float2 join_wave(const Parts& p, float c) {
 // O and L of one row out of two lists of parts, by one workgroup; sums in a fixed
 // order.
 template <int D, bool BF16>
-__device__ __forceinline__ void join_row(JoinShared<D>& sh, const Parts& a, const Parts& b, float c,
+__device__ __forceinline__ void join_row(JoinShared<D>& sh, const Parts& a, const Parts& b,
                                          uint16_t* __restrict__ o, float* __restrict__ lse) {
   constexpr int PER = D / 4, SIDE = kJoinThreads / PER, WAVES = kJoinThreads / 64;
   const int tid = threadIdx.x, wave = tid >> 6;
@@ -563,7 +566,7 @@ __device__ __forceinline__ void join_row(JoinShared<D>& sh, const Parts& a, cons
     if (i0 > 0) __syncthreads();
     for (int i = tid; i < m; i += kJoinThreads) {
       const float2 x = ml(i0 + i);   // an empty part: (-inf, 0), or NaN
-      const float e = x.x == -INFINITY ? x.y : x.y * exp2_hw((x.x - M) * c);
+      const float e = x.x == -INFINITY ? x.y : x.y * exp2_hw(x.x - M);
       sh.w[i] = e;
       z += e;
     }
@@ -592,7 +595,7 @@ __device__ __forceinline__ void join_row(JoinShared<D>& sh, const Parts& a, cons
     for (int r = 0; r < 4; ++r) v[r] += sh.acc[i][d + r];
   const float inv = z == 0.f ? 0.f : 1.f / z;   // a NaN sum: NaN
   *reinterpret_cast<u32x2*>(o + d) = u32x2{pack2<BF16>(v[0] * inv, v[1] * inv), pack2<BF16>(v[2] * inv, v[3] * inv)};
-  if (tid == 0) *lse = z == 0.f ? -INFINITY : fmaf(M, c, log2_hw(z)) * kLn2;
+  if (tid == 0) *lse = z == 0.f ? -INFINITY : (M + log2_hw(z)) * kLn2;
 }
 
 }  // namespace stream
