@@ -161,14 +161,15 @@ __global__ void __launch_bounds__(kThreads) fa_rope_kernel(const Args a) {
     if constexpr (APPEND) p = (a.pos ? (int64_t)a.pos[b] : (int64_t)a.start[b]) + t;
     else p = a.pos ? a.pos[b * a.pos_stride + t] : t;
     // In turns and 64 bits up to the fraction of a turn: 32 would leave the
-    // angle of position 100000 off by 0.004.
+    // angle of position 100000 off by 0.004. v_sin_f32 and v_cos_f32 take turns;
+    // they are off by 2^-22.9 at most (measured over 2^26 values of [-1/2, 1/2]).
     constexpr double kTurn = 0.15915494309189533577;
     const double pd = (double)p;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const double x = pd * (a.freqs[8 * u + j] * kTurn);
-      float s, c;
-      sincospif(2.f * (float)(x - rint(x)), &s, &c);
+      const float f = (float)(x - rint(x));
+      const float s = __builtin_amdgcn_sinf(f), c = __builtin_amdgcn_cosf(f);
       cs[j] = c * a.scale;
       sn[j] = (a.back ? -s : s) * a.scale;
     }

@@ -2,9 +2,9 @@
 their restatement in 64 bits (oracle/rotary.py).
 
 A value is off by
-  - its factors cos and sin: the angle in half turns is rounded to 32 bits once
-    (pi 2^-25), the functions are within 4 units of 2^-24 and the scale's product
-    rounds once more: 7 units of 2^-24 in all, of |x1| + |x2|;
+  - its factors cos and sin: the angle in turns is rounded to 32 bits once (at most
+    2 pi 2^-26), the functions are within 2.2 units of 2^-24 and the scale's product
+    rounds once more: 5 units of 2^-24 in all, of |x1| + |x2|; 7 are allowed;
   - a product and a fused product: 2 more of the same units;
   - the rounding to its type: half a step, or half of the smallest step.
 """
