@@ -53,11 +53,58 @@ fa_weights_chunk_kernel(const uint16_t* __restrict__ q, const char* __restrict__
   const int h = hk * group + 16 * sub + col;
   const bool live = 16 * sub + col < group;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  chunk_body<D, BF16, NT, true>(sh, wave, q, k_pool, v_pool, page_table + (size_t)r.b * max_pages, r.p0, r.p1,
-                                r.ctx, r.bad, live, ((int64_t)r.b * H + h) * D, hk, Hkv, num_pages, c,
-                                scores + ((int64_t)r.b * H + h - col) * score_row(max_pages),
-                                score_row(max_pages), min(16, group - 16 * sub), part_o, part_ml,
-                                (int64_t)at.number * H + h);
+  const ScoresOut scores_out{scores + ((int64_t)r.b * H + h - col) * score_row(max_pages),
+                             score_row(max_pages), min(16, group - 16 * sub)};
+  const PartOut<D> out{part_o, part_ml, (int64_t)at.number * H + h};
+  chunk_body<D, BF16, NT>(sh, wave, q, k_pool, v_pool, Pages{page_table + (size_t)r.b * max_pages, r.ctx},
+                          r.p0, r.p1, r.bad, live, ((int64_t)r.b * H + h) * D, hk, Hkv, num_pages, c,
+                          scores_out, out, out);
+}
+
+// Short contexts, a workgroup of kOneWaves waves for a sequence and KV head: the scores
+// stay in LDS until the sums are known, and one launch writes everything. Taken for tables
+// of up to kOnePages pages and up to two workgroups a CU. A call by itself, us, in one
+// launch and in chunks: D = 64, 64 workgroups, 4 pages 3.9 and 8.4, 32 pages 6.3 and 8.8;
+// D = 128, 256 workgroups, 4 pages 4.8 and 9.5, 32 pages 10.7 and 15.0; 1024 workgroups
+// of 24 pages 34.1 and 34.3.
+constexpr int kOneWaves = 8;
+constexpr int kOnePages = 32, kOneBlocks = 512;
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(64 * kOneWaves)
+fa_weights_one_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_pool,
+                      const char* __restrict__ v_pool, const int32_t* __restrict__ page_table,
+                      const int32_t* __restrict__ ctx_lens, const float* w_in, float* w_out,
+                      uint16_t* __restrict__ o, float* __restrict__ lse, int H, int Hkv, int max_pages,
+                      int num_pages, float c) {
+  constexpr int STRIDE = kOnePages * kTokens + 4;
+  __shared__ Shared<D, kOneWaves> sh;
+  __shared__ __attribute__((aligned(16))) float scores[16 * STRIDE];
+  __shared__ float2 J[16];   // of a group's heads: reference, 1 / sum
+  const int hk = blockIdx.x, b = blockIdx.y, G = H / Hkv;
+  const int col = threadIdx.x & 15, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int ctx = __builtin_amdgcn_readfirstlane(ctx_lens[b]), pages = pages_of(ctx, max_pages);
+  const bool live = col < G;
+  const int64_t row = (int64_t)b * H + hk * G + col;
+  const RowOut<D, BF16> out{o, lse, row};
+  chunk_body<D, BF16, false>(sh, wave, q, k_pool, v_pool, Pages{page_table + (size_t)b * max_pages, ctx}, 0,
+                             pages, ctx < 0 || (ctx > 0 && pages == 0), live, row * D, hk, Hkv, num_pages,
+                             c, ScoresKept{scores, STRIDE}, out, [&](float mc, float z) {
+                               out(mc, z);
+                               J[col] = make_float2(mc, 1.f / z);
+                             });
+  __syncthreads();
+  const int width = max_pages * kPageSize, n = min(max(ctx, 0), width);
+  const int64_t at = ((int64_t)b * Hkv + hk) * width;
+  for (int j = threadIdx.x; j < (w_in == w_out ? n : width); j += 64 * kOneWaves) {
+    float w = w_in[at + j];
+    if (j < n) {
+      float sum = 0.f;
+      for (int g = 0; g < G; ++g) sum = fmaf(exp2_hw(fmaf(scores[g * STRIDE + j], c, -J[g].x)), J[g].y, sum);
+      w += sum;
+    }
+    w_out[at + j] = w;
+  }
 }
 
 constexpr int kChunk = 4 * kJoinThreads;   // slots of a workgroup that writes weights
@@ -126,6 +173,11 @@ fa_weights_join_kernel(const float* __restrict__ part_o, const float2* __restric
   if (there) *reinterpret_cast<f32x4*>(w_out + at) = w;
 }
 
+// Whether a call is one launch.
+static bool in_one(int64_t B, int64_t H, int64_t Hkv, int64_t max_pages) {
+  return max_pages <= kOnePages && H / Hkv <= 16 && B * Hkv <= kOneBlocks;
+}
+
 // The workspace, in floats: the scores first, then the
 // chunks' partial O, their maxima and sums, the sequences' first chunks and, of
 // more sequences than a wave plans, the table of chunks.
@@ -150,6 +202,14 @@ static int decode_weights(const void* q, const void* k_pool, const void* v_pool,
                           float* ws, void* o, float* lse, float* w_out, void* stream) {
   const float c = (float)(1.0 / sqrt((double)D)) * kLog2e;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (in_one(B, H, Hkv, max_pages)) {
+    hipLaunchKernelGGL((fa_weights_one_kernel<D, BF16>), dim3((unsigned)Hkv, (unsigned)B),
+                       dim3(64 * kOneWaves), 0, s, (const uint16_t*)q, (const char*)k_pool,
+                       (const char*)v_pool, page_table, ctx_lens, w_in, w_out, (uint16_t*)o, lse, (int)H,
+                       (int)Hkv, (int)max_pages, (int)num_pages, c);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? FA_OK : -(int)e;
+  }
   const Workspace w = workspace_of(B, H, Hkv, D, max_pages);
   const int64_t groups = head_groups(H, Hkv), rows = B * H;
   const Plan plan = plan_of(groups);
@@ -525,6 +585,7 @@ extern "C" int64_t fa_decode_weights_workspace_floats(int64_t B, int64_t H, int6
   if (B <= 0 || B > 65535 || H <= 0 || H > 65535 || H_kv <= 0 || H % H_kv != 0 ||
       (D != 64 && D != 128) || max_pages <= 0 || max_pages > kIndexes / 16 || B > kIndexes / max_pages)
     return 0;
+  if (fa::cache::in_one(B, H, H_kv, max_pages)) return 0;
   return fa::cache::workspace_of(B, H, H_kv, D, max_pages).floats;
 }
 

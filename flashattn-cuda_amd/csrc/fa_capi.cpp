@@ -319,7 +319,7 @@ extern "C" int fa_validate_decode_shared(const void* q, const void* k_pool, cons
                                     max_pages, num_pages, /*num_splits=*/1);
   if (st != FA_OK) return st;
   if (H_kv <= 0 || H % H_kv != 0) return FA_ERR_KV_HEADS;
-  if (!prefix_table || !prefix_len || !workspace || !o || !lse) return FA_ERR_NULL_POINTER;
+  if (!prefix_table || !prefix_len || !o || !lse) return FA_ERR_NULL_POINTER;
   if (prefix_pages <= 0) return FA_ERR_MAX_PAGES;
   if (!aligned16(workspace) || !aligned16(o)) return FA_ERR_ALIGNMENT;
   const auto a4 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; };
@@ -327,6 +327,8 @@ extern "C" int fa_validate_decode_shared(const void* q, const void* k_pool, cons
   // Positions within the prefix and rows (b, h) are 32-bit numbers.
   if (prefix_pages > (int64_t(1) << 27) - 8 || num_pages > kMaxGrid) return FA_ERR_TOO_LARGE;
   if (B * H > (int64_t(1) << 24)) return FA_ERR_TOO_LARGE;
+  if (!workspace && fa_decode_shared_workspace_floats(B, H, H_kv, D, prefix_pages, max_pages) > 0)
+    return FA_ERR_NULL_POINTER;
   return FA_OK;
 }
 
@@ -340,7 +342,9 @@ extern "C" int fa_validate_decode_weights(const void* q, const void* k_pool, con
                                     max_pages, num_pages, /*num_splits=*/1);
   if (st != FA_OK) return st;
   if (H_kv <= 0 || H % H_kv != 0) return FA_ERR_KV_HEADS;
-  if (!weights || !weights_out || !workspace || !o || !lse) return FA_ERR_NULL_POINTER;
+  if (!weights || !weights_out || !o || !lse) return FA_ERR_NULL_POINTER;
+  if (!workspace && fa_decode_weights_workspace_floats(B, H, H_kv, D, max_pages) > 0)
+    return FA_ERR_NULL_POINTER;
   if (!aligned16(workspace) || !aligned16(o) || !aligned16(weights) || !aligned16(weights_out))
     return FA_ERR_ALIGNMENT;
   if (reinterpret_cast<uintptr_t>(lse) & 3u) return FA_ERR_ALIGNMENT;

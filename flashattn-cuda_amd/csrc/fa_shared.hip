@@ -308,9 +308,10 @@ fa_shared_chunk_kernel(const uint16_t* __restrict__ q, const char* __restrict__ 
     const bool live = r < rows;
     const int64_t row = live ? (int64_t)(r / group) * H + hk * group + r % group : 0;
     const int p0 = (int)((int64_t)pages * at.number / n), p1 = (int)((int64_t)pages * (at.number + 1) / n);
-    chunk_body<D, BF16, NT, false>(sh, wave, q, k_pool, v_pool, prefix_table, p0, p1, P,
-                                   P < 0 || (P > 0 && pages == 0), live, row * D, hk, Hkv, num_pages, c,
-                                   nullptr, 0, 0, pre_o, pre_ml, (int64_t)at.number * B * H + row);
+    const PartOut<D> out{pre_o, pre_ml, (int64_t)at.number * B * H + row};
+    chunk_body<D, BF16, NT>(sh, wave, q, k_pool, v_pool, Pages{prefix_table, P}, p0, p1,
+                            P < 0 || (P > 0 && pages == 0), live, row * D, hk, Hkv, num_pages, c, NoScores{},
+                            out, out);
     return;
   }
   const Place at = place_of((int)blockIdx.x - pre_blocks, Hkv * ngrp);
@@ -320,9 +321,10 @@ fa_shared_chunk_kernel(const uint16_t* __restrict__ q, const char* __restrict__ 
   const int hk = at.hg / ngrp, sub = at.hg - hk * ngrp;
   const int h = hk * group + 16 * sub + col;
   const bool live = 16 * sub + col < group;
-  chunk_body<D, BF16, NT, false>(sh, wave, q, k_pool, v_pool, page_table + (size_t)r.b * max_pages, r.p0, r.p1,
-                                 r.ctx, r.bad, live, ((int64_t)r.b * H + h) * D, hk, Hkv, num_pages, c,
-                                 nullptr, 0, 0, own_o, own_ml, (int64_t)at.number * H + h);
+  const PartOut<D> out{own_o, own_ml, (int64_t)at.number * H + h};
+  chunk_body<D, BF16, NT>(sh, wave, q, k_pool, v_pool, Pages{page_table + (size_t)r.b * max_pages, r.ctx},
+                          r.p0, r.p1, r.bad, live, ((int64_t)r.b * H + h) * D, hk, Hkv, num_pages, c,
+                          NoScores{}, out, out);
 }
 
 // Workgroups [0, units): runs of tiles of the prefix. The others: two chunks of the
@@ -361,10 +363,37 @@ fa_shared_tile_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k
   const int hk = hg / ngrp, sub = hg - hk * ngrp;
   const int h = hk * group + 16 * sub + col;
   const bool live = r.b >= 0 && 16 * sub + col < group;
-  chunk_body<D, BF16, NT, false>(sh.chunk[half], wave % kWaves, q, k_pool, v_pool,
-                                 page_table + (size_t)max(r.b, 0) * max_pages, r.p0, r.p1, r.ctx, r.bad, live,
-                                 ((int64_t)r.b * H + h) * D, hk, Hkv, num_pages, c, nullptr, 0, 0, own_o,
-                                 own_ml, (int64_t)number * H + h);
+  const PartOut<D> out{own_o, own_ml, (int64_t)number * H + h};
+  chunk_body<D, BF16, NT>(sh.chunk[half], wave % kWaves, q, k_pool, v_pool,
+                          Pages{page_table + (size_t)max(r.b, 0) * max_pages, r.ctx}, r.p0, r.p1, r.bad, live,
+                          ((int64_t)r.b * H + h) * D, hk, Hkv, num_pages, c, NoScores{}, out, out);
+}
+
+// Short calls in one launch, a workgroup of kOneWaves waves for a sequence and 16 heads of
+// a KV head: it walks the prefix's pages and then its own.
+constexpr int kOneWaves = 8;
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(64 * kOneWaves)
+fa_shared_one_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_pool,
+                     const char* __restrict__ v_pool, const int32_t* __restrict__ prefix_table,
+                     const int32_t* __restrict__ prefix_len, const int32_t* __restrict__ page_table,
+                     const int32_t* __restrict__ ctx_lens, uint16_t* __restrict__ o,
+                     float* __restrict__ lse, int H, int Hkv, int group, int ngrp, int prefix_pages,
+                     int max_pages, int num_pages, float c) {
+  __shared__ Shared<D, kOneWaves> sh;
+  const int hk = (int)blockIdx.x / ngrp, sub = (int)blockIdx.x - hk * ngrp, b = blockIdx.y;
+  const int col = threadIdx.x & 15, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int P = __builtin_amdgcn_readfirstlane(prefix_len[0]);
+  const int ctx = __builtin_amdgcn_readfirstlane(ctx_lens[b]);
+  const int np = pages_of(P, prefix_pages), own = pages_of(ctx, max_pages);
+  const bool bad = P < 0 || (P > 0 && np == 0) || ctx < 0 || (ctx > 0 && own == 0);
+  const int64_t row = (int64_t)b * H + hk * group + 16 * sub + col;
+  const RowOut<D, BF16> out{o, lse, row};
+  chunk_body<D, BF16, false>(sh, wave, q, k_pool, v_pool,
+                             JoinedPages{prefix_table, page_table + (size_t)b * max_pages, np, P, ctx}, 0,
+                             np + own, bad, 16 * sub + col < group, row * D, hk, Hkv, num_pages, c,
+                             NoScores{}, out, out);
 }
 
 // O and L of row blockIdx.x out of the partials of the prefix (SP of them, or, of
@@ -385,13 +414,25 @@ fa_shared_join_kernel(const float* __restrict__ pre_o, const float2* __restrict_
                     o + (int64_t)row * D, lse + row);
 }
 
+// The cuts are made for the 256 CUs of a whole MI355X, whatever the device has: the
+// workspace follows from the sizes alone.
+constexpr int kCus = 256;
+
+// A call is one launch, a workgroup for a sequence and 16 heads, where nothing would be
+// gained by cutting it: up to a workgroup a CU and kOneWork dims of the pages of both
+// tables (36 pages of D = 128), or two and half of it. A call by itself, us, in one launch
+// and cut: D = 64, 32 workgroups, 16 pages 4.9 and 8.4, 64 pages 8.7 and 8.4, 96 pages 11.3
+// and 8.5; D = 128, 36 pages of 32 workgroups 8.7 and 8.9, of 256 9.1 and 15.4; 512
+// workgroups of 16 pages 11.7 and 16.6.
+constexpr int kOneWork = 36 * 128;
+static bool in_one(int64_t blocks, int64_t pages, int64_t D) {
+  return blocks <= 2 * kCus && pages * D * (blocks <= kCus ? 1 : 2) <= kOneWork;
+}
+
 // Query rows of a KV head up to which the prefix goes through the chunk pass: one
 // or two workgroups of 16 rows for a chunk.
 constexpr int kFewRows = 32;
 constexpr int kMaxSplits = 256;   // of the prefix
-// The cut is made for the 256 CUs of a whole MI355X, whatever the device has: the
-// workspace follows from the sizes alone.
-constexpr int kCus = 256;
 // Units of the prefix pass in the launch of tiles: five eighths of the CUs, so that the
 // own pages are read beside the tiles' products and not after them, and chunks of the
 // own pages that make kTileFill workgroups' halves (32 sequences of 50 to 1500 tokens
@@ -405,7 +446,7 @@ constexpr int64_t kPassThrough = 64 << 20;   // bytes of pools read past the cac
 // How a call is cut: the prefix pass and its splits, the own pages' chunks, and the
 // workspace in floats.
 struct Cut {
-  bool few;
+  bool one, few;
   int row_blocks, sp;
   Plan plan;   // of the own pages' chunks
   int64_t rows, own, pre_ml, own_o, own_ml, first, table, floats;
@@ -413,6 +454,7 @@ struct Cut {
 
 static Cut cut_of(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t prefix_pages, int64_t max_pages) {
   Cut p;
+  p.one = in_one(B * head_groups(H, Hkv), prefix_pages + max_pages, D);
   p.rows = B * (H / Hkv);
   p.few = p.rows <= kFewRows;
   int64_t sp, most;
@@ -446,6 +488,15 @@ static int launch(const Cut& p, const void* q, const void* k_pool, const void* v
                   float* lse, hipStream_t s) {
   const float c = (float)(1.0 / sqrt((double)D)) * kLog2e;
   const int64_t groups = head_groups(H, Hkv);
+  if (p.one) {
+    hipLaunchKernelGGL((fa_shared_one_kernel<D, BF16>), dim3((unsigned)groups, (unsigned)B),
+                       dim3(64 * kOneWaves), 0, s, (const uint16_t*)q, (const char*)k_pool,
+                       (const char*)v_pool, prefix_table, prefix_len, page_table, ctx_lens, (uint16_t*)o,
+                       lse, (int)H, (int)Hkv, (int)(H / Hkv), (int)(groups / Hkv), (int)prefix_pages,
+                       (int)max_pages, (int)num_pages, c);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? FA_OK : -(int)e;
+  }
   const Plan plan = p.plan;
   float* own_o = ws + p.own_o;
   float2* pre_ml = (float2*)(ws + p.pre_ml);
@@ -495,7 +546,8 @@ extern "C" int64_t fa_decode_shared_workspace_floats(int64_t B, int64_t H, int64
       max_pages <= 0 || B > 65535 || H > 65535 || prefix_pages > (1 << 27) - 8 ||
       max_pages > kIndexes / 16 || B > kIndexes / max_pages)
     return 0;
-  return fa::shared::cut_of(B, H, H_kv, D, prefix_pages, max_pages).floats;
+  const fa::shared::Cut p = fa::shared::cut_of(B, H, H_kv, D, prefix_pages, max_pages);
+  return p.one ? 0 : p.floats;
 }
 
 extern "C" int fa_decode_shared(const void* q, const void* k_pool, const void* v_pool,

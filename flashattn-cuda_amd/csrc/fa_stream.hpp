@@ -1,6 +1,6 @@
 // fa_stream.hpp — decode attention over runs of 16-bit pages, for the kernels
 // that run it: one query token per sequence, cut into chunks of pages that a
-// later launch joins by their references and sums (see part_ml below).
+// later launch joins by their references and sums (see chunk_body), or, of short sequences, whole.
 //
 // Bound by memory: a page of 16 tokens of one KV head is 32 D bytes each of K and
 // V, read once for up to 16 query rows. A wave loads whole pages straight into
@@ -275,29 +275,61 @@ __device__ __forceinline__ void turn_k(u32x4& a, u32x4& b, bool upper) {
 }
 
 // LDS of a workgroup: its waves' parts, heads in different banks.
-template <int D>
+template <int D, int WAVES = kWaves>
 struct Shared {
-  __attribute__((aligned(16))) float o[kWaves][16][D + 4];
-  float m[kWaves][16], l[kWaves][16];
-  int bad[kWaves];
+  __attribute__((aligned(16))) float o[WAVES][16][D + 4];
+  float m[WAVES][16], l[WAVES][16];
+  int bad[WAVES];
 };
 
-// One chunk by kWaves waves, `wave` their number: pages p0 .. p1 - 1 of a list `pt` of a
-// sequence of ctx tokens, for up to 16 query rows. Column col of the products is
-// the query row at element qoff of q (live: there is one), and takes partial
-// number `part`: part_o[part * D ..] normalised, part_ml[part] = (reference, sum of
-// weights to it, in units of log 2): (-inf, 0) of no pages, a NaN sum where a page or
-// the length is invalid. scores (SCORES): where the scores of column 0 go, K Q^T unscaled, a float
-// a slot of the sequence, and score_stride on those of the next of `heads` columns.
-// NT: pages are read with the non-temporal hint. Has one barrier of the workgroup, so
-// waves without a chunk call it too, with no pages and no live row.
-template <int D, bool BF16, bool NT, bool SCORES>
+// Where the tokens are: the page id of place p in a list, and the tokens from its
+// first on (of the last place, fewer than 16).
+struct Pages {
+  const int32_t* pt;
+  int ctx;
+  __device__ int id(int p) const { return pt[p]; }
+  __device__ int tokens(int p) const { return ctx - p * kTokens; }
+};
+// The pages of a prefix, np of them, and then a sequence's own.
+struct JoinedPages {
+  const int32_t *prefix, *own;
+  int np, P, ctx;
+  __device__ int id(int p) const { return p < np ? prefix[p] : own[p - np]; }
+  __device__ int tokens(int p) const { return p < np ? P - p * kTokens : ctx - (p - np) * kTokens; }
+};
+
+// Scores of a chunk that go to memory, K Q^T unscaled, a float a slot of the
+// sequence: column 0's, and `stride` on those of the next of `heads` columns.
+struct NoScores {
+  static constexpr bool kThere = false;
+};
+struct ScoresOut {
+  static constexpr bool kThere = true, kKept = false;
+  float* to;
+  int64_t stride;
+  int heads;
+};
+// Scores that stay in LDS: rows of `stride` floats for the columns, places from 0 on.
+struct ScoresKept {
+  static constexpr bool kThere = true, kKept = true;
+  float* rows;
+  int stride;
+};
+
+// One chunk by WAVES waves, `wave` their number: places p0 .. p1 - 1 of the pages, for
+// up to 16 query rows. Column col of the products is the query row at element qoff of
+// q (live: there is one). At the end row(d, v) is called for its dims d .. d + 3,
+// normalised, by some lane of the column, and stat(reference, sum) by one: of the
+// weights, in units of log 2; (-inf, 0) of no tokens, a NaN sum where a page or the
+// length (bad) is invalid. NT: pages are read with the non-temporal hint. Has one
+// barrier of the workgroup, so waves without a chunk call it too, with no pages and no
+// live row.
+template <int D, bool BF16, bool NT, int WAVES, typename Where, typename Scores, typename Row, typename Stat>
 __device__ __forceinline__ void
-chunk_body(Shared<D>& sh, const int wave, const uint16_t* __restrict__ q, const char* __restrict__ k_pool,
-           const char* __restrict__ v_pool, const int32_t* __restrict__ pt, int p0, int p1, int ctx,
-           bool bad, bool live, int64_t qoff, int hk, int Hkv, int num_pages, float c,
-           float* __restrict__ scores, int64_t score_stride, int heads, float* __restrict__ part_o,
-           float2* __restrict__ part_ml, int64_t part) {
+chunk_body(Shared<D, WAVES>& sh, const int wave, const uint16_t* __restrict__ q,
+           const char* __restrict__ k_pool, const char* __restrict__ v_pool, const Where& pages, int p0,
+           int p1, bool bad, bool live, int64_t qoff, int hk, int Hkv, int num_pages, float c,
+           const Scores& scores, Row&& row, Stat&& stat) {
   constexpr int BYTES = kTokens * D * 2;   // a page of one head
   constexpr int KS = D / 32;               // steps of S = K Q^T, K pieces of a lane
   constexpr int DB = D / 16;               // blocks of O^T
@@ -306,13 +338,13 @@ chunk_body(Shared<D>& sh, const int wave, const uint16_t* __restrict__ q, const 
   const int lane = threadIdx.x & 63;
   const int col = lane & 15, grp = lane >> 4;
   // This wave's pages, in whole batches but for the last wave's.
-  const int per = ((p1 - p0 + kBatch - 1) / kBatch + kWaves - 1) / kWaves * kBatch;
+  const int per = ((p1 - p0 + kBatch - 1) / kBatch + WAVES - 1) / WAVES * kBatch;
   const int w0 = min(p0 + per * wave, p1), w1 = min(w0 + per, p1);
 
   // Ids of 64 pages a load, lane i that of page 64 j + i; first of all, as the
   // pages wait for them.
   int ids = 0;
-  const auto load_ids = [&](int w) { ids = pt[min(w + lane, w1 - 1)]; };
+  const auto load_ids = [&](int w) { ids = pages.id(min(w + lane, w1 - 1)); };
   if (w0 < w1) load_ids(w0);
   u32x4 qf[KS];   // column col, dims 32 kb + 8 grp .. + 7
 #pragma unroll
@@ -331,26 +363,15 @@ chunk_body(Shared<D>& sh, const int wave, const uint16_t* __restrict__ q, const 
   const uint32_t voff = 4 * grp * (2 * D) + col * (4 * VW);   // tokens 4 grp + r, dims D/16 col ..
   u32x4 xk[kBatch][KS];
   uint32_t xv[kBatch][4][VW];
-  // Scores wait in the wave's part of sh.o, D/16 pages of them, and go out in long
-  // rows, a head's 64 D/16 bytes at a time: stored page by page, the next loads
-  // waited for every store before them.
-  const auto store_scores = [&](int from, int to) {   // pages
-    const int per_row = 4 * DB;                        // lanes of a row, 4 slots each
-    const int n = (to - from) * kTokens;
-#pragma unroll
-    for (int h = 0; h < 16; h += 64 / per_row) {
-      const int g = h + lane / per_row, j = 4 * (lane % per_row);
-      if (g < heads && j < n)
-        *reinterpret_cast<f32x4*>(scores + g * score_stride + (int64_t)from * kTokens + j) =
-            *reinterpret_cast<const f32x4*>(&sh.o[wave][g][j]);
-    }
-  };
   for (int w = w0; w < w1; w += kBatch) {
     if (((w - w0) & 63) == 0) {
       if (w != w0) load_ids(w);
       const bool no = ids < 0 || ids >= num_pages;
       bad |= no;
       ids = no ? 0 : ids;   // read in place of a page that is not there; the result is NaN
+      // Used up here: after the branch the compiler would wait for the load on either
+      // path, and with it, every batch, for the scores' stores.
+      asm volatile("" : "+v"(ids));
     }
     // Past the wave's last page the last one again, masked below.
 #pragma unroll
@@ -374,8 +395,13 @@ chunk_body(Shared<D>& sh, const int wave, const uint16_t* __restrict__ q, const 
         }
       }
     }
-    // Tokens of the batch that the wave has; from the lane's first.
-    const int rem = min(ctx, w1 * kTokens) - w * kTokens, lim = rem - 4 * grp;
+    int n[kBatch];   // tokens of the pages
+    bool tail = false;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      n[i] = w + i < w1 ? min(pages.tokens(w + i), kTokens) : 0;
+      tail |= n[i] < kTokens;
+    }
     f32x4 s[kBatch];
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
@@ -385,24 +411,43 @@ chunk_body(Shared<D>& sh, const int wave, const uint16_t* __restrict__ q, const 
 #pragma unroll
       for (int kb = 0; kb < KS; ++kb) s[i] = mma16<BF16>(xk[i][kb], qf[kb], s[i]);
     }
-    if (rem < kBatch * kTokens) {   // wave-uniform
-      asm volatile("");             // a branch: not selects in every batch
+    if (tail) {           // wave-uniform
+      asm volatile("");   // a branch: not selects in every batch
       // Rows past the context may hold NaN, and 0 NaN is NaN: V's become zeros.
 #pragma unroll
       for (int i = 0; i < kBatch; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const bool in = kTokens * i + r < lim;
+          const bool in = 4 * grp + r < n[i];
           s[i][r] = in ? s[i][r] : -INFINITY;
 #pragma unroll
           for (int j = 0; j < VW; ++j) xv[i][r][j] = in ? xv[i][r][j] : 0u;
         }
     }
-    if constexpr (SCORES) {
+    if constexpr (Scores::kThere) {
+      if constexpr (Scores::kKept) {
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i)
-        *reinterpret_cast<f32x4*>(&sh.o[wave][col][((w - w0 + i) % DB) * kTokens + 4 * grp]) = s[i];
-      if ((w - w0) % DB == DB - kBatch || w + kBatch >= w1) store_scores(w0 + (w - w0) / DB * DB, min(w + kBatch, w1));
+        for (int i = 0; i < kBatch; ++i)
+          if (w + i < w1)
+            *reinterpret_cast<f32x4*>(scores.rows + col * scores.stride + (w + i) * kTokens + 4 * grp) = s[i];
+      } else {
+        // They wait in the wave's part of sh.o, D/16 pages of them, and go out in long
+        // rows, a head's 64 D/16 bytes at a time.
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+          *reinterpret_cast<f32x4*>(&sh.o[wave][col][((w - w0 + i) % DB) * kTokens + 4 * grp]) = s[i];
+        if ((w - w0) % DB == DB - kBatch || w + kBatch >= w1) {
+          const int from = w0 + (w - w0) / DB * DB, slots = (min(w + kBatch, w1) - from) * kTokens;
+          constexpr int LANES = 4 * DB;   // of a row, 4 slots each
+#pragma unroll
+          for (int h = 0; h < 16; h += 64 / LANES) {
+            const int g = h + lane / LANES, j = 4 * (lane % LANES);
+            if (g < scores.heads && j < slots)
+              *reinterpret_cast<f32x4*>(scores.to + g * scores.stride + (int64_t)from * kTokens + j) =
+                  *reinterpret_cast<const f32x4*>(&sh.o[wave][g][j]);
+          }
+        }
+      }
     }
     float top = s[0][0];
 #pragma unroll
@@ -468,38 +513,60 @@ chunk_body(Shared<D>& sh, const int wave, const uint16_t* __restrict__ q, const 
   __syncthreads();
   bool any_bad = false;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) any_bad |= sh.bad[w] != 0;
+  for (int w = 0; w < WAVES; ++w) any_bad |= sh.bad[w] != 0;
   // A row's columns are written by its lane column: lanes (col, grp) of all waves.
   if (!live) return;
   float M = sh.m[0][col];
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) M = fmaxf(M, sh.m[w][col]);
-  float e[kWaves], z = 0.f;
+  for (int w = 1; w < WAVES; ++w) M = fmaxf(M, sh.m[w][col]);
+  float e[WAVES], z = 0.f;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
+  for (int w = 0; w < WAVES; ++w) {
     const float wl = sh.l[w][col];
     e[w] = wl == 0.f ? 0.f : exp2_hw((sh.m[w][col] - M) * c);   // without pages: m = -inf, sums 0
     z = fmaf(e[w], wl, z);
   }
   if (any_bad) z = NAN;
   const float inv = z == 0.f ? 0.f : 1.f / z;
-  for (int d = 4 * (4 * wave + grp); d < D; d += 16 * kWaves) {
+  for (int d = 4 * (4 * wave + grp); d < D; d += 16 * WAVES) {
     f32x4 a = f32x4{};
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
       const f32x4 v = *reinterpret_cast<const f32x4*>(&sh.o[w][col][d]);
 #pragma unroll
       for (int j = 0; j < 4; ++j) a[j] = fmaf(e[w], v[j], a[j]);
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) a[j] *= inv;
-    *reinterpret_cast<f32x4*>(part_o + part * D + d) = a;
+    row(d, a);
   }
   // The reference is the scaled maximum, rounded; the sum takes up what that left.
   const float mc = M * c;
-  if (wave == 0 && grp == 0)
-    part_ml[part] = make_float2(mc, mc == -INFINITY ? z : z * exp2_hw(fmaf(M, c, -mc)));
+  if (wave == 0 && grp == 0) stat(mc, mc == -INFINITY ? z : z * exp2_hw(fmaf(M, c, -mc)));
 }
+
+// row and stat of chunk_body: partial number `part`, part_o[part * D ..] and
+// part_ml[part]; or the result itself.
+template <int D>
+struct PartOut {
+  float* o;
+  float2* ml;
+  int64_t part;
+  __device__ void operator()(int d, f32x4 a) const { *reinterpret_cast<f32x4*>(o + part * D + d) = a; }
+  __device__ void operator()(float mc, float z) const { ml[part] = make_float2(mc, z); }
+};
+template <int D, bool BF16>
+struct RowOut {
+  uint16_t* o;
+  float* lse;
+  int64_t row;
+  __device__ void operator()(int d, f32x4 a) const {
+    *reinterpret_cast<u32x2*>(o + row * D + d) = u32x2{pack2<BF16>(a[0], a[1]), pack2<BF16>(a[2], a[3])};
+  }
+  __device__ void operator()(float mc, float z) const {
+    lse[row] = z == 0.f ? -INFINITY : (mc + log2_hw(z)) * kLn2;
+  }
+};
 
 // Partials of one row: number at + i * stride, i < n.
 struct Parts {

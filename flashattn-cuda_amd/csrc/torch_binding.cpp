@@ -842,16 +842,17 @@ std::vector<torch::Tensor> decode_shared(torch::Tensor q, torch::Tensor k_pool, 
               "decode tensors must be on the same device");
   const c10::DeviceGuard guard(q.device());
   const auto f32 = q.options().dtype(torch::kFloat);
-  auto ws = at::empty({fa_decode_shared_workspace_floats(a.B, a.H, a.Hkv, a.D, prefix_table.size(0),
-                                                         a.max_pages)}, f32);
+  const int64_t floats =
+      fa_decode_shared_workspace_floats(a.B, a.H, a.Hkv, a.D, prefix_table.size(0), a.max_pages);
+  const auto ws = floats > 0 ? at::empty({floats}, f32) : torch::Tensor();
   auto o = at::empty({a.B, a.H, a.D}, q.options());
   auto lse = at::empty({a.B, a.H}, f32);
   const int st = fa_decode_shared(
       q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), prefix_table.data_ptr<int32_t>(),
       prefix_len.data_ptr<int32_t>(), page_table.data_ptr<int32_t>(), ctx_lens.data_ptr<int32_t>(), a.B,
       a.H, a.Hkv, a.D, a.page_size, prefix_table.size(0), a.max_pages, a.num_pages,
-      ws.data_ptr<float>(), o.data_ptr(), lse.data_ptr<float>(), q.scalar_type() == torch::kBFloat16,
-      current_stream(q));
+      floats > 0 ? ws.data_ptr<float>() : nullptr, o.data_ptr(), lse.data_ptr<float>(),
+      q.scalar_type() == torch::kBFloat16, current_stream(q));
   check_status(st, "fa_decode_shared");
   return {o, lse};
 }
@@ -874,15 +875,16 @@ std::vector<torch::Tensor> decode_paged_weights(torch::Tensor q, torch::Tensor k
   check_weights(weights, a.B, a.Hkv, a.max_pages, q.device());
   const c10::DeviceGuard guard(q.device());
   const auto f32 = q.options().dtype(torch::kFloat);
-  auto ws = at::empty({fa_decode_weights_workspace_floats(a.B, a.H, a.Hkv, a.D, a.max_pages)}, f32);
+  const int64_t floats = fa_decode_weights_workspace_floats(a.B, a.H, a.Hkv, a.D, a.max_pages);
+  const auto ws = floats > 0 ? at::empty({floats}, f32) : torch::Tensor();
   auto o = at::empty({a.B, a.H, a.D}, q.options());
   auto lse = at::empty({a.B, a.H}, f32);
   auto w = inplace ? weights : at::empty(weights.sizes(), f32);
   const int st = fa_decode_paged_weights(
       q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), page_table.data_ptr<int32_t>(),
       ctx_lens.data_ptr<int32_t>(), weights.data_ptr<float>(), a.B, a.H, a.Hkv, a.D, a.page_size,
-      a.max_pages, a.num_pages, ws.data_ptr<float>(), o.data_ptr(), lse.data_ptr<float>(),
-      w.data_ptr<float>(), q.scalar_type() == torch::kBFloat16, current_stream(q));
+      a.max_pages, a.num_pages, floats > 0 ? ws.data_ptr<float>() : nullptr, o.data_ptr(),
+      lse.data_ptr<float>(), w.data_ptr<float>(), q.scalar_type() == torch::kBFloat16, current_stream(q));
   check_status(st, "fa_decode_paged_weights");
   return {o, lse, w};
 }

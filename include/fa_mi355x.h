@@ -596,7 +596,8 @@ int fa_decode_shared(const void* q, const void* k_pool, const void* v_pool,
                      int64_t max_pages, int64_t num_pages, float* workspace, void* o, float* lse,
                      int bf16, void* stream);
 
-/* Floats of fa_decode_shared's workspace; 0 for invalid sizes. */
+/* Floats of fa_decode_shared's workspace (NULL where 0): 0 for invalid sizes, and for
+ * calls of one launch (few pages and workgroups). */
 int64_t fa_decode_shared_workspace_floats(int64_t B, int64_t H, int64_t H_kv, int64_t D,
                                           int64_t prefix_pages, int64_t max_pages);
 
@@ -629,7 +630,8 @@ int fa_decode_paged_weights(const void* q, const void* k_pool, const void* v_poo
                             int64_t page_size, int64_t max_pages, int64_t num_pages, float* workspace,
                             void* o, float* lse, float* weights_out, int bf16, void* stream);
 
-/* Floats of fa_decode_paged_weights' workspace; 0 for invalid sizes. */
+/* Floats of fa_decode_paged_weights' workspace (NULL where 0): 0 for invalid sizes, and
+ * for calls of one launch (few pages a sequence, up to 16 heads a KV head). */
 int64_t fa_decode_weights_workspace_floats(int64_t B, int64_t H, int64_t H_kv, int64_t D,
                                            int64_t max_pages);
 

@@ -40,14 +40,16 @@ def _check_weights(got, case, dtype, tag=""):
 CASES = [(1, 1, 1, 64, [1]), (2, 8, 2, 64, [0, 5]), (3, 4, 4, 128, [1, 16, 17]), (4, 8, 8, 64, [300, 0, 2, 64]),
          (2, 32, 8, 128, [33, 1700]), (3, 40, 2, 64, [100, 2500, 17]), (1, 128, 1, 128, [800]), (2, 36, 2, 128, [1023, 1025]),
          (20, 4, 2, 64, [13 * i for i in range(20)]), (1, 300, 1, 64, [1100]), (300, 4, 2, 64, [7 * i % 90 for i in range(300)]),
-         (1500, 2, 1, 64, [i % 5 for i in range(1500)]), (1, 8, 1, 128, [9000]), (65, 2, 2, 128, [40] * 64 + [3000])]
+         (1500, 2, 1, 64, [i % 5 for i in range(1500)]), (1, 8, 1, 128, [9000]), (65, 2, 2, 128, [40] * 64 + [3000]),
+         (3, 36, 4, 128, [512, 0, 497]), (2, 16, 1, 64, [255, 256]), (256, 2, 2, 128, [i % 300 for i in range(256)])]
 
 
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("wide", [0, 40])   # short tables are walked in one launch, wide ones in chunks
 @pytest.mark.parametrize("i", range(len(CASES)))
-def test_weights_match_oracle(fa, dev, i, dtype):
+def test_weights_match_oracle(fa, dev, i, wide, dtype):
     B, H, Hkv, D, ctx = CASES[i]
-    case = _paged(dev, i, B, H, Hkv, D, ctx, dtype, extra=i % 3)
+    case = _paged(dev, i, B, H, Hkv, D, ctx, dtype, extra=i % 3 + wide)
     before = case[5].clone()
     got = fa.decode_paged_weights(*case)
     _check_weights(got, case, dtype, f"{CASES[i]}")
@@ -74,11 +76,12 @@ def test_weights_large_scores(fa, dev):
         _check_weights(fa.decode_paged_weights(*case), case, "fp16", f"amp {amp}")
 
 
+@pytest.mark.parametrize("wide", [0, 40])
 @pytest.mark.parametrize("D", [64, 128])
-def test_weights_invalid(fa, dev, D):
+def test_weights_invalid(fa, dev, D, wide):
     """An invalid page or length: O, L and the weights up to the context, cut to the table, are NaN; the rest is kept."""
     ctx = [40, 300, 40, 64, 0]
-    q, kp, vp, table, c, w = _paged(dev, 5, 5, 8, 2, D, ctx, "fp16")
+    q, kp, vp, table, c, w = _paged(dev, 5, 5, 8, 2, D, ctx, "fp16", extra=wide)
     good = fa.decode_paged_weights(q, kp, vp, table, c, w)
     t, n = table.clone(), c.clone()
     t[0, 2], t[1, 9] = -1, kp.shape[0]

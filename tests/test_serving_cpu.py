@@ -83,7 +83,8 @@ def _shared(**kw):
 
 SHARED = [
     (dict(), "FA_OK"), (dict(q=0), "FA_ERR_NULL_POINTER"), (dict(pt=0), "FA_ERR_NULL_POINTER"), (dict(pl=0), "FA_ERR_NULL_POINTER"),
-    (dict(ws=0), "FA_ERR_NULL_POINTER"), (dict(o=0), "FA_ERR_NULL_POINTER"), (dict(l=0), "FA_ERR_NULL_POINTER"), (dict(H=30), "FA_ERR_KV_HEADS"),
+    (dict(ws=0), "FA_ERR_NULL_POINTER"), (dict(ws=0, pp=16, mp=20), "FA_OK"), (dict(ws=0, pp=17, mp=20), "FA_ERR_NULL_POINTER"),
+    (dict(o=0), "FA_ERR_NULL_POINTER"), (dict(l=0), "FA_ERR_NULL_POINTER"), (dict(H=30), "FA_ERR_KV_HEADS"),
     (dict(Hkv=0), "FA_ERR_KV_HEADS"), (dict(D=96), "FA_ERR_HEAD_DIM"), (dict(B=0), "FA_ERR_BATCH_HEADS"), (dict(size=8), "FA_ERR_PAGE_SIZE"),
     (dict(pp=0), "FA_ERR_MAX_PAGES"), (dict(mp=0), "FA_ERR_MAX_PAGES"), (dict(pages=0), "FA_ERR_NUM_PAGES"), (dict(ws=A + 4), "FA_ERR_ALIGNMENT"),
     (dict(pl=A + 2), "FA_ERR_ALIGNMENT"), (dict(o=A + 2), "FA_ERR_ALIGNMENT"), (dict(pp=1 << 27), "FA_ERR_TOO_LARGE"),
@@ -107,7 +108,8 @@ def _weights(**kw):
 
 
 WEIGHTS = [
-    (dict(), "FA_OK"), (dict(w=0), "FA_ERR_NULL_POINTER"), (dict(wo=0), "FA_ERR_NULL_POINTER"), (dict(ws=0), "FA_ERR_NULL_POINTER"),
+    (dict(), "FA_OK"), (dict(w=0), "FA_ERR_NULL_POINTER"), (dict(wo=0), "FA_ERR_NULL_POINTER"), (dict(ws=0, mp=33), "FA_ERR_NULL_POINTER"),
+    (dict(ws=0, mp=32), "FA_OK"), (dict(ws=0, H=136), "FA_ERR_NULL_POINTER"),
     (dict(l=0), "FA_ERR_NULL_POINTER"), (dict(H=30), "FA_ERR_KV_HEADS"),
     (dict(D=32), "FA_ERR_HEAD_DIM"), (dict(w=A + 4), "FA_ERR_ALIGNMENT"), (dict(wo=A + 8), "FA_ERR_ALIGNMENT"), (dict(l=A + 1), "FA_ERR_ALIGNMENT"),
     (dict(mp=1 << 20, B=2000, Hkv=32), "FA_OK"), (dict(mp=1 << 20, B=2000, H=64, Hkv=64), "FA_ERR_TOO_LARGE"), (dict(B=40000, H=1000, Hkv=1), "FA_ERR_TOO_LARGE"),
@@ -157,7 +159,7 @@ def test_status_strings(capi):
                                              (300, 32, 32, 64, 625, 1), (1, 128, 1, 128, 50, 2), (2000, 8, 8, 64, 10, 4000), (65535, 1, 1, 64, 4, 8)])
 def test_workspaces(capi, B, H, Hkv, D, pp, mp):
     """Room for a part of the prefix and a chunk a sequence at least, at most 256 parts and 4096 workgroups' chunks or a
-    chunk for 8 pages beside one a sequence; none for sizes that are refused."""
+    chunk for 8 pages beside one a sequence; none for calls of one launch and for sizes that are refused."""
     lib = capi.load()
     part = B * H * (D + 2)
     chunk = H * (D + 2)
@@ -165,10 +167,17 @@ def test_workspaces(capi, B, H, Hkv, D, pp, mp):
     most = min(B * mp // 8, -(-4096 // groups)) + B
     small = 3 + 2 * B + (4 * (1 + most) if B > 256 else 0)
     n = lib.fa_decode_shared_workspace_floats(B, H, Hkv, D, pp, mp)
-    assert part + B * chunk <= n <= min(256, -(-pp // 4)) * part + most * chunk + small
+    blocks = B * Hkv * -(-H // Hkv // 16)
+    if blocks <= 256 and (pp + mp) * D <= 4608 or blocks <= 512 and (pp + mp) * D <= 2304:
+        assert n == 0
+    else:
+        assert part + B * chunk <= n <= min(256, -(-pp // 4)) * part + most * chunk + small
     w = lib.fa_decode_weights_workspace_floats(B, H, Hkv, D, mp)
     scores = B * H * (((16 * mp + 63) // 64) | 1) * 64   # rows of an odd number of 256 bytes
-    assert scores + B * chunk <= w <= scores + most * chunk + small
+    if mp <= 32 and H // Hkv <= 16 and B * Hkv <= 512:
+        assert w == 0
+    else:
+        assert scores + B * chunk <= w <= scores + most * chunk + small
     for bad in ((0, H, Hkv, D, pp, mp), (B, H, H + 1, D, pp, mp), (B, H, Hkv, 96, pp, mp), (B, H, Hkv, D, 0, mp), (B, H, Hkv, D, pp, -1),
                 (B, 70000, 1, D, pp, mp), (B, H, Hkv, D, 1 << 27, mp), (65535, H, Hkv, D, pp, 1 << 16)):
         assert lib.fa_decode_shared_workspace_floats(*bad) == 0

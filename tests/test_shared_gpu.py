@@ -76,14 +76,17 @@ CASES = [
     (1, 128, 1, 128, 800, [20]), (3, 40, 2, 64, 2100, [100, 0, 17]), (2, 2, 1, 128, 0, [70, 0]), (2, 4, 2, 64, 15, [0, 0]),
     (40, 32, 8, 128, 70, [2] * 40), (300, 2, 1, 64, 90, [5 * i % 70 for i in range(300)]), (600, 4, 4, 128, 40, [i % 3 for i in range(600)]),
     (16, 2, 1, 64, 1500, [3] * 16), (17, 2, 1, 64, 1500, [40] * 16 + [2000]),
+    (3, 40, 2, 128, 160, [333, 0, 17]), (64, 4, 4, 64, 515, [i % 33 for i in range(64)]), (128, 4, 4, 64, 300, [i % 120 for i in range(128)]),
+    (1, 8, 8, 128, 0, [575]), (2, 3, 1, 64, 1151, [1, 0]), (512, 1, 1, 128, 17, [i % 160 for i in range(512)]),
 ]
 
 
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("wide", [0, 80])   # short tables are walked in one launch, wide ones in chunks
 @pytest.mark.parametrize("i", range(len(CASES)))
-def test_matches_oracle(fa, dev, i, dtype):
+def test_matches_oracle(fa, dev, i, wide, dtype):
     B, H, Hkv, D, P, ctx = CASES[i]
-    case = _case(dev, i, B, H, Hkv, D, P, ctx, dtype, extra=i % 3)
+    case = _case(dev, i, B, H, Hkv, D, P, ctx, dtype, extra=i % 3 + wide)
     got = fa.decode_shared(*case)
     _check(got, _want(case, dtype), dtype, f"case {CASES[i][:5]}")
     again = fa.decode_shared(*case)
@@ -91,10 +94,11 @@ def test_matches_oracle(fa, dev, i, dtype):
 
 
 @pytest.mark.parametrize("P", [1, 15, 16, 17, 31, 32, 33, 48, 63, 64, 65, 127, 128, 129, 191, 193, 255, 256, 257])
+@pytest.mark.parametrize("wide", [0, 80])
 @pytest.mark.parametrize("D,dtype", [(64, "bf16"), (128, "fp16")])
-def test_prefix_lengths(fa, dev, P, D, dtype):
+def test_prefix_lengths(fa, dev, P, D, dtype, wide):
     """The prefix ends at every place of a page, a tile and the ring of tiles."""
-    case = _case(dev, P, 3, 8, 2, D, P, [5, 0, 31], dtype)
+    case = _case(dev, P, 3, 8, 2, D, P, [5, 0, 31], dtype, extra=wide)
     _check(fa.decode_shared(*case), _want(case, dtype), dtype)
 
 
@@ -119,12 +123,13 @@ def test_many_tiles_a_workgroup(fa, dev):
     _check([x[some] for x in got], _want((q[some], kp, vp, prefix, plen, table[some], ctx[some]), "fp16"), "fp16")
 
 
+@pytest.mark.parametrize("wide", [0, 80])
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
 @pytest.mark.parametrize("D", [64, 128])
-def test_invalid_pages_and_lengths(fa, dev, D, dtype):
+def test_invalid_pages_and_lengths(fa, dev, D, dtype, wide):
     """An invalid own page or length makes its sequence NaN, an invalid prefix all of them."""
     ctx = [40, 40, 40, 0, 16]
-    case = list(_case(dev, 4, 5, 8, 2, D, 200, ctx, dtype, spare=1))
+    case = list(_case(dev, 4, 5, 8, 2, D, 200, ctx, dtype, spare=1, extra=wide))
     good = fa.decode_shared(*case)
     pages = case[1].shape[0]
     t = case[5].clone()
