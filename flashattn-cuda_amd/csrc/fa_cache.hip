@@ -6,9 +6,13 @@
 // token j of sequence b gets from the G query heads that share a KV head
 //   W'[j] = W[j] + sum_g exp(s_gj - L_g),
 // s the scaled scores and L their logsumexp over the whole context. L is known
-// only after the last key, so the split pass keeps its scores (4 G bytes a token
+// only after the last key, so the chunk pass keeps its scores (4 G bytes a token
 // and KV head beside the 4 D of its K and V rows) and the launch that joins the
-// splits turns them into weights; a second pass over K would read 2 D bytes.
+// chunks turns them into weights; a second pass over K would read 2 D bytes.
+//
+// Bound: memory. 16 sequences of 2000 to 32768 tokens, H32 over 8, D = 128 (1.14 GB
+// of K and V, 36 MB of scores written and read again): 227 us, the chunks 215 and the join
+// 13; without their scores the chunks take 186 us, and the decode without weights 180.
 #include <hip/hip_runtime.h>
 
 #include <math.h>
@@ -24,17 +28,6 @@ namespace cache {
 
 using namespace stream;
 using pages::kPageSize;
-
-// Pools from this size on do not stay in the caches between two steps; their pages
-// are read with the non-temporal hint.
-constexpr int64_t kPassThrough = 64 << 20;
-
-// Floats from a head's scores to the next head's: an odd number of 256 bytes, not
-// the table's power of two, at which all heads' scores of a page would meet in the
-// same memory channels.
-__host__ __device__ inline int64_t score_row(int64_t max_pages) {
-  return ((max_pages * kPageSize + 63) / 64 | 1) * 64;
-}
 
 template <int D, bool BF16, bool NT>
 __global__ void __launch_bounds__(stream::kThreads)
@@ -53,8 +46,8 @@ fa_weights_chunk_kernel(const uint16_t* __restrict__ q, const char* __restrict__
   const int h = hk * group + 16 * sub + col;
   const bool live = 16 * sub + col < group;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const ScoresOut scores_out{scores + ((int64_t)r.b * H + h - col) * score_row(max_pages),
-                             score_row(max_pages), min(16, group - 16 * sub)};
+  const int64_t width = (int64_t)max_pages * kPageSize;
+  const ScoresOut scores_out{scores + ((int64_t)r.b * H + h - col) * width, width, min(16, group - 16 * sub)};
   const PartOut<D> out{part_o, part_ml, (int64_t)at.number * H + h};
   chunk_body<D, BF16, NT>(sh, wave, q, k_pool, v_pool, Pages{page_table + (size_t)r.b * max_pages, r.ctx},
                           r.p0, r.p1, r.bad, live, ((int64_t)r.b * H + h) * D, hk, Hkv, num_pages, c,
@@ -155,11 +148,10 @@ fa_weights_join_kernel(const float* __restrict__ part_o, const float2* __restric
       }
       __syncthreads();
       if (there && j < ctx) {
-        const int64_t next = score_row(max_pages);
-        const float* sc = scores + ((int64_t)b * H + hk * G + g0) * next + j;
+        const float* sc = scores + ((int64_t)b * H + hk * G + g0) * width + j;
 #pragma unroll 4
         for (int g = 0; g < gs; ++g) {
-          const f32x4 x = *reinterpret_cast<const f32x4*>(sc + g * next);
+          const f32x4 x = *reinterpret_cast<const f32x4*>(sc + g * width);
           const float2 Jg = J[g];
 #pragma unroll
           for (int i = 0; i < 4; ++i) sum[i] = fmaf(exp2_hw(fmaf(x[i], c, -Jg.x)), Jg.y, sum[i]);
@@ -187,7 +179,7 @@ struct Workspace {
 static Workspace workspace_of(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t max_pages) {
   Workspace w;
   w.most = most_chunks(B, max_pages, plan_of(head_groups(H, Hkv)));
-  w.part_o = B * H * score_row(max_pages);
+  w.part_o = B * H * max_pages * kPageSize;
   w.part_ml = w.part_o + w.most * H * D;
   w.table = w.part_ml + (2 * w.most * H + 3) / 4 * 4;
   w.first = w.table + (B > kWavePlan ? 4 * (1 + w.most) : 0);
@@ -220,7 +212,7 @@ static int decode_weights(const void* q, const void* k_pool, const void* v_pool,
   if (table != nullptr)
     hipLaunchKernelGGL(fa_stream_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, ctx_lens, (int)B,
                        (int)max_pages, plan, table);
-  const bool nt = num_pages * Hkv * kPageSize * D * 4 >= kPassThrough;
+  const bool nt = pass_through(num_pages, Hkv, D);
   const auto kernel = nt ? fa_weights_chunk_kernel<D, BF16, true> : fa_weights_chunk_kernel<D, BF16, false>;
   hipLaunchKernelGGL(kernel, dim3((unsigned)chunk_blocks(w.most, groups)), dim3(stream::kThreads), 0, s,
                      (const uint16_t*)q, (const char*)k_pool, (const char*)v_pool, page_table, ctx_lens,
@@ -525,11 +517,10 @@ fa_evict_list_kernel(const float* __restrict__ weights, const Selection* __restr
   }
 }
 
-constexpr int kMoveRows = 4;   // rows a thread has in flight
-
-// The stayers' rows into the new pages: 16-byte pieces, each row read and written
-// once, the reads past the caches. Bound: memory, by the gather of 2 D byte rows.
-// Slots, page ids and rows each are asked for together.
+// The stayers' rows into the new pages, a 16-byte piece of K and of V a thread, each row
+// read and written once. Bound: memory, by the gather of 2 D byte rows (8 sequences of 8
+// heads, 4096 of up to 32000 tokens, D = 128: 268 MB in 55 us, 4.9 TB/s, as a plain copy
+// of that size). Four rows a thread and non-temporal loads gained nothing.
 template <int D>
 __global__ void __launch_bounds__(kMoveThreads)
 fa_evict_move_kernel(u32x4* k_pool, u32x4* v_pool, const int32_t* __restrict__ page_table,
@@ -539,40 +530,21 @@ fa_evict_move_kernel(u32x4* k_pool, u32x4* v_pool, const int32_t* __restrict__ p
   constexpr int CH = D / 8;                // pieces of a row
   constexpr int SIDE = kMoveThreads / CH;  // rows side by side
   const int hk = blockIdx.y, b = blockIdx.z;
-  const int c = (int)threadIdx.x % CH;
-  const int32_t* kp = kept + ((size_t)b * Hkv + hk) * keep;
-  int j[kMoveRows], old[kMoveRows], from[kMoveRows], to[kMoveRows];
-  u32x4 x[kMoveRows], y[kMoveRows];
-  bool miss = false;
-#pragma unroll
-  for (int i = 0; i < kMoveRows; ++i) {
-    j[i] = ((int)blockIdx.x * kMoveRows + i) * SIDE + (int)threadIdx.x / CH;
-    old[i] = kp[min(j[i], keep - 1)];
-    to[i] = new_table[(size_t)b * new_max_pages + min(j[i], keep - 1) / kPageSize];
+  const int c = (int)threadIdx.x % CH, j = (int)blockIdx.x * SIDE + (int)threadIdx.x / CH;
+  if (j >= keep) return;
+  const int old = kept[((size_t)b * Hkv + hk) * keep + j];
+  const int to = new_table[(size_t)b * new_max_pages + j / kPageSize];
+  if (old < 0) return;
+  const int from = page_table[(size_t)b * max_pages + old / kPageSize];
+  if (from < 0 || from >= num_pages || to < 0 || to >= num_pages) {
+    bad[b] = 1;   // the same value from every writer
+    return;
   }
-#pragma unroll
-  for (int i = 0; i < kMoveRows; ++i) {
-    if (j[i] >= keep) old[i] = -1;
-    from[i] = page_table[(size_t)b * max_pages + max(old[i], 0) / kPageSize];
-  }
-#pragma unroll
-  for (int i = 0; i < kMoveRows; ++i) {
-    const bool ok = from[i] >= 0 && from[i] < num_pages && to[i] >= 0 && to[i] < num_pages;
-    miss |= old[i] >= 0 && !ok;
-    if (!ok) old[i] = -1;
-    // Rows that do not move read the pool's first one.
-    const int64_t src = old[i] < 0 ? c : (((int64_t)from[i] * Hkv + hk) * kPageSize + old[i] % kPageSize) * CH + c;
-    x[i] = __builtin_nontemporal_load(k_pool + src);
-    y[i] = __builtin_nontemporal_load(v_pool + src);
-  }
-#pragma unroll
-  for (int i = 0; i < kMoveRows; ++i) {
-    if (old[i] < 0) continue;
-    const int64_t dst = (((int64_t)to[i] * Hkv + hk) * kPageSize + j[i] % kPageSize) * CH + c;
-    k_pool[dst] = x[i];
-    v_pool[dst] = y[i];
-  }
-  if (miss) bad[b] = 1;   // the same value from every writer
+  const int64_t src = (((int64_t)from * Hkv + hk) * kPageSize + old % kPageSize) * CH + c;
+  const int64_t dst = (((int64_t)to * Hkv + hk) * kPageSize + j % kPageSize) * CH + c;
+  const u32x4 x = k_pool[src], y = v_pool[src];
+  k_pool[dst] = x;
+  v_pool[dst] = y;
 }
 
 }  // namespace cache
@@ -640,7 +612,7 @@ extern "C" int fa_kv_evict(void* k_pool, void* v_pool, const int32_t* page_table
                        dim3(kMoveThreads), 0, s, weights, sel, kept, new_weights, (int)H_kv,
                        (int)max_pages, (int)new_max_pages, (int)keep, (int)recent);
   }
-  const int64_t rows = kMoveRows * (kMoveThreads / (D / 8));
+  const int64_t rows = kMoveThreads / (D / 8);
   const dim3 grid((unsigned)((keep + rows - 1) / rows), (unsigned)H_kv, (unsigned)B);
   const auto move = D == 128 ? fa_evict_move_kernel<128> : fa_evict_move_kernel<64>;
   hipLaunchKernelGGL(move, grid, dim3(kMoveThreads), 0, s, (fa::u32x4*)k_pool, (fa::u32x4*)v_pool,

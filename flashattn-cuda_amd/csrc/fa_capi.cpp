@@ -324,9 +324,10 @@ extern "C" int fa_validate_decode_shared(const void* q, const void* k_pool, cons
   if (!aligned16(workspace) || !aligned16(o)) return FA_ERR_ALIGNMENT;
   const auto a4 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; };
   if (!a4(prefix_table) || !a4(prefix_len) || !a4(lse)) return FA_ERR_ALIGNMENT;
-  // Positions within the prefix and rows (b, h) are 32-bit numbers.
+  // Positions within the prefix are 32-bit numbers; the chunks and the join have a
+  // workgroup of 256 threads for a row (b, h) and some more, fewer than 2^32 threads.
   if (prefix_pages > (int64_t(1) << 27) - 8 || num_pages > kMaxGrid) return FA_ERR_TOO_LARGE;
-  if (B * H > (int64_t(1) << 24)) return FA_ERR_TOO_LARGE;
+  if (B * H >= int64_t(1) << 23) return FA_ERR_TOO_LARGE;
   if (!workspace && fa_decode_shared_workspace_floats(B, H, H_kv, D, prefix_pages, max_pages) > 0)
     return FA_ERR_NULL_POINTER;
   return FA_OK;
@@ -348,10 +349,10 @@ extern "C" int fa_validate_decode_weights(const void* q, const void* k_pool, con
   if (!aligned16(workspace) || !aligned16(o) || !aligned16(weights) || !aligned16(weights_out))
     return FA_ERR_ALIGNMENT;
   if (reinterpret_cast<uintptr_t>(lse) & 3u) return FA_ERR_ALIGNMENT;
-  // The join has a workgroup for 1024 slots of a (b, KV head), and one for a row.
-  const int64_t chunks = (max_pages * 16 + 1023) / 1024;
-  if (num_pages > kMaxGrid || B * H > (int64_t(1) << 24) || B * H_kv > ((int64_t(1) << 30) - 1) / chunks)
-    return FA_ERR_TOO_LARGE;
+  // The join has a workgroup of 256 threads for 1024 slots of a (b, KV head), and one
+  // for a row: fewer than 2^32 threads.
+  const int64_t chunks = (max_pages * 16 + 1023) / 1024, most = int64_t(1) << 23;
+  if (num_pages > kMaxGrid || B * H >= most || B * H_kv > (most - 1) / chunks) return FA_ERR_TOO_LARGE;
   return FA_OK;
 }
 
@@ -376,9 +377,9 @@ extern "C" int fa_validate_kv_evict(const void* k_pool, const void* v_pool, cons
   for (const void* p : words)
     if (reinterpret_cast<uintptr_t>(p) & 3u) return FA_ERR_ALIGNMENT;
   if (B > 65535 || H_kv > 65535 || num_pages > kMaxGrid) return FA_ERR_TOO_LARGE;
-  // Slots are 32-bit numbers, and a thread's steps of 1024 past the last one too.
-  constexpr int64_t kMaxSlotPages = (int64_t(1) << 27) - 128;
-  if (max_pages > kMaxSlotPages || new_max_pages > kMaxSlotPages) return FA_ERR_TOO_LARGE;
+  // Slots are 32-bit numbers, and a thread's steps of 1024 past the last one too; the
+  // copy has up to 16 threads for a new slot, fewer than 2^32.
+  if (max_pages > (int64_t(1) << 27) - 128 || new_max_pages > (int64_t(1) << 24) - 128) return FA_ERR_TOO_LARGE;
   if (keep < 1 || keep > new_max_pages * 16 || recent < 0 || recent > keep) return FA_ERR_BUDGET;
   return FA_OK;
 }

@@ -12,6 +12,13 @@
 // walks over heads of q, k (and v) with them, so the trigonometry is shared by
 // the heads and needs no table in memory. Rows are addressed by strides: the
 // [B, N, H, D] a projection leaves is read as it is and written head-major.
+//
+// Kernel times, us: 4 x 4096 tokens, 16 + 16 heads of D = 128, bf16: 51, 5.2 TB/s, as a
+// plain copy of that size. Gradients of 2 x 2000 tokens, 32 + 8 heads of D = 128, fp32 to
+// bf16: 25, 4.9 TB/s. The append of two prompts of up to 1777 tokens, 32 heads over 8,
+// D = 128: 17.4. One token of 8 sequences: 4.5; 1024 tokens, 8 + 8 heads of D = 64: 3.8,
+// with the library's sine and cosine 4.3. Loads and stores with the non-temporal hint:
+// 25 -> 36, 17.4 -> 20.5.
 #include <hip/hip_runtime.h>
 
 #include <stdint.h>
@@ -248,7 +255,10 @@ __global__ void __launch_bounds__(kThreads) fa_rope_kernel(const Args a) {
   }
 }
 
-// Tokens of a workgroup, the heads a thread walks over and the grid.
+// Tokens of a workgroup, the heads a thread walks over and the grid: about 2048
+// workgroups, where the angles are shared by as many heads as leave the chip full. The
+// three calls above, us, for 512, 1024, 2048, 4096 and 8192: 69.0 58.4 51.3 50.7 49.5;
+// 26.3 26.8 24.6 25.3 25.0; 19.9 17.2 17.4 18.7 18.7.
 static dim3 plan(Args& a, int64_t B, bool append) {
   const int units = a.D / 16;
   int tt = 0;

@@ -25,7 +25,7 @@ using namespace stream;
 
 constexpr int kTile = 64;     // keys of a tile: 4 pages
 constexpr int kStages = 4;    // tiles in LDS, three of them in flight
-constexpr float kSlack = 8.f;   // of weights' exponents; see there
+constexpr float kSlack = 8.f;   // of weights' exponents; see its use
 constexpr int kKeyGroups = 2; // waves side by side over the keys of a tile
 constexpr int kRowGroups = 4, kTileRows = 32 * kRowGroups;   // and over the query rows of a unit
 constexpr int kTileWaves = kKeyGroups * kRowGroups;
@@ -48,6 +48,11 @@ struct TileShared {
 // those of the forward: S^T = K Q^T with Q in registers, O^T += V^T P^T with P^T
 // straight from the accumulators (fa_tile.hpp), P rounded to the operands' type beside
 // an unrounded sum, as the forward rounds it.
+//
+// Bound by LDS: a tile of 64 keys for 128 rows at D = 128 takes about 1.1 us of a CU, in
+// which each of the eight waves reads half of K and V (16 KiB) out of LDS for its 32 rows;
+// the copies, exponentials or the second product left out change that by little. Beside
+// the tiles a unit costs about 8 us, and storing 16.8 MB of partials 7 us at the end.
 template <int D, bool BF16>
 __device__ __forceinline__ void
 tile_unit(TileShared<D>& sh, const int unit, const int units, const f16* __restrict__ q,
@@ -162,7 +167,8 @@ tile_unit(TileShared<D>& sh, const int unit, const int units, const f16* __restr
     for (int r = 1; r < 16; ++r) mx = fmaxf(mx, sc[r]);
     mx = max_xor32(mx) * c;
     // The reference follows the maximum only where that is kSlack above it: of 32 rows
-    // one has a new maximum in most steps. Weights reach 2^kSlack.
+    // one has a new maximum in most steps (64 sequences under 32768: a call 83 us without,
+    // 75 with). Weights reach 2^kSlack, far from the types' ends.
     if (__any(mx > mc + kSlack)) {
       const float m_new = fmaxf(mc, mx);
       const float alpha = m_new == mc ? 1.f : exp2_hw(mc - m_new);
@@ -429,19 +435,18 @@ static bool in_one(int64_t blocks, int64_t pages, int64_t D) {
   return blocks <= 2 * kCus && pages * D * (blocks <= kCus ? 1 : 2) <= kOneWork;
 }
 
-// Query rows of a KV head up to which the prefix goes through the chunk pass: one
-// or two workgroups of 16 rows for a chunk.
+// Query rows of a KV head up to which the prefix goes through the chunk pass, one or two
+// workgroups of 16 rows for a chunk and kCus in all. A call, us, through chunks and tiles,
+// H32 over 8, D = 128, 50 to 200 tokens under 8000 and 32000: 16 rows 15.1 28.4 and 20.5
+// 36.7, 32 rows 15.7 35.6 and 21.2 37.8, 64 rows 21.1 59.1 and 19.5 39.8. The chunks of 32
+// rows under 32000, for 256, 512 and 1024 workgroups: 35.6 38.9 42.5.
 constexpr int kFewRows = 32;
-constexpr int kMaxSplits = 256;   // of the prefix
 // Units of the prefix pass in the launch of tiles: five eighths of the CUs, so that the
-// own pages are read beside the tiles' products and not after them, and chunks of the
-// own pages that make kTileFill workgroups' halves (32 sequences of 50 to 1500 tokens
-// under 7999, H32 over 8 D128: 33.3 us, with 256 units 38, with chunks for 1024 halves
-// 36.9, in launches of their own 17 + 20.4; 64 of 20 to 1000 under 32768: 69, 83, 74,
-// 48.5 + 24.7). Where the own pages are few, by their table, all CUs (64 of one token
-// under 30000: 61.2 -> 52.6).
-constexpr int kTileUnits = 160, kTileFill = 512;
-constexpr int64_t kPassThrough = 64 << 20;   // bytes of pools read past the caches
+// own pages are read beside the tiles' products and not after them (32 sequences of 50 to
+// 1500 tokens under 7999, H32 over 8 D128: 33.3 us, with 256 units 38, in launches of
+// their own 17 + 20.4; 64 of 20 to 1000 under 32768: 69, 83, 48.5 + 24.7). Where the own
+// pages are few, by their table, all CUs (64 of one token under 30000: 61.2 -> 52.6).
+constexpr int kTileUnits = 160;
 
 // How a call is cut: the prefix pass and its splits, the own pages' chunks, and the
 // workspace in floats.
@@ -460,7 +465,7 @@ static Cut cut_of(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t prefix_p
   int64_t sp, most;
   if (p.few) {
     p.row_blocks = (int)((p.rows + 15) / 16);
-    sp = kFill / (Hkv * p.row_blocks);
+    sp = kCus / (Hkv * p.row_blocks);
     most = prefix_pages / kMinChunk;
   } else {
     p.row_blocks = (int)((p.rows + kTileRows - 1) / kTileRows);
@@ -468,8 +473,8 @@ static Cut cut_of(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t prefix_p
     most = (prefix_pages * kTokens + kTile - 1) / kTile;
   }
   sp = sp > most ? most : sp;
-  p.sp = (int)(sp < 1 ? 1 : (sp > kMaxSplits ? kMaxSplits : sp));
-  p.plan = plan_of(head_groups(H, Hkv), p.few ? kFill : kTileFill);
+  p.sp = (int)(sp < 1 ? 1 : sp);
+  p.plan = plan_of(head_groups(H, Hkv));
   p.own = most_chunks(B, max_pages, p.plan);
   p.own_o = B * H * p.sp * D;
   p.pre_ml = p.own_o + p.own * H * D;
@@ -506,7 +511,7 @@ static int launch(const Cut& p, const void* q, const void* k_pool, const void* v
   if (table != nullptr)
     hipLaunchKernelGGL(fa_stream_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, ctx_lens, (int)B,
                        (int)max_pages, plan, table);
-  const bool nt = num_pages * Hkv * kTokens * D * 4 >= kPassThrough;
+  const bool nt = pass_through(num_pages, Hkv, D);
   if (p.few) {
     const int64_t pre_blocks = chunk_blocks(p.sp, Hkv * p.row_blocks);
     const auto kernel = nt ? fa_shared_chunk_kernel<D, BF16, true> : fa_shared_chunk_kernel<D, BF16, false>;

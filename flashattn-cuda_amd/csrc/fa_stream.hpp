@@ -40,15 +40,25 @@ constexpr int kXcds = 8;
 // lengths, from lengths that only the device knows. The grid has the most
 // chunks that any lengths can give, and the rest end at once. C is what makes
 // kFill workgroups, between kMinChunk and kMaxChunk pages; beyond that, what
-// makes kMost.
-constexpr int kFill = 1024, kMost = 4096;
+// makes kMost. Weights of 8 sequences of 200 to 4000 tokens, H32 over 8, D = 128, for kFill
+// 256, 512 and 1024: 24.6, 26.1 and 26.8 us a call; 32 of 50 to 1500 under a prefix of
+// 7999: 40.4, 39.0 and 38.7. kMaxChunk 128: 16 of 2000 to 32768 tokens 227 -> 232 us, the
+// last chunks run alone; 16: 64 of 20 to 1000 under 32768 75 -> 80.
+constexpr int kFill = 512, kMost = 4096;
 constexpr int kMinChunk = kWaves * kBatch, kMaxChunk = 32;
+
+// Pools from 64 MiB on do not stay in the caches between two steps; their pages are
+// read with the non-temporal hint (the 1.14 GB of the above: 251 -> 227 us; 91 MB
+// that are read again at once: 25.8 -> 26.7).
+inline bool pass_through(int64_t num_pages, int64_t Hkv, int64_t D) {
+  return num_pages * Hkv * kTokens * D * 4 >= (int64_t)64 << 20;
+}
 
 struct Plan {
   unsigned fill, most;   // chunks along the pages that make kFill and kMost workgroups
 };
-inline Plan plan_of(int64_t groups, int64_t fill = kFill) {
-  return {(unsigned)((fill + groups - 1) / groups), (unsigned)((kMost + groups - 1) / groups)};
+inline Plan plan_of(int64_t groups) {
+  return {(unsigned)((kFill + groups - 1) / groups), (unsigned)((kMost + groups - 1) / groups)};
 }
 
 // Pages of a chunk where the batch has `total`.

@@ -531,7 +531,8 @@ int fa_decode_paged_mx(const void* q, const void* k_pool, const void* v_pool,
  * positions[b * pos_stride + n] (pos_stride 0: one row for all; NULL: n). back !=
  * 0 rotates by -a: the transpose, which takes gradients of the outputs to
  * gradients of the inputs. in_type, out_type: FA_F16, FA_BF16 or FA_F32, alike or
- * in_type FA_F32. Arithmetic in fp32, one rounding to out_type.
+ * in_type FA_F32. Arithmetic in fp32, one rounding to out_type. Outputs must not
+ * overlap inputs.
  */
 int fa_rope(const void* q, const int64_t q_strides[3], const void* k, const int64_t k_strides[3],
             const double* freqs, const int32_t* positions, int64_t pos_stride, void* q_out,
@@ -585,7 +586,9 @@ int fa_validate_kv_append_rope(const void* q, const int64_t q_strides[3], const 
  * (b, h). A page id outside [0, num_pages), a negative length or one beyond its
  * table makes o and lse of the sequence NaN, of every sequence where it is the
  * prefix's. q, pools, o fp16 (bf16 != 0: bfloat16); weights of the prefix are
- * rounded to that type for their product with V, as in the forward. workspace:
+ * rounded to that type for their product with V, as in the forward. How the pages
+ * are shared out follows from the lengths of the whole batch, so a sequence's last
+ * bits may depend on the others' lengths; the same call gives the same bits. workspace:
  * fa_decode_shared_workspace_floats(...) floats, 16-byte aligned, need not be
  * cleared; calls that may overlap need one each.
  */

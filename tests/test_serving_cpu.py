@@ -89,6 +89,7 @@ SHARED = [
     (dict(pp=0), "FA_ERR_MAX_PAGES"), (dict(mp=0), "FA_ERR_MAX_PAGES"), (dict(pages=0), "FA_ERR_NUM_PAGES"), (dict(ws=A + 4), "FA_ERR_ALIGNMENT"),
     (dict(pl=A + 2), "FA_ERR_ALIGNMENT"), (dict(o=A + 2), "FA_ERR_ALIGNMENT"), (dict(pp=1 << 27), "FA_ERR_TOO_LARGE"),
     (dict(B=40000, H=1000, Hkv=1), "FA_ERR_TOO_LARGE"), (dict(B=70000), "FA_ERR_TOO_LARGE"),
+    (dict(B=65535, H=128), "FA_OK"), (dict(B=65535, H=136), "FA_ERR_TOO_LARGE"),
 ]
 
 
@@ -112,7 +113,8 @@ WEIGHTS = [
     (dict(ws=0, mp=32), "FA_OK"), (dict(ws=0, H=136), "FA_ERR_NULL_POINTER"),
     (dict(l=0), "FA_ERR_NULL_POINTER"), (dict(H=30), "FA_ERR_KV_HEADS"),
     (dict(D=32), "FA_ERR_HEAD_DIM"), (dict(w=A + 4), "FA_ERR_ALIGNMENT"), (dict(wo=A + 8), "FA_ERR_ALIGNMENT"), (dict(l=A + 1), "FA_ERR_ALIGNMENT"),
-    (dict(mp=1 << 20, B=2000, Hkv=32), "FA_OK"), (dict(mp=1 << 20, B=2000, H=64, Hkv=64), "FA_ERR_TOO_LARGE"), (dict(B=40000, H=1000, Hkv=1), "FA_ERR_TOO_LARGE"),
+    (dict(mp=1 << 17, B=2000, Hkv=2), "FA_OK"), (dict(mp=1 << 17, B=2100, Hkv=2), "FA_ERR_TOO_LARGE"), (dict(B=40000, H=1000, Hkv=1), "FA_ERR_TOO_LARGE"),
+    (dict(B=65535, H=128), "FA_OK"), (dict(B=65535, H=136), "FA_ERR_TOO_LARGE"),
 ]
 
 
@@ -136,7 +138,8 @@ EVICT = [
     (dict(D=96), "FA_ERR_HEAD_DIM"), (dict(B=0), "FA_ERR_BATCH_HEADS"), (dict(size=4), "FA_ERR_PAGE_SIZE"), (dict(mp=0), "FA_ERR_MAX_PAGES"),
     (dict(nmp=0), "FA_ERR_MAX_PAGES"), (dict(pages=-1), "FA_ERR_NUM_PAGES"), (dict(kp=A + 8), "FA_ERR_ALIGNMENT"), (dict(kept=A + 2), "FA_ERR_ALIGNMENT"),
     (dict(keep=0), "FA_ERR_BUDGET"), (dict(keep=113), "FA_ERR_BUDGET"), (dict(keep=112), "FA_OK"), (dict(recent=-1), "FA_ERR_BUDGET"),
-    (dict(recent=101), "FA_ERR_BUDGET"), (dict(recent=100), "FA_OK"), (dict(mp=1 << 27), "FA_ERR_TOO_LARGE"), (dict(Hkv=70000), "FA_ERR_TOO_LARGE"),
+    (dict(recent=101), "FA_ERR_BUDGET"), (dict(recent=100), "FA_OK"), (dict(mp=1 << 27), "FA_ERR_TOO_LARGE"), (dict(nmp=1 << 24), "FA_ERR_TOO_LARGE"),
+    (dict(nmp=(1 << 24) - 128, keep=(1 << 28) - 2048), "FA_OK"), (dict(Hkv=70000), "FA_ERR_TOO_LARGE"),
 ]
 
 
@@ -173,7 +176,7 @@ def test_workspaces(capi, B, H, Hkv, D, pp, mp):
     else:
         assert part + B * chunk <= n <= min(256, -(-pp // 4)) * part + most * chunk + small
     w = lib.fa_decode_weights_workspace_floats(B, H, Hkv, D, mp)
-    scores = B * H * (((16 * mp + 63) // 64) | 1) * 64   # rows of an odd number of 256 bytes
+    scores = B * H * 16 * mp
     if mp <= 32 and H // Hkv <= 16 and B * Hkv <= 512:
         assert w == 0
     else:
