@@ -519,8 +519,8 @@ fa_evict_list_kernel(const float* __restrict__ weights, const Selection* __restr
 
 // The stayers' rows into the new pages, a 16-byte piece of K and of V a thread, each row
 // read and written once. Bound: memory, by the gather of 2 D byte rows (8 sequences of 8
-// heads, 4096 of up to 32000 tokens, D = 128: 268 MB in 55 us, 4.9 TB/s, as a plain copy
-// of that size). Four rows a thread and non-temporal loads gained nothing.
+// heads, 4096 of up to 32000 tokens, D = 128: 268 MB in 57 us, 4.7 TB/s, near a plain copy
+// of that size). Four rows a thread and non-temporal loads gained 2 us of it at most.
 template <int D>
 __global__ void __launch_bounds__(kMoveThreads)
 fa_evict_move_kernel(u32x4* k_pool, u32x4* v_pool, const int32_t* __restrict__ page_table,
