@@ -49,10 +49,14 @@ struct TileShared {
 // straight from the accumulators (fa_tile.hpp), P rounded to the operands' type beside
 // an unrounded sum, as the forward rounds it.
 //
-// Bound by LDS: a tile of 64 keys for 128 rows at D = 128 takes about 1.1 us of a CU, in
-// which each of the eight waves reads half of K and V (16 KiB) out of LDS for its 32 rows;
-// the copies, exponentials or the second product left out change that by little. Beside
-// the tiles a unit costs about 8 us, and storing 16.8 MB of partials 7 us at the end.
+// Bound, with 128 rows a KV head, by memory: 256 units at D = 128 take 1.55 us a tile,
+// 5.4 TB/s. With more, the row blocks of a tile find it in their L2 and a tile takes 1.15
+// to 1.2 us of a CU, 0.93 PFLOP/s over the chip, bound by LDS: each of the eight waves
+// reads 16 KiB a tile for its 32 rows, 1 KiB a matrix instruction. The copies,
+// exponentials or the second product left out change that by little, and no more do key
+// groups that take turns at products and exponentials, or V in blocks of 32 columns. Waves
+// of 64 rows would read half, but need more than the 256 registers of two waves a SIMD.
+// Beside the tiles a unit costs about 8 us, and 16.8 MB of partials 7 us at the end.
 template <int D, bool BF16>
 __device__ __forceinline__ void
 tile_unit(TileShared<D>& sh, const int unit, const int units, const f16* __restrict__ q,
