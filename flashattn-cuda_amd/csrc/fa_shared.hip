@@ -23,6 +23,10 @@ namespace shared {
 
 using namespace stream;
 
+// The cuts are made for the 256 CUs of a whole MI355X, whatever the device has: the
+// workspace follows from the sizes alone.
+constexpr int kCus = 256;
+
 constexpr int kTile = 64;     // keys of a tile: 4 pages
 constexpr int kStages = 4;    // tiles in LDS, three of them in flight
 constexpr float kSlack = 8.f;   // of weights' exponents; see its use
@@ -40,7 +44,7 @@ struct TileShared {
   int bad;
 };
 
-// Prefix pass, unit g of `units`: (KV head, run of tiles, kTileRows query rows) by
+// Prefix pass, unit g of all: (KV head, one of S runs of tiles, kTileRows query rows) by
 // kRowGroups x 2 waves, wave (rm, kg) with rows 32 rm .. + 31 and the tile's keys 32
 // kg .. + 31; rm the slow one, so that of a few rows every SIMD has some. Tiles are
 // copied global -> LDS (buffer_load ... lds), the rows past the prefix as zeros (the
@@ -59,11 +63,10 @@ struct TileShared {
 // Beside the tiles a unit costs about 8 us, and 16.8 MB of partials 7 us at the end.
 template <int D, bool BF16>
 __device__ __forceinline__ void
-tile_unit(TileShared<D>& sh, const int unit, const int units, const f16* __restrict__ q,
-          const f16* __restrict__ kpool, const f16* __restrict__ vpool,
-          const int32_t* __restrict__ prefix_table, const int32_t* __restrict__ prefix_len,
-          float* __restrict__ part_o, float2* __restrict__ part_ml, int rows, int H, int Hkv,
-          int max_pages, int num_pages, int S, int row_blocks, int nxcd, float c) {
+tile_unit(TileShared<D>& sh, const int unit, const f16* __restrict__ q, const f16* __restrict__ kpool,
+          const f16* __restrict__ vpool, const int32_t* __restrict__ prefix_table, int P, bool bad,
+          float* __restrict__ part_o, float2* __restrict__ part_ml, int rows, int H, int Hkv, int num_pages,
+          int S, int most, int row_blocks, int nxcd, float c) {
   constexpr int WM = kRowGroups, NW = kTileWaves;
   constexpr int PAGE = TileShared<D>::kPage, STAGE = TileShared<D>::kStage;
   constexpr int CPR = D / 8;
@@ -74,7 +77,7 @@ tile_unit(TileShared<D>& sh, const int unit, const int units, const f16* __restr
   static_assert(NW * DB * 8 * 64 * 4 <= kStages * STAGE, "merge area within the ring");
 
   // Row blocks that read the same tiles are neighbours on one XCD.
-  const int g = xcd_remap(unit, units, nxcd);
+  const int g = xcd_remap(unit, Hkv * S * row_blocks, nxcd);
   const int rb = g % row_blocks, s = (g / row_blocks) % S, hk = g / row_blocks / S;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -83,9 +86,6 @@ tile_unit(TileShared<D>& sh, const int unit, const int units, const f16* __restr
 
   if (tid == 0) sh.bad = 0;
   __syncthreads();
-  int P = prefix_len[0];
-  bool bad = P < 0 || P > max_pages * kTokens;
-  if (bad) P = 0;
   const int pages = (P + kTokens - 1) / kTokens;
   const int tiles = (pages + PAGES - 1) / PAGES;
   const int t0 = (int)((int64_t)tiles * s / S), t1 = (int)((int64_t)tiles * (s + 1) / S);
@@ -276,13 +276,13 @@ tile_unit(TileShared<D>& sh, const int unit, const int units, const f16* __restr
     for (int r4 = 0; r4 < 4; ++r4)
       *reinterpret_cast<f32x4*>(mine + (lane & 31) * ROW + 32 * h + 8 * r4 + 4 * (lane >> 5)) =
           f32x4{v[h][4 * r4], v[h][4 * r4 + 1], v[h][4 * r4 + 2], v[h][4 * r4 + 3]};
-  if (kg == 0 && lane < 32 && live) part_ml[(size_t)qrow * S + s] = make_float2(M, nan ? NAN : z);
+  if (kg == 0 && lane < 32 && live) part_ml[(size_t)qrow * most + s] = make_float2(M, nan ? NAN : z);
   constexpr int PER = D / 8;   // lanes of a row's half
 #pragma unroll 4
   for (int i = 0; i < 32; i += 64 / PER) {
     const int x = i + lane / PER, r = (rb * WM + rm) * 32 + x, d = 4 * (lane % PER);
     if (r >= rows) continue;
-    const size_t at = ((size_t)(r / G) * H + hk * G + r % G) * S + s;
+    const size_t at = ((size_t)(r / G) * H + hk * G + r % G) * most + s;
     *reinterpret_cast<f32x4*>(part_o + at * D + kg * (D / 2) + d) = *reinterpret_cast<const f32x4*>(mine + x * ROW + d);
   }
 }
@@ -337,7 +337,28 @@ fa_shared_chunk_kernel(const uint16_t* __restrict__ q, const char* __restrict__ 
                           NoScores{}, out, out);
 }
 
-// Workgroups [0, units): runs of tiles of the prefix. The others: two chunks of the
+// Splits of the prefix in the launch of tiles, from the lengths that only the device
+// knows: as many units as make the prefix's share of the CUs that of its work, in us of a
+// CU, so that the own pages are read beside the tiles and neither is left over; of
+// kUnitTiles tiles at least. `per` units a split, `pages` own pages. Against 160 units for
+// any lengths, us a call, H32 over 8, D = 128: 32 sequences of 50 to 1500 tokens under 7999
+// 38.6 -> 34.0, 128 of 20 to 500 under 32768 122 -> 117, 64 of 500 to 2000 107 -> 105, of
+// 20 to 1000 76 and 76, 36 of 30 to 120 under 2500 19.4 -> 21.4; 18 such sets in the mean
+// 1 % less. In launches of their own the first took 17 + 20.4 and the fourth 48.5 + 24.7.
+// kUnitTime 0.5, 3, 8 and 13: the mean 39.9, 39.1, 40.0, 39.8 (a unit's own time is 8);
+// kUnitTiles 4, 6, 8 and 10: 39.2, 39.1, 39.2, 40.1.
+template <int D>
+__device__ __forceinline__ int tile_splits(int tiles, int per, int pages, int Hkv, int most) {
+  constexpr float kTileTime = 1.15f * D / 128, kUnitTime = 3.f, kPageTime = 0.4f * D / 128;
+  constexpr int kUnitTiles = 6;
+  const float t = kTileTime * tiles * per, own = kPageTime * pages * Hkv;
+  const float x = t + own - kCus * kUnitTime;   // kUnitTime u^2 + x u - kCus t = 0
+  const float u = (__builtin_sqrtf(x * x + 4 * kUnitTime * kCus * t) - x) / (2 * kUnitTime);
+  return max(min(min((int)(u / per + 0.5f), tiles / kUnitTiles), most), 1);
+}
+
+// Workgroups [0, units): runs of tiles of the prefix, at most SP a KV head and row block;
+// those past the planned ones end at once. The others: two chunks of the
 // own pages each, of neighbouring head groups (see place_of: here an XCD's chunks and
 // head groups follow one another over its workgroups' halves). The own pages are bound
 // by memory and the tiles by their products, so one launch has both under way.
@@ -350,7 +371,8 @@ fa_shared_tile_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k
                       float* __restrict__ pre_o, float2* __restrict__ pre_ml, float* __restrict__ own_o,
                       float2* __restrict__ own_ml, int2* __restrict__ first, int B, int H, int Hkv,
                       int group, int ngrp, int rows, int units, int row_blocks, int SP,
-                      int prefix_pages, int max_pages, int num_pages, Plan plan, int nxcd, float c) {
+                      int* __restrict__ splits, int prefix_pages, int max_pages, int num_pages, Plan plan,
+                      int nxcd, float c) {
   constexpr int kHalves = kTileWaves / kWaves;
   __shared__ union Lds {
     TileShared<D> tile;
@@ -358,9 +380,16 @@ fa_shared_tile_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k
     __device__ Lds() {}
   } sh;
   if ((int)blockIdx.x < units) {
-    tile_unit<D, BF16>(sh.tile, blockIdx.x, units, (const f16*)q, (const f16*)k_pool, (const f16*)v_pool,
-                       prefix_table, prefix_len, pre_o, pre_ml, rows, H, Hkv, prefix_pages, num_pages, SP,
-                       row_blocks, nxcd, c);
+    int P = prefix_len[0];
+    const bool bad = P < 0 || P > prefix_pages * kTokens;
+    if (bad) P = 0;
+    const int S = tile_splits<D>((P + kTile - 1) / kTile, Hkv * row_blocks,
+                                 total_pages(ctx_lens, table, B, max_pages), Hkv, SP);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *splits = S;
+    if ((int)blockIdx.x >= Hkv * S * row_blocks) return;
+    tile_unit<D, BF16>(sh.tile, blockIdx.x, (const f16*)q, (const f16*)k_pool, (const f16*)v_pool,
+                       prefix_table, P, bad, pre_o, pre_ml, rows, H, Hkv, num_pages, S, SP, row_blocks, nxcd,
+                       c);
     return;
   }
   const int w = (int)blockIdx.x - units, col = threadIdx.x & 15;
@@ -406,27 +435,23 @@ fa_shared_one_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_
                              NoScores{}, out, out);
 }
 
-// O and L of row blockIdx.x out of the partials of the prefix (SP of them, or, of
-// few rows, as many as the prefix's length gives) and of the own pages.
+// O and L of row blockIdx.x out of the partials of the prefix (of few rows, as many as
+// the prefix's length gives, else *splits) and of the own pages.
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kJoinThreads)
 fa_shared_join_kernel(const float* __restrict__ pre_o, const float2* __restrict__ pre_ml,
                       const float* __restrict__ own_o, const float2* __restrict__ own_ml,
-                      const int2* __restrict__ first, const int32_t* __restrict__ prefix_len,
-                      uint16_t* __restrict__ o, float* __restrict__ lse, int H, int rows, int SP,
-                      int few, int prefix_pages) {
+                      const int2* __restrict__ first, const int* __restrict__ splits,
+                      const int32_t* __restrict__ prefix_len, uint16_t* __restrict__ o,
+                      float* __restrict__ lse, int H, int rows, int SP, int few, int prefix_pages) {
   __shared__ JoinShared<D> sh;
   const int row = blockIdx.x, b = row / H;
   const int2 f = first[b];
-  const int n = few ? prefix_splits(prefix_len[0], prefix_pages, SP) : SP;
+  const int n = few ? prefix_splits(prefix_len[0], prefix_pages, SP) : *splits;
   const Parts pre = few ? Parts{pre_o, pre_ml, row, rows, n} : Parts{pre_o, pre_ml, (int64_t)row * SP, 1, n};
   join_row<D, BF16>(sh, pre, Parts{own_o, own_ml, (int64_t)f.x * H + (row - b * H), H, f.y},
                     o + (int64_t)row * D, lse + row);
 }
-
-// The cuts are made for the 256 CUs of a whole MI355X, whatever the device has: the
-// workspace follows from the sizes alone.
-constexpr int kCus = 256;
 
 // A call is one launch, a workgroup for a sequence and 16 heads, where nothing would be
 // gained by cutting it: up to a workgroup a CU and kOneWork dims of the pages of both
@@ -445,12 +470,6 @@ static bool in_one(int64_t blocks, int64_t pages, int64_t D) {
 // 36.7, 32 rows 15.7 35.6 and 21.2 37.8, 64 rows 21.1 59.1 and 19.5 39.8. The chunks of 32
 // rows under 32000, for 256, 512 and 1024 workgroups: 35.6 38.9 42.5.
 constexpr int kFewRows = 32;
-// Units of the prefix pass in the launch of tiles: five eighths of the CUs, so that the
-// own pages are read beside the tiles' products and not after them (32 sequences of 50 to
-// 1500 tokens under 7999, H32 over 8 D128: 33.3 us, with 256 units 38, in launches of
-// their own 17 + 20.4; 64 of 20 to 1000 under 32768: 69, 83, 48.5 + 24.7). Where the own
-// pages are few, by their table, all CUs (64 of one token under 30000: 61.2 -> 52.6).
-constexpr int kTileUnits = 160;
 
 // How a call is cut: the prefix pass and its splits, the own pages' chunks, and the
 // workspace in floats.
@@ -466,16 +485,10 @@ static Cut cut_of(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t prefix_p
   p.one = in_one(B * head_groups(H, Hkv), prefix_pages + max_pages, D);
   p.rows = B * (H / Hkv);
   p.few = p.rows <= kFewRows;
-  int64_t sp, most;
-  if (p.few) {
-    p.row_blocks = (int)((p.rows + 15) / 16);
-    sp = kCus / (Hkv * p.row_blocks);
-    most = prefix_pages / kMinChunk;
-  } else {
-    p.row_blocks = (int)((p.rows + kTileRows - 1) / kTileRows);
-    sp = (4 * B * max_pages < prefix_pages ? kCus : kTileUnits) / (Hkv * p.row_blocks);
-    most = (prefix_pages * kTokens + kTile - 1) / kTile;
-  }
+  const int64_t block = p.few ? 16 : kTileRows, part = p.few ? kMinChunk : kTile / kTokens;
+  p.row_blocks = (int)((p.rows + block - 1) / block);
+  int64_t sp = kCus / (Hkv * p.row_blocks);
+  const int64_t most = (prefix_pages + part - 1) / part;
   sp = sp > most ? most : sp;
   p.sp = (int)(sp < 1 ? 1 : sp);
   p.plan = plan_of(head_groups(H, Hkv));
@@ -485,7 +498,7 @@ static Cut cut_of(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t prefix_p
   p.own_ml = p.pre_ml + 2 * B * H * p.sp;
   p.table = p.own_ml + (2 * p.own * H + 3) / 4 * 4;
   p.first = p.table + (B > kWavePlan ? 4 * (1 + p.own) : 0);
-  p.floats = p.first + 2 * B;
+  p.floats = p.first + 2 * B + 1;
   return p;
 }
 
@@ -511,6 +524,7 @@ static int launch(const Cut& p, const void* q, const void* k_pool, const void* v
   float2* pre_ml = (float2*)(ws + p.pre_ml);
   float2* own_ml = (float2*)(ws + p.own_ml);
   int2* first = (int2*)(ws + p.first);
+  int* splits = (int*)(ws + p.first + 2 * B);
   int4* table = B > kWavePlan ? (int4*)(ws + p.table) : nullptr;
   if (table != nullptr)
     hipLaunchKernelGGL(fa_stream_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, ctx_lens, (int)B,
@@ -534,11 +548,11 @@ static int launch(const Cut& p, const void* q, const void* k_pool, const void* v
                        (const uint16_t*)q, (const char*)k_pool, (const char*)v_pool, prefix_table,
                        prefix_len, page_table, ctx_lens, table, ws, pre_ml, own_o, own_ml, first, (int)B,
                        (int)H, (int)Hkv, (int)(H / Hkv), (int)(groups / Hkv), (int)p.rows, (int)units,
-                       p.row_blocks, p.sp, (int)prefix_pages, (int)max_pages, (int)num_pages, plan,
-                       topo.xcds, c);
+                       p.row_blocks, p.sp, splits, (int)prefix_pages, (int)max_pages, (int)num_pages,
+                       plan, topo.xcds, c);
   }
   hipLaunchKernelGGL((fa_shared_join_kernel<D, BF16>), dim3((unsigned)(B * H)), dim3(kJoinThreads), 0, s,
-                     ws, pre_ml, own_o, own_ml, first, prefix_len, (uint16_t*)o, lse, (int)H, (int)(B * H),
+                     ws, pre_ml, own_o, own_ml, first, splits, prefix_len, (uint16_t*)o, lse, (int)H, (int)(B * H),
                      p.sp, (int)p.few, (int)prefix_pages);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? FA_OK : -(int)e;

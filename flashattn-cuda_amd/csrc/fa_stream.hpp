@@ -138,8 +138,21 @@ __device__ __forceinline__ Chunk chunk_of(const int32_t* __restrict__ ctx_lens, 
   return r;
 }
 
-// The chunks of a batch of any size: table[0] has their number, table[1 + x] chunk
-// x as (sequence, its length, split, splits). One workgroup, a run of sequences a
+// Pages of the batch, by a whole wave.
+__device__ __forceinline__ int total_pages(const int32_t* __restrict__ ctx_lens, const int4* __restrict__ table,
+                                           int B, int max_pages) {
+  if (table != nullptr) return table[0].y;
+  int pages = 0;
+#pragma unroll
+  for (int k = 0; k < kWavePlan / 64; ++k) {
+    const int i = 64 * k + (int)(threadIdx.x & 63);
+    pages += i < B ? pages_of(ctx_lens[i], max_pages) : 0;
+  }
+  return __builtin_amdgcn_readlane(scan_sum(pages), 63);
+}
+
+// The chunks of a batch of any size: table[0] has their number and the pages of the
+// batch, table[1 + x] chunk x as (sequence, its length, split, splits). One workgroup, a run of sequences a
 // thread; a sequence's entries are written by the whole wave.
 constexpr int kPlanThreads = 1024;
 static __global__ void __launch_bounds__(kPlanThreads)
@@ -168,7 +181,7 @@ fa_stream_plan_kernel(const int32_t* __restrict__ ctx_lens, int B, int max_pages
     if (w < wave) e += sh[1][w];
     chunks += sh[1][w];
   }
-  if (tid == 0) table[0] = int4{chunks, 0, 0, 0};
+  if (tid == 0) table[0] = int4{chunks, total, 0, 0};
   for (int k = 0; k < per; ++k) {
     const int i = i0 + k;
     const int ctx = i < i1 ? ctx_lens[i] : 0;
