@@ -99,9 +99,10 @@ def test_weights_invalid(fa, dev, D, wide):
     assert torch.equal(O[0], good[0][0]) and torch.equal(W[0], good[2][0])
 
 
-def test_weights_graph(fa, dev):
+@pytest.mark.parametrize("wide", [0, 40])
+def test_weights_graph(fa, dev, wide):
     """The weights added up in place by a captured step, replayed, against eager steps."""
-    q, kp, vp, table, c, w = _paged(dev, 6, 4, 16, 4, 64, [90, 0, 17, 200], "bf16", poison=False)
+    q, kp, vp, table, c, w = _paged(dev, 6, 4, 16, 4, 64, [90, 0, 17, 200], "bf16", poison=False, extra=wide)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
@@ -118,6 +119,22 @@ def test_weights_graph(fa, dev):
         want = fa.decode_paged_weights(q, kp, vp, table, c, mine, inplace=True)
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(out, want)), i
+
+
+@pytest.mark.parametrize("wide", [0, 40])
+def test_weights_two_streams(fa, dev, wide):
+    cases = [_paged(dev, 30 + i, 4, 16, 4, 128, [90 + i, 0, 300, 5], "fp16", extra=wide) for i in range(2)]
+    want = [fa.decode_paged_weights(*c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(fa.decode_paged_weights(*cases[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, y) for out in got[i] for x, y in zip(out, want[i]))
 
 
 # ---------------------------------------------------------------------------

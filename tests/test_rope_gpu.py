@@ -387,3 +387,34 @@ def test_graph_and_streams(fa, dev):
         want = step(mine)
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip([*out, *pools], [*want, *mine])), i
+
+
+def test_step_graph(fa, dev):
+    """A captured step, rope and its way back and the rotated append, replayed with new rows and positions."""
+    q, k, v, pools, table, start, i32 = _append_case(dev, 8, 3, 8, 2, 1, 64, "bf16", [0, 15, 40])
+    freqs, scale = fa.rope_frequencies(64, scaling="by_parts", factor=4.0, original_len=256, device=dev)
+    pos = i32([7, 100, 41])
+
+    def step(pools):
+        rows = fa.rope(q, k, freqs, pos[:, None], scale=scale)
+        back = fa.rope_backward(*rows, freqs, pos[:, None], scale=scale)
+        return [*rows, *back, *fa.kv_append_rope(q, k, v, *pools, table, start, freqs, pos, scale=scale, want_k=True)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step([x.clone() for x in pools])
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(pools)
+    for i in range(4):
+        q.copy_(torch.randn_like(q))
+        v.copy_(torch.randn_like(v))
+        start.add_(i)
+        pos.add_(1000 * i)
+        mine = [x.clone() for x in pools]
+        graph.replay()
+        want = step(mine)
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip([*out, *pools], [*want, *mine])), i
