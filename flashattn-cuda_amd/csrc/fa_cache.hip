@@ -244,6 +244,12 @@ constexpr int kMostKeys = 32;              // of a thread's keys in registers
 constexpr int kListKeys = 4;               // up to which the selection also lists the stayers
 constexpr int kSubRuns = 4, kRuns = kSelWaves * kSubRuns;   // of a wave's slots, of the candidates
 
+// Sum of the first `waves` of a workgroup's waves' counts, by a whole wave.
+__device__ __forceinline__ int sum_before(const int* sh, int waves) {
+  const int lane = threadIdx.x & 63;
+  return __builtin_amdgcn_readlane(scan_sum(lane < waves ? sh[lane] : 0), 63);
+}
+
 // What is known of a (b, KV head) after its selection: tokens with keys above
 // `key` stay, and of those equal to it the first `left`. The candidates, all but
 // the newest tokens, are cut into runs: kSelWaves of `per` slots, of each kSubRuns
@@ -351,7 +357,7 @@ fa_evict_select_kernel(const float* __restrict__ weights, const int32_t* __restr
     if (lane == 63) sh_sum[wave] = above;
     above -= c0 + c1;
     __syncthreads();
-    for (int i = 0; i < wave; ++i) above += sh_sum[i];   // tokens of larger digits
+    above += sum_before(sh_sum, wave);   // tokens of larger digits
     if (above < left && above + c0 + c1 >= left) {        // exactly one thread
       const bool first = above + c0 >= left;
       sh_digit = kBins - 1 - 2 * tid - (first ? 0 : 1);
@@ -373,11 +379,8 @@ fa_evict_select_kernel(const float* __restrict__ weights, const int32_t* __restr
       sh_eq[wave] = eq;
     }
     __syncthreads();
-    gt = eq = 0;
-    for (int i = 0; i < wave; ++i) {
-      gt += sh_gt[i];
-      eq += sh_eq[i];
-    }
+    gt = sum_before(sh_gt, wave);
+    eq = sum_before(sh_eq, wave);
     const uint64_t below = ((uint64_t)1 << lane) - 1;
     each([&](int at, uint32_t k) {
       const uint64_t mg = __ballot(k > prefix), me = __ballot(k == prefix);
@@ -411,15 +414,12 @@ fa_evict_select_kernel(const float* __restrict__ weights, const int32_t* __restr
     sh_eq[wave] = eq;
   }
   __syncthreads();
-  if (tid < kRuns) {
-    gt = sh_run[0][tid];   // of a run that there is not: nothing, never read
-    eq = sh_run[1][tid];
-    for (int i = 0; i < tid / kSubRuns; ++i) {
-      gt += sh_gt[i];
-      eq += sh_eq[i];
-    }
-    out[bh].gt[tid] = gt;
-    out[bh].eq[tid] = eq;
+  if (wave == 0) {
+    static_assert(kRuns == 64, "a lane for each run");
+    const int of = lane / kSubRuns, first = lane % kSubRuns == 0;   // the run's wave
+    // Of a run that there is not: nothing, never read.
+    out[bh].gt[tid] = sh_run[0][tid] + scan_sum(first ? sh_gt[of] : 0) - sh_gt[of];
+    out[bh].eq[tid] = sh_run[1][tid] + scan_sum(first ? sh_eq[of] : 0) - sh_eq[of];
     if (tid == 0) {
       out[bh].per = per;
       out[bh].sub = sub;
