@@ -242,7 +242,6 @@ constexpr int kSelWaves = kSelThreads / 64;
 constexpr int kBins = 2048, kCopies = 4;   // counters of a digit, side by side for lanes of a wave
 constexpr int kMostKeys = 32;              // of a thread's keys in registers
 constexpr int kListKeys = 4;               // up to which the selection also lists the stayers
-constexpr int kSubRuns = 4, kRuns = kSelWaves * kSubRuns;   // of a wave's slots, of the candidates
 
 // Sum of the first `waves` of a workgroup's waves' counts, by a whole wave.
 __device__ __forceinline__ int sum_before(const int* sh, int waves) {
@@ -252,12 +251,12 @@ __device__ __forceinline__ int sum_before(const int* sh, int waves) {
 
 // What is known of a (b, KV head) after its selection: tokens with keys above
 // `key` stay, and of those equal to it the first `left`. The candidates, all but
-// the newest tokens, are cut into runs: kSelWaves of `per` slots, of each kSubRuns
-// of `sub`. gt and eq count the keys above and equal before a run.
+// the newest tokens, are cut into kSelWaves runs of `per` slots; gt and eq count the
+// keys above and equal before a run.
 struct Selection {
-  int n, cand, per, sub, left;   // n: the length, 0 of an invalid one; cand 0: every token stays
+  int n, cand, per, left;   // n: the length, 0 of an invalid one; cand 0: every token stays
   uint32_t key;
-  int gt[kRuns], eq[kRuns];
+  int gt[kSelWaves], eq[kSelWaves];
 };
 constexpr int kSelWords = sizeof(Selection) / 4;
 
@@ -269,7 +268,7 @@ constexpr int kSelWords = sizeof(Selection) / 4;
 // beside real ones they come last, so none of them ever stays. With up to kListKeys
 // keys a thread it also writes the stayers' old slots and weights, in order; beyond,
 // that is spread over the chip (fa_evict_list_kernel: 32000 slots of 64 heads 28 us in
-// one launch, 17 + 6.5 in two; 1100 slots of 32 heads 6.9 and 6.9 + 3.6).
+// one launch, 15.0 + 5.5 in two; 1100 slots of 32 heads 6.1, and 6.1 + 3.6).
 template <int E>
 __global__ void __launch_bounds__(kSelThreads)
 fa_evict_select_kernel(const float* __restrict__ weights, const int32_t* __restrict__ ctx_lens,
@@ -281,7 +280,6 @@ fa_evict_select_kernel(const float* __restrict__ weights, const int32_t* __restr
   __shared__ __attribute__((aligned(16))) uint32_t hist[kBins * kCopies];
   __shared__ uint32_t sh_digit, sh_above;
   __shared__ int sh_sum[kSelWaves], sh_gt[kSelWaves], sh_eq[kSelWaves];
-  __shared__ int sh_run[2][kRuns];
   const int hk = blockIdx.x, b = blockIdx.y;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -368,19 +366,19 @@ fa_evict_select_kernel(const float* __restrict__ weights, const int32_t* __restr
     left -= (int)sh_above;
   }
   if (need == 0) prefix = 0xffffffffu;   // of no number: every NaN has 0
+  int gt = 0, eq = 0;   // of the wave, then before it
+  each([&](int, uint32_t k) {
+    gt += __popcll(__ballot(k > prefix));
+    eq += __popcll(__ballot(k == prefix));
+  });
+  if (lane == 0) {
+    sh_gt[wave] = gt;
+    sh_eq[wave] = eq;
+  }
+  __syncthreads();
+  gt = sum_before(sh_gt, wave);
+  eq = sum_before(sh_eq, wave);
   if constexpr (LIST) {
-    int gt = 0, eq = 0;
-    each([&](int, uint32_t k) {
-      gt += __popcll(__ballot(k > prefix));
-      eq += __popcll(__ballot(k == prefix));
-    });
-    if (lane == 0) {
-      sh_gt[wave] = gt;
-      sh_eq[wave] = eq;
-    }
-    __syncthreads();
-    gt = sum_before(sh_gt, wave);
-    eq = sum_before(sh_eq, wave);
     const uint64_t below = ((uint64_t)1 << lane) - 1;
     each([&](int at, uint32_t k) {
       const uint64_t mg = __ballot(k > prefix), me = __ballot(k == prefix);
@@ -395,44 +393,21 @@ fa_evict_select_kernel(const float* __restrict__ weights, const int32_t* __restr
     });
     return;
   }
-  const int sub = (per / 64 + kSubRuns - 1) / kSubRuns * 64;
-  int gt = 0, eq = 0, next = 0, r = wave * kSubRuns;
-  each([&](int at, uint32_t k) {
-    if (at == next) {   // a run starts
-      if (lane == 0) {
-        sh_run[0][r] = gt;
-        sh_run[1][r] = eq;
-      }
-      next += sub;
-      ++r;
-    }
-    gt += __popcll(__ballot(k > prefix));
-    eq += __popcll(__ballot(k == prefix));
-  });
   if (lane == 0) {
-    sh_gt[wave] = gt;
-    sh_eq[wave] = eq;
+    out[bh].gt[wave] = gt;
+    out[bh].eq[wave] = eq;
   }
-  __syncthreads();
-  if (wave == 0) {
-    static_assert(kRuns == 64, "a lane for each run");
-    const int of = lane / kSubRuns, first = lane % kSubRuns == 0;   // the run's wave
-    // Of a run that there is not: nothing, never read.
-    out[bh].gt[tid] = sh_run[0][tid] + scan_sum(first ? sh_gt[of] : 0) - sh_gt[of];
-    out[bh].eq[tid] = sh_run[1][tid] + scan_sum(first ? sh_eq[of] : 0) - sh_eq[of];
-    if (tid == 0) {
-      out[bh].per = per;
-      out[bh].sub = sub;
-      out[bh].left = left;
-      out[bh].key = prefix;
-    }
+  if (tid == 0) {
+    out[bh].per = per;
+    out[bh].left = left;
+    out[bh].key = prefix;
   }
 }
 
 constexpr int kMoveThreads = 256;
-constexpr int kListSlots = 512;   // slots that a workgroup looks through at a time
+constexpr int kListSlots = 1024;   // slots that a workgroup looks through at a time
 
-// Old slots and weights of the stayers, in order. Workgroups x < kRuns have a run of
+// Old slots and weights of the stayers, in order. Workgroups x < kSelWaves have a run of
 // candidates, the others kListSlots of the tokens that stay unseen (the newest, or
 // all of a short cache).
 __global__ void __launch_bounds__(kMoveThreads)
@@ -451,10 +426,10 @@ fa_evict_list_kernel(const float* __restrict__ weights, const Selection* __restr
   int32_t* kp = kept + bh * keep;
   float* wn = w_new + bh * ((size_t)new_max_pages * kPageSize);
   const int cand = se.cand;
-  if (blockIdx.x >= kRuns) {
+  if (blockIdx.x >= kSelWaves) {
     const int stay = cand > 0 ? recent : se.n;    // tokens cand .. + stay - 1
     const int to = cand > 0 ? keep - recent : 0;
-    const int first = ((int)blockIdx.x - kRuns) * kListSlots;
+    const int first = ((int)blockIdx.x - kSelWaves) * kListSlots;
     for (int i = first + tid; i < min(first + kListSlots, stay); i += kMoveThreads) {
       kp[to + i] = cand + i;
       wn[to + i] = w[cand + i];
@@ -462,9 +437,7 @@ fa_evict_list_kernel(const float* __restrict__ weights, const Selection* __restr
     return;
   }
   if (cand == 0) return;
-  const int per = se.per, sub = se.sub, left = se.left;
-  const int start = (int)blockIdx.x / kSubRuns * per, lo = start + (int)blockIdx.x % kSubRuns * sub;
-  const int hi = min(min(lo + sub, start + per), cand);
+  const int left = se.left, lo = (int)blockIdx.x * se.per, hi = min(lo + se.per, cand);
   if (lo >= hi) return;
   const uint32_t key = se.key;
   int gt = se.gt[blockIdx.x], eq = se.eq[blockIdx.x];
@@ -608,7 +581,7 @@ extern "C" int fa_kv_evict(void* k_pool, void* v_pool, const int32_t* page_table
                      (int)recent, (int)(new_max_pages * kPageSize));
   if (keys > kListKeys) {
     const int64_t plain = ((keep < width ? keep : width) + kListSlots - 1) / kListSlots;
-    hipLaunchKernelGGL(fa_evict_list_kernel, dim3((unsigned)(kRuns + plain), (unsigned)H_kv, (unsigned)B),
+    hipLaunchKernelGGL(fa_evict_list_kernel, dim3((unsigned)(kSelWaves + plain), (unsigned)H_kv, (unsigned)B),
                        dim3(kMoveThreads), 0, s, weights, sel, kept, new_weights, (int)H_kv,
                        (int)max_pages, (int)new_max_pages, (int)keep, (int)recent);
   }
