@@ -10,7 +10,7 @@
 //                    c D/16 + db, P^T straight from the S accumulators)
 // K's pieces are operands as they lie; V's tokens are paired by v_perm. Nothing
 // goes through LDS, so a CU has three waves a SIMD with 16 KiB each in flight (D
-// = 128). Lane l has query row l % 16 in both products, so a row's maximum and
+// = 128; held to the registers of four, 1.14 GB took 240 us against 215, with two 219). Lane l has query row l % 16 in both products, so a row's maximum and
 // sum stay in its lane column.
 //
 // Maxima are kept as K Q^T gives them and differences are scaled, so that no
