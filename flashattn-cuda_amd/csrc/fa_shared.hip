@@ -54,13 +54,12 @@ struct TileShared {
 // an unrounded sum, as the forward rounds it.
 //
 // Bound, with 128 rows a KV head, by memory: 256 units at D = 128 take 1.55 us a tile,
-// 5.4 TB/s. With more, the row blocks of a tile find it in their L2 and a tile takes 1.15
-// to 1.2 us of a CU, 0.93 PFLOP/s over the chip, bound by LDS: each of the eight waves
-// reads 16 KiB a tile for its 32 rows, 1 KiB a matrix instruction. The copies,
-// exponentials or the second product left out change that by little, and no more do key
-// groups that take turns at products and exponentials, or V in blocks of 32 columns. Waves
-// of 64 rows would read half, but need more than the 256 registers of two waves a SIMD.
-// Beside the tiles a unit costs about 8 us, and 16.8 MB of partials 7 us at the end.
+// 5.4 TB/s. With more, the row blocks of a tile find it in their L2 and a tile takes 1.2
+// us of a CU, 0.9 PFLOP/s over the chip, the forward's rate, and no part of it by itself:
+// 1.04 without the copies, 1.16 with half of the reads from LDS, 1.24 without the
+// exponentials. Key groups that take turns at products and exponentials, or V in blocks
+// of 32 columns, change it by 2 % at most. Beside the tiles a unit costs about 8 us, and
+// 16.8 MB of partials 7 us at the end.
 template <int D, bool BF16>
 __device__ __forceinline__ void
 tile_unit(TileShared<D>& sh, const int unit, const f16* __restrict__ q, const f16* __restrict__ kpool,

@@ -1,6 +1,7 @@
 // fa_stream.hpp — decode attention over runs of 16-bit pages, for the kernels
 // that run it: one query token per sequence, cut into chunks of pages that a
-// later launch joins by their references and sums (see chunk_body), or, of short sequences, whole.
+// later launch joins by their references and sums (see chunk_body), or, of short
+// sequences, whole.
 //
 // Bound by memory: a page of 16 tokens of one KV head is 32 D bytes each of K and
 // V, read once for up to 16 query rows. A wave loads whole pages straight into
@@ -10,8 +11,9 @@
 //                    c D/16 + db, P^T straight from the S accumulators)
 // K's pieces are operands as they lie; V's tokens are paired by v_perm. Nothing
 // goes through LDS, so a CU has three waves a SIMD with 16 KiB each in flight (D
-// = 128; held to the registers of four, 1.14 GB took 240 us against 215, with two 219). Lane l has query row l % 16 in both products, so a row's maximum and
-// sum stay in its lane column.
+// = 128; held to the registers of four, 1.14 GB took 240 us against 215, with two
+// 219). Lane l has query row l % 16 in both products, so a row's maximum and sum stay
+// in its lane column.
 //
 // Maxima are kept as K Q^T gives them and differences are scaled, so that no
 // weight passes 1 however large the scores are. P goes into its product as two
