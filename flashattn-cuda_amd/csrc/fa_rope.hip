@@ -162,6 +162,24 @@ __global__ void __launch_bounds__(kThreads) fa_rope_kernel(const Args a) {
   const bool turn = u < a.R / 16;
   const int ea = turn && !INTER ? 8 * u : 16 * u;
   const int eb = turn && !INTER ? a.R / 2 + 8 * u : 16 * u + 8;
+  // Rows are asked for before the angles are worked out.
+  Vec<IN> xa[kBatch], xb[kBatch];
+  const auto load = [&](int i) {
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const int hj = h + j * HS;
+      xa[j] = Vec<IN>{};
+      xb[j] = Vec<IN>{};
+      if (i + j < a.per_wg && hj < heads && live) {
+        const Rows& r = hj < a.H ? a.in[0] : (!APPEND || hj < a.H + a.Hkv ? a.in[1] : a.in[2]);
+        const int hh = hj < a.H ? hj : (hj < a.H + a.Hkv ? hj - a.H : hj - a.H - a.Hkv);
+        const EI* src = (const EI*)r.p + b * r.sb + hh * r.sh + t * r.sn;
+        xa[j] = load8<IN>(src + ea);
+        xb[j] = load8<IN>(src + eb);
+      }
+    }
+  };
+  load(0);
   float cs[8], sn[8];
   if (turn && h < a.H + a.Hkv) {
     int64_t p;
@@ -183,20 +201,7 @@ __global__ void __launch_bounds__(kThreads) fa_rope_kernel(const Args a) {
   }
 
   for (int i = 0; i < a.per_wg; i += kBatch, h += kBatch * HS) {
-    Vec<IN> xa[kBatch], xb[kBatch];
-#pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
-      const int hj = h + j * HS;
-      xa[j] = Vec<IN>{};
-      xb[j] = Vec<IN>{};
-      if (i + j < a.per_wg && hj < heads && live) {
-        const Rows& r = hj < a.H ? a.in[0] : (!APPEND || hj < a.H + a.Hkv ? a.in[1] : a.in[2]);
-        const int hh = hj < a.H ? hj : (hj < a.H + a.Hkv ? hj - a.H : hj - a.H - a.Hkv);
-        const EI* src = (const EI*)r.p + b * r.sb + hh * r.sh + t * r.sn;
-        xa[j] = load8<IN>(src + ea);
-        xb[j] = load8<IN>(src + eb);
-      }
-    }
+    if (i > 0) load(i);
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
       const int hj = h + j * HS;
