@@ -13,12 +13,12 @@
 // the heads and needs no table in memory. Rows are addressed by strides: the
 // [B, N, H, D] a projection leaves is read as it is and written head-major.
 //
-// Kernel times, us: 4 x 4096 tokens, 16 + 16 heads of D = 128, bf16: 51, 5.2 TB/s, as a
-// plain copy of that size. Gradients of 2 x 2000 tokens, 32 + 8 heads of D = 128, fp32 to
-// bf16: 25, 4.9 TB/s. The append of two prompts of up to 1777 tokens, 32 heads over 8,
-// D = 128: 17.4. One token of 8 sequences: 4.5; 1024 tokens, 8 + 8 heads of D = 64: 3.8,
-// with the library's sine and cosine 4.3. Loads and stores with the non-temporal hint:
-// 25 -> 36, 17.4 -> 20.5.
+// Kernel times, us: 4 x 4096 tokens, 16 + 16 heads of D = 128, bf16: 42.6, 6.3 TB/s (a
+// plain copy of 256 MB 5.4). Gradients of 2 x 2000 tokens, 32 + 8 heads of D = 128, fp32 to
+// bf16: 21.3, 5.8 TB/s. The append of two prompts of up to 1777 tokens, 32 heads over 8,
+// D = 128: 16.3. One token of 8 sequences: 4.1; 1024 tokens, 8 + 8 heads of D = 64: 3.2.
+// Rows asked for after the angles: 51.4, 24.7, 17.3, 4.6 and 3.7. Loads and stores with the
+// non-temporal hint: 25 -> 36, 17.4 -> 20.5; the library's sine and cosine: 3.8 -> 4.3.
 #include <hip/hip_runtime.h>
 
 #include <stdint.h>
@@ -113,7 +113,8 @@ struct Args {
   int max_pages, num_pages;
 };
 
-constexpr int kBatch = 4;   // heads whose loads a thread has in flight
+constexpr int kBatch = 2;   // heads whose loads a thread has in flight (1, 2, 4, 8: 44.0 42.6 43.9 45.6 us of
+                            // the first call above, 21.1 21.3 22.5 32.8 of the second)
 
 // Thread (hs, tok, u): 8 pairs u of token tok, heads hs, hs + HS, ...: HS =
 // 256 / (tokens * D/16) heads side by side, so that a call of single tokens
@@ -262,8 +263,8 @@ __global__ void __launch_bounds__(kThreads) fa_rope_kernel(const Args a) {
 
 // Tokens of a workgroup, the heads a thread walks over and the grid: about 2048
 // workgroups, where the angles are shared by as many heads as leave the chip full. The
-// three calls above, us, for 512, 1024, 2048, 4096 and 8192: 69.0 58.4 51.3 50.7 49.5;
-// 26.3 26.8 24.6 25.3 25.0; 19.9 17.2 17.4 18.7 18.7.
+// first three calls above, us, for 2048 and 4096: 42.6 43.9; 21.3 21.1; 16.3 17.2; four
+// heads in flight and 512, 1024, 2048, 4096: 51.6 51.8 43.9 44.0.
 static dim3 plan(Args& a, int64_t B, bool append) {
   const int units = a.D / 16;
   int tt = 0;
