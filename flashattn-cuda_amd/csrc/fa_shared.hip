@@ -25,7 +25,7 @@ using namespace stream;
 
 // The cuts are made for the 256 CUs of a whole MI355X, whatever the device has: the
 // workspace follows from the sizes alone.
-constexpr int kCus = 256;
+constexpr int kCus = 256, kMostUnits = 192;   // units: of the prefix pass in tiles
 
 constexpr int kTile = 64;     // keys of a tile: 4 pages
 constexpr int kStages = 4;    // tiles in LDS, three of them in flight
@@ -339,17 +339,19 @@ fa_shared_chunk_kernel(const uint16_t* __restrict__ q, const char* __restrict__ 
 // Splits of the prefix in the launch of tiles, from the lengths that only the device
 // knows: as many units as make the prefix's share of the CUs that of its work, in us of a
 // CU, so that the own pages are read beside the tiles and neither is left over; of
-// kUnitTiles tiles at least. `per` units a split, `pages` own pages. Against 160 units for
-// any lengths, us a call, H32 over 8, D = 128: 32 sequences of 50 to 1500 tokens under 7999
-// 38.6 -> 34.0, 128 of 20 to 500 under 32768 122 -> 117, 64 of 500 to 2000 107 -> 105, of
-// 20 to 1000 76 and 76, 36 of 30 to 120 under 2500 19.4 -> 21.4; 18 such sets in the mean
-// 1 % less. In launches of their own the first took 17 + 20.4 and the fourth 48.5 + 24.7.
-// kUnitTime 0.5, 3, 8 and 13: the mean 39.9, 39.1, 40.0, 39.8 (a unit's own time is 8);
-// kUnitTiles 4, 6, 8 and 10: 39.2, 39.1, 39.2, 40.1.
+// kUnitTiles tiles at least, and kMostUnits at most (more, and the own pages of a short
+// batch wait for a CU: 16 sequences of 50 to 200 under 8000 20 -> 23.5 us). `per` units a
+// split, `pages` own pages. Against 160 units for any lengths, us a call, H32 over 8, D =
+// 128: 32 sequences of 50 to 1500 tokens under 7999 38.6 -> 33.7, 128 of 20 to 500 under
+// 32768 122 -> 115, 64 of 500 to 2000 107 -> 105, of 20 to 1000 75 and 75, 36 of 30 to 120
+// under 2500 19.4 -> 22.2; 18 such sets in the mean 2 % less. In launches of their own
+// the first took 17 + 20.4 and the fourth 48.5 + 24.7. kUnitTime 0.5, 3, 8 and 13: the mean
+// 39.9, 39.1, 40.0, 39.8 (a unit's own time is 8); kUnitTiles 1, 2, 3, 4 and 6, 8 sets of
+// short prefixes: 16.8, 16.6, 16.6, 17.0, 18.0.
 template <int D>
 __device__ __forceinline__ int tile_splits(int tiles, int per, int pages, int Hkv, int most) {
   constexpr float kTileTime = 1.15f * D / 128, kUnitTime = 3.f, kPageTime = 0.4f * D / 128;
-  constexpr int kUnitTiles = 6;
+  constexpr int kUnitTiles = 3;
   const float t = kTileTime * tiles * per, own = kPageTime * pages * Hkv;
   const float x = t + own - kCus * kUnitTime;   // kUnitTime u^2 + x u - kCus t = 0
   const float u = (__builtin_sqrtf(x * x + 4 * kUnitTime * kCus * t) - x) / (2 * kUnitTime);
@@ -486,7 +488,7 @@ static Cut cut_of(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t prefix_p
   p.few = p.rows <= kFewRows;
   const int64_t block = p.few ? 16 : kTileRows, part = p.few ? kMinChunk : kTile / kTokens;
   p.row_blocks = (int)((p.rows + block - 1) / block);
-  int64_t sp = kCus / (Hkv * p.row_blocks);
+  int64_t sp = (p.few ? kCus : kMostUnits) / (Hkv * p.row_blocks);
   const int64_t most = (prefix_pages + part - 1) / part;
   sp = sp > most ? most : sp;
   p.sp = (int)(sp < 1 ? 1 : sp);
