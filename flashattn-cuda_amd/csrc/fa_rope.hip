@@ -14,11 +14,12 @@
 // [B, N, H, D] a projection leaves is read as it is and written head-major.
 //
 // Kernel times, us: 4 x 4096 tokens, 16 + 16 heads of D = 128, bf16: 42.6, 6.3 TB/s (a
-// plain copy of 256 MB 5.4). Gradients of 2 x 2000 tokens, 32 + 8 heads of D = 128, fp32 to
-// bf16: 21.3, 5.8 TB/s. The append of two prompts of up to 1777 tokens, 32 heads over 8,
-// D = 128: 16.3. One token of 8 sequences: 4.1; 1024 tokens, 8 + 8 heads of D = 64: 3.2.
-// Rows asked for after the angles: 51.4, 24.7, 17.3, 4.6 and 3.7. Loads and stores with the
-// non-temporal hint: 25 -> 36, 17.4 -> 20.5; the library's sine and cosine: 3.8 -> 4.3.
+// plain copy of 256 MB 5.4; calls in turn on other rows 52). Gradients of 2 x 2000 tokens,
+// 32 + 8 heads of D = 128, fp32 to bf16: 21.3, 5.8 TB/s. The append of two prompts of up to
+// 1777 tokens, 32 heads over 8, D = 128: 16.3. One token of 8 sequences: 4.2; 1024 tokens,
+// 8 + 8 heads of D = 64: 3.4, with the library's sine and cosine half a us more. Rows asked
+// for after the angles: 51.4, 24.7, 17.3, 4.6 and 3.7. Loads and stores with the
+// non-temporal hint: 25 -> 36, 17.4 -> 20.5.
 #include <hip/hip_runtime.h>
 
 #include <stdint.h>
