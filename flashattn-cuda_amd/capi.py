@@ -80,7 +80,7 @@ SIGNATURES = {
     "fa_decode_weights_workspace_floats": (_i64, [_i64] * 5),
     "fa_validate_decode_weights": (C.c_int, [_vp] * 6 + [_i64] * 7 + [_vp] * 4),
     "fa_kv_evict": (C.c_int, [_vp] * 11 + [_i64] * 9 + [_vp]),
-    "fa_kv_evict_workspace_words": (_i64, [_i64] * 2),
+    "fa_kv_evict_workspace_words": (_i64, [_i64] * 3),
     "fa_validate_kv_evict": (C.c_int, [_vp] * 11 + [_i64] * 9),
     "fa_probe_fwd_variant": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, C.c_int, C.c_int, _vp]),
     "fa_probe_fwd_variants": (C.c_int, [_vp, C.c_int, _i64, C.c_int]),

@@ -295,15 +295,17 @@ fa_evict_select_kernel(const float* __restrict__ weights, const int32_t* __restr
     if (j < keep) kept[bh * keep + j] = -1;
   }
   const int cand = n > keep ? n - recent : 0, need = keep - recent;   // 0 <= need < cand
+  constexpr bool LIST = E > 0 && E <= kListKeys;
   if (tid == 0) {
-    out[bh].n = n;
-    out[bh].cand = cand;
+    if constexpr (!LIST) {
+      out[bh].n = n;
+      out[bh].cand = cand;
+    }
     if (hk == 0) {
       new_lens[b] = m;
       bad[b] = invalid;
     }
   }
-  constexpr bool LIST = E > 0 && E <= kListKeys;
   if constexpr (LIST) {   // those that stay unseen
     const int stay = cand > 0 ? recent : n, to = cand > 0 ? need : 0;
     for (int j = tid; j < stay; j += kSelThreads) {
@@ -551,9 +553,11 @@ extern "C" int fa_decode_paged_weights(const void* q, const void* k_pool, const 
             o, lse, weights_out, stream);
 }
 
-extern "C" int64_t fa_kv_evict_workspace_words(int64_t B, int64_t H_kv) {
+extern "C" int64_t fa_kv_evict_workspace_words(int64_t B, int64_t H_kv, int64_t max_pages) {
+  using namespace fa::cache;
   if (B <= 0 || H_kv <= 0 || B > 65535 || H_kv > 65535) return 0;
-  return B * H_kv * fa::cache::kSelWords;
+  if (max_pages <= kListKeys * kSelThreads / kPageSize) return 0;
+  return B * H_kv * kSelWords;
 }
 
 extern "C" int fa_kv_evict(void* k_pool, void* v_pool, const int32_t* page_table,

@@ -364,8 +364,9 @@ extern "C" int fa_validate_kv_evict(const void* k_pool, const void* v_pool, cons
                                     int64_t H_kv, int64_t D, int64_t keep, int64_t recent, int64_t page_size,
                                     int64_t max_pages, int64_t new_max_pages, int64_t num_pages) {
   if (!k_pool || !v_pool || !page_table || !ctx_lens || !weights || !new_page_table || !kept ||
-      !new_weights || !new_lens || !bad || !workspace)
+      !new_weights || !new_lens || !bad)
     return FA_ERR_NULL_POINTER;
+  if (!workspace && fa_kv_evict_workspace_words(B, H_kv, max_pages) > 0) return FA_ERR_NULL_POINTER;
   if (D != 64 && D != 128) return FA_ERR_HEAD_DIM;
   if (B <= 0 || H_kv <= 0) return FA_ERR_BATCH_HEADS;
   if (page_size != 16) return FA_ERR_PAGE_SIZE;

@@ -925,14 +925,15 @@ std::vector<torch::Tensor> kv_evict(torch::Tensor k_pool, torch::Tensor v_pool, 
   auto new_weights = at::empty({B, Hkv, 16 * new_page_table.size(1)}, weights.options());
   auto new_lens = at::empty({B}, page_table.options());
   auto bad = at::empty({B}, page_table.options());
-  auto ws = at::empty({fa_kv_evict_workspace_words(B, Hkv)}, page_table.options());
+  const int64_t words = fa_kv_evict_workspace_words(B, Hkv, max_pages);
+  const auto ws = words > 0 ? at::empty({words}, page_table.options()) : torch::Tensor();
   const int st = fa_kv_evict(k_pool.data_ptr(), v_pool.data_ptr(), page_table.data_ptr<int32_t>(),
                              ctx_lens.data_ptr<int32_t>(), weights.data_ptr<float>(),
                              new_page_table.data_ptr<int32_t>(), kept.data_ptr<int32_t>(),
                              new_weights.data_ptr<float>(), new_lens.data_ptr<int32_t>(),
-                             bad.data_ptr<int32_t>(), ws.data_ptr<int32_t>(), B, Hkv, k_pool.size(3), keep,
-                             recent, k_pool.size(2), max_pages, new_page_table.size(1), k_pool.size(0),
-                             current_stream(k_pool));
+                             bad.data_ptr<int32_t>(), words > 0 ? ws.data_ptr<int32_t>() : nullptr, B, Hkv,
+                             k_pool.size(3), keep, recent, k_pool.size(2), max_pages,
+                             new_page_table.size(1), k_pool.size(0), current_stream(k_pool));
   check_status(st, "fa_kv_evict");
   return {kept, new_weights, new_lens, bad};
 }

@@ -658,9 +658,9 @@ int fa_validate_decode_weights(const void* q, const void* k_pool, const void* v_
  * invalid are not copied and set bad[b] to 1; a negative length, or one beyond the
  * table, sets bad[b] and new_lens[b] = 0; every other bad[b] is set to 0. Pages of
  * new_page_table that the call writes must not be among those it reads. 16-bit
- * rows of any type. 0 <= recent <= keep <= new_max_pages * 16. workspace:
- * fa_kv_evict_workspace_words(...) words of 4 bytes that need not be cleared; calls
- * that may overlap need one each.
+ * rows of any type. 0 <= recent <= keep <= new_max_pages * 16, keep > 0. workspace:
+ * fa_kv_evict_workspace_words(...) words of 4 bytes (NULL where 0) that need not be
+ * cleared; calls that may overlap need one each.
  */
 int fa_kv_evict(void* k_pool, void* v_pool, const int32_t* page_table, const int32_t* ctx_lens,
                 const float* weights, const int32_t* new_page_table, int32_t* kept,
@@ -668,8 +668,9 @@ int fa_kv_evict(void* k_pool, void* v_pool, const int32_t* page_table, const int
                 int64_t H_kv, int64_t D, int64_t keep, int64_t recent, int64_t page_size,
                 int64_t max_pages, int64_t new_max_pages, int64_t num_pages, void* stream);
 
-/* Words of fa_kv_evict's workspace; 0 for invalid sizes. */
-int64_t fa_kv_evict_workspace_words(int64_t B, int64_t H_kv);
+/* Words of fa_kv_evict's workspace; 0 for invalid sizes, and for tables of up to 256
+ * pages. */
+int64_t fa_kv_evict_workspace_words(int64_t B, int64_t H_kv, int64_t max_pages);
 
 /* Host-only argument check of fa_kv_evict. */
 int fa_validate_kv_evict(const void* k_pool, const void* v_pool, const int32_t* page_table,

@@ -134,7 +134,8 @@ def _evict(**kw):
 
 
 EVICT = [
-    (dict(), "FA_OK"), *((({x: 0}), "FA_ERR_NULL_POINTER") for x in ("kp", "vp", "t", "c", "w", "nt", "kept", "nw", "nl", "bad", "ws")),
+    (dict(), "FA_OK"), *((({x: 0}), "FA_ERR_NULL_POINTER") for x in ("kp", "vp", "t", "c", "w", "nt", "kept", "nw", "nl", "bad")),
+    (dict(ws=0), "FA_OK"), (dict(ws=0, mp=256), "FA_OK"), (dict(ws=0, mp=257), "FA_ERR_NULL_POINTER"),
     (dict(D=96), "FA_ERR_HEAD_DIM"), (dict(B=0), "FA_ERR_BATCH_HEADS"), (dict(size=4), "FA_ERR_PAGE_SIZE"), (dict(mp=0), "FA_ERR_MAX_PAGES"),
     (dict(nmp=0), "FA_ERR_MAX_PAGES"), (dict(pages=-1), "FA_ERR_NUM_PAGES"), (dict(kp=A + 8), "FA_ERR_ALIGNMENT"), (dict(kept=A + 2), "FA_ERR_ALIGNMENT"),
     (dict(keep=0), "FA_ERR_BUDGET"), (dict(keep=113), "FA_ERR_BUDGET"), (dict(keep=112), "FA_OK"), (dict(recent=-1), "FA_ERR_BUDGET"),
@@ -185,7 +186,7 @@ def test_workspaces(capi, B, H, Hkv, D, pp, mp):
                 (B, 70000, 1, D, pp, mp), (B, H, Hkv, D, 1 << 27, mp), (65535, H, Hkv, D, pp, 1 << 16)):
         assert lib.fa_decode_shared_workspace_floats(*bad) == 0
         if bad[0] == 0 or bad[1] == 70000:
-            assert lib.fa_kv_evict_workspace_words(bad[0], bad[1]) == 0
+            assert lib.fa_kv_evict_workspace_words(bad[0], bad[1], 300) == 0
         if bad[4] not in (0, 1 << 27):
             assert lib.fa_decode_weights_workspace_floats(*bad[:4], bad[5]) == 0
 
