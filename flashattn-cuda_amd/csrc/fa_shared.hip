@@ -507,8 +507,7 @@ template <int D, bool BF16>
 static int launch(const Cut& p, const void* q, const void* k_pool, const void* v_pool,
                   const int32_t* prefix_table, const int32_t* prefix_len, const int32_t* page_table,
                   const int32_t* ctx_lens, int64_t B, int64_t H, int64_t Hkv, int64_t prefix_pages,
-                  int64_t max_pages, int64_t num_pages, const Topology& topo, float* ws, void* o,
-                  float* lse, hipStream_t s) {
+                  int64_t max_pages, int64_t num_pages, float* ws, void* o, float* lse, hipStream_t s) {
   const float c = (float)(1.0 / sqrt((double)D)) * kLog2e;
   const int64_t groups = head_groups(H, Hkv);
   if (p.one) {
@@ -550,7 +549,7 @@ static int launch(const Cut& p, const void* q, const void* k_pool, const void* v
                        prefix_len, page_table, ctx_lens, table, ws, pre_ml, own_o, own_ml, first, (int)B,
                        (int)H, (int)Hkv, (int)(H / Hkv), (int)(groups / Hkv), (int)p.rows, (int)units,
                        p.row_blocks, p.sp, splits, (int)prefix_pages, (int)max_pages, (int)num_pages,
-                       plan, topo.xcds, c);
+                       plan, stream_topology(s).xcds, c);
   }
   hipLaunchKernelGGL((fa_shared_join_kernel<D, BF16>), dim3((unsigned)(B * H)), dim3(kJoinThreads), 0, s,
                      ws, pre_ml, own_o, own_ml, first, splits, prefix_len, (uint16_t*)o, lse, (int)H, (int)(B * H),
@@ -591,5 +590,5 @@ extern "C" int fa_decode_shared(const void* q, const void* k_pool, const void* v
   const auto fn = D == 128 ? (bf16 ? launch<128, true> : launch<128, false>)
                            : (bf16 ? launch<64, true> : launch<64, false>);
   return fn(p, q, k_pool, v_pool, prefix_table, prefix_len, page_table, ctx_lens, B, H, H_kv,
-            prefix_pages, max_pages, num_pages, stream_topology(s), workspace, o, lse, s);
+            prefix_pages, max_pages, num_pages, workspace, o, lse, s);
 }
