@@ -217,6 +217,9 @@ def rope_frequencies(rot_dim: int, base: float = 10000.0, scaling=None, factor: 
       "by_parts"  those that make fewer than slow_turns turns within original_len
                   divided by factor, those that make more than fast_turns kept, a
                   linear ramp over their index between the two; scale is 0.1 ln factor + 1
+                  (YaRN, Peng et al. 2023). The ramp's ends, rounded outwards, may lie
+                  before the first frequency or past the last one: a trained length
+                  above 2 pi base leaves even the slowest partly kept
 
     scale is 1 otherwise. It multiplies the rotated dims of Q and of K.
     """
@@ -241,9 +244,8 @@ def rope_frequencies(rot_dim: int, base: float = 10000.0, scaling=None, factor: 
         def index(turns):   # of the frequency that makes so many turns within original_len
             return rot_dim * math.log(original_len / (2.0 * math.pi * turns)) / (2.0 * math.log(base))
 
-        lo = max(math.floor(index(fast_turns)), 0)
-        hi = min(math.ceil(index(slow_turns)), half - 1)
-        ramp = torch.clamp((i - lo) / max(hi - lo, 1e-3), 0.0, 1.0)   # 0: kept, 1: divided
+        lo, hi = math.floor(index(fast_turns)), math.ceil(index(slow_turns))   # lo < hi
+        ramp = torch.clamp((i - lo) / (hi - lo), 0.0, 1.0)   # 0: kept, 1: divided
         freqs = freqs * (1.0 - ramp) + freqs / factor * ramp
         scale = 0.1 * math.log(factor) + 1.0
     elif scaling not in (None, "ntk"):

@@ -235,6 +235,43 @@ def test_frequencies(fa):
         assert torch.allclose(same, f, rtol=1e-14) and scale == 1.0
 
 
+@pytest.mark.parametrize("R,base,n,slow,fast", [(128, 1e4, 131072, 1, 32), (128, 1e4, 65536, 1, 32), (16, 1e4, 65536, 1, 32), (64, 1e4, 1 << 20, 2, 20),
+                                                (64, 5e5, 1 << 22, 1, 4), (128, 1e4, 150, 1, 32), (32, 1e4, 5, 1, 32), (64, 100.0, 4096, 1, 32),
+                                                (16, 1e4, 4096, 1, 32), (8, 1e4, 40, 0.5, 1000)])
+def test_frequencies_by_parts_ramp(fa, R, base, n, slow, fast):
+    """The ramp's ends lie where the number of turns within the trained length is fast_turns and slow_turns, out of
+    the frequencies there are too (a trained length above 2 pi base, or below 2 pi fast_turns): each frequency's share
+    of the division is read off the line between the places, rounded outwards, found here by bisection over a real index."""
+    def place(turns):
+        lo, hi = -4.0 * R, 5.0 * R
+        for _ in range(200):
+            mid = (lo + hi) / 2
+            lo, hi = (mid, hi) if n / (2 * math.pi) * base ** (-2 * mid / R) > turns else (lo, mid)
+        return (lo + hi) / 2
+
+    a, b = math.floor(place(fast)), math.ceil(place(slow))
+    want = [min(max((i - a) / (b - a), 0.0), 1.0) for i in range(R // 2)]
+    f = fa.rope_frequencies(R, base, device="cpu")[0].numpy()
+    got, scale = fa.rope_frequencies(R, base, "by_parts", 8.0, n, slow_turns=slow, fast_turns=fast, device="cpu")
+    assert scale == pytest.approx(0.1 * math.log(8) + 1)
+    # five roundings of 2^-53 each in the ramp, its complement, the two products and the sum
+    assert np.allclose(got.numpy(), [x * (1 - r) + x / 8 * r for x, r in zip(f, want)], rtol=2e-15, atol=0)
+    turns = n * f / (2 * math.pi)
+    step = base ** (2 / R)   # from one frequency to the next; beyond a place rounded outwards the ends are reached
+    assert (got.numpy()[turns >= fast * step] == f[turns >= fast * step]).all()
+    assert np.allclose(got.numpy()[turns <= slow / step], f[turns <= slow / step] / 8, rtol=2e-15, atol=0)
+
+
+def test_frequencies_by_parts_by_hand(fa):
+    """128 dims, base 10000, trained on 131072 positions, 8 times as long: fast_turns 32 at index 64 log(131072 / (64 pi)) / log
+    10000 = 45.03, slow_turns 1 at 64 log(131072 / (2 pi)) / log 10000 = 69.11, past the last of the 64 frequencies. The ramp goes
+    from 45 to 70: the last, of 2.4 turns, has 18 / 25 of the division, the one of index 50 a fifth of it."""
+    f, _ = fa.rope_frequencies(128, 10000.0, device="cpu")
+    g, _ = fa.rope_frequencies(128, 10000.0, "by_parts", 8.0, 131072, device="cpu")
+    r = (g / f).numpy()
+    assert np.allclose(r[[45, 50, 63]], [1, 1 - 0.2 * 7 / 8, 1 - 0.72 * 7 / 8], rtol=1e-14) and (r[:46] == 1).all()
+
+
 def test_frequencies_refuse(fa):
     for kw, word in ((dict(rot_dim=0), "rot_dim"), (dict(rot_dim=15), "rot_dim"), (dict(rot_dim=16, base=1.0), "base"),
                      (dict(rot_dim=16, factor=0.5), "factor"), (dict(rot_dim=16, scaling="ramp"), "scaling"),
