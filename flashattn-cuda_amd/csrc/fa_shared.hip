@@ -497,7 +497,7 @@ static Cut cut_of(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t prefix_p
   p.own_o = B * H * p.sp * D;
   p.pre_ml = p.own_o + p.own * H * D;
   p.own_ml = p.pre_ml + 2 * B * H * p.sp;
-  p.table = p.own_ml + (2 * p.own * H + 3) / 4 * 4;
+  p.table = (p.own_ml + 2 * p.own * H + 3) / 4 * 4;   // entries of 16 bytes
   p.first = p.table + (B > kWavePlan ? 4 * (1 + p.own) : 0);
   p.floats = p.first + 2 * B + 1;
   return p;

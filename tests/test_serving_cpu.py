@@ -191,6 +191,15 @@ def test_workspaces(capi, B, H, Hkv, D, pp, mp):
             assert lib.fa_decode_weights_workspace_floats(*bad[:4], bad[5]) == 0
 
 
+@pytest.mark.parametrize("B,H,Hkv,D,pp,mp", [(257, 1, 1, 64, 20, 80), (301, 3, 1, 128, 9, 40), (257, 1, 1, 64, 24, 80), (1001, 5, 5, 64, 30, 9)])
+def test_workspace_table_is_aligned(capi, B, H, Hkv, D, pp, mp):
+    """Above 256 sequences the chunks' table, entries of 16 bytes, and then two words a sequence and one more end the
+    workspace: the table lies on 16 bytes where what comes before it, and it, are multiples of four words."""
+    lib = capi.load()
+    assert (lib.fa_decode_shared_workspace_floats(B, H, Hkv, D, pp, mp) - 2 * B - 1) % 4 == 0
+    assert (lib.fa_decode_weights_workspace_floats(B, H, Hkv, D, mp) - 2 * B) % 4 == 0
+
+
 def test_binding_refuses_host_tensors(fa):
     x = torch.zeros(1, 2, 3, 64)
     i = torch.zeros(1, dtype=torch.int32)

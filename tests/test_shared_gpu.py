@@ -272,3 +272,10 @@ def test_two_streams(fa, dev):
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(a, want[i][0]) and torch.equal(b, want[i][1]) for a, b in got[i])
+
+
+@pytest.mark.parametrize("B,H,Hkv,D,P", [(257, 1, 1, 64, 300), (301, 3, 1, 128, 130)])
+def test_odd_batch_planned_on_the_device(fa, dev, B, H, Hkv, D, P):
+    """More sequences than a wave plans, with an odd number of the prefix's parts: the chunks' table behind them lies on 16 bytes."""
+    case = _case(dev, B, B, H, Hkv, D, P, [7 * i % 90 for i in range(B)], "bf16", extra=80)
+    _check(fa.decode_shared(*case), _want(case, "bf16"), "bf16")
