@@ -73,18 +73,18 @@ fa_weights_one_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k
   constexpr int STRIDE = kOnePages * kTokens + 4;
   __shared__ Shared<D, kOneWaves> sh;
   __shared__ __attribute__((aligned(16))) float scores[16 * STRIDE];
-  __shared__ float2 J[16];   // of a group's heads: reference, 1 / sum
+  __shared__ float2 J[16];   // of a group's heads: maximum, 1 / sum
   const int hk = blockIdx.x, b = blockIdx.y, G = H / Hkv;
   const int col = threadIdx.x & 15, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ctx = __builtin_amdgcn_readfirstlane(ctx_lens[b]), pages = pages_of(ctx, max_pages);
   const bool live = col < G;
   const int64_t row = (int64_t)b * H + hk * G + col;
-  const RowOut<D, BF16> out{o, lse, row};
+  const RowOut<D, BF16> out{o, lse, row, c};
   chunk_body<D, BF16, false>(sh, wave, q, k_pool, v_pool, Pages{page_table + (size_t)b * max_pages, ctx}, 0,
                              pages, ctx < 0 || (ctx > 0 && pages == 0), live, row * D, hk, Hkv, num_pages,
-                             c, ScoresKept{scores, STRIDE}, out, [&](float mc, float z) {
-                               out(mc, z);
-                               J[col] = make_float2(mc, 1.f / z);
+                             c, ScoresKept{scores, STRIDE}, out, [&](float m, float z) {
+                               out(m, z);
+                               J[col] = make_float2(m, 1.f / z);
                              });
   __syncthreads();
   const int width = max_pages * kPageSize, n = min(max(ctx, 0), width);
@@ -93,7 +93,7 @@ fa_weights_one_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k
     float w = w_in[at + j];
     if (j < n) {
       float sum = 0.f;
-      for (int g = 0; g < G; ++g) sum = fmaf(exp2_hw(fmaf(scores[g * STRIDE + j], c, -J[g].x)), J[g].y, sum);
+      for (int g = 0; g < G; ++g) sum = fmaf(exp2_hw((scores[g * STRIDE + j] - J[g].x) * c), J[g].y, sum);
       w += sum;
     }
     w_out[at + j] = w;
@@ -118,7 +118,7 @@ fa_weights_join_kernel(const float* __restrict__ part_o, const float2* __restric
     const int row = blockIdx.x, b = row / H;
     const int2 f = first_of[b];
     const Parts a{part_o, part_ml, (int64_t)f.x * H + (row - b * H), H, f.y};
-    join_row<D, BF16>(sh, a, Parts{part_o, part_ml, 0, 0, 0}, o + (int64_t)row * D, lse + row);
+    join_row<D, BF16>(sh, a, Parts{part_o, part_ml, 0, 0, 0}, c, o + (int64_t)row * D, lse + row);
     return;
   }
   const int unit = (int)blockIdx.x - rows;
@@ -136,14 +136,14 @@ fa_weights_join_kernel(const float* __restrict__ part_o, const float2* __restric
   f32x4 w = f32x4{};
   if (there) w = *reinterpret_cast<const f32x4*>(w_in + at);
   if (start < ctx) {
-    __shared__ float2 J[kJoinThreads];   // of a group's heads: reference, 1 / sum
+    __shared__ float2 J[kJoinThreads];   // of a group's heads: maximum, 1 / sum
     const int2 f = first_of[b];
     f32x4 sum = f32x4{};
     for (int g0 = 0; g0 < G; g0 += kJoinThreads) {
       const int gs = min(kJoinThreads, G - g0);
       if (g0 > 0) __syncthreads();
       for (int g = wave; g < gs; g += kJoinThreads / 64) {
-        const float2 x = join_wave(Parts{part_o, part_ml, (int64_t)f.x * H + hk * G + g0 + g, H, f.y});
+        const float2 x = join_wave(Parts{part_o, part_ml, (int64_t)f.x * H + hk * G + g0 + g, H, f.y}, c);
         if ((tid & 63) == 0) J[g] = make_float2(x.x, 1.f / x.y);
       }
       __syncthreads();
@@ -154,7 +154,7 @@ fa_weights_join_kernel(const float* __restrict__ part_o, const float2* __restric
           const f32x4 x = *reinterpret_cast<const f32x4*>(sc + g * width);
           const float2 Jg = J[g];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) sum[i] = fmaf(exp2_hw(fmaf(x[i], c, -Jg.x)), Jg.y, sum[i]);
+          for (int i = 0; i < 4; ++i) sum[i] = fmaf(exp2_hw((x[i] - Jg.x) * c), Jg.y, sum[i]);
         }
       }
     }

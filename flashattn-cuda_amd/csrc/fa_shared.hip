@@ -8,7 +8,7 @@
 // share a KV head, B * H / H_kv of them, form one product with them, as in a
 // forward pass without a mask. Few rows (kFewRows) go through the chunks of
 // fa_stream.hpp instead, as the own pages do, and in their launch. One launch joins
-// the partials of both by their references and sums.
+// the partials of both by their maxima and sums.
 #include <hip/hip_runtime.h>
 
 #include <math.h>
@@ -30,6 +30,7 @@ constexpr int kCus = 256, kMostUnits = 192;   // units: of the prefix pass in ti
 constexpr int kTile = 64;     // keys of a tile: 4 pages
 constexpr int kStages = 4;    // tiles in LDS, three of them in flight
 constexpr float kSlack = 8.f;   // of weights' exponents; see its use
+constexpr float kFar = 4096.f;  // scores, in units of log 2, from which on differences are scaled; see m
 constexpr int kKeyGroups = 2; // waves side by side over the keys of a tile
 constexpr int kRowGroups = 4, kTileRows = 32 * kRowGroups;   // and over the query rows of a unit
 constexpr int kTileWaves = kKeyGroups * kRowGroups;
@@ -40,7 +41,7 @@ struct TileShared {
   static constexpr int kPage = kTokens * D * 2;
   static constexpr int kStage = 2 * (kTile / kTokens) * kPage;   // K, then V
   __attribute__((aligned(1024))) char ring[kStages * kStage];
-  float m[kTileWaves][64], l[kTileWaves][64];
+  float m[kTileWaves][64], l[kTileWaves][64], over[kTileWaves][64];
   int bad;
 };
 
@@ -136,7 +137,14 @@ tile_unit(TileShared<D>& sh, const int unit, const f16* __restrict__ q, const f1
     }
   };
 
-  float mc = -INFINITY, l = 0.f;   // reference of the weights, in units of log 2; their sum
+  // Reference of the weights, as K Q^T gives it (-inf: no score yet), and their sum. A weight is
+  // 2^(s c - mu), mu the scaled reference, rounded: all of a row are off by the same 2^rest, which
+  // the sum is freed of. Where a row of the wave has |mu| >= kFar the reference is taken off the
+  // scores first, which is exact however large they are (a mu of 2^27 is rounded by 2^3, of 2^31 by
+  // 2^7, past all types); always done, a tile pass of 28.8 us takes 29.4, and 46.3 at D = 64 49.3.
+  float m = -INFINITY, l = 0.f, mu = 0.f;
+  bool far = false;   // the same in the whole wave
+  const auto rest = [&](float m, float mu, bool far) { return far || m == -INFINITY ? 0.f : fmaf(m, c, -mu); };
   f32x16 o[DB];
 #pragma unroll
   for (int db = 0; db < DB; ++db) o[db] = f32x16{};
@@ -168,21 +176,30 @@ tile_unit(TileShared<D>& sh, const int unit, const f16* __restrict__ q, const f1
     float mx = sc[0];
 #pragma unroll
     for (int r = 1; r < 16; ++r) mx = fmaxf(mx, sc[r]);
-    mx = max_xor32(mx) * c;
+    mx = max_xor32(mx);
     // The reference follows the maximum only where that is kSlack above it: of 32 rows
     // one has a new maximum in most steps (64 sequences under 32768: a call 83 us without,
     // 75 with). Weights reach 2^kSlack, far from the types' ends.
-    if (__any(mx > mc + kSlack)) {
-      const float m_new = fmaxf(mc, mx);
-      const float alpha = m_new == mc ? 1.f : exp2_hw(mc - m_new);
+    if (__any((mx - m) * c > kSlack)) {   // of -inf and -inf a NaN: no
+      const float m_new = fmaxf(m, mx);
+      const bool far_new = __any(m_new != -INFINITY && fabsf(m_new) * c >= kFar);
+      const float mu_new = far_new || m_new == -INFINITY ? 0.f : m_new * c;
+      const float alpha = m == -INFINITY ? 1.f : exp2_hw((m - m_new) * c + (rest(m_new, mu_new, far_new) - rest(m, mu, far)));
       l *= alpha;
 #pragma unroll
       for (int db = 0; db < DB; ++db)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
-      mc = m_new;
+      m = m_new;
+      mu = mu_new;
+      far = far_new;
     }
-    const float mu = mc == -INFINITY ? 0.f : mc;   // no score above -inf so far: weights of 0
+    if (far) {            // wave-uniform
+      asm volatile("");   // a branch: not selects in every step
+      const float by = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sc[r] -= by;
+    }
     __builtin_amdgcn_sched_barrier(0);
     const uint32_t vb = col_base<D>(lds0 + (k % kStages) * STAGE + PAGES * PAGE + kg * (32 * 2 * D), lane);
     f16x8 vf[2][DB];
@@ -194,7 +211,7 @@ tile_unit(TileShared<D>& sh, const int unit, const f16* __restrict__ q, const f1
     f32x16 sn;
     if constexpr (decltype(next)::value) sn = scores();
 #pragma unroll
-    for (int r = 0; r < 16; ++r) sc[r] = exp2_hw(fmaf(sc[r], c, -mu));
+    for (int r = 0; r < 16; ++r) sc[r] = exp2_hw(fmaf(sc[r], c, -mu));   // of -inf, with no reference too: 0
     f16x8 p[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) p[j] = pack_px<BF16>(sc, j);
@@ -230,6 +247,7 @@ tile_unit(TileShared<D>& sh, const int unit, const f16* __restrict__ q, const f1
     if (some) step(n - 1, sc, std::false_type{});
   }
   l = sum_xor32(l);
+  const float over = exp2_hw(-rest(m, mu, far));   // of the weights that reach the sum and the products
 
   // Merge the two key groups through LDS, each for half of the columns: a wave
   // leaves the other's half register by register, lanes of the two hold the same
@@ -245,24 +263,26 @@ tile_unit(TileShared<D>& sh, const int unit, const f16* __restrict__ q, const f1
     for (int h = 0; h < HB; ++h)
 #pragma unroll
       for (int r = 0; r < 16; ++r) to[(h * 16 + r) * 64 + lane] = kg == 0 ? o[HB + h][r] : o[h][r];
-    sh.m[wave][lane] = mc;
+    sh.m[wave][lane] = m;
     sh.l[wave][lane] = l;
+    sh.over[wave][lane] = over;
   }
   __syncthreads();
   const int other = wave ^ 1;   // the same rows, the other keys
-  const float m1 = sh.m[other][lane], M = fmaxf(mc, m1);
-  const float e0 = mc == -INFINITY ? 0.f : exp2_hw(mc - M), e1 = m1 == -INFINITY ? 0.f : exp2_hw(m1 - M);
+  const float m1 = sh.m[other][lane], M = fmaxf(m, m1);
+  const float e0 = m == -INFINITY ? 0.f : exp2_hw((m - M) * c) * over;
+  const float e1 = m1 == -INFINITY ? 0.f : exp2_hw((m1 - M) * c) * sh.over[other][lane];
   const float z = e0 * l + e1 * sh.l[other][lane];
   const bool nan = sh.bad || z != z;
   const float inv = nan ? NAN : (z > 0.f ? 1.f / z : 0.f);
   const float f0 = e0 * inv, f1 = e1 * inv;
   float v[HB][16];
-  const float* from = area + other * XCH;
+  const float* theirs = area + other * XCH;
 #pragma unroll
   for (int h = 0; h < HB; ++h)
 #pragma unroll
     for (int r = 0; r < 16; ++r)
-      v[h][r] = f0 * (kg == 0 ? o[h][r] : o[HB + h][r]) + f1 * from[(h * 16 + r) * 64 + lane];
+      v[h][r] = f0 * (kg == 0 ? o[h][r] : o[HB + h][r]) + f1 * theirs[(h * 16 + r) * 64 + lane];
   __syncthreads();
   // Through LDS once more, rows of the wave's half in a row: 32 rows of D / 2 (and 4
   // words, for the banks), stored a row's 2 D bytes at a time.
@@ -429,7 +449,7 @@ fa_shared_one_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_
   const int np = pages_of(P, prefix_pages), own = pages_of(ctx, max_pages);
   const bool bad = P < 0 || (P > 0 && np == 0) || ctx < 0 || (ctx > 0 && own == 0);
   const int64_t row = (int64_t)b * H + hk * group + 16 * sub + col;
-  const RowOut<D, BF16> out{o, lse, row};
+  const RowOut<D, BF16> out{o, lse, row, c};
   chunk_body<D, BF16, false>(sh, wave, q, k_pool, v_pool,
                              JoinedPages{prefix_table, page_table + (size_t)b * max_pages, np, P, ctx}, 0,
                              np + own, bad, 16 * sub + col < group, row * D, hk, Hkv, num_pages, c,
@@ -444,13 +464,13 @@ fa_shared_join_kernel(const float* __restrict__ pre_o, const float2* __restrict_
                       const float* __restrict__ own_o, const float2* __restrict__ own_ml,
                       const int2* __restrict__ first, const int* __restrict__ splits,
                       const int32_t* __restrict__ prefix_len, uint16_t* __restrict__ o,
-                      float* __restrict__ lse, int H, int rows, int SP, int few, int prefix_pages) {
+                      float* __restrict__ lse, int H, int rows, int SP, int few, int prefix_pages, float c) {
   __shared__ JoinShared<D> sh;
   const int row = blockIdx.x, b = row / H;
   const int2 f = first[b];
   const int n = few ? prefix_splits(prefix_len[0], prefix_pages, SP) : *splits;
   const Parts pre = few ? Parts{pre_o, pre_ml, row, rows, n} : Parts{pre_o, pre_ml, (int64_t)row * SP, 1, n};
-  join_row<D, BF16>(sh, pre, Parts{own_o, own_ml, (int64_t)f.x * H + (row - b * H), H, f.y},
+  join_row<D, BF16>(sh, pre, Parts{own_o, own_ml, (int64_t)f.x * H + (row - b * H), H, f.y}, c,
                     o + (int64_t)row * D, lse + row);
 }
 
@@ -553,7 +573,7 @@ static int launch(const Cut& p, const void* q, const void* k_pool, const void* v
   }
   hipLaunchKernelGGL((fa_shared_join_kernel<D, BF16>), dim3((unsigned)(B * H)), dim3(kJoinThreads), 0, s,
                      ws, pre_ml, own_o, own_ml, first, splits, prefix_len, (uint16_t*)o, lse, (int)H, (int)(B * H),
-                     p.sp, (int)p.few, (int)prefix_pages);
+                     p.sp, (int)p.few, (int)prefix_pages, c);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? FA_OK : -(int)e;
 }

@@ -1,6 +1,6 @@
 // fa_stream.hpp — decode attention over runs of 16-bit pages, for the kernels
 // that run it: one query token per sequence, cut into chunks of pages that a
-// later launch joins by their references and sums (see chunk_body), or, of short
+// later launch joins by their maxima and sums (see chunk_body), or, of short
 // sequences, whole.
 //
 // Bound by memory: a page of 16 tokens of one KV head is 32 D bytes each of K and
@@ -15,8 +15,9 @@
 // 219). Lane l has query row l % 16 in both products, so a row's maximum and sum stay
 // in its lane column.
 //
-// Maxima are kept as K Q^T gives them and differences are scaled, so that no
-// weight passes 1 however large the scores are. P goes into its product as two
+// Maxima are kept as K Q^T gives them, in the partials and the joins too, and differences
+// are scaled, so that no weight passes 1 however large the scores are: a scaled maximum
+// of 2^31 is rounded by up to 2^7, a factor of 2^128. P goes into its product as two
 // 16-bit terms, rounded and then what that leaves out (22 bits in fp16, 16 in
 // bf16), beside a sum of P that is not rounded.
 #pragma once
@@ -365,9 +366,8 @@ struct ScoresKept {
 // One chunk by WAVES waves, `wave` their number: places p0 .. p1 - 1 of the pages, for
 // up to 16 query rows. Column col of the products is the query row at element qoff of
 // q (live: there is one). At the end row(d, v) is called for its dims d .. d + 3,
-// normalised, by some lane of the column, and stat(reference, sum) by one: of the
-// weights, in units of log 2; (-inf, 0) of no tokens, a NaN sum where a page or the
-// length (bad) is invalid. NT: pages are read with the non-temporal hint. Has one
+// normalised, by some lane of the column, and stat(maximum, sum of the weights) by one:
+// (-inf, 0) of no tokens, a NaN sum where a page or the length (bad) is invalid. NT: pages are read with the non-temporal hint. Has one
 // barrier of the workgroup, so waves without a chunk call it too, with no pages and no
 // live row.
 template <int D, bool BF16, bool NT, int WAVES, typename Where, typename Scores, typename Row, typename Stat>
@@ -586,9 +586,7 @@ chunk_body(Shared<D, WAVES>& sh, const int wave, const uint16_t* __restrict__ q,
     for (int j = 0; j < 4; ++j) a[j] *= inv;
     row(d, a);
   }
-  // The reference is the scaled maximum, rounded; the sum takes up what that left.
-  const float mc = M * c;
-  if (wave == 0 && grp == 0) stat(mc, mc == -INFINITY ? z : z * exp2_hw(fmaf(M, c, -mc)));
+  if (wave == 0 && grp == 0) stat(M, z);
 }
 
 // row and stat of chunk_body: partial number `part`, part_o[part * D ..] and
@@ -599,19 +597,22 @@ struct PartOut {
   float2* ml;
   int64_t part;
   __device__ void operator()(int d, f32x4 a) const { *reinterpret_cast<f32x4*>(o + part * D + d) = a; }
-  __device__ void operator()(float mc, float z) const { ml[part] = make_float2(mc, z); }
+  __device__ void operator()(float m, float z) const { ml[part] = make_float2(m, z); }
 };
+// L from the maximum of the products K Q^T and the sum of the weights.
+__device__ __forceinline__ float lse_of(float m, float z, float c) {
+  return z == 0.f ? -INFINITY : fmaf(m, c, log2_hw(z)) * kLn2;
+}
 template <int D, bool BF16>
 struct RowOut {
   uint16_t* o;
   float* lse;
   int64_t row;
+  float c;
   __device__ void operator()(int d, f32x4 a) const {
     *reinterpret_cast<u32x2*>(o + row * D + d) = u32x2{pack2<BF16>(a[0], a[1]), pack2<BF16>(a[2], a[3])};
   }
-  __device__ void operator()(float mc, float z) const {
-    lse[row] = z == 0.f ? -INFINITY : (mc + log2_hw(z)) * kLn2;
-  }
+  __device__ void operator()(float m, float z) const { lse[row] = lse_of(m, z, c); }
 };
 
 // Partials of one row: number at + i * stride, i < n.
@@ -632,21 +633,21 @@ struct JoinShared {
   float acc[4 * kJoinThreads / D][D];
 };
 
-// Reference and sum over a row's parts, for the whole wave: (-inf, 0) of empty
+// Maximum and sum over a row's parts, for the whole wave: (-inf, 0) of empty
 // ones, a NaN sum where one is.
-__device__ __forceinline__ float2 join_wave(const Parts& p) {
+__device__ __forceinline__ float2 join_wave(const Parts& p, float c) {
   const int lane = threadIdx.x & 63;
   float M = -INFINITY, z = 0.f;
   for (int i = lane; i < p.n; i += 64) {
     const float2 x = p.ml[p.at + i * p.stride];
     if (x.x > M) {
-      z *= exp2_hw(M - x.x);   // M = -inf: z is 0 or NaN
+      z *= exp2_hw((M - x.x) * c);   // M = -inf: z is 0 or NaN
       M = x.x;
     }
-    z += x.x == -INFINITY ? x.y : x.y * exp2_hw(x.x - M);
+    z += x.x == -INFINITY ? x.y : x.y * exp2_hw((x.x - M) * c);
   }
   const float top = wave_max(M);
-  return make_float2(top, wave_sum(M == -INFINITY ? z : z * exp2_hw(M - top)));
+  return make_float2(top, wave_sum(M == -INFINITY ? z : z * exp2_hw((M - top) * c)));
 }
 
 // O and L of one row out of two lists of parts, by one workgroup; sums in a fixed
@@ -654,7 +655,7 @@ __device__ __forceinline__ float2 join_wave(const Parts& p) {
 // to 16 parts 5.2 us (5.7 with shuffles over LDS for the wave's maxima and sums). Parts
 // asked for before their weights, one, two or four a thread: 5.5, 6.1, 6.6.
 template <int D, bool BF16>
-__device__ __forceinline__ void join_row(JoinShared<D>& sh, const Parts& a, const Parts& b,
+__device__ __forceinline__ void join_row(JoinShared<D>& sh, const Parts& a, const Parts& b, float c,
                                          uint16_t* __restrict__ o, float* __restrict__ lse) {
   constexpr int PER = D / 4, SIDE = kJoinThreads / PER, WAVES = kJoinThreads / 64;
   const int tid = threadIdx.x, wave = tid >> 6;
@@ -680,7 +681,7 @@ __device__ __forceinline__ void join_row(JoinShared<D>& sh, const Parts& a, cons
     if (i0 > 0) __syncthreads();
     for (int i = tid; i < m; i += kJoinThreads) {
       const float2 x = i0 + i < kJoinThreads ? mine : ml(i0 + i);   // an empty part: (-inf, 0), or NaN
-      const float e = x.x == -INFINITY ? x.y : x.y * exp2_hw(x.x - M);
+      const float e = x.x == -INFINITY ? x.y : x.y * exp2_hw((x.x - M) * c);
       sh.w[i] = e;
       z += e;
     }
@@ -708,7 +709,7 @@ __device__ __forceinline__ void join_row(JoinShared<D>& sh, const Parts& a, cons
     for (int r = 0; r < 4; ++r) v[r] += sh.acc[i][d + r];
   const float inv = z == 0.f ? 0.f : 1.f / z;   // a NaN sum: NaN
   *reinterpret_cast<u32x2*>(o + d) = u32x2{pack2<BF16>(v[0] * inv, v[1] * inv), pack2<BF16>(v[2] * inv, v[3] * inv)};
-  if (tid == 0) *lse = z == 0.f ? -INFINITY : (M + log2_hw(z)) * kLn2;
+  if (tid == 0) *lse = lse_of(M, z, c);
 }
 
 }  // namespace stream

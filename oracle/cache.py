@@ -42,6 +42,31 @@ def attend(q, k, v, half):
     return o, lse, p, tol_o, rel + 2.0 ** -22 * np.abs(lse), p * rel[:, None] + 2.0 ** -30
 
 
+def attend_exact(s, v, half, p_half):
+    """attend() for products s [G, n] = q k that the kernels have exactly, whatever their size: what bounds the weights
+    are the differences to the largest, x = (s - max) / sqrt(D) in units of log 2, not the scores. With u = 2^-24:
+
+    - the scale is off by 3 u, its product with the difference and a sum with a constant by u each, an exponential by
+      2 u, where a weight is taken in parts (in its wave, up to eight new maxima, waves, chunks, 32 lanes of a join) each
+      of them and a product: u (5 |x| + 80) in all;
+    - a sum of n weights, and of n products, in up to 16 parts: (n / 16 + 64) u;
+    - P is off by p_half of itself, or 2^-25 of the largest below fp16's normal numbers; O by half of itself.
+    """
+    D, u = v.shape[-1], 2.0 ** -24
+    m = s.max(1, keepdims=True)
+    x = (s - m) / np.sqrt(D) / np.log(2)
+    e = np.exp2(x)
+    z = e.sum(1, keepdims=True)
+    p = e / z
+    o, lse = p @ v, (m / np.sqrt(D) + np.log(z))[:, 0]
+    rel = p * u * (5 * np.abs(np.maximum(x, -200)) + 80)
+    adds = (s.shape[1] / 16 + 64) * u
+    w = rel.sum(1, keepdims=True) + adds
+    av = p @ np.abs(v)
+    tol_o = rel @ np.abs(v) + (w + half) * np.abs(o) + (adds + p_half) * av + 2.0 ** -25 * (np.abs(v).sum(0) / z + 1)
+    return o, lse, p, tol_o, w[:, 0] + 8 * u * np.abs(lse), rel + p * w + 2.0 ** -126
+
+
 def decode_shared(q, k_pool, v_pool, prefix, prefix_len, table, ctx, half):
     """(o [B, H, D], lse [B, H], tol_o, tol_l)."""
     B, H, D = q.shape

@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from oracle import cache, rotary
-from test_shared_gpu import HALF, TYPES, _case, _check, _i32
+from test_shared_gpu import HALF, HUGE, TYPES, _case, _check, _huge_scores, _i32
 
 pytestmark = pytest.mark.gpu
 
@@ -372,3 +372,32 @@ def test_a_budget_as_used(fa, dev):
     # twelve steps' weights, each off by less than 2.1 times a score's error (above, 0.05 here) of itself
     err = np.abs(_f64(weights) - plain)
     assert (err <= 0.1 * np.maximum(plain, 1e-6) + 1e-6).all()
+
+
+@pytest.mark.parametrize("ctx,wide", [([1], 0), ([2, 17, 0, 500], 0), ([3000, 33, 1100], 0), ([333, 5], 40), ([20000], 0)])
+@pytest.mark.parametrize("D,dtype", [(64, "fp16"), (128, "fp16"), (64, "bf16"), (128, "bf16")])
+def test_weights_huge_scores(fa, dev, D, dtype, ctx, wide):
+    """Scores (in units of log 2) of 2^17 to 2^33 in fp16 and to 2^90 in bf16, of both signs: O, L and the weights follow from the
+    scores' differences."""
+    b, qs = HUGE[dtype]
+    B = len(ctx)
+    q, kp, vp, _, _, table, c = _huge_scores(_case(dev, B, B, 16, 2, D, 0, ctx, dtype, extra=wide), b, qs)
+    w = torch.rand((B, 2, 16 * table.shape[1]), device=dev)
+    got = fa.decode_paged_weights(q, kp, vp, table, c, w)
+    qf, kf, vf, tf, want = [_f64(x) for x in (q, kp, vp, table, w)]
+    res = [np.zeros((B, 16, D)), np.full((B, 16), -np.inf), np.zeros((B, 16, D)), np.zeros((B, 16))]
+    tw = np.zeros(want.shape)
+    for i, n in enumerate(ctx):
+        for h in range(2 if n else 0):
+            g = slice(8 * h, 8 * h + 8)
+            k, v = (cache.rows(x, tf[i, :-(-n // 16)], n, h) for x in (kf, vf))
+            s = qf[i, g] @ k.T
+            assert np.array_equal(s.astype(np.float32), s)
+            o, l, p, to, tl, tp = cache.attend_exact(s, v, HALF[dtype], HALF[dtype] ** 2)
+            for x, y in zip(res, (o, l, to, tl)):
+                x[i, g] = y
+            want[i, h, :n] += p.sum(0)
+            tw[i, h, :n] = tp.sum(0) + 9 * 2.0 ** -24 * want[i, h, :n]   # the sum's roundings
+    _check(got[:2], res, dtype, f"{ctx}")
+    err = np.abs(_f64(got[2]) - want)
+    assert (err <= tw).all(), f"{ctx} W: worst {np.nanmax(err / np.maximum(tw, 1e-300)):.2f} of the bound, {np.isnan(err).sum()} NaN"

@@ -279,3 +279,95 @@ def test_odd_batch_planned_on_the_device(fa, dev, B, H, Hkv, D, P):
     """More sequences than a wave plans, with an odd number of the prefix's parts: the chunks' table behind them lies on 16 bytes."""
     case = _case(dev, B, B, H, Hkv, D, P, [7 * i % 90 for i in range(B)], "bf16", extra=80)
     _check(fa.decode_shared(*case), _want(case, "bf16"), "bf16")
+
+
+STEPS = np.array([0, 1, 2, 3, 4, 6, 8, 12]) / 8   # numbers that both types hold beside a power of two
+
+
+def _huge_scores(case, b, qs):
+    """The case with products of q and k far beyond 2^24, as rows of one KV head per b and query heads per (b, a): every value
+    of a K row is b but the first, b f with f of STEPS; every value of a query is a but the first, which makes the products
+    a b (D - 1) +- 8 f g with g the last place of the product in 32 bits, so that each is a number of 24 bits and any
+    order of its sum is exact. Slots that no sequence has keep their NaN."""
+    q, kp, vp = case[:3]
+    D, dt = q.shape[-1], q.dtype
+    rng = np.random.default_rng(3)
+    f = torch.from_numpy(rng.choice(STEPS, (kp.shape[0], 16))).to(kp.device)
+    k = torch.tensor(b, dtype=torch.float64, device=kp.device)[None, :, None, None].expand(kp.shape[0], -1, 16, D).clone()
+    k[..., 0] *= f[:, None]
+    kp.copy_(torch.where(torch.isnan(kp), kp.double(), k))
+    for h in range(q.shape[1]):
+        bh, a = b[h // len(qs)], qs[h % len(qs)]
+        g = 2.0 ** (math.floor(math.log2(D * abs(a) * bh)) - 23)
+        q[:, h] = a
+        q[:, h, 0] = 8 * g / bh * (1 if h % 2 else -1)
+        assert float(q[0, h, 1]) == a and abs(float(q[0, h, 0])) == 8 * g / bh
+    return case
+
+
+HUGE = {"fp16": ([1024.0, 16384.0], [512.0, 1023.0, -2047.0, -1024.0, 16384.0, 4096.0, -640.0, 8192.0]),
+        "bf16": ([1024.0, 2.0 ** 45], [512.0, 1020.0, -2040.0, -2.0 ** 41, 1.5, 2.0 ** 20, -96.0, 2.0 ** 30])}
+
+
+@pytest.mark.parametrize("B,P,ctx,wide", [(2, 200, [9, 0], 0), (2, 700, [50, 333], 80), (6, 700, [50, 0, 333, 5, 1, 17], 80),
+                                          (17, 3000, [7 * i for i in range(17)], 80), (40, 257, [i % 30 for i in range(40)], 80)])
+@pytest.mark.parametrize("D,dtype", [(64, "fp16"), (128, "fp16"), (64, "bf16"), (128, "bf16")])
+def test_huge_scores(fa, dev, D, dtype, B, P, ctx, wide):
+    """Scores (in units of log 2) of 2^17 to 2^33 in fp16 and to 2^90 in bf16, of both signs: the weights follow from the scores'
+    differences. 16 to 320 query rows of a KV head: one launch, chunks, and tiles."""
+    b, qs = HUGE[dtype]
+    case = _huge_scores(_case(dev, B + P, B, 16, 2, D, P, ctx, dtype, extra=wide), b, qs)
+    O, L = fa.decode_shared(*case)
+    # weights of a prefix in tiles have the type's bits; the others' two terms keep more, within the same bound
+    _check((O, L), _want_exact(case, HALF[dtype], HALF[dtype]), dtype, f"B {B}")
+
+
+def _want_exact(case, half, p_half):
+    """_want() of a case whose products of q and k the kernels have exactly."""
+    q, kp, vp, prefix, plen, table, ctx = [x.cpu().double().numpy() for x in case]
+    B, H, D = q.shape
+    Hkv = kp.shape[1]
+    G = H // Hkv
+    want = [np.zeros((B, H, D)), np.zeros((B, H)), np.zeros((B, H, D)), np.zeros((B, H))]
+    for b in range(B):
+        P, n = int(plen[0]), int(ctx[b])
+        for h in range(Hkv):
+            g = slice(G * h, G * h + G)
+            k, v = (np.concatenate([cache.rows(x, prefix, P, h), cache.rows(x, table[b, :-(-n // 16)], n, h)]) for x in (kp, vp))
+            s = q[b, g] @ k.T
+            assert np.array_equal(s.astype(np.float32), s)
+            o, l, _, to, tl, _ = cache.attend_exact(s, v, half, p_half)
+            for x, y in zip(want, (o, l, to, tl)):
+                x[b, g] = y
+    return want
+
+
+def _climbing_scores(case):
+    """Products of q and k that rise along a sequence's keys, prefix and then own, from below -A 256 to A 256, A from 1/16 to 512 and of
+    both signs, with up to 16 beside that: multiples of 1/16 below 2^18, so each is a number of 24 bits and exact."""
+    q, kp, vp, prefix, plen, table, ctx = case
+    P, H, dev = int(plen), q.shape[1], q.device
+    total = P + int(ctx.max())
+    rng = np.random.default_rng(5)
+    k0 = lambda at: torch.from_numpy(np.floor(at / total * 512) - 256).to(dev, kp.dtype)
+    for ids, first, n in [(prefix, 0, P)] + [(t, P, int(n)) for t, n in zip(table, ctx)]:
+        for j in range(-(-n // 16)):
+            m = min(16, n - 16 * j)
+            page = int(ids[j])
+            kp[page, :, :m, 0] = k0(first + 16 * j + np.arange(m))
+            kp[page, :, :m, 1] = torch.from_numpy(rng.integers(0, 256, (kp.shape[1], m))).to(dev, kp.dtype)
+    q.zero_()
+    scale = torch.tensor([64, -64, 1, -1 / 16, 512, -512, 0.25, 16], device=dev, dtype=q.dtype)
+    q[..., 0] = scale[torch.arange(H, device=dev) % 8]
+    q[..., 1] = 1 / 16
+    return case
+
+
+@pytest.mark.parametrize("B,H,Hkv,P,ctx,wide", [(2, 8, 1, 300, [20, 9], 0), (3, 8, 1, 2500, [300, 0, 77], 80), (40, 8, 2, 2500, [3 * i for i in range(40)], 80),
+                                                (40, 8, 1, 9000, [i % 7 for i in range(40)], 0), (9, 32, 4, 700, [600 - i for i in range(9)], 80)])
+@pytest.mark.parametrize("D,dtype", [(64, "fp16"), (128, "fp16"), (64, "bf16"), (128, "bf16")])
+def test_climbing_scores(fa, dev, D, dtype, B, H, Hkv, P, ctx, wide):
+    """The maximum moves along the keys, by less and by more than the weights' slack, from far scores over near ones to far ones,
+    in rows side by side: one launch, chunks, and tiles."""
+    case = _climbing_scores(_case(dev, P, B, H, Hkv, D, P, ctx, dtype, extra=wide))
+    _check(fa.decode_shared(*case), _want_exact(case, HALF[dtype], HALF[dtype]), dtype, f"B {B}")
