@@ -30,6 +30,10 @@ constexpr int kCus = 256, kMostUnits = 192;   // units: of the prefix pass in ti
 constexpr int kTile = 64;     // keys of a tile: 4 pages
 constexpr int kStages = 4;    // tiles in LDS, three of them in flight
 constexpr float kSlack = 8.f;   // of weights' exponents; see its use
+// Of bf16 the slack is above the reference and not below it: its V reach 2^127, which a
+// weight above 1 would take out of range, while fp16's weights have no bits to lose at the lower end.
+template <bool BF16>
+constexpr float kShift = BF16 ? kSlack : 0.f;
 constexpr float kFar = 4096.f;  // scores, in units of log 2, from which on differences are scaled; see m
 constexpr int kKeyGroups = 2; // waves side by side over the keys of a tile
 constexpr int kRowGroups = 4, kTileRows = 32 * kRowGroups;   // and over the query rows of a unit
@@ -138,13 +142,15 @@ tile_unit(TileShared<D>& sh, const int unit, const f16* __restrict__ q, const f1
   };
 
   // Reference of the weights, as K Q^T gives it (-inf: no score yet), and their sum. A weight is
-  // 2^(s c - mu), mu the scaled reference, rounded: all of a row are off by the same 2^rest, which
-  // the sum is freed of. Where a row of the wave has |mu| >= kFar the reference is taken off the
+  // 2^(s c - mu), mu the scaled reference and kShift, rounded: all of a row are off by the same
+  // 2^rest, which the sums are freed of. Where a row of the wave has |mu| >= kFar the reference is taken off the
   // scores first, which is exact however large they are (a mu of 2^27 is rounded by 2^3, of 2^31 by
   // 2^7, past all types); always done, a tile pass of 28.8 us takes 29.4, and 46.3 at D = 64 49.3.
   float m = -INFINITY, l = 0.f, mu = 0.f;
   bool far = false;   // the same in the whole wave
-  const auto rest = [&](float m, float mu, bool far) { return far || m == -INFINITY ? 0.f : fmaf(m, c, -mu); };
+  const auto rest = [&](float m, float mu, bool far) {
+    return m == -INFINITY ? 0.f : (far ? -kShift<BF16> : fmaf(m, c, -mu));
+  };
   f32x16 o[DB];
 #pragma unroll
   for (int db = 0; db < DB; ++db) o[db] = f32x16{};
@@ -179,11 +185,11 @@ tile_unit(TileShared<D>& sh, const int unit, const f16* __restrict__ q, const f1
     mx = max_xor32(mx);
     // The reference follows the maximum only where that is kSlack above it: of 32 rows
     // one has a new maximum in most steps (64 sequences under 32768: a call 83 us without,
-    // 75 with). Weights reach 2^kSlack, far from the types' ends.
+    // 75 with). fp16's weights reach 2^kSlack, bf16's 1.
     if (__any((mx - m) * c > kSlack)) {   // of -inf and -inf a NaN: no
       const float m_new = fmaxf(m, mx);
       const bool far_new = __any(m_new != -INFINITY && fabsf(m_new) * c >= kFar);
-      const float mu_new = far_new || m_new == -INFINITY ? 0.f : m_new * c;
+      const float mu_new = far_new || m_new == -INFINITY ? kShift<BF16> : fmaf(m_new, c, kShift<BF16>);
       const float alpha = m == -INFINITY ? 1.f : exp2_hw((m - m_new) * c + (rest(m_new, mu_new, far_new) - rest(m, mu, far)));
       l *= alpha;
 #pragma unroll
@@ -270,7 +276,7 @@ tile_unit(TileShared<D>& sh, const int unit, const f16* __restrict__ q, const f1
   __syncthreads();
   const int other = wave ^ 1;   // the same rows, the other keys
   const float m1 = sh.m[other][lane], M = fmaxf(m, m1);
-  const float e0 = m == -INFINITY ? 0.f : exp2_hw((m - M) * c) * over;
+  const float e0 = m == -INFINITY ? 0.f : exp2_hw((m - M) * c) * over;   // over: 2^(kSlack + 1/2) at most
   const float e1 = m1 == -INFINITY ? 0.f : exp2_hw((m1 - M) * c) * sh.over[other][lane];
   const float z = e0 * l + e1 * sh.l[other][lane];
   const bool nan = sh.bad || z != z;

@@ -574,6 +574,8 @@ chunk_body(Shared<D, WAVES>& sh, const int wave, const uint16_t* __restrict__ q,
   }
   if (any_bad) z = NAN;
   const float inv = z == 0.f ? 0.f : 1.f / z;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) e[w] *= inv;   // before the sums: bf16's V reaches 2^127
   for (int d = 4 * (4 * wave + grp); d < D; d += 16 * WAVES) {
     f32x4 a = f32x4{};
 #pragma unroll
@@ -582,8 +584,6 @@ chunk_body(Shared<D, WAVES>& sh, const int wave, const uint16_t* __restrict__ q,
 #pragma unroll
       for (int j = 0; j < 4; ++j) a[j] = fmaf(e[w], v[j], a[j]);
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) a[j] *= inv;
     row(d, a);
   }
   if (wave == 0 && grp == 0) stat(M, z);
@@ -650,6 +650,13 @@ __device__ __forceinline__ float2 join_wave(const Parts& p, float c) {
   return make_float2(top, wave_sum(M == -INFINITY ? z : z * exp2_hw((M - top) * c)));
 }
 
+// Parts are joined by 2^-kJoinShift of their sums, which add up to as many as there are tokens (2^8
+// times that of tiles): V near bf16's end that a part's own sums hold, of a 2^14th of the tokens at
+// least, stay in range. At the lower end a V of 2^-118 is 2^-16 off. Weights that add up to 1
+// would wait for their sum: 2048 rows 5.0 -> 5.9 us.
+template <bool BF16>
+constexpr float kJoinShift = BF16 ? 16.f : 0.f;
+
 // O and L of one row out of two lists of parts, by one workgroup; sums in a fixed
 // order. Bound by the chain of a launch, the parts' weights and the parts: 2048 rows of 10
 // to 16 parts 5.2 us (5.7 with shuffles over LDS for the wave's maxima and sums). Parts
@@ -681,7 +688,7 @@ __device__ __forceinline__ void join_row(JoinShared<D>& sh, const Parts& a, cons
     if (i0 > 0) __syncthreads();
     for (int i = tid; i < m; i += kJoinThreads) {
       const float2 x = i0 + i < kJoinThreads ? mine : ml(i0 + i);   // an empty part: (-inf, 0), or NaN
-      const float e = x.x == -INFINITY ? x.y : x.y * exp2_hw((x.x - M) * c);
+      const float e = x.x == -INFINITY ? x.y : x.y * exp2_hw(fmaf(x.x - M, c, -kJoinShift<BF16>));
       sh.w[i] = e;
       z += e;
     }
@@ -709,7 +716,7 @@ __device__ __forceinline__ void join_row(JoinShared<D>& sh, const Parts& a, cons
     for (int r = 0; r < 4; ++r) v[r] += sh.acc[i][d + r];
   const float inv = z == 0.f ? 0.f : 1.f / z;   // a NaN sum: NaN
   *reinterpret_cast<u32x2*>(o + d) = u32x2{pack2<BF16>(v[0] * inv, v[1] * inv), pack2<BF16>(v[2] * inv, v[3] * inv)};
-  if (tid == 0) *lse = lse_of(M, z, c);
+  if (tid == 0) *lse = lse_of(M, z * exp2_hw(kJoinShift<BF16>), c);
 }
 
 }  // namespace stream

@@ -401,3 +401,22 @@ def test_weights_huge_scores(fa, dev, D, dtype, ctx, wide):
     _check(got[:2], res, dtype, f"{ctx}")
     err = np.abs(_f64(got[2]) - want)
     assert (err <= tw).all(), f"{ctx} W: worst {np.nanmax(err / np.maximum(tw, 1e-300)):.2f} of the bound, {np.isnan(err).sum()} NaN"
+
+
+@pytest.mark.parametrize("top", [118, -118])
+@pytest.mark.parametrize("H,Hkv,ctx", [(4, 1, [500]), (4, 1, [20000]), (8, 8, [3000, 700, 40]), (1, 1, [131072])])
+@pytest.mark.parametrize("D", [64, 128])
+def test_weights_range_of_bf16(fa, dev, D, H, Hkv, ctx, top):
+    """V of 2^118 and of 2^-118 in equal weights: what up to 131072 of them add up to is past the range, O is V. Equal weights' sums
+    are (n / 16 + 64) 2^-24 off, twice: 2^-10, below half a place of O."""
+    q, kp, vp, table, c, w = _paged(dev, 3, len(ctx), H, Hkv, D, ctx, "bf16", poison=False)
+    kp.zero_()
+    sign = torch.where(torch.arange(D, device=dev) % 3 == 0, -1.0, 1.0)
+    vp.copy_((sign * 2.0 ** top).expand_as(vp))
+    O, L, W = fa.decode_paged_weights(q, kp, vp, table, c, w)
+    assert torch.equal(O, (sign * 2.0 ** top).to(O.dtype).expand_as(O))
+    for b, n in enumerate(ctx):
+        off = (n / 16 + 64) * 2.0 ** -24 + 2.0 ** -21
+        assert (L[b].double() - math.log(n)).abs().max() <= off + 2.0 ** -21 * math.log(n)
+        add = (W[b, :, :n].double() - w[b, :, :n].double()) * n * Hkv / H
+        assert (add - 1).abs().max() <= off + 2.0 ** -24 * 4 * n * Hkv / H   # and the sum with weights of up to 3

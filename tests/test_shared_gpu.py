@@ -371,3 +371,21 @@ def test_climbing_scores(fa, dev, D, dtype, B, H, Hkv, P, ctx, wide):
     in rows side by side: one launch, chunks, and tiles."""
     case = _climbing_scores(_case(dev, P, B, H, Hkv, D, P, ctx, dtype, extra=wide))
     _check(fa.decode_shared(*case), _want_exact(case, HALF[dtype], HALF[dtype]), dtype, f"B {B}")
+
+
+@pytest.mark.parametrize("top", [118, -110])
+@pytest.mark.parametrize("B,H,Hkv,P,ctx,wide", [(2, 8, 2, 250, [200, 0], 0), (2, 8, 2, 20000, [3000, 70], 0), (40, 32, 8, 20000, [9 * i for i in range(40)], 80),
+                                                (17, 4, 2, 130000, [5] * 17, 0), (1, 2, 1, 0, [131072], 0)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_range_of_bf16(fa, dev, D, B, H, Hkv, P, ctx, wide, top):
+    """V of 2^118 and 2^-110 in equal weights, in one launch, over chunks and over tiles: what up to 131072 of them add up to is past
+    the range, O is V. Equal weights' sums are (n / 16 + 64) 2^-24 off, twice: 2^-10, below half a place of O."""
+    q, kp, vp, prefix, plen, table, c = _case(dev, 3, B, H, Hkv, D, P, ctx, "bf16", poison=False, extra=wide)
+    kp.zero_()
+    sign = torch.where(torch.arange(D, device=dev) % 3 == 0, -1.0, 1.0)
+    vp.copy_((sign * 2.0 ** top).expand_as(vp))
+    O, L = fa.decode_shared(q, kp, vp, prefix, plen, table, c)
+    assert torch.equal(O, (sign * 2.0 ** top).to(O.dtype).expand_as(O))
+    n = (c + plen).double().cpu().numpy()
+    want = np.log(n)[:, None]
+    assert (np.abs(L.double().cpu().numpy() - want) <= (n[:, None] / 16 + 64) * 2.0 ** -24 + 2.0 ** -21 * want).all()
