@@ -29,6 +29,13 @@ namespace cache {
 using namespace stream;
 using pages::kPageSize;
 
+// What the scores of a head are turned into weights by, from their maximum and sum: (maximum, 1 /
+// sum). Where every score is -inf, O is 0, L -inf and every weight 0: (0, 0), as -inf has no
+// difference to itself; a NaN sum keeps its NaN.
+__device__ __forceinline__ float2 by_head(float m, float z) {
+  return make_float2(m == -INFINITY ? 0.f : m, z == 0.f ? 0.f : 1.f / z);
+}
+
 template <int D, bool BF16, bool NT>
 __global__ void __launch_bounds__(stream::kThreads)
 fa_weights_chunk_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k_pool,
@@ -73,7 +80,7 @@ fa_weights_one_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k
   constexpr int STRIDE = kOnePages * kTokens + 4;
   __shared__ Shared<D, kOneWaves> sh;
   __shared__ __attribute__((aligned(16))) float scores[16 * STRIDE];
-  __shared__ float2 J[16];   // of a group's heads: maximum, 1 / sum
+  __shared__ float2 J[16];   // of a group's heads, see by_head
   const int hk = blockIdx.x, b = blockIdx.y, G = H / Hkv;
   const int col = threadIdx.x & 15, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ctx = __builtin_amdgcn_readfirstlane(ctx_lens[b]), pages = pages_of(ctx, max_pages);
@@ -84,7 +91,7 @@ fa_weights_one_kernel(const uint16_t* __restrict__ q, const char* __restrict__ k
                              pages, ctx < 0 || (ctx > 0 && pages == 0), live, row * D, hk, Hkv, num_pages,
                              c, ScoresKept{scores, STRIDE}, out, [&](float m, float z) {
                                out(m, z);
-                               J[col] = make_float2(m, 1.f / z);
+                               J[col] = by_head(m, z);
                              });
   __syncthreads();
   const int width = max_pages * kPageSize, n = min(max(ctx, 0), width);
@@ -136,7 +143,7 @@ fa_weights_join_kernel(const float* __restrict__ part_o, const float2* __restric
   f32x4 w = f32x4{};
   if (there) w = *reinterpret_cast<const f32x4*>(w_in + at);
   if (start < ctx) {
-    __shared__ float2 J[kJoinThreads];   // of a group's heads: maximum, 1 / sum
+    __shared__ float2 J[kJoinThreads];   // of a group's heads, see by_head
     const int2 f = first_of[b];
     f32x4 sum = f32x4{};
     for (int g0 = 0; g0 < G; g0 += kJoinThreads) {
@@ -144,7 +151,7 @@ fa_weights_join_kernel(const float* __restrict__ part_o, const float2* __restric
       if (g0 > 0) __syncthreads();
       for (int g = wave; g < gs; g += kJoinThreads / 64) {
         const float2 x = join_wave(Parts{part_o, part_ml, (int64_t)f.x * H + hk * G + g0 + g, H, f.y}, c);
-        if ((tid & 63) == 0) J[g] = make_float2(x.x, 1.f / x.y);
+        if ((tid & 63) == 0) J[g] = by_head(x.x, x.y);
       }
       __syncthreads();
       if (there && j < ctx) {

@@ -621,7 +621,8 @@ int fa_validate_decode_shared(const void* q, const void* k_pool, const void* v_p
  * fp32 [B, H_kv, max_pages * 16], 16-byte aligned; slots past the context keep
  * their value. weights_out may be weights (in place), but not overlap it
  * otherwise. Where o and lse are NaN (an invalid page or length), so are the
- * sequence's weights up to its context, cut to the table. How the pages are shared
+ * sequence's weights up to its context, cut to the table; a head whose scores are all
+ * -inf (o 0, lse -inf) adds nothing. How the pages are shared
  * out follows from the lengths of the whole batch, so a sequence's last bits may
  * depend on the others' lengths; the same call gives the same bits. workspace:
  * fa_decode_weights_workspace_floats(...) floats, 16-byte aligned, need not be

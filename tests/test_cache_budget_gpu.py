@@ -420,3 +420,25 @@ def test_weights_range_of_bf16(fa, dev, D, H, Hkv, ctx, top):
         assert (L[b].double() - math.log(n)).abs().max() <= off + 2.0 ** -21 * math.log(n)
         add = (W[b, :, :n].double() - w[b, :, :n].double()) * n * Hkv / H
         assert (add - 1).abs().max() <= off + 2.0 ** -24 * 4 * n * Hkv / H   # and the sum with weights of up to 3
+
+
+@pytest.mark.parametrize("wide", [0, 40])
+@pytest.mark.parametrize("D,dtype", [(64, "fp16"), (128, "bf16")])
+def test_weights_masked_by_minus_infinity(fa, dev, D, dtype, wide):
+    """Keys whose scores are -inf get no weight; where all of a head are, O is 0, L -inf and the weights stay as they were."""
+    q, kp, vp, table, c, w = _paged(dev, 8, 3, 8, 2, D, [300, 33, 16], dtype, extra=wide)
+    q[..., 0] = q[..., 0].abs() + 0.5
+    k = kp.clone()
+    for b, n in ((0, 300), (1, 33)):
+        k[table[b, :-(-n // 16)].long(), 0, :, 0] = -math.inf      # KV head 0: all
+    k[table[0, :10].long(), 1, :, 0] = -math.inf                   # and of head 1 the first 160 keys
+    O, L, W = fa.decode_paged_weights(q, k, vp, table, c, w)
+    assert (O[:2, :4] == 0).all() and torch.isneginf(L[:2, :4]).all() and torch.equal(W[:2, 0], w[:2, 0])
+    assert torch.equal(W[0, 1, :160], w[0, 1, :160])
+    for b, h, skip in ((0, 1, 160), (1, 1, 0), (2, 0, 0), (2, 1, 0)):
+        n, g = int(c[b]), slice(4 * h, 4 * h + 4)
+        kk, vv = (cache.rows(_f64(x), table[b, :-(-n // 16)].cpu().numpy(), n, h)[skip:] for x in (kp, vp))
+        o, l, p, to, tl, tp = cache.attend(_f64(q[b, g]), kk, vv, HALF[dtype])
+        assert (np.abs(_f64(O[b, g]) - o) <= to).all() and (np.abs(_f64(L[b, g]) - l) <= tl).all()
+        want = _f64(w[b, h, skip:n]) + p.sum(0)
+        assert (np.abs(_f64(W[b, h, skip:n]) - want) <= tp.sum(0) + 5 * 2.0 ** -24 * want).all()
