@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from oracle import cache, rotary
-from test_shared_gpu import HALF, HUGE, TYPES, _case, _check, _huge_scores, _i32
+from test_shared_gpu import HALF, HUGE, TYPES, _case, _check, _climbing_scores, _huge_scores, _i32
 
 pytestmark = pytest.mark.gpu
 
@@ -442,3 +442,152 @@ def test_weights_masked_by_minus_infinity(fa, dev, D, dtype, wide):
         assert (np.abs(_f64(O[b, g]) - o) <= to).all() and (np.abs(_f64(L[b, g]) - l) <= tl).all()
         want = _f64(w[b, h, skip:n]) + p.sum(0)
         assert (np.abs(_f64(W[b, h, skip:n]) - want) <= tp.sum(0) + 5 * 2.0 ** -24 * want).all()
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("B,H,Hkv,D,ctx", [(8, 32, 8, 128, [200, 0, 777, 4, 1025, 16, 90, 3]), (3, 16, 8, 64, [2000, 33, 515])])
+def test_weights_of_a_large_pool(fa, dev, B, H, Hkv, D, ctx, dtype):
+    """Pools from 64 MiB on: pages are read past the caches."""
+    pages = (64 << 20) // (Hkv * 16 * D * 4)
+    case = _paged(dev, 11, B, H, Hkv, D, ctx, dtype, spare=pages, extra=40)
+    got = fa.decode_paged_weights(*case)
+    _check_weights(got, case, dtype)
+    again = fa.decode_paged_weights(*case)
+    assert all(torch.equal(x, y) for x, y in zip(got, again))
+
+
+@pytest.mark.parametrize("wide", [0, 40])
+def test_weights_far_pages(fa, dev, wide):
+    """Pages past 2^31 values of a pool, in one launch and in chunks; the same call on a small pool gives its bits."""
+    Hkv, D = 8, 128
+    pages = (1 << 31) // (Hkv * 16 * D) + 100
+    q, kp, vp, table, c, w = _paged(dev, 12, 3, 16, Hkv, D, [150, 0, 33], "bf16", spare=0, extra=wide)
+    n = kp.shape[0]
+    far = []
+    for x in (kp, vp):
+        y = torch.empty(pages, Hkv, 16, D, dtype=x.dtype, device=dev)
+        y[pages - n:] = x
+        far.append(y)
+    got = fa.decode_paged_weights(q, *far, torch.where(table >= 0, table + (pages - n), table), c, w)
+    want = fa.decode_paged_weights(q, kp, vp, table, c, w)
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+    _check_weights(got, (q, kp, vp, table, c, w), "bf16")
+
+
+@pytest.mark.parametrize("ctx,wide", [([400, 9], 0), ([2500, 77, 0], 0), ([300, 5], 40)])
+@pytest.mark.parametrize("D,dtype", [(64, "fp16"), (128, "bf16")])
+def test_weights_climbing_scores(fa, dev, D, dtype, ctx, wide):
+    """The maximum moves along the keys, by little and by far."""
+    B = len(ctx)
+    q, kp, vp, prefix, plen, table, c = _climbing_scores(_case(dev, 5, B, 16, 2, D, 0, ctx, dtype, extra=wide))
+    w = torch.rand((B, 2, 16 * table.shape[1]), device=dev)
+    O, L, W = fa.decode_paged_weights(q, kp, vp, table, c, w)
+    want, tol = _f64(w), np.zeros(w.shape)
+    for b, n in enumerate(ctx):
+        for h in range(2 if n else 0):
+            g = slice(8 * h, 8 * h + 8)
+            k, v = (cache.rows(_f64(x), table[b, :-(-n // 16)].cpu().numpy(), n, h) for x in (kp, vp))
+            o, l, p, to, tl, tp = cache.attend_exact(_f64(q[b, g]) @ k.T, v, HALF[dtype], HALF[dtype] ** 2)
+            assert (np.abs(_f64(O[b, g]) - o) <= to).all() and (np.abs(_f64(L[b, g]) - l) <= tl).all()
+            want[b, h, :n] += p.sum(0)
+            tol[b, h, :n] = tp.sum(0) + 9 * 2.0 ** -24 * want[b, h, :n]
+    assert (np.abs(_f64(W) - want) <= tol).all()
+
+
+# Tables of the eviction: up to 256 pages the selection lists what stays, beyond a launch of its own does; up to 1024, to 2048 and
+# more pages it has 16, 32 and no keys of a thread in registers.
+WIDE = [300, 1100, 2100]
+
+
+@pytest.mark.parametrize("wide", WIDE)
+@pytest.mark.parametrize("kind", ["zeros", "one value", "nan", "negative", "infinite", "steps", "bits"])
+def test_evict_odd_weights_of_wide_tables(fa, dev, kind, wide):
+    """As test_evict_odd_weights."""
+    ctx, keep, recent = [700, 90, 2500], 100, 9
+    pools, table, c, w, new_table = _evict_case(dev, 20, 2, 64, ctx, keep, wide=wide)
+    rng = np.random.default_rng(5)
+    if kind == "zeros":
+        w[:] = np.where(rng.random(w.shape) < 0.5, 0.0, -0.0)
+    elif kind == "one value":
+        w[:] = 0.25
+    elif kind == "nan":
+        w[rng.random(w.shape) < 0.97] = np.nan
+    elif kind == "negative":
+        w[:] = rng.standard_normal(w.shape)
+    elif kind == "infinite":
+        w[rng.random(w.shape) < 0.3] = np.inf
+        w[rng.random(w.shape) < 0.3] = -np.inf
+    elif kind == "steps":
+        w[:] = np.float32(1) + rng.integers(0, 40, w.shape).astype(np.float32) * np.float32(2.0 ** -23)
+    else:
+        w[:] = rng.integers(0, 2 ** 32, w.shape, dtype=np.uint32).view(np.float32)
+    _check_evict(fa, dev, pools, table, c, w, new_table, keep, recent, kind)
+
+
+@pytest.mark.parametrize("wide", WIDE)
+def test_evict_invalid_of_wide_tables(fa, dev, wide):
+    """As test_evict_invalid."""
+    ctx, keep, recent = [100, 100, 100, 100, 30, 100], 40, 8
+    pools, table, c, w, new_table = _evict_case(dev, 21, 2, 64, ctx, keep, wide=wide)
+    pages = pools[0].shape[0]
+    table[0, 6] = pages
+    new_table[1, 1] = -7
+    c[2], c[3] = -1, 16 * table.shape[1] + 1
+    new_table[4, 0] = pages
+    _check_evict(fa, dev, pools, table, c, w, new_table, keep, recent)
+    got = _run_evict(fa, dev, pools, table, c, w, new_table, keep, recent)
+    assert got[5].tolist() == [1, 1, 1, 1, 1, 0] and got[4].tolist() == [40, 40, 0, 0, 30, 40]
+
+
+@pytest.mark.parametrize("wide", [0, *WIDE])
+@pytest.mark.parametrize("keep,recent", [(64, 0), (64, 1), (64, 63), (64, 64), (1500, 1500), (1500, 20), (1, 0), (1, 1)])
+def test_evict_mixed_batches(fa, dev, keep, recent, wide):
+    """Caches above, at and below the budget, empty ones and an invalid length side by side; nothing but the newest, and nothing of them."""
+    ctx = [1, 64, 65, 0, 4000, 63, 1500, 1501, 17]
+    case = _evict_case(dev, 24, 2, 64, ctx, keep, "bf16", wide=wide)
+    case[2][8] = -3
+    _check_evict(fa, dev, *case, keep, recent, f"{keep} {recent}")
+
+
+@pytest.mark.parametrize("ctx,keep,recent", [([20000], 4096, 256), ([17000, 300, 32768, 16385], 1000, 0), ([33000], 4096, 4096)])
+def test_evict_long(fa, dev, ctx, keep, recent):
+    """Lengths that fill tables of 1025 pages and more."""
+    _check_evict(fa, dev, *_evict_case(dev, 25, 2, 64, ctx, keep, "bf16"), keep, recent)
+
+
+def test_graphs_of_one_pool(fa, dev):
+    """A decode with weights and an eviction, captured with one memory pool, so that their workspaces share memory, replayed in
+    turn with new queries and lengths, eager calls between."""
+    q, kp, vp, table, c, w = _paged(dev, 26, 3, 16, 2, 64, [600, 90, 300], "fp16", poison=False, extra=300, spare=60)
+    t, n = table.clone().clamp_(min=0), kp.shape[0]
+    used = set(table[table >= 0].tolist())
+    new = torch.tensor([i for i in range(n) if i not in used][:24], dtype=torch.int32, device=dev).reshape(3, 8)
+
+    def decode(w):
+        return fa.decode_paged_weights(q, kp, vp, t, c, w)
+
+    def evict(k, v):
+        return fa.kv_evict(k, v, t, c, w, new, 100, 10)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        decode(w), evict(kp.clone(), vp.clone())
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs, pool = [], [], None
+    for call in (lambda: decode(w), lambda: evict(kp, vp)):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool):
+            outs.append(call())
+        pool = graph.pool()
+        graphs.append(graph)
+    for i in range(4):
+        q.copy_(torch.randn_like(q))
+        w.copy_(torch.rand_like(w))
+        c[0] = 600 - 100 * i
+        pools = kp.clone(), vp.clone()
+        for graph in graphs:
+            graph.replay()
+        want = [*decode(w), *evict(*pools)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip([*outs[0], *outs[1], kp, vp], [*want, *pools])), i

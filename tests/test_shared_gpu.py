@@ -389,3 +389,192 @@ def test_range_of_bf16(fa, dev, D, B, H, Hkv, P, ctx, wide, top):
     n = (c + plen).double().cpu().numpy()
     want = np.log(n)[:, None]
     assert (np.abs(L.double().cpu().numpy() - want) <= (n[:, None] / 16 + 64) * 2.0 ** -24 + 2.0 ** -21 * want).all()
+
+
+# ---------------------------------------------------------------------------
+# The prefix in tiles: more than 32 query rows a KV head, tables too wide for one launch
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("P", [0, 1, 15, 16, 17, 31, 32, 33, 48, 63, 64, 65, 127, 128, 129, 191, 193, 255, 256, 257, 319, 321])
+@pytest.mark.parametrize("D,dtype", [(64, "bf16"), (128, "fp16")])
+def test_tiles_prefix_lengths(fa, dev, P, D, dtype):
+    """The prefix ends at every place of a page, a tile and the ring of tiles; an empty one too."""
+    case = _case(dev, P, 12, 8, 2, D, P, [5, 0, 31] * 4, dtype, extra=80)
+    got = fa.decode_shared(*case)
+    _check(got, _want(case, dtype), dtype)
+    again = fa.decode_shared(*case)
+    assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_tiles_invalid_pages_and_lengths(fa, dev, D, dtype):
+    """An invalid own page or length makes its sequence NaN, an invalid prefix all of them."""
+    B, ctx = 40, [40, 40, 40, 0, 16] + [7] * 35
+    case = list(_case(dev, 4, B, 8, 2, D, 200, ctx, dtype, spare=1, extra=80))
+    good = fa.decode_shared(*case)
+    pages = case[1].shape[0]
+    t = case[5].clone()
+    t[0, 1], t[1, 2] = -1, pages
+    c = case[6].clone()
+    c[2] = 16 * t.shape[1] + 1
+    c[4] = -1
+    O, L = fa.decode_shared(*case[:5], t, c)
+    for b in (0, 1, 2, 4):
+        assert torch.isnan(O[b]).all() and torch.isnan(L[b]).all(), b
+    assert torch.isfinite(O[3]).all() and torch.isfinite(O[5:]).all() and torch.isfinite(L[5:]).all()
+    t = case[5].clone()
+    t[0, 1], t[1, 2] = -1, pages   # the lengths as they were: the rest keep their bits
+    O, L = fa.decode_shared(*case[:5], t, case[6])
+    assert torch.isnan(O[:2]).all() and torch.equal(O[2:], good[0][2:]) and torch.equal(L[2:], good[1][2:])
+    for at, page in ((0, -5), (12, pages), (5, 2 ** 31 - 1)):
+        p = case[3].clone()
+        p[at] = page
+        O, L = fa.decode_shared(*case[:3], p, *case[4:])
+        assert torch.isnan(O).all() and torch.isnan(L).all(), (at, page)
+    for n in (-1, 16 * case[3].numel() + 1, 2 ** 31 - 1):
+        O, L = fa.decode_shared(*case[:4], _i32(dev, [n]), *case[5:])
+        assert torch.isnan(O).all() and torch.isnan(L).all(), n
+    p = case[3].clone()   # entries past the prefix are not looked at
+    p[4:] = -1
+    O, L = fa.decode_shared(*case[:3], p, _i32(dev, [64]), *case[5:])
+    assert torch.isfinite(O).all() and torch.isfinite(L).all()
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_tiles_no_keys(fa, dev, dtype):
+    """Neither a prefix nor own tokens: O 0 and L -inf, beside sequences that have some."""
+    case = _case(dev, 5, 40, 8, 2, 128, 0, [0, 100, 1, 0, 777] * 8, dtype, extra=80)
+    got = fa.decode_shared(*case)
+    _check(got, _want(case, dtype), dtype)
+    assert (got[0][3] == 0).all() and torch.isneginf(got[1][3]).all()
+
+
+def test_tiles_prefix_in_the_own_pages(fa, dev):
+    """The same keys shared, and as the start of every sequence's own pages: one result within the bounds."""
+    ctx = [30, 1, 0, 64, 15, 16] * 4
+    case = _case(dev, 6, 24, 16, 4, 64, 160, ctx, "bf16", extra=80)
+    q, kp, vp, prefix, plen, table, c = case
+    joined = torch.cat((prefix[:10].expand(24, 10), table), 1).contiguous()
+    _check(fa.decode_shared(q, kp, vp, prefix, plen * 0, joined, c + 160), _want(case, "bf16"), "bf16")
+    _check(fa.decode_shared(*case), _want(case, "bf16"), "bf16")
+
+
+@pytest.mark.parametrize("D,dtype", [(64, "fp16"), (128, "bf16")])
+@pytest.mark.parametrize("amp", [8.0, 60.0])
+def test_tiles_sharp_and_large_scores(fa, dev, amp, D, dtype):
+    """Scores of hundreds: a few keys carry the weight, and the maximum moves along the keys by more than the weights' slack."""
+    case = _case(dev, 7, 40, 8, 2, D, 1700, [50, 0, 3, 100] * 10, dtype, amp=amp, extra=80)
+    _check(fa.decode_shared(*case), _want(case, dtype), dtype, f"amp {amp}")
+
+
+@pytest.mark.parametrize("D,dtype", [(64, "fp16"), (128, "bf16")])
+def test_tiles_masked_by_minus_infinity(fa, dev, D, dtype):
+    """Keys whose scores are -inf have no weight: the first tiles, a page's part, the whole prefix of a KV head, every key of a row."""
+    B, P = 40, 256
+    q, kp, vp, prefix, plen, table, ctx = _case(dev, 8, B, 4, 2, D, P, [16, 3] * 20, dtype, extra=80)
+    q[..., 0] = q[..., 0].abs() + 0.5
+    live = np.ones((2, P), bool)
+    live[0, :128] = live[0, 195:201] = False
+    live[1] = False
+    for h in range(2):
+        for j in range(P):
+            if not live[h, j]:
+                kp[prefix[j // 16].long(), h, j % 16, 0] = -math.inf
+    kp[table[2, 0].long(), 1, :, 0] = -math.inf   # sequence 2, KV head 1: all
+    O, L = fa.decode_shared(q, kp, vp, prefix, plen, table, ctx)
+    f = lambda t: t.cpu().double().numpy()
+    for b in (0, 1, 2, 39):
+        for h in range(4):
+            if b == 2 and h >= 2:
+                assert (O[b, h] == 0).all() and torch.isneginf(L[b, h])
+                continue
+            k, v = (np.concatenate([cache.rows(f(x), prefix.cpu().numpy(), P, h // 2)[live[h // 2]],
+                                    cache.rows(f(x), table[b].cpu().numpy(), int(ctx[b]), h // 2)]) for x in (kp, vp))
+            o, l, _, to, tl, _ = cache.attend(f(q[b, h:h + 1]), k, v, HALF[dtype])
+            assert (np.abs(f(O[b, h]) - o[0]) <= to[0]).all() and abs(float(L[b, h]) - l[0]) <= tl[0]
+
+
+@pytest.mark.parametrize("D,dtype", [(64, "fp16"), (128, "bf16")])
+def test_tiles_nan_stays_in_its_head(fa, dev, D, dtype):
+    """A NaN in a key or a value of the prefix, or in an own value, reaches every query that sees it and no other."""
+    case = _case(dev, 9, 24, 8, 4, D, 100, [20] * 24, dtype, extra=80)
+    q, kp, vp, prefix, plen, table, ctx = case
+    good = fa.decode_shared(*case)
+    kp[int(prefix[2]), 1, 5, 7] = math.nan
+    vp[int(prefix[6]), 0, 3, 11] = math.nan
+    vp[int(table[2, 0]), 3, 4, 9] = math.nan
+    O, L = fa.decode_shared(*case)
+    assert torch.isnan(O[:, 2:4]).all() and torch.isnan(L[:, 2:4]).all()
+    assert torch.isnan(O[:, :2, 11]).all() and torch.isnan(O[2, 6:8, 9]).all()
+    same = torch.ones(24, 8, D, dtype=torch.bool, device=dev)
+    same[:, 2:4] = False
+    same[:, :2, 11] = False
+    same[2, 6:8, 9] = False
+    assert torch.equal(O[same], good[0][same])
+    keep = torch.tensor([0, 1, 4, 5, 6, 7], device=dev)
+    assert torch.equal(L[:, keep], good[1][:, keep])
+
+
+@pytest.mark.parametrize("few", [True, False])
+def test_far_pages_of_chunks_and_tiles(fa, dev, few):
+    """Pages past 2^31 values of a pool, in chunks and in tiles that pass the caches; the same call on a small pool gives its bits."""
+    Hkv, D = 8, 128
+    pages = (1 << 31) // (Hkv * 16 * D) + 200
+    B = 2 if few else 20
+    case = _case(dev, 10, B, 16, Hkv, D, 350, [40, 9] * (B // 2), "bf16", spare=0, extra=80)
+    q, kp, vp, prefix, plen, table, ctx = case
+    n = kp.shape[0]
+    far = []
+    for x in (kp, vp):
+        y = torch.empty(pages, Hkv, 16, D, dtype=x.dtype, device=dev)
+        y[pages - n:] = x
+        far.append(y)
+    shift = lambda t: torch.where(t >= 0, t + (pages - n), t)
+    got = fa.decode_shared(q, *far, shift(prefix), plen, shift(table), ctx)
+    want = fa.decode_shared(*case)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    _check(got, _want(case, "bf16"), "bf16")
+
+
+def test_tiles_two_streams(fa, dev):
+    cases = [_case(dev, 13 + i, 24, 16, 4, 128, 600 + 100 * i, [40, 0, 9, 100, 1, 64] * 4, "bf16", extra=80) for i in range(2)]
+    want = [fa.decode_shared(*c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(fa.decode_shared(*cases[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(a, want[i][0]) and torch.equal(b, want[i][1]) for a, b in got[i])
+
+
+def test_graphs_of_one_pool(fa, dev):
+    """Captured calls, in tiles and in chunks, of one memory pool, so that their workspaces share memory, replayed in turn with new
+    lengths and queries, eager calls between."""
+    side = torch.cuda.Stream()
+    runs, pool = [], None
+    for seed, shape in ((11, (40, 8, 2, 64, 300, [50, 3, 0, 7] * 10)), (12, (3, 8, 2, 128, 900, [5, 80, 0])), (13, (24, 32, 8, 128, 900, [5 * i for i in range(24)]))):
+        case = _case(dev, seed, *shape, "fp16", poison=False, extra=80)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            fa.decode_shared(*case)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool):
+            out = fa.decode_shared(*case)
+        pool = graph.pool()
+        runs.append((case, graph, out))
+    for i in range(4):
+        for case, graph, out in runs:
+            case[0].copy_(torch.randn_like(case[0]))
+            case[4].fill_(17 * i + 1)
+            case[6].clamp_(max=40 - 9 * i)
+            graph.replay()
+        for case, graph, out in runs:
+            want = fa.decode_shared(*case)
+            torch.cuda.synchronize()
+            assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1]), i
+            _check(out, _want(case, "fp16"), "fp16")
