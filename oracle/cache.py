@@ -52,6 +52,8 @@ def attend_exact(s, v, half, p_half):
     - a sum of n weights, and of n products, in up to 16 parts: (n / 16 + 64) u;
     - P is off by p_half of itself, or 2^-25 of the largest below fp16's normal numbers; O by half of itself.
     """
+    if s.shape[1] == 0:
+        return attend(np.zeros((len(s), v.shape[-1])), v, v, half)
     D, u = v.shape[-1], 2.0 ** -24
     m = s.max(1, keepdims=True)
     x = (s - m) / np.sqrt(D) / np.log(2)

@@ -9,7 +9,8 @@ import pytest
 import torch
 
 from oracle import cache, rotary
-from test_shared_gpu import HALF, HUGE, TYPES, _case, _check, _climbing_scores, _huge_scores, _i32
+from test_shared_gpu import (HALF, HUGE, TYPES, _case, _check, _climbing_scores, _coherent_roundings, _huge_scores, _i32, _one_term,
+                             _want_exact)
 
 pytestmark = pytest.mark.gpu
 
@@ -591,3 +592,14 @@ def test_graphs_of_one_pool(fa, dev):
         want = [*decode(w), *evict(*pools)]
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip([*outs[0], *outs[1], kp, vp], [*want, *pools])), i
+
+
+@pytest.mark.parametrize("ctx,wide", [([320, 16], 0), ([320, 16], 40), ([4000, 0], 0)])
+@pytest.mark.parametrize("D,dtype", [(64, "fp16"), (128, "fp16"), (64, "bf16"), (128, "bf16")])
+def test_weighted_values_keep_two_terms(fa, dev, D, dtype, ctx, wide):
+    """P has two terms of the type, 22 bits in fp16 and 16 in bf16, in one launch and in chunks."""
+    case = _coherent_roundings(_case(dev, 3, 2, 8, 2, D, 0, ctx, dtype, poison=False, extra=wide))
+    want = _want_exact(case, HALF[dtype], HALF[dtype] ** 2)
+    assert not _one_term(case, want, 0, ctx[0])
+    q, kp, vp, _, _, table, c = case
+    _check(fa.decode_paged_weights(q, kp, vp, table, c, torch.zeros(2, 2, 16 * table.shape[1], device=dev))[:2], want, dtype)

@@ -578,3 +578,42 @@ def test_graphs_of_one_pool(fa, dev):
             torch.cuda.synchronize()
             assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1]), i
             _check(out, _want(case, "fp16"), "fp16")
+
+
+def _coherent_roundings(case):
+    """Keys of two weights, e^(-a / sqrt(D)) and e^(-b / sqrt(D)) of the largest, one that the type rounds up by nearly half a step and
+    one that it rounds down, with values that cancel: what P's rounding does to O adds up, and O's own does not hide it. The first
+    slot of each page has the largest weight, which is 1 in every part, and no value."""
+    q, kp, vp = case[:3]
+    D, dt, dev = q.shape[-1], q.dtype, q.device
+    steps = torch.arange(1, 128, dtype=torch.float64) / 32
+    p = torch.exp(-steps / math.sqrt(D))
+    off = (p.to(dt).double() - p) / p
+    a, b = int(off.argmax()), int(off.argmin())
+    kp.zero_(), vp.zero_(), q.zero_()
+    q[..., 0] = 1
+    kp[:, :, 1::2, 0], kp[:, :, 2::2, 0] = -float(steps[a]), -float(steps[b])
+    sign = torch.where(torch.arange(D, device=dev) % 3 == 0, -1.0, 1.0).to(dt)
+    vp[:, :, 1::2] = sign
+    vp[:, :, 2::2] = sign * -float(8 * p[a] / (7 * p[b]))
+    return case
+
+
+def _one_term(case, want, b, n):
+    """Whether O of sequence b, of n keys of page 0's kind, would pass the bounds if P were rounded to the type once."""
+    q, kp, vp = case[:3]
+    k, v = (x[0, 0].cpu().double().repeat(-(-n // 16), 1)[:n] for x in (kp, vp))
+    s = k @ q[b, 0].cpu().double() / math.sqrt(q.shape[-1])
+    e = torch.exp(s - s.max())
+    o = (e.to(q.dtype).double() @ v / e.sum()).numpy()
+    return (np.abs(o - want[0][b, 0]) <= 4 * want[2][b, 0]).any()
+
+
+@pytest.mark.parametrize("B,P,ctx,wide", [(2, 160, [160, 0], 0), (2, 160, [160, 0], 80), (3, 4000, [320, 16, 0], 0), (40, 0, [320] * 40, 80)])
+@pytest.mark.parametrize("D,dtype", [(64, "fp16"), (128, "fp16"), (64, "bf16"), (128, "bf16")])
+def test_weights_keep_two_terms(fa, dev, D, dtype, B, P, ctx, wide):
+    """P has two terms of the type, 22 bits in fp16 and 16 in bf16, in one launch, in chunks of a prefix, and in own pages."""
+    case = _coherent_roundings(_case(dev, 3, B, 8, 2, D, P, ctx, dtype, poison=False, extra=wide))
+    want = _want_exact(case, HALF[dtype], HALF[dtype] ** 2)
+    assert not _one_term(case, want, 0, P + ctx[0])
+    _check(fa.decode_shared(*case), want, dtype)
