@@ -300,7 +300,8 @@ def decode_shared(q, k_pool, v_pool, prefix_table, prefix_len, page_table, ctx_l
     then its own paged K/V, as one softmax; decode_paged's dtypes.
 
     The prefix is the first prefix_len (int32, one value, on the device) tokens of the
-    pages prefix_table (int32 [prefix_pages]), read once for the whole batch;
+    pages prefix_table (int32 [prefix_pages]), read once for every 128 query rows (b, h)
+    of a KV head, for every 16 where there are up to 32, and of short tables once a sequence;
     page_table and ctx_lens are those of the sequences' own tokens (lengths may be 0).
     An invalid prefix makes every O and L NaN, an invalid own page those of its sequence.
     """
@@ -313,7 +314,7 @@ def decode_paged_weights(q, k_pool, v_pool, page_table, ctx_lens, weights, inpla
 
     inplace: W is weights itself. Slots past a context keep their value; where O and L
     are NaN (an invalid page or length), W is NaN over the context. The split over the
-    pages follows the batch's lengths, on the device.
+    pages follows the batch's lengths, on the device, and the table's width.
     """
     return _C.decode_paged_weights(q, k_pool, v_pool, page_table, ctx_lens, weights, inplace)
 

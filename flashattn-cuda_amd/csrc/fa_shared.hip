@@ -24,7 +24,8 @@ namespace shared {
 using namespace stream;
 
 // The cuts are made for the 256 CUs of a whole MI355X, whatever the device has: the
-// workspace follows from the sizes alone.
+// workspace follows from the sizes alone. A partition of fewer CUs gets the same results by
+// cuts that are not its own.
 constexpr int kCus = 256, kMostUnits = 192;   // units: of the prefix pass in tiles
 
 constexpr int kTile = 64;     // keys of a tile: 4 pages
@@ -56,7 +57,10 @@ struct TileShared {
 // copy's range ends there), and wait in a ring of kStages. Scores and products are
 // those of the forward: S^T = K Q^T with Q in registers, O^T += V^T P^T with P^T
 // straight from the accumulators (fa_tile.hpp), P rounded to the operands' type beside
-// an unrounded sum, as the forward rounds it.
+// an unrounded sum, as the forward rounds it. O is then 1.35 times as far from 64 bits as its own
+// rounding; the chunks' second term would cost bf16 its products again and 40 vector instructions
+// a tile: 28.8 -> 34.5 us for 32 sequences of 50 to 1500 tokens under 7999, 68.4 -> 86.7 for 64 of
+// 20 to 1000 under 32768 (H32 over 8, D = 128).
 //
 // Bound, with 128 rows a KV head, by memory: 256 units at D = 128 take 1.55 us a tile,
 // 5.4 TB/s. With more, the row blocks of a tile find it in their L2 and a tile takes 1.2
@@ -480,12 +484,13 @@ fa_shared_join_kernel(const float* __restrict__ pre_o, const float2* __restrict_
                     o + (int64_t)row * D, lse + row);
 }
 
-// A call is one launch, a workgroup for a sequence and 16 heads, where nothing would be
+// A call is one launch, a workgroup for a sequence and 16 heads, where little would be
 // gained by cutting it: up to a workgroup a CU and kOneWork dims of the pages of both
 // tables (36 pages of D = 128), or two and half of it. A call by itself, us, in one launch
-// and cut: D = 64, 32 workgroups, 16 pages 4.9 and 8.4, 64 pages 8.7 and 8.4, 96 pages 11.3
-// and 8.5; D = 128, 36 pages of 32 workgroups 8.7 and 8.9, of 256 9.1 and 15.4; 512
-// workgroups of 16 pages 11.7 and 16.6.
+// and cut: D = 64, 16 pages of 32 workgroups 4.8 and 8.3, 56 8.0 and 8.3, 72 9.4 and 8.3, of 128
+// 9.2 and 14.7, of 256 10.0 and 17.4, 36 of 512 11.6 and 18.0; D = 128, 36 pages of 32 8.8 and
+// 8.8, of 256 9.9 and 18.7, 18 of 512 12.4 and 18.7. One bound whatever the number of
+// workgroups: few of them lose up to 1.1 us past 56 pages of D = 64.
 constexpr int kOneWork = 36 * 128;
 static bool in_one(int64_t blocks, int64_t pages, int64_t D) {
   return blocks <= 2 * kCus && pages * D * (blocks <= kCus ? 1 : 2) <= kOneWork;

@@ -582,13 +582,15 @@ int fa_validate_kv_append_rope(const void* q, const int64_t q_strides[3], const 
  * prefix_pages), the same for every b, and to the ctx_lens[b] tokens of its own
  * pages (page_table, as in fa_decode_paged_gqa_f16; prefix_len: int32 [1] on the
  * device). o, lse are those of one softmax over both; o = 0 and lse = -inf where
- * both are empty. The prefix is read once per KV head for up to 128 query rows
- * (b, h). A page id outside [0, num_pages), a negative length or one beyond its
- * table makes o and lse of the sequence NaN, of every sequence where it is the
- * prefix's. q, pools, o fp16 (bf16 != 0: bfloat16); weights of the prefix are
- * rounded to that type for their product with V, as in the forward. How the pages
- * are shared out follows from the lengths of the whole batch, so a sequence's last
- * bits may depend on the others' lengths; the same call gives the same bits. workspace:
+ * both are empty. With R = B H / H_kv query rows a KV head, the prefix is read once
+ * for every 128 of them, up to R = 32 for every 16, and in calls of one launch (see
+ * the workspace) for every sequence and 16 heads. A page id outside [0, num_pages),
+ * a negative length or one beyond its table makes o and lse of the sequence NaN, of
+ * every sequence where it is the prefix's. q, pools, o fp16 (bf16 != 0: bfloat16); where the prefix is read for 128
+ * rows its weights are rounded to that type for their product with V, as in the
+ * forward, else they keep two terms of it. How the pages are shared out follows from
+ * the lengths of the whole batch and the widths of the tables, so a sequence's last
+ * bits may depend on these; the same call gives the same bits. workspace:
  * fa_decode_shared_workspace_floats(...) floats, 16-byte aligned, need not be
  * cleared; calls that may overlap need one each.
  */
@@ -623,8 +625,8 @@ int fa_validate_decode_shared(const void* q, const void* k_pool, const void* v_p
  * otherwise. Where o and lse are NaN (an invalid page or length), so are the
  * sequence's weights up to its context, cut to the table; a head whose scores are all
  * -inf (o 0, lse -inf) adds nothing. How the pages are shared
- * out follows from the lengths of the whole batch, so a sequence's last bits may
- * depend on the others' lengths; the same call gives the same bits. workspace:
+ * out follows from the lengths of the whole batch and the table's width, so a
+ * sequence's last bits may depend on these; the same call gives the same bits. workspace:
  * fa_decode_weights_workspace_floats(...) floats, 16-byte aligned, need not be
  * cleared; calls that may overlap need one each.
  */
