@@ -244,7 +244,8 @@ def rope_frequencies(rot_dim: int, base: float = 10000.0, scaling=None, factor: 
         def index(turns):   # of the frequency that makes so many turns within original_len
             return rot_dim * math.log(original_len / (2.0 * math.pi * turns)) / (2.0 * math.log(base))
 
-        lo, hi = math.floor(index(fast_turns)), math.ceil(index(slow_turns))   # lo < hi
+        lo = math.floor(index(fast_turns))
+        hi = max(math.ceil(index(slow_turns)), lo + 1)   # both one index: kept up to it
         ramp = torch.clamp((i - lo) / (hi - lo), 0.0, 1.0)   # 0: kept, 1: divided
         freqs = freqs * (1.0 - ramp) + freqs / factor * ramp
         scale = 0.1 * math.log(factor) + 1.0

@@ -281,6 +281,16 @@ def test_frequencies_by_parts_by_hand(fa):
     assert np.allclose(r[[45, 50, 63]], [1, 1 - 0.2 * 7 / 8, 1 - 0.72 * 7 / 8], rtol=1e-14) and (r[:46] == 1).all()
 
 
+def test_frequencies_by_parts_one_place(fa):
+    """Numbers of turns so near to each other that both places are one index: kept up to it, divided from the next on."""
+    R, base, n = 16, 1e4, 4096
+    f, _ = fa.rope_frequencies(R, base, device="cpu")
+    for k in (5, 7):
+        slow = n / (2 * math.pi) * base ** (-2 * k / R)
+        g, _ = fa.rope_frequencies(R, base, "by_parts", 8.0, n, slow_turns=slow, fast_turns=math.nextafter(slow, math.inf), device="cpu")
+        assert torch.equal(g[:k + 1], f[:k + 1]) and torch.allclose(g[k + 1:], f[k + 1:] / 8, rtol=2e-15, atol=0)
+
+
 def test_frequencies_refuse(fa):
     for kw, word in ((dict(rot_dim=0), "rot_dim"), (dict(rot_dim=15), "rot_dim"), (dict(rot_dim=16, base=1.0), "base"),
                      (dict(rot_dim=16, factor=0.5), "factor"), (dict(rot_dim=16, scaling="ramp"), "scaling"),
