@@ -31,11 +31,11 @@ constexpr int kCus = 256, kMostUnits = 192;   // units: of the prefix pass in ti
 constexpr int kTile = 64;     // keys of a tile: 4 pages
 constexpr int kStages = 4;    // tiles in LDS, three of them in flight
 constexpr float kSlack = 8.f;   // of weights' exponents; see its use
-// Of bf16 the slack is above the reference and not below it: its V reach 2^127, which a
-// weight above 1 would take out of range, while fp16's weights have no bits to lose at the lower end.
+// bf16's weights are 2^-kShift of those of the reference, up to 1: its V reach 2^127, which a
+// weight above 1 would take out of range, while fp16's have no bits to lose at the lower end.
 template <bool BF16>
 constexpr float kShift = BF16 ? kSlack : 0.f;
-constexpr float kFar = 4096.f;  // scores, in units of log 2, from which on differences are scaled; see m
+constexpr float kFar = 4096.f;  // references, in units of log 2, from which on differences are scaled
 constexpr int kKeyGroups = 2; // waves side by side over the keys of a tile
 constexpr int kRowGroups = 4, kTileRows = 32 * kRowGroups;   // and over the query rows of a unit
 constexpr int kTileWaves = kKeyGroups * kRowGroups;
@@ -57,10 +57,10 @@ struct TileShared {
 // copy's range ends there), and wait in a ring of kStages. Scores and products are
 // those of the forward: S^T = K Q^T with Q in registers, O^T += V^T P^T with P^T
 // straight from the accumulators (fa_tile.hpp), P rounded to the operands' type beside
-// an unrounded sum, as the forward rounds it. O is then 1.35 times as far from 64 bits as its own
-// rounding; the chunks' second term would cost bf16 its products again and 40 vector instructions
-// a tile: 28.8 -> 34.5 us for 32 sequences of 50 to 1500 tokens under 7999, 68.4 -> 86.7 for 64 of
-// 20 to 1000 under 32768 (H32 over 8, D = 128).
+// an unrounded sum, as the forward rounds it. O is then 1.35 times as far from 64 bits as
+// its own rounding puts it; the chunks' second term would cost bf16 a second product and 40
+// vector instructions a tile: 28.8 -> 34.5 us for 32 sequences of 50 to 1500 tokens under
+// 7999, 68.4 -> 86.7 for 64 of 20 to 1000 under 32768 (H32 over 8, D = 128).
 //
 // Bound, with 128 rows a KV head, by memory: 256 units at D = 128 take 1.55 us a tile,
 // 5.4 TB/s. With more, the row blocks of a tile find it in their L2 and a tile takes 1.2
@@ -146,10 +146,11 @@ tile_unit(TileShared<D>& sh, const int unit, const f16* __restrict__ q, const f1
   };
 
   // Reference of the weights, as K Q^T gives it (-inf: no score yet), and their sum. A weight is
-  // 2^(s c - mu), mu the scaled reference and kShift, rounded: all of a row are off by the same
-  // 2^rest, which the sums are freed of. Where a row of the wave has |mu| >= kFar the reference is taken off the
-  // scores first, which is exact however large they are (a mu of 2^27 is rounded by 2^3, of 2^31 by
-  // 2^7, past all types); always done, a tile pass of 28.8 us takes 29.4, and 46.3 at D = 64 49.3.
+  // 2^(s c - mu), mu the scaled reference and kShift, rounded: all of a row are off by the
+  // same 2^rest, which the sums are freed of. Where a row of the wave has a scaled reference
+  // of kFar or more, references are taken off the scores first, which holds however large
+  // they are (a mu of 2^27 is rounded by 2^3, of 2^31 by 2^7, past all types); always done, a
+  // tile pass of 28.8 us takes 29.4, and one of 46.3 at D = 64 49.3.
   float m = -INFINITY, l = 0.f, mu = 0.f;
   bool far = false;   // the same in the whole wave
   const auto rest = [&](float m, float mu, bool far) {
@@ -194,7 +195,8 @@ tile_unit(TileShared<D>& sh, const int unit, const f16* __restrict__ q, const f1
       const float m_new = fmaxf(m, mx);
       const bool far_new = __any(m_new != -INFINITY && fabsf(m_new) * c >= kFar);
       const float mu_new = far_new || m_new == -INFINITY ? kShift<BF16> : fmaf(m_new, c, kShift<BF16>);
-      const float alpha = m == -INFINITY ? 1.f : exp2_hw((m - m_new) * c + (rest(m_new, mu_new, far_new) - rest(m, mu, far)));
+      const float rests = rest(m_new, mu_new, far_new) - rest(m, mu, far);
+      const float alpha = m == -INFINITY ? 1.f : exp2_hw((m - m_new) * c + rests);
       l *= alpha;
 #pragma unroll
       for (int db = 0; db < DB; ++db)

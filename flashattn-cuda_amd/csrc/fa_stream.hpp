@@ -367,9 +367,9 @@ struct ScoresKept {
 // up to 16 query rows. Column col of the products is the query row at element qoff of
 // q (live: there is one). At the end row(d, v) is called for its dims d .. d + 3,
 // normalised, by some lane of the column, and stat(maximum, sum of the weights) by one:
-// (-inf, 0) of no tokens, a NaN sum where a page or the length (bad) is invalid. NT: pages are read with the non-temporal hint. Has one
-// barrier of the workgroup, so waves without a chunk call it too, with no pages and no
-// live row.
+// (-inf, 0) of no tokens, a NaN sum where a page or the length (bad) is invalid. NT:
+// pages are read with the non-temporal hint. Has one barrier of the workgroup, so waves
+// without a chunk call it too, with no pages and no live row.
 template <int D, bool BF16, bool NT, int WAVES, typename Where, typename Scores, typename Row, typename Stat>
 __device__ __forceinline__ void
 chunk_body(Shared<D, WAVES>& sh, const int wave, const uint16_t* __restrict__ q,
